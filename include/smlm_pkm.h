@@ -537,6 +537,76 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
                              int dilation, float eps, float *dh, void *dk, void *dv, float *dwh, float *dwk, float *dwv,
                              float *dconv, float *parts, void *stream);
 
+/*
+ * Cross entropy of the logits s = x W^T without storing them (F.cross_entropy(lm_head(x).float(), targets),
+ * smlm/model.py:286-293): per token logsumexp(s_n) - s_n[targets[n]], 0 where targets[n] == ignore_index, NaN where it
+ * is any other index outside the vocabulary; their mean over the tokens that are not ignored (NaN if none), or sum.
+ *   x (M, d) and w (V, d) bf16, rows of x_row_stride / w_row_stride elements (multiples of 8, 16-byte aligned, at most
+ *   2^23), d a multiple of 8; targets (M,) int64
+ *   loss  SMLM_REDUCE_NONE: (M,) fp32; otherwise fp32[2]: the loss, and the number of tokens that are not ignored
+ *   lse   (M,) fp32: the tokens' logsumexp, which the gradient needs
+ * workspace: smlm_linear_ce_workspace(M, V, d, 0) bytes, 16-byte aligned, free again when the call's work is done.
+ * Logits and sums in fp32, the sum over the tokens in fp64; the same result on every call.
+ */
+enum smlm_reduction { SMLM_REDUCE_NONE = 0, SMLM_REDUCE_MEAN = 1, SMLM_REDUCE_SUM = 2 };
+int64_t smlm_linear_ce_workspace(int64_t M, int64_t V, int64_t d, int grad);
+int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w_row_stride, const int64_t *targets,
+                   int64_t ignore_index, int reduction, int64_t M, int64_t V, int64_t d, float *loss, float *lse,
+                   void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its gradient: dx = G W (M, d) and dw = G^T x (V, d), contiguous bf16, either NULL if not wanted, with
+ * G[n, v] = c_n (softmax(s_n)[v] - [v == targets[n]]), formed in bf16 in pieces of the vocabulary of at most 512 MB (or 128
+ * columns).  grad: per_token ? (M,) fp32, c_n = grad[n] : one fp32, c_n = grad[0] / (count ? count[0] : 1), applied in
+ * fp32 behind the sums.  c_n = 0 for ignored tokens.  lse from the forward; workspace: smlm_linear_ce_workspace(M, V, d,
+ * 1) bytes, 16-byte aligned.  fp32 sums in a fixed order.
+ */
+int smlm_linear_ce_backward(const float *grad, const float *count, int per_token, const void *x, int64_t x_row_stride,
+                            const void *w, int64_t w_row_stride, const int64_t *targets, int64_t ignore_index,
+                            const float *lse, int64_t M, int64_t V, int64_t d, void *dx, void *dw, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
+/*
+ * The gated feed-forward block y = (silu(a) * b) w2^T, a | b = the halves of x w13^T (smlm/model.py:110-118).
+ *   x (M, d), w13 (2 * hidden, d), w2 (n_out, hidden) bf16 with row strides as above, d, hidden and n_out multiples of 8
+ *   act (M, hidden) bf16: scratch; y (M, n_out) contiguous bf16
+ * a, b and the gate in fp32, act and y rounded once each.
+ */
+int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w13, int64_t w13_row_stride, const void *w2,
+                   int64_t w2_row_stride, int64_t M, int64_t d, int64_t hidden, int64_t n_out, void *act, void *y,
+                   void *stream);
+
+/*
+ * Its gradients from dy (M, n_out) and the inputs alone (a and b are formed again): dx (M, d), dw13 (2 * hidden, d), dw2
+ * (n_out, hidden), contiguous bf16, each NULL if not wanted.  workspace: smlm_gated_ffn_workspace(...) bytes, 16-byte
+ * aligned.  fp32 sums in a fixed order; the gradients of a and b are rounded to bf16 as operands of their products.
+ */
+int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out);
+int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, const void *x, int64_t x_row_stride, const void *w13,
+                            int64_t w13_row_stride, const void *w2, int64_t w2_row_stride, int64_t M, int64_t d,
+                            int64_t hidden, int64_t n_out, void *dx, void *dw13, void *dw2, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
+/*
+ * Residual add and RMSNorm of a recorded pass (smlm/model.py:124-126, 156-163): xs = x + delta rounded to x's type,
+ * h = xs * rstd * w, rstd = rsqrt(mean(xs^2) + eps) in fp32.
+ *   x, xs (M, C) of x_dtype; delta (M, C) of delta_dtype or NULL (xs is then not written and may be NULL); w (C,) of
+ *   w_dtype; h (M, C) of h_dtype; rstd (M,) fp32.  Types SMLM_F32 or SMLM_BF16; all contiguous.
+ */
+int smlm_rmsnorm_train(const void *x, int x_dtype, const void *delta, int delta_dtype, const void *w, int w_dtype,
+                       float eps, int64_t M, int64_t C, void *xs, void *h, int h_dtype, float *rstd, void *stream);
+
+/*
+ * Its gradients: dx (M, C) of x_dtype = rstd (gw - hat mean(gw hat)) + dxs with gw = dh w, hat = xs rstd, and, if not
+ * NULL, the same in ddelta (delta_dtype); dw (C,) of w_dtype = sum over the rows of dh hat (NULL if not wanted).  dxs
+ * (M, C) of x_dtype, the gradient of xs, or NULL; dh or NULL likewise (not both).
+ * parts: caller-owned scratch of smlm_rmsnorm_parts(M, C) floats.  The same result on every call.
+ */
+int64_t smlm_rmsnorm_parts(int64_t M, int64_t C);
+int smlm_rmsnorm_train_backward(const void *dxs, const void *dh, int h_dtype, const void *xs, int x_dtype, const void *w,
+                                int w_dtype, const float *rstd, int64_t M, int64_t C, void *dx, void *ddelta,
+                                int delta_dtype, void *dw, float *parts, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,452 @@
+// The language model's loss over its vocabulary, from the hidden states and the output embedding, with its gradient
+// (F.cross_entropy(lm_head(x).float(), targets) of smlm/model.py:286-293), without ever holding the logits:
+//   s_n = x_n W^T, loss_n = logsumexp(s_n) - s_n[t_n], dx = G W, dW = G^T x, G = c_n (softmax(s_n) - 1[t_n]).
+//
+// Forward: a workgroup takes 256 tokens and a range of the vocabulary, forms 128 columns of logits at a time in its
+// accumulators and keeps a running maximum and sum of exponentials per lane, each lane over its own columns (no exchange
+// between lanes until the range ends).  The (maximum, sum) of every range go to a small array, which a second kernel joins,
+// one wavefront per token; the target's logit is picked from the accumulators, so that it is the very value in the sum.
+// A third launch adds the tokens' losses up (in fp64, in a fixed order).  Only lse (fp32 per token) is kept.
+//
+// Gradient, in pieces of the vocabulary: the logits of a piece again, G of the piece as bf16 (c_n is 0 or 1 where the loss
+// is a mean or sum, so that G needs no scale: 1 / count goes on at the end), then its two products (lm_mm.hip): dW's
+// rows of the piece are final, dx gathers over the pieces in fp32.
+//
+// Bound by the products: 2 M V d operations forward, three times that in the gradient (one third for the logits again, which
+// is what not keeping them costs), with d = 384 a short sum: 12 chunks of 32 per 128 x 256 tile, then 128 exponentials a
+// lane.  The chunks of successive tiles run through one pipeline, so that a tile's first loads are on their way during its
+// predecessor's exponentials.
+#include "lm_mm.h"
+
+#include <algorithm>
+
+namespace smlm {
+namespace {
+
+constexpr int kLsCols = 128;                              // vocabulary columns per tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kLsFinishRows = 16;                         // tokens per workgroup of the joining kernel
+constexpr int64_t kLsPieceBytes = 512LL << 20;            // most bytes of one piece's G
+constexpr int kNoTarget = -0x40000000;
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct LossArgs {
+  const uint16_t *x, *w;
+  int64_t ldx, ldw, M, d, v0, v1, V;                      // vocabulary columns [v0, v1) of V
+  const int64_t *targets;
+  int64_t ignore;
+  int nsplit, tiles;                                      // ranges of the vocabulary, and its 128-column tiles
+  float2 *parts;                                          // forward: (maximum, sum) [M][2 nsplit]
+  float *picked;                                          // forward: the target's logit [M]
+  const float *lse, *coef, *grad, *count;                 // gradient: coef per token, or null; grad and count: see below
+  float *scale;                                           // gradient: *grad / *count (count null: *grad), written here
+  uint16_t *g;                                            // gradient: G of the piece [M][ldg]
+  int64_t ldg;
+};
+
+template <int NJ, bool GRAD>
+__global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
+  constexpr int NI = 4;
+  typedef MmTile<kLsCols, true, 16> FT;
+  typedef MmTile<32 * NJ, true, 0> TT;
+  typedef MmLoop<FT, TT, NI, NJ> Loop;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int64_t nt = (a.M + TT::kRows - 1) / TT::kRows;
+  if (GRAD && blockIdx.x == 0 && threadIdx.x == 0 && a.grad)   // for the products that follow
+    *a.scale = a.count ? (*a.count > 0.f ? *a.grad / *a.count : 0.f) : *a.grad;
+  const int64_t unit = mm_tile_of(blockIdx.x, nt * a.nsplit);
+  if (unit < 0) return;  // workgroup-uniform
+  // the token tiles of one range are neighbours: an XCD reads its ranges of W from memory once
+  const int64_t t0 = unit % nt * TT::kRows;
+  const int split = (int)(unit / nt);
+  const int first = (int)((int64_t)a.tiles * split / a.nsplit), last = (int)((int64_t)a.tiles * (split + 1) / a.nsplit);
+  const int wave = threadIdx.x / kWave, wf = (wave & 1) * 16 * NI, wt = (wave >> 1) * 16 * NJ;
+  const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
+
+  int target[NJ];                     // column in [v0, ..), kNoTarget: not in this piece or none
+  float m[NJ], l[NJ], c[NJ];          // forward: running maximum and sum; gradient: m = lse, c = the coefficient
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int64_t t = t0 + wt + 16 * j + r;
+    const int64_t y = t < a.M ? a.targets[t] : a.ignore;
+    const bool valid = y != a.ignore && y >= a.v0 && y < a.v1;
+    target[j] = valid ? (int)(y - a.v0) : kNoTarget;
+    m[j] = -__builtin_inff();
+    l[j] = c[j] = 0.f;
+    if (GRAD && t < a.M) {
+      m[j] = a.lse[t];
+      // an index outside the vocabulary makes its token's gradient NaN, as its loss
+      c[j] = y == a.ignore ? 0.f : y < 0 || y >= a.V ? __builtin_nanf("") : a.coef ? a.coef[t] : 1.f;
+    }
+  }
+
+  Loop L;
+  L.init(smem, a.ldw, a.ldx, wf, wt);
+  const int nch = (int)((a.d + kMmK - 1) / kMmK);
+  // the loads run two chunks ahead of the products, over the ends of tiles
+  int ahead_tile = first, ahead_ch = 0;
+  uint32_t ahead = 0;
+  auto issue = [&]() {
+    const int64_t f0 = a.v0 + (int64_t)ahead_tile * kLsCols, k0 = (int64_t)ahead_ch * kMmK;
+    L.template issue_one<FT>(a.w, a.ldw, a.V, a.d, k0, [&](int u) { return f0 + 64 * u; }, L.fo, L.lds + ahead);
+    L.template issue_one<TT>(a.x, a.ldx, a.M, a.d, k0, [&](int u) { return t0 + 64 * u; }, L.to, L.lds + ahead + FT::kBytes);
+    ahead = ahead == 2 * Loop::kStage ? 0 : ahead + Loop::kStage;
+    if (++ahead_ch == nch) {
+      ahead_ch = 0;
+      ++ahead_tile;
+    }
+  };
+  floatx4 acc[NI][NJ];
+  int left = (last - first) * nch;    // chunks not yet multiplied
+  if (left > 0) issue();
+  if (left > 1) issue();
+  uint32_t now = 0;
+  for (int tile = first; tile < last; ++tile) {
+    mm_zero(acc);
+    for (int ch = 0; ch < nch; ++ch, --left) {
+      if (left > 1) mm_wait_barrier<Loop::kLoads>();
+      else mm_wait_barrier<0>();
+      if (left > 2) issue();
+      L.compute(now, acc);
+      now = now == 2 * Loop::kStage ? 0 : now + Loop::kStage;
+    }
+
+    // lane (r, g): columns c0 .. c0 + 15 of token r of each 16
+    const int c0 = tile * kLsCols + wf + 16 * g;
+    const int64_t end = (GRAD ? a.v1 : a.V) - a.v0;
+    if ((int64_t)(tile + 1) * kLsCols > end) {          // columns past the end count for nothing
+      const int valid = (int)(end - c0);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = 4 * i + e < valid ? acc[i][j][e] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const unsigned rel = (unsigned)(target[j] - c0);
+      if constexpr (!GRAD) {
+        if (__any(rel < 16u)) {                         // about one 16-token group in 50 at 50,304 columns
+          float v = 0.f;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
+          if (rel < 16u) a.picked[t0 + wt + 16 * j + r] = v;
+        }
+        float top = m[j];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[q / 4][j][q % 4]);
+        const float ref = top == -__builtin_inff() ? 0.f : top;   // nothing yet: every exponential is 0
+        float sum = l[j] * exp2_hw((m[j] - ref) * kLog2e);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum += exp2_hw((acc[q / 4][j][q % 4] - ref) * kLog2e);
+        m[j] = top;
+        l[j] = sum;
+      } else {
+        const int64_t t = t0 + wt + 16 * j + r;
+        float p[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) p[q] = exp2_hw((acc[q / 4][j][q % 4] - m[j]) * kLog2e);
+        if (__any(rel < 16u)) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) p[q] = rel == (unsigned)q ? p[q] - 1.f : p[q];
+        }
+        uint32_t o[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o[q] = c[j] == 0.f ? 0u : pack_bf16x2(p[2 * q] * c[j], p[2 * q + 1] * c[j]);
+        if (t < a.M) {
+          uint4 *out = (uint4 *)(a.g + t * a.ldg + c0);
+          out[0] = uint4{o[0], o[1], o[2], o[3]};
+          out[1] = uint4{o[4], o[5], o[6], o[7]};
+        }
+      }
+    }
+  }
+
+  if constexpr (!GRAD) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int o = 16; o <= 32; o *= 2) {
+        const float m2 = __shfl_xor(m[j], o, kWave), l2 = __shfl_xor(l[j], o, kWave);
+        const float top = fmaxf(m[j], m2), ref = top == -__builtin_inff() ? 0.f : top;
+        l[j] = l[j] * exp2_hw((m[j] - ref) * kLog2e) + l2 * exp2_hw((m2 - ref) * kLog2e);
+        m[j] = top;
+      }
+      const int64_t t = t0 + wt + 16 * j + r;
+      if (g == 0 && t < a.M) a.parts[t * 2 * a.nsplit + 2 * split + (wave & 1)] = make_float2(m[j], l[j]);
+    }
+  }
+}
+
+// Joins the ranges of kLsFinishRows tokens: lse, and the losses (each) or their sum and number (sums, counts).
+__global__ void __launch_bounds__(256)
+    loss_join_kernel(const float2 *__restrict__ parts, int nparts, const float *__restrict__ picked,
+                     const int64_t *__restrict__ targets, int64_t ignore, int64_t M, int64_t V, float *__restrict__ lse,
+                     float *__restrict__ each, double *__restrict__ sums) {
+  __shared__ double sum[4];
+  __shared__ int num[4];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  double total = 0.0;
+  int count = 0;
+  for (int q = 0; q < kLsFinishRows / 4; ++q) {
+    const int64_t t = (int64_t)blockIdx.x * kLsFinishRows + wave * (kLsFinishRows / 4) + q;
+    if (t >= M) break;
+    float m = -__builtin_inff(), l = 0.f;
+    for (int p = lane; p < nparts; p += kWave) {
+      const float2 v = parts[t * nparts + p];
+      const float top = fmaxf(m, v.x), ref = top == -__builtin_inff() ? 0.f : top;
+      l = l * exp2_hw((m - ref) * kLog2e) + v.y * exp2_hw((v.x - ref) * kLog2e);
+      m = top;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor(m, o, kWave), l2 = __shfl_xor(l, o, kWave);
+      const float top = fmaxf(m, m2), ref = top == -__builtin_inff() ? 0.f : top;
+      l = l * exp2_hw((m - ref) * kLog2e) + l2 * exp2_hw((m2 - ref) * kLog2e);
+      m = top;
+    }
+    const float z = m + logf(l);
+    const int64_t y = targets[t];
+    const float loss = y == ignore ? 0.f : y < 0 || y >= V ? __builtin_nanf("") : z - picked[t];
+    if (lane == 0) {
+      lse[t] = z;
+      if (each) each[t] = loss;
+    }
+    total += loss;
+    count += y != ignore;
+  }
+  if (!sums) return;  // workgroup-uniform
+  if (lane == 0) {
+    sum[wave] = total;
+    num[wave] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sums[2 * (int64_t)blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
+    sums[2 * (int64_t)blockIdx.x + 1] = num[0] + num[1] + num[2] + num[3];
+  }
+}
+
+// out[0] = the loss, out[1] = the number of tokens that count.
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict__ sums, int64_t n, int mean, float *out) {
+  __shared__ double s[2][16];
+  double v[2] = {0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    v[0] += sums[2 * i];
+    v[1] += sums[2 * i + 1];
+  }
+  for (int o = 32; o > 0; o >>= 1)
+    for (int q = 0; q < 2; ++q) v[q] += __shfl_xor(v[q], o, kWave);
+  if (threadIdx.x % kWave == 0)
+    for (int q = 0; q < 2; ++q) s[q][threadIdx.x / kWave] = v[q];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double a = 0.0, b = 0.0;
+    for (int i = 0; i < 16; ++i) {
+      a += s[0][i];
+      b += s[1][i];
+    }
+    out[0] = (float)(mean ? a / b : a);  // no token counts: NaN, as F.cross_entropy
+    out[1] = (float)b;
+  }
+}
+
+template <int NJ, bool GRAD>
+int launch_loss(LossArgs a, hipStream_t stream, const char *what) {
+  constexpr int kLds = kMmStages * (kLsCols + 32 * NJ) * kMmK * 2;
+  const hipError_t e = hipFuncSetAttribute((const void *)loss_kernel<NJ, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           kLds);
+  if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
+  const int64_t n = ceil_div(a.M, 32 * NJ) * a.nsplit;
+  if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
+  hipLaunchKernelGGL((loss_kernel<NJ, GRAD>), dim3((unsigned)mm_grid(n)), dim3(kMmThreads), kLds, stream, a);
+  return launch_status(what);
+}
+
+// Tokens of a tile: 16 NJ per wavefront.
+int tile_nj(int64_t M) { return M > 128 ? 8 : M > 64 ? 4 : 2; }
+
+template <bool GRAD>
+int dispatch_loss(const LossArgs &a, hipStream_t stream, const char *what) {
+  switch (tile_nj(a.M)) {
+    case 8: return launch_loss<8, GRAD>(a, stream, what);
+    case 4: return launch_loss<4, GRAD>(a, stream, what);
+    default: return launch_loss<2, GRAD>(a, stream, what);
+  }
+}
+
+// Ranges of `tiles` vocabulary tiles: two workgroups for each CU, all of them at once on the card.
+int range_count(int64_t M, int64_t tiles) {
+  const int64_t nt = ceil_div(M, 32 * tile_nj(M));
+  return (int)std::min<int64_t>(tiles, std::max<int64_t>(1, 512 / nt));
+}
+
+struct GradPlan {
+  int64_t cols, pieces, splits, g_bytes, part_bytes;
+};
+GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
+  GradPlan p;
+  const int64_t most = std::max<int64_t>(kLsPieceBytes / (2 * M) / kLsCols, 1) * kLsCols;
+  p.pieces = ceil_div(V, most);
+  p.cols = ceil_div(ceil_div(V, p.pieces), kLsCols) * kLsCols;
+  p.pieces = ceil_div(V, p.cols);
+  p.splits = mm_splits(M, d, p.cols, 512);
+  p.g_bytes = M * p.cols * 2;
+  p.part_bytes = p.pieces * p.splits > 1 ? p.splits * M * d * 4 : 0;
+  return p;
+}
+
+int check_loss(const char *what, const void *x, int64_t x_stride, const void *w, int64_t w_stride, const void *targets,
+               int64_t M, int64_t V, int64_t d) {
+  if (!x || !w || !targets) return fail(SMLM_EINVAL, "%s: null x, weight or targets pointer", what);
+  if (M < 0 || V < 1 || d < 1)
+    return fail(SMLM_EINVAL, "%s: bad shape M=%lld V=%lld d=%lld", what, (long long)M, (long long)V, (long long)d);
+  if (d % 8) return fail(SMLM_EUNSUPPORTED, "%s: d=%lld must be a multiple of 8", what, (long long)d);
+  if (V > (1 << 30) || d > (1 << 20) || M > (1LL << 36) / d)
+    return fail(SMLM_EUNSUPPORTED, "%s: M=%lld V=%lld d=%lld too large", what, (long long)M, (long long)V, (long long)d);
+  // the lanes' 32-bit byte offsets span 64 rows
+  if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > (1 << 23) || w_stride > (1 << 23) ||
+      ((uintptr_t)x | (uintptr_t)w) % 16 || (uintptr_t)targets % 8)
+    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^23 elements (x %lld, "
+                "weight %lld)", what, (long long)x_stride, (long long)w_stride);
+  return SMLM_OK;
+}
+
+}  // namespace
+}  // namespace smlm
+
+extern "C" int64_t smlm_linear_ce_workspace(int64_t M, int64_t V, int64_t d, int grad) {
+  using namespace smlm;
+  if (M < 1 || V < 1 || d < 1) return 0;
+  if (grad) {
+    const GradPlan p = grad_plan(M, V, d);
+    return 256 + p.g_bytes + p.part_bytes;
+  }
+  // (maximum, sum) of every range, the picked logits, and the partial sums of the losses
+  return M * 2 * range_count(M, ceil_div(V, kLsCols)) * 8 + ceil_div(M, 4) * 16 + ceil_div(M, kLsFinishRows) * 16;
+}
+
+extern "C" int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w_row_stride,
+                              const int64_t *targets, int64_t ignore_index, int reduction, int64_t M, int64_t V, int64_t d,
+                              float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace smlm;
+  const char *what = "smlm_linear_ce";
+  if (const int rc = check_loss(what, x, x_row_stride, w, w_row_stride, targets, M, V, d)) return rc;
+  if (!loss || !lse) return fail(SMLM_EINVAL, "%s: null loss or lse pointer", what);
+  if (reduction < SMLM_REDUCE_NONE || reduction > SMLM_REDUCE_SUM)
+    return fail(SMLM_EINVAL, "%s: unknown reduction %d", what, reduction);
+  if (M == 0) return reduction == SMLM_REDUCE_NONE ? SMLM_OK : fail(SMLM_EINVAL, "%s: nothing to reduce", what);
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < smlm_linear_ce_workspace(M, V, d, 0))
+    return fail(SMLM_EINVAL, "%s: the workspace needs %lld bytes, 16-byte aligned", what,
+                (long long)smlm_linear_ce_workspace(M, V, d, 0));
+  hipStream_t s = (hipStream_t)stream;
+  LossArgs a{};
+  a.x = (const uint16_t *)x;
+  a.w = (const uint16_t *)w;
+  a.ldx = x_row_stride;
+  a.ldw = w_row_stride;
+  a.M = M;
+  a.d = d;
+  a.v0 = 0;
+  a.v1 = a.V = V;
+  a.targets = targets;
+  a.ignore = ignore_index;
+  a.tiles = (int)ceil_div(V, kLsCols);
+  a.nsplit = range_count(M, a.tiles);
+  char *ws = (char *)workspace;
+  a.parts = (float2 *)ws;
+  ws += M * 2 * a.nsplit * 8;
+  a.picked = (float *)ws;
+  double *sums = reduction == SMLM_REDUCE_NONE ? nullptr : (double *)(ws + ceil_div(M, 4) * 16);
+  if (const int rc = dispatch_loss<false>(a, s, what)) return rc;
+  const int64_t blocks = ceil_div(M, kLsFinishRows);
+  if (blocks > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: M=%lld too large", what, (long long)M);
+  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a.parts, 2 * a.nsplit, a.picked, targets,
+                     ignore_index, M, V, lse, reduction == SMLM_REDUCE_NONE ? loss : nullptr, sums);
+  if (const int rc = launch_status(what)) return rc;
+  if (!sums) return SMLM_OK;
+  hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, sums, blocks, reduction == SMLM_REDUCE_MEAN ? 1 : 0, loss);
+  return launch_status(what);
+}
+
+extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, int per_token, const void *x,
+                                       int64_t x_row_stride, const void *w, int64_t w_row_stride, const int64_t *targets,
+                                       int64_t ignore_index, const float *lse, int64_t M, int64_t V, int64_t d, void *dx,
+                                       void *dw, void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace smlm;
+  const char *what = "smlm_linear_ce_backward";
+  if (const int rc = check_loss(what, x, x_row_stride, w, w_row_stride, targets, M, V, d)) return rc;
+  if (!grad || !lse || (!dx && !dw)) return fail(SMLM_EINVAL, "%s: null grad, lse or gradient pointers", what);
+  if (((uintptr_t)dx | (uintptr_t)dw) % 16) return fail(SMLM_EINVAL, "%s: dx and dw must be 16-byte aligned", what);
+  if (M < 1) return fail(SMLM_EINVAL, "%s: no tokens", what);
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < smlm_linear_ce_workspace(M, V, d, 1))
+    return fail(SMLM_EINVAL, "%s: the workspace needs %lld bytes, 16-byte aligned", what,
+                (long long)smlm_linear_ce_workspace(M, V, d, 1));
+  hipStream_t s = (hipStream_t)stream;
+  const GradPlan p = grad_plan(M, V, d);
+  LossArgs a{};
+  a.x = (const uint16_t *)x;
+  a.w = (const uint16_t *)w;
+  a.ldx = x_row_stride;
+  a.ldw = w_row_stride;
+  a.M = M;
+  a.d = d;
+  a.V = V;
+  a.targets = targets;
+  a.ignore = ignore_index;
+  a.lse = lse;
+  a.coef = per_token ? grad : nullptr;
+  a.grad = per_token ? nullptr : grad;
+  a.count = count;
+  a.scale = (float *)workspace;
+  a.g = (uint16_t *)((char *)workspace + 256);
+  a.ldg = p.cols;
+  float *parts = (float *)((char *)workspace + 256 + p.g_bytes);
+  const float *scale = per_token ? nullptr : a.scale;
+  for (int64_t piece = 0; piece < p.pieces; ++piece) {
+    a.v0 = piece * p.cols;
+    a.v1 = std::min(V, a.v0 + p.cols);
+    const int64_t n = a.v1 - a.v0;
+    a.tiles = (int)ceil_div(n, kLsCols);
+    a.nsplit = range_count(M, a.tiles);
+    if (const int rc = dispatch_loss<true>(a, s, what)) return rc;
+    if (dx) {   // the sum over the piece's columns
+      MmArgs m{};
+      m.feat = a.w + a.v0 * a.ldw;
+      m.ldf = a.ldw;
+      m.Kf = n;
+      m.tok = a.g;
+      m.ldt = a.ldg;
+      m.F = d;
+      m.T = M;
+      m.K = (n + 7) / 8 * 8;
+      m.f32 = p.part_bytes > 0;
+      m.out = m.f32 ? (void *)parts : dx;
+      m.ldo = d;
+      m.nsplit = p.splits;
+      m.k_per = mm_k_per(m.K, p.splits);
+      m.scale = scale;
+      m.accumulate = piece > 0;
+      if (const int rc = mm_launch(m, false, true, s, what)) return rc;
+    }
+    if (dw) {   // the sum over the tokens
+      MmArgs m{};
+      m.feat = a.x;
+      m.ldf = a.ldx;
+      m.Kf = m.K = M;
+      m.tok = a.g;
+      m.ldt = a.ldg;
+      m.F = d;
+      m.T = n;
+      m.out = (uint16_t *)dw + a.v0 * d;
+      m.ldo = d;
+      m.nsplit = 1;
+      m.k_per = mm_k_per(M, 1);
+      m.scale = scale;
+      if (const int rc = mm_launch(m, false, false, s, what)) return rc;
+    }
+  }
+  if (dx && p.part_bytes > 0) return mm_reduce_launch(parts, p.splits, M, d, scale, dx, d, s, what);
+  return SMLM_OK;
+}

@@ -1,0 +1,218 @@
+// The K loop of the training step's products on the matrix cores (v_mfma_f32_16x16x32_bf16, fp32 sums): a tile of
+// TT rows ("tokens") x FT columns ("features") from two bf16 operands, each of which may have the summed dimension k
+// contiguous (rows of k: a linear layer's input and weight) or strided (rows of tokens or features, k the slow dimension:
+// the operands of a weight's gradient).
+//
+// Workgroup = 4 wavefronts, WF x WT of them over the tile, 16 NI features x 16 NJ tokens each.  At the matrix cores' rate a
+// wavefront's tile of 64 features x 128 tokens reads 96 of the 128 bytes per clock that the LDS has, one of 64 x 64 all
+// of them: hence 128 x 256 tiles where there are enough of them.
+// k streams through three LDS stages of 32, two chunks ahead, loaded straight from memory into LDS (buffer_load ... lds,
+// no registers in between); one barrier per chunk both publishes a chunk and frees the stage that is loaded next.  A
+// stage takes 24 KB for 128 x 256, so that two workgroups fit a CU: one's epilogue runs under the other's products.
+//
+// LDS layouts (16-byte pieces; banks repeat every 256 bytes):
+//   k contiguous: 64-byte rows, piece c of row R at c ^ swz(R), so that the 16 rows of a fragment read fall on distinct
+//     banks; read with ds_read_b128.  Feature rows are read permuted (lane r of tile i takes row 4 NI (r / 4) + 4 i +
+//     r % 4), which leaves each lane 4 NI consecutive features of a token in its accumulators: 32-byte stores.
+//   k strided: rows of 32 k, piece c of row k at c ^ v(k), read with ds_read_b64_tr_b16, which gives lane r four k of
+//     column r.  Lane group g takes k = 8 g .. 8 g + 7 in both layouts.
+// Out of range rows and k read as zeros (the buffer's record count; the k beyond the end of contiguous rows by an offset
+// out of range), so tails need no other care than not storing what lies outside.
+#pragma once
+
+#include "pkm_common.h"
+
+namespace smlm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+constexpr int kMmThreads = 256, kMmK = 32, kMmStages = 3, kMmXcds = 8;
+
+// 16 bytes per lane from a buffer straight into LDS at lds + 16 * lane (wave-uniform lds).  Inline assembly, so that the
+// compiler adds no wait for it before every LDS read; the kernels wait themselves (mm_wait).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void mm_load_lds(intx4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds)
+               : "m0");
+}
+#pragma clang diagnostic pop
+
+// At most N vector memory operations on their way and every LDS read done; then the barrier.  Loads complete in order:
+// with N = the loads issued after a chunk's, that chunk has landed.
+template <int N>
+__device__ __forceinline__ void mm_wait_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Descriptor of `bytes` bytes from p (clipped to 32 bits; no offset used reaches the clip).
+__device__ __forceinline__ intx4 mm_rsrc(const uint16_t *p, int64_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t n = bytes <= 0 ? 0u : bytes > 0xFFFFFFF0LL ? 0xFFFFFFF0u : (uint32_t)bytes;
+  return intx4{(int)(uint32_t)a, (int)(uint32_t)((a >> 32) & 0xFFFF), (int)n, 0x00020000};
+}
+
+constexpr uint32_t kMmOutside = 0xFFFFFFF0u;  // an offset that no record count reaches
+
+// One operand's LDS tile of ROWS rows (tokens or features) x 32 k.  PERM: features per lane group (4 NI) of a permuted
+// fragment, 0 for a plain one.
+template <int ROWS, bool KC, int PERM>
+struct MmTile {
+  static constexpr bool kContiguous = KC;
+  static constexpr int kRows = ROWS, kBytes = ROWS * kMmK * 2;
+  static constexpr int kLoads = kBytes / 4096;                       // per thread and chunk
+  static constexpr int kRowBytes = KC ? kMmK * 2 : ROWS * 2;
+  static constexpr int kRowsPerLoad = 4096 / kRowBytes;              // LDS rows that one load of the workgroup fills
+  static_assert(kBytes % 4096 == 0, "a whole number of loads");
+
+  static __device__ __forceinline__ int swz(int row) {               // KC
+    return (PERM ? row / PERM : row / 4) & 3;
+  }
+  static __device__ __forceinline__ int vsw(int k) {                 // k strided
+    return ROWS >= 128 ? 2 * ((k & 3) | ((k >> 3 & 1) << 2)) : 2 * ((k >> 1 & 1) | ((k >> 3 & 1) << 1));
+  }
+
+  // Loads whose offsets from their own bases differ (k strided, 256 rows: the swizzle of an odd load is another).
+  static constexpr int kOffsets = !KC && ROWS == 256 ? 2 : 1;
+  // This thread's byte offset of load u (u < kOffsets stands for all u of its parity) from the load's base.
+  static __device__ __forceinline__ uint32_t offset(int u, int tid, int64_t ld) {
+    if constexpr (KC) {
+      const int row = tid / 4;                                       // 64 rows a load: one swizzle for all of them
+      return (uint32_t)(row * ld * 2 + first_k(tid) * 2);
+    } else {
+      const int per = kRowBytes / 16, k = u * kRowsPerLoad + tid / per;
+      return (uint32_t)((tid / per) * ld * 2 + (((tid % per) ^ vsw(k)) * 16));
+    }
+  }
+  static __device__ __forceinline__ int first_k(int tid) { return 8 * ((tid % 4) ^ swz(tid / 4)); }   // KC
+  // Descriptor of load u: rows from row0 (KC: the load's own first row), k from k0, of an operand of `rows` rows and K.
+  static __device__ __forceinline__ intx4 rsrc(const uint16_t *p, int64_t ld, int64_t rows, int64_t K, int64_t row0,
+                                               int64_t k0, int u) {
+    if constexpr (KC) {
+      return mm_rsrc(p + row0 * ld + k0, row0 < rows ? ((rows - 1 - row0) * ld + (K - k0)) * 2 : 0);
+    } else {
+      const int64_t k = k0 + u * kRowsPerLoad;
+      return mm_rsrc(p + k * ld + row0, k < K ? ((K - 1 - k) * ld + (rows - row0)) * 2 : 0);
+    }
+  }
+
+  // LDS address (from the tile's base) that lane (r, g) reads the wavefront's row group i from, its rows starting at w0.
+  static __device__ __forceinline__ uint32_t frag_at(int w0, int i, int r, int g) {
+    if constexpr (KC) {                       // w0 a multiple of 4 * PERM or 16: the swizzle is that of i = 0
+      const int R = PERM ? w0 + PERM * (r / 4) + r % 4 : w0 + r;
+      return R * kRowBytes + ((g ^ swz(R)) * 16) + i * (PERM ? 4 : 16) * kRowBytes;
+    } else {
+      const int k = 8 * g + r / 4;
+      const int col = PERM ? w0 + PERM * (r % 4) + 4 * i : w0 + 16 * i + 4 * (r % 4);
+      return k * kRowBytes + (((col / 8) ^ vsw(k)) * 16) + (col % 8) * 2;
+    }
+  }
+  static __device__ __forceinline__ bf16x8 frag(uint32_t at) {
+    if constexpr (KC) {
+      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)at;
+    } else {
+      typedef __attribute__((address_space(3))) bf16x4 *p4;
+      const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)at);
+      const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(at + 4 * kRowBytes));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// The loop's state of one thread for an F tile of features and a T tile of tokens: a stage holds F, then T.
+template <class F, class T, int NI, int NJ>
+struct MmLoop {
+  static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads;
+  uint32_t fo[F::kOffsets], to[T::kOffsets], fa[NI], ta[NJ], lds;
+
+  // wf, wt: first feature and token row of this wavefront in the tile
+  __device__ __forceinline__ void init(const unsigned char *smem, int64_t ldf, int64_t ldt, int wf, int wt) {
+    const int tid = threadIdx.x, lane = tid % kWave, r = lane & 15, g = lane >> 4;
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_byte *)smem;
+#pragma unroll
+    for (int u = 0; u < F::kOffsets; ++u) fo[u] = F::offset(u, tid, ldf);
+#pragma unroll
+    for (int u = 0; u < T::kOffsets; ++u) to[u] = T::offset(u, tid, ldt);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) fa[i] = base + F::frag_at(wf, i, r, g);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) ta[j] = base + F::kBytes + T::frag_at(wt, j, r, g);
+    lds = base + __builtin_amdgcn_readfirstlane(tid / kWave) * 1024;
+  }
+
+  // Loads of one operand's chunk of k from k0 on into `stage` (a byte offset).  row0: the first row of load u.
+  template <class O, class ROW0>
+  __device__ __forceinline__ void issue_one(const uint16_t *p, int64_t ld, int64_t rows, int64_t K, int64_t k0, ROW0 row0,
+                                            const uint32_t *off, uint32_t at) {
+    uint32_t o[O::kOffsets];
+#pragma unroll
+    for (int u = 0; u < O::kOffsets; ++u) o[u] = off[u];
+    if constexpr (O::kContiguous) {
+      if (k0 + kMmK > K) o[0] = k0 + O::first_k(threadIdx.x) < K ? o[0] : kMmOutside;
+    }
+#pragma unroll
+    for (int u = 0; u < O::kLoads; ++u)
+      mm_load_lds(O::rsrc(p, ld, rows, K, row0(u), k0, u), o[u % O::kOffsets], at + u * 4096);
+  }
+
+  __device__ __forceinline__ void compute(uint32_t stage, floatx4 (&acc)[NI][NJ]) const {
+    bf16x8 a[NI], b[NJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) a[i] = F::frag(fa[i] + stage);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) b[j] = T::frag(ta[j] + stage);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+  }
+};
+
+template <int NI, int NJ>
+__device__ __forceinline__ void mm_zero(floatx4 (&acc)[NI][NJ]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+}
+
+// Tile t of `n`, so that each XCD (workgroup id % 8) walks neighbours; -1 for the padding of the grid (mm_grid).
+__device__ __forceinline__ int64_t mm_tile_of(int64_t id, int64_t n) {
+  const int64_t per = (n + kMmXcds - 1) / kMmXcds, t = id % kMmXcds * per + id / kMmXcds;
+  return id / kMmXcds < per && t < n ? t : -1;
+}
+inline int64_t mm_grid(int64_t n) { return (n + kMmXcds - 1) / kMmXcds * kMmXcds; }
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- plain products (lm_mm.hip) ----------------------------------------------------------------------------------------
+// out[t, f] = sum_k tok[t, k] feat[f, k]; an operand with *_kc = false is stored [k][row].  Rows and strides in elements,
+// rows of 16-byte pieces.  nsplit > 1 or f32: fp32 parts [nsplit][T][F] (with accumulate added to what is there), split s
+// summing k_per (a multiple of 32) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
+// F a multiple of 8; K one too where an operand has k contiguous, that operand's k from the sum's end up to it zeros; a k
+// strided tok has rows of at least T rounded up to 8.  Kf: the k that a k strided feat has (the last of K may lack).
+struct MmArgs {
+  const uint16_t *feat, *tok;
+  int64_t ldf, ldt, F, T, K, Kf;
+  void *out;
+  int64_t ldo;
+  int64_t nsplit, k_per;
+  const float *scale;
+  int f32, accumulate;
+};
+int mm_launch(const MmArgs &a, bool feat_kc, bool tok_kc, hipStream_t stream, const char *what);
+// Splits of k for T x F outputs over K: as many as fill the card, each of at least min_k.
+int64_t mm_splits(int64_t T, int64_t F, int64_t K, int64_t min_k);
+int64_t mm_k_per(int64_t K, int64_t nsplit);
+// out bf16 [T][ldo] = scale * sum of `parts` fp32 [nsplit][T][F] in order
+int mm_reduce_launch(const float *parts, int64_t nsplit, int64_t T, int64_t F, const float *scale, void *out, int64_t ldo,
+                     hipStream_t stream, const char *what);
+
+}  // namespace smlm

@@ -78,9 +78,20 @@ EXPORTS = {
     "smlm_engram_mix": (_i, [_p] * 7 + [_i, _p, _p, _i64, _i64, _i, _i, _i, _f, _p, _p]),
     "smlm_engram_mix_parts": (_i64, [_i64, _i64, _i, _i]),
     "smlm_engram_mix_backward": (_i, [_p] * 8 + [_i64, _i64, _i, _i, _i, _f] + [_p] * 9),
+    "smlm_linear_ce_workspace": (_i64, [_i64, _i64, _i64, _i]),
+    "smlm_linear_ce": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
+    "smlm_linear_ce_backward": (_i, [_p, _p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,
+                                     _p]),
+    "smlm_gated_ffn": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p]),
+    "smlm_gated_ffn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "smlm_gated_ffn_backward": (_i, [_p, _i64] * 4 + [_i64] * 4 + [_p] * 4 + [_i64, _p]),
+    "smlm_rmsnorm_train": (_i, [_p, _i, _p, _i, _p, _i, _f, _i64, _i64, _p, _p, _i, _p, _p]),
+    "smlm_rmsnorm_parts": (_i64, [_i64, _i64]),
+    "smlm_rmsnorm_train_backward": (_i, [_p, _p, _i, _p, _i, _p, _i, _p, _i64, _i64, _p, _p, _i, _p, _p, _p]),
     "smlm_row_gather": (_i, [_p, _i64, _p, _i, _i64, _i, _p, _p]),
 }
 ADAM_F32, ADAM_BF16, ADAM_INT8 = 0, 1, 2
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2      # smlm_reduction
 
 _lib = None
 

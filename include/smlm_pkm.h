@@ -542,7 +542,7 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
  * smlm/model.py:286-293): per token logsumexp(s_n) - s_n[targets[n]], 0 where targets[n] == ignore_index, NaN where it
  * is any other index outside the vocabulary; their mean over the tokens that are not ignored (NaN if none), or sum.
  *   x (M, d) and w (V, d) bf16, rows of x_row_stride / w_row_stride elements (multiples of 8, 16-byte aligned, at most
- *   2^23), d a multiple of 8; targets (M,) int64
+ *   2^22), d a multiple of 8; targets (M,) int64
  *   loss  SMLM_REDUCE_NONE: (M,) fp32; otherwise fp32[2]: the loss, and the number of tokens that are not ignored
  *   lse   (M,) fp32: the tokens' logsumexp, which the gradient needs
  * workspace: smlm_linear_ce_workspace(M, V, d, 0) bytes, 16-byte aligned, free again when the call's work is done.

@@ -40,11 +40,12 @@ __global__ void __launch_bounds__(kMmThreads, 2) gate_kernel(GateArgs p) {
   typedef MmLoop<ST, TT, 2, NJ> Out;
   constexpr uint32_t kStage = Gate::kStage;               // the larger of the two
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t nf = (p.hidden + kGateFeat - 1) / kGateFeat, nt = (p.M + TT::kRows - 1) / TT::kRows;
-  const int64_t tile = mm_tile_of(blockIdx.x, nf * nt);
+  const unsigned nf = (unsigned)((p.hidden + kGateFeat - 1) / kGateFeat), nt = (unsigned)((p.M + TT::kRows - 1) / TT::kRows);
+  const int tile = mm_tile_of(blockIdx.x, nf * nt);
   if (tile < 0) return;  // workgroup-uniform
-  // the token tiles of a feature tile are spread, the feature tiles of a token tile neighbours: its rows are read once
-  const int64_t f0 = tile % nf * kGateFeat, t0 = tile / nf * TT::kRows;
+  // the feature tiles of a token tile are neighbours: on one XCD its rows are read from memory once
+  const unsigned row = tile / nf;
+  const int64_t f0 = (int64_t)(tile - row * nf) * kGateFeat, t0 = (int64_t)row * TT::kRows;
   const int wave = threadIdx.x / kWave, wf = (wave & 1) * 32, wt = (wave >> 1) * 16 * NJ;
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
 
@@ -54,37 +55,60 @@ __global__ void __launch_bounds__(kMmThreads, 2) gate_kernel(GateArgs p) {
   for (int i = 0; i < 2; ++i) A.fa[2 + i] = A.fa[i] + kGateFeat * FT::kRowBytes;   // b's rows: the same swizzle
   Out B;
   if constexpr (GRAD) B.init(smem, p.ldw2, p.lddy, wf, wt);
-  const int n1 = (int)((p.d + kMmK - 1) / kMmK), n2 = GRAD ? (int)((p.n_out + kMmK - 1) / kMmK) : 0, n = n1 + n2;
+  const int n1 = (int)((p.d + kMmK - 1) / kMmK), n2 = GRAD ? (int)((p.n_out + kMmK - 1) / kMmK) : 0;
+  // rows of a beyond hidden are b's, whose results are not stored; rows of b beyond the weight read as zeros
+  MmSource<FT> as, bs;
+  MmSource<TT> xs, ys;
+  MmSource<ST> ss;
+  as.init(p.w13, p.ldw13, 2 * p.hidden, p.d, f0, 0);
+  bs.init(p.w13, p.ldw13, 2 * p.hidden, p.d, p.hidden + f0 - kGateFeat, 0);   // load 1 adds 64 rows
+  xs.init(p.x, p.ldx, p.M, p.d, t0, 0);
+  if constexpr (GRAD) {
+    ss.init(p.w2, p.ldw2, p.hidden, p.n_out, f0, 0);
+    ys.init(p.dy, p.lddy, p.M, p.n_out, t0, 0);
+  }
   uint32_t ahead = 0;
-  auto issue = [&](int ch) {
-    const uint32_t at = A.lds + ahead;
-    if (ch < n1) {
-      const int64_t k0 = (int64_t)ch * kMmK;
-      // rows of a beyond hidden are b's, whose results are not stored; rows of b beyond the weight read as zeros
-      A.template issue_one<FT>(p.w13, p.ldw13, 2 * p.hidden, p.d, k0,
-                               [&](int u) { return u == 0 ? f0 : p.hidden + f0; }, A.fo, at);
-      A.template issue_one<TT>(p.x, p.ldx, p.M, p.d, k0, [&](int u) { return t0 + 64 * u; }, A.to, at + FT::kBytes);
-    } else if constexpr (GRAD) {
-      const int64_t k0 = (int64_t)(ch - n1) * kMmK;
-      B.template issue_one<ST>(p.w2, p.ldw2, p.hidden, p.n_out, k0, [&](int) { return f0; }, B.fo, at);
-      B.template issue_one<TT>(p.dy, p.lddy, p.M, p.n_out, k0, [&](int u) { return t0 + 64 * u; }, B.to, at + ST::kBytes);
-    }
-    ahead = ahead == 2 * kStage ? 0 : ahead + kStage;
+  auto issue_ab = [&]() {
+    Gate::template load<FT>(as, A.fo, A.lds + ahead, 0, 1);
+    Gate::template load<FT>(bs, A.fo, A.lds + ahead, 1, 2);
+    Gate::template load<TT>(xs, A.to, A.lds + ahead + FT::kBytes);
+    as.next();
+    bs.next();
+    xs.next();
+    ahead = mm_next_stage(ahead, kStage);
   };
-  floatx4 ab[4][NJ], dact[2][NJ];
+  auto issue_out = [&]() {
+    B.issue(ss, ys, ahead);
+    ahead = mm_next_stage(ahead, kStage);
+  };
+  // chunk ch of both sums in a row
+  auto issue = [&](int ch) {
+    if (ch < n1) issue_ab();
+    else if (ch < n1 + n2) issue_out();
+  };
+  floatx4 ab[4][NJ];
   mm_zero(ab);
-  mm_zero(dact);
   issue(0);
-  if (n > 1) issue(1);
+  issue(1);
   uint32_t now = 0;
-  for (int ch = 0; ch < n; ++ch) {
-    if (ch + 1 >= n) mm_wait_barrier<0>();
-    else if (ch + 1 < n1) mm_wait_barrier<Gate::kLoads>();
-    else mm_wait_barrier<Out::kLoads>();
-    if (ch + 2 < n) issue(ch + 2);
-    if (ch < n1) A.compute(now, ab);
-    else if constexpr (GRAD) B.compute(now, dact);
-    now = now == 2 * kStage ? 0 : now + kStage;
+  for (int ch = 0; ch < n1; ++ch) {
+    if (ch + 1 < n1) mm_wait_barrier<Gate::kLoads>();
+    else if (n2 > 0) mm_wait_barrier<Out::kLoads>();
+    else mm_wait_barrier<0>();
+    issue(ch + 2);
+    A.compute(now, ab);
+    now = mm_next_stage(now, kStage);
+  }
+  floatx4 dact[2][NJ];
+  mm_zero(dact);
+  if constexpr (GRAD) {
+    for (int ch = 0; ch < n2; ++ch) {
+      if (ch + 1 < n2) mm_wait_barrier<Out::kLoads>();
+      else mm_wait_barrier<0>();
+      if (ch + 2 < n2) issue_out();
+      B.compute(now, dact);
+      now = mm_next_stage(now, kStage);
+    }
   }
 
   // lane (r, g): features f .. f + 7 of token r of each 16
@@ -142,8 +166,8 @@ int check_ffn(const char *what, const void *x, int64_t ldx, const void *w13, int
     return fail(SMLM_EUNSUPPORTED, "%s: M=%lld d=%lld hidden=%lld n_out=%lld too large", what, (long long)M, (long long)d,
                 (long long)hidden, (long long)n_out);
   if (ldx < d || ldw13 < d || ldw2 < hidden || ldx % 8 || ldw13 % 8 || ldw2 % 8 || std::max(std::max(ldx, ldw13), ldw2) >
-      (1 << 23) || ((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2) % 16)
-    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^23 elements (x %lld, "
+      (1 << 22) || ((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2) % 16)
+    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^22 elements (x %lld, "
                 "w13 %lld, w2 %lld)", what, (long long)ldx, (long long)ldw13, (long long)ldw2);
   return SMLM_OK;
 }
@@ -229,8 +253,8 @@ extern "C" int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, co
   using namespace smlm;
   const char *what = "smlm_gated_ffn_backward";
   if (const int rc = check_ffn(what, x, x_row_stride, w13, w13_row_stride, w2, w2_row_stride, M, d, hidden, n_out)) return rc;
-  if (!dy || dy_row_stride < n_out || dy_row_stride % 8 || dy_row_stride > (1 << 23) || (uintptr_t)dy % 16)
-    return fail(SMLM_EINVAL, "%s: dy must have 16-byte aligned rows with a stride from %lld to 2^23 elements", what,
+  if (!dy || dy_row_stride < n_out || dy_row_stride % 8 || dy_row_stride > (1 << 22) || (uintptr_t)dy % 16)
+    return fail(SMLM_EINVAL, "%s: dy must have 16-byte aligned rows with a stride from %lld to 2^22 elements", what,
                 (long long)n_out);
   if ((!dx && !dw13 && !dw2) || ((uintptr_t)dx | (uintptr_t)dw13 | (uintptr_t)dw2) % 16)
     return fail(SMLM_EINVAL, "%s: dx, dw13 and dw2 must be 16-byte aligned, one of them at least given", what);

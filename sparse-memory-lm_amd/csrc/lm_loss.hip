@@ -52,14 +52,14 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
   typedef MmTile<32 * NJ, true, 0> TT;
   typedef MmLoop<FT, TT, NI, NJ> Loop;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t nt = (a.M + TT::kRows - 1) / TT::kRows;
+  const unsigned nt = (unsigned)((a.M + TT::kRows - 1) / TT::kRows);
   if (GRAD && blockIdx.x == 0 && threadIdx.x == 0 && a.grad)   // for the products that follow
     *a.scale = a.count ? (*a.count > 0.f ? *a.grad / *a.count : 0.f) : *a.grad;
-  const int64_t unit = mm_tile_of(blockIdx.x, nt * a.nsplit);
+  const int unit = mm_tile_of(blockIdx.x, nt * a.nsplit);
   if (unit < 0) return;  // workgroup-uniform
   // the token tiles of one range are neighbours: an XCD reads its ranges of W from memory once
-  const int64_t t0 = unit % nt * TT::kRows;
-  const int split = (int)(unit / nt);
+  const int split = unit / nt;
+  const int64_t t0 = (int64_t)(unit - split * nt) * TT::kRows;
   const int first = (int)((int64_t)a.tiles * split / a.nsplit), last = (int)((int64_t)a.tiles * (split + 1) / a.nsplit);
   const int wave = threadIdx.x / kWave, wf = (wave & 1) * 16 * NI, wt = (wave >> 1) * 16 * NJ;
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
@@ -85,18 +85,23 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
   L.init(smem, a.ldw, a.ldx, wf, wt);
   const int nch = (int)((a.d + kMmK - 1) / kMmK);
   // the loads run two chunks ahead of the products, over the ends of tiles
-  int ahead_tile = first, ahead_ch = 0;
+  int ahead_tile = first;
   uint32_t ahead = 0;
+  MmSource<FT> fs;
+  MmSource<TT> ts;
+  auto tile_starts = [&]() {
+    fs.init(a.w, a.ldw, a.V, a.d, a.v0 + (int64_t)ahead_tile * kLsCols, 0);
+    ts.init(a.x, a.ldx, a.M, a.d, t0, 0);
+  };
   auto issue = [&]() {
-    const int64_t f0 = a.v0 + (int64_t)ahead_tile * kLsCols, k0 = (int64_t)ahead_ch * kMmK;
-    L.template issue_one<FT>(a.w, a.ldw, a.V, a.d, k0, [&](int u) { return f0 + 64 * u; }, L.fo, L.lds + ahead);
-    L.template issue_one<TT>(a.x, a.ldx, a.M, a.d, k0, [&](int u) { return t0 + 64 * u; }, L.to, L.lds + ahead + FT::kBytes);
-    ahead = ahead == 2 * Loop::kStage ? 0 : ahead + Loop::kStage;
-    if (++ahead_ch == nch) {
-      ahead_ch = 0;
+    L.issue(fs, ts, ahead);
+    ahead = mm_next_stage(ahead, Loop::kStage);
+    if (fs.k <= 0) {
       ++ahead_tile;
+      tile_starts();
     }
   };
+  tile_starts();
   floatx4 acc[NI][NJ];
   int left = (last - first) * nch;    // chunks not yet multiplied
   if (left > 0) issue();
@@ -109,7 +114,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
       else mm_wait_barrier<0>();
       if (left > 2) issue();
       L.compute(now, acc);
-      now = now == 2 * Loop::kStage ? 0 : now + Loop::kStage;
+      now = mm_next_stage(now, Loop::kStage);
     }
 
     // lane (r, g): columns c0 .. c0 + 15 of token r of each 16
@@ -305,10 +310,10 @@ int check_loss(const char *what, const void *x, int64_t x_stride, const void *w,
   if (d % 8) return fail(SMLM_EUNSUPPORTED, "%s: d=%lld must be a multiple of 8", what, (long long)d);
   if (V > (1 << 30) || d > (1 << 20) || M > (1LL << 36) / d)
     return fail(SMLM_EUNSUPPORTED, "%s: M=%lld V=%lld d=%lld too large", what, (long long)M, (long long)V, (long long)d);
-  // the lanes' 32-bit byte offsets span 64 rows
-  if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > (1 << 23) || w_stride > (1 << 23) ||
+  // the lanes' 32-bit byte offsets span 256 rows
+  if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > (1 << 22) || w_stride > (1 << 22) ||
       ((uintptr_t)x | (uintptr_t)w) % 16 || (uintptr_t)targets % 8)
-    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^23 elements (x %lld, "
+    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^22 elements (x %lld, "
                 "weight %lld)", what, (long long)x_stride, (long long)w_stride);
   return SMLM_OK;
 }

@@ -52,13 +52,6 @@ __device__ __forceinline__ void mm_wait_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Descriptor of `bytes` bytes from p (clipped to 32 bits; no offset used reaches the clip).
-__device__ __forceinline__ intx4 mm_rsrc(const uint16_t *p, int64_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  const uint32_t n = bytes <= 0 ? 0u : bytes > 0xFFFFFFF0LL ? 0xFFFFFFF0u : (uint32_t)bytes;
-  return intx4{(int)(uint32_t)a, (int)(uint32_t)((a >> 32) & 0xFFFF), (int)n, 0x00020000};
-}
-
 constexpr uint32_t kMmOutside = 0xFFFFFFF0u;  // an offset that no record count reaches
 
 // One operand's LDS tile of ROWS rows (tokens or features) x 32 k.  PERM: features per lane group (4 NI) of a permuted
@@ -73,36 +66,22 @@ struct MmTile {
   static_assert(kBytes % 4096 == 0, "a whole number of loads");
 
   static __device__ __forceinline__ int swz(int row) {               // KC
-    return (PERM ? row / PERM : row / 4) & 3;
+    return -(PERM ? row / PERM : row / 4) & 3;
   }
   static __device__ __forceinline__ int vsw(int k) {                 // k strided
     return ROWS >= 128 ? 2 * ((k & 3) | ((k >> 3 & 1) << 2)) : 2 * ((k >> 1 & 1) | ((k >> 3 & 1) << 1));
   }
 
-  // Loads whose offsets from their own bases differ (k strided, 256 rows: the swizzle of an odd load is another).
-  static constexpr int kOffsets = !KC && ROWS == 256 ? 2 : 1;
-  // This thread's byte offset of load u (u < kOffsets stands for all u of its parity) from the load's base.
+  // This thread's byte offset of load u from the chunk's first byte.
   static __device__ __forceinline__ uint32_t offset(int u, int tid, int64_t ld) {
     if constexpr (KC) {
-      const int row = tid / 4;                                       // 64 rows a load: one swizzle for all of them
-      return (uint32_t)(row * ld * 2 + first_k(tid) * 2);
+      return (uint32_t)((u * kRowsPerLoad + tid / 4) * ld * 2 + first_k(tid) * 2);
     } else {
       const int per = kRowBytes / 16, k = u * kRowsPerLoad + tid / per;
-      return (uint32_t)((tid / per) * ld * 2 + (((tid % per) ^ vsw(k)) * 16));
+      return (uint32_t)(k * ld * 2 + (((tid % per) ^ vsw(k)) * 16));
     }
   }
   static __device__ __forceinline__ int first_k(int tid) { return 8 * ((tid % 4) ^ swz(tid / 4)); }   // KC
-  // Descriptor of load u: rows from row0 (KC: the load's own first row), k from k0, of an operand of `rows` rows and K.
-  static __device__ __forceinline__ intx4 rsrc(const uint16_t *p, int64_t ld, int64_t rows, int64_t K, int64_t row0,
-                                               int64_t k0, int u) {
-    if constexpr (KC) {
-      return mm_rsrc(p + row0 * ld + k0, row0 < rows ? ((rows - 1 - row0) * ld + (K - k0)) * 2 : 0);
-    } else {
-      const int64_t k = k0 + u * kRowsPerLoad;
-      return mm_rsrc(p + k * ld + row0, k < K ? ((K - 1 - k) * ld + (rows - row0)) * 2 : 0);
-    }
-  }
-
   // LDS address (from the tile's base) that lane (r, g) reads the wavefront's row group i from, its rows starting at w0.
   static __device__ __forceinline__ uint32_t frag_at(int w0, int i, int r, int g) {
     if constexpr (KC) {                       // w0 a multiple of 4 * PERM or 16: the swizzle is that of i = 0
@@ -126,20 +105,45 @@ struct MmTile {
   }
 };
 
+// Where an operand's next chunk comes from: wave-uniform, stepped from chunk to chunk.  `left` is exact: the bytes from the
+// chunk's first to the operand's last, which the record count of its loads is clipped to.
+template <class O>
+struct MmSource {
+  const uint16_t *p;
+  int64_t left, step, k;                                 // step in bytes; k: what is left of the sum
+  // rows from row0 (< rows) on and k from k0 (< K) on of an operand of `rows` rows and K
+  __device__ __forceinline__ void init(const uint16_t *base, int64_t ld, int64_t rows, int64_t K, int64_t row0, int64_t k0) {
+    const int64_t major = O::kContiguous ? row0 : k0, minor = O::kContiguous ? k0 : row0;
+    p = base + major * ld + minor;
+    left = (((O::kContiguous ? rows : K) - 1 - major) * ld + (O::kContiguous ? K : rows) - minor) * 2;
+    step = O::kContiguous ? kMmK * 2 : kMmK * 2 * ld;
+    k = K - k0;
+  }
+  __device__ __forceinline__ intx4 rsrc() const {
+    const uint64_t a = (uint64_t)p;
+    return intx4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(left >> 32 ? 0xFFFFFFF0u : (uint32_t)left), 0x00020000};
+  }
+  __device__ __forceinline__ void next() {
+    p += step / 2;
+    left -= step;
+    k -= kMmK;
+  }
+};
+
 // The loop's state of one thread for an F tile of features and a T tile of tokens: a stage holds F, then T.
 template <class F, class T, int NI, int NJ>
 struct MmLoop {
   static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads;
-  uint32_t fo[F::kOffsets], to[T::kOffsets], fa[NI], ta[NJ], lds;
+  uint32_t fo[F::kLoads], to[T::kLoads], fa[NI], ta[NJ], lds;
 
   // wf, wt: first feature and token row of this wavefront in the tile
   __device__ __forceinline__ void init(const unsigned char *smem, int64_t ldf, int64_t ldt, int wf, int wt) {
     const int tid = threadIdx.x, lane = tid % kWave, r = lane & 15, g = lane >> 4;
     const uint32_t base = (uint32_t)(uintptr_t)(lds_byte *)smem;
 #pragma unroll
-    for (int u = 0; u < F::kOffsets; ++u) fo[u] = F::offset(u, tid, ldf);
+    for (int u = 0; u < F::kLoads; ++u) fo[u] = F::offset(u, tid, ldf);
 #pragma unroll
-    for (int u = 0; u < T::kOffsets; ++u) to[u] = T::offset(u, tid, ldt);
+    for (int u = 0; u < T::kLoads; ++u) to[u] = T::offset(u, tid, ldt);
 #pragma unroll
     for (int i = 0; i < NI; ++i) fa[i] = base + F::frag_at(wf, i, r, g);
 #pragma unroll
@@ -147,19 +151,27 @@ struct MmLoop {
     lds = base + __builtin_amdgcn_readfirstlane(tid / kWave) * 1024;
   }
 
-  // Loads of one operand's chunk of k from k0 on into `stage` (a byte offset).  row0: the first row of load u.
-  template <class O, class ROW0>
-  __device__ __forceinline__ void issue_one(const uint16_t *p, int64_t ld, int64_t rows, int64_t K, int64_t k0, ROW0 row0,
-                                            const uint32_t *off, uint32_t at) {
-    uint32_t o[O::kOffsets];
+  // Loads first .. last - 1 of an operand's next chunk into LDS at `at`.
+  template <class O>
+  static __device__ __forceinline__ void load(const MmSource<O> &s, const uint32_t *off, uint32_t at, int first = 0,
+                                              int last = O::kLoads) {
+    const intx4 rsrc = s.rsrc();
+    if (O::kContiguous && s.k < kMmK) {                  // wave-uniform, and rare: a path of its own
+      const bool inside = O::first_k(threadIdx.x) < s.k;
 #pragma unroll
-    for (int u = 0; u < O::kOffsets; ++u) o[u] = off[u];
-    if constexpr (O::kContiguous) {
-      if (k0 + kMmK > K) o[0] = k0 + O::first_k(threadIdx.x) < K ? o[0] : kMmOutside;
+      for (int u = 0; u < O::kLoads; ++u)
+        if (u >= first && u < last) mm_load_lds(rsrc, inside ? off[u] : kMmOutside, at + u * 4096);
+    } else {
+#pragma unroll
+      for (int u = 0; u < O::kLoads; ++u)
+        if (u >= first && u < last) mm_load_lds(rsrc, off[u], at + u * 4096);
     }
-#pragma unroll
-    for (int u = 0; u < O::kLoads; ++u)
-      mm_load_lds(O::rsrc(p, ld, rows, K, row0(u), k0, u), o[u % O::kOffsets], at + u * 4096);
+  }
+  __device__ __forceinline__ void issue(MmSource<F> &f, MmSource<T> &t, uint32_t stage) {
+    load<F>(f, fo, lds + stage);
+    load<T>(t, to, lds + stage + F::kBytes);
+    f.next();
+    t.next();
   }
 
   __device__ __forceinline__ void compute(uint32_t stage, floatx4 (&acc)[NI][NJ]) const {
@@ -175,6 +187,10 @@ struct MmLoop {
   }
 };
 
+__device__ __forceinline__ uint32_t mm_next_stage(uint32_t stage, uint32_t bytes) {
+  return stage == 2 * bytes ? 0 : stage + bytes;
+}
+
 template <int NI, int NJ>
 __device__ __forceinline__ void mm_zero(floatx4 (&acc)[NI][NJ]) {
 #pragma unroll
@@ -184,9 +200,9 @@ __device__ __forceinline__ void mm_zero(floatx4 (&acc)[NI][NJ]) {
 }
 
 // Tile t of `n`, so that each XCD (workgroup id % 8) walks neighbours; -1 for the padding of the grid (mm_grid).
-__device__ __forceinline__ int64_t mm_tile_of(int64_t id, int64_t n) {
-  const int64_t per = (n + kMmXcds - 1) / kMmXcds, t = id % kMmXcds * per + id / kMmXcds;
-  return id / kMmXcds < per && t < n ? t : -1;
+__device__ __forceinline__ int mm_tile_of(unsigned id, unsigned n) {
+  const unsigned per = (n + kMmXcds - 1) / kMmXcds, t = id % kMmXcds * per + id / kMmXcds;
+  return id / kMmXcds < per && t < n ? (int)t : -1;
 }
 inline int64_t mm_grid(int64_t n) { return (n + kMmXcds - 1) / kMmXcds * kMmXcds; }
 

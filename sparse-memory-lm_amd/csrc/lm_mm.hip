@@ -14,33 +14,33 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm_kernel(MmArgs a) {
   typedef MmTile<32 * NJ, TKC, 0> TT;
   typedef MmLoop<FT, TT, NI, NJ> Loop;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int64_t nf = (a.F + FT::kRows - 1) / FT::kRows, nt = (a.T + TT::kRows - 1) / TT::kRows;
-  const int64_t tile = mm_tile_of(blockIdx.x, nf * nt * a.nsplit);
+  const unsigned nf = (unsigned)((a.F + FT::kRows - 1) / FT::kRows), nt = (unsigned)((a.T + TT::kRows - 1) / TT::kRows);
+  const int tile = mm_tile_of(blockIdx.x, nf * nt * (unsigned)a.nsplit);   // the host has checked that they are this few
   if (tile < 0) return;  // workgroup-uniform
   // the feature tiles of one token tile are neighbours: on one XCD its rows come from memory once
-  const int64_t f0 = tile % nf * FT::kRows, t0 = tile / nf % nt * TT::kRows, s = tile / (nf * nt);
+  const unsigned row = tile / nf, split = row / nt;
+  const int64_t f0 = (int64_t)(tile - row * nf) * FT::kRows, t0 = (int64_t)(row - split * nt) * TT::kRows, s = split;
   const int64_t k_begin = s * a.k_per, k_end = min(a.K, k_begin + a.k_per);
   const int wave = threadIdx.x / kWave, wf = (wave & 1) * 16 * NI, wt = (wave >> 1) * 16 * NJ;
   Loop L;
   L.init(smem, a.ldf, a.ldt, wf, wt);
-  auto issue = [&](int64_t k0, uint32_t stage) {
-    L.template issue_one<FT>(a.feat, a.ldf, a.F, FKC ? a.K : a.Kf, k0, [&](int u) { return FKC ? f0 + 64 * u : f0; }, L.fo, L.lds + stage);
-    L.template issue_one<TT>(a.tok, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, k0, [&](int u) { return TKC ? t0 + 64 * u : t0; }, L.to,
-                             L.lds + stage + FT::kBytes);
-  };
   floatx4 acc[NI][NJ];
   mm_zero(acc);
   const int nch = k_end > k_begin ? (int)((k_end - k_begin + kMmK - 1) / kMmK) : 0;
-  if (nch > 0) issue(k_begin, 0);
-  if (nch > 1) issue(k_begin + kMmK, Loop::kStage);
+  MmSource<FT> fs;
+  MmSource<TT> ts;
+  fs.init(a.feat, a.ldf, a.F, FKC ? a.K : a.Kf, f0, k_begin);
+  ts.init(a.tok, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, t0, k_begin);
+  if (nch > 0) L.issue(fs, ts, 0);
+  if (nch > 1) L.issue(fs, ts, Loop::kStage);
   uint32_t now = 0, next = 2 * Loop::kStage;
   for (int ch = 0; ch < nch; ++ch) {
     if (ch + 1 < nch) mm_wait_barrier<Loop::kLoads>();
     else mm_wait_barrier<0>();
-    if (ch + 2 < nch) issue(k_begin + (int64_t)(ch + 2) * kMmK, next);  // the stage of chunk ch - 1, which all have read
+    if (ch + 2 < nch) L.issue(fs, ts, next);             // into the stage of chunk ch - 1, which all have read
     L.compute(now, acc);
-    now = now == 2 * Loop::kStage ? 0 : now + Loop::kStage;
-    next = next == 2 * Loop::kStage ? 0 : next + Loop::kStage;
+    now = mm_next_stage(now, Loop::kStage);
+    next = mm_next_stage(next, Loop::kStage);
   }
 
   // lane (r, g): features 4 NI g .. (permuted) or 4 g .. of each 16, of token r of each 16

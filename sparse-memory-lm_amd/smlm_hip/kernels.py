@@ -1163,7 +1163,7 @@ def _one_device(name, first, *others):
             raise ValueError(f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
 
 
-MAX_ROW_STRIDE = 1 << 23      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
+MAX_ROW_STRIDE = 1 << 22      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
 
 
 def _mm_rows(t, rows, cols):

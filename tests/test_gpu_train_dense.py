@@ -515,7 +515,7 @@ def test_a_run_of_them_together():
     xs = xs + (F.silu(a) * b) @ w2.T
     ref_loss = F.cross_entropy(F.rms_norm(xs, nw.shape, nw, 1e-5) @ emb.T, ins[2])
     ref = torch.autograd.grad(ref_loss, (x, delta, nw, w13, w2, emb))
-    assert abs(float(loss) - float(ref_loss)) <= 2e-3 * float(ref_loss)
+    assert abs(loss.item() - ref_loss.item()) <= 2e-3 * ref_loss.item()
     for name, p, q in zip(("x", "delta", "norm", "w13", "w2", "emb"), got, ref):
         # a chain of eight bf16 roundings, each at most 2^-8 of its value
         assert float((p.double() - q).norm() / q.norm()) <= 8 * HALF, name

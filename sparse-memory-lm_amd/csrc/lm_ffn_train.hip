@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) gate_kernel(GateArgs p) {
   for (int i = 0; i < 2; ++i) A.fa[2 + i] = A.fa[i] + kGateFeat * FT::kRowBytes;   // b's rows: the same swizzle
   Out B;
   if constexpr (GRAD) B.init(smem, p.ldw2, p.lddy, wf, wt);
-  const int n1 = (int)((p.d + kMmK - 1) / kMmK), n2 = GRAD ? (int)((p.n_out + kMmK - 1) / kMmK) : 0;
+  const int n1 = mm_chunks(p.d), n2 = GRAD ? mm_chunks(p.n_out) : 0;
   // rows of a beyond hidden are b's, whose results are not stored; rows of b beyond the weight read as zeros
   MmSource<FT> as, bs;
   MmSource<TT> xs, ys;
@@ -67,49 +67,111 @@ __global__ void __launch_bounds__(kMmThreads, 2) gate_kernel(GateArgs p) {
     ss.init(p.w2, p.ldw2, p.hidden, p.n_out, f0, 0);
     ys.init(p.dy, p.lddy, p.M, p.n_out, t0, 0);
   }
-  uint32_t ahead = 0;
-  auto issue_ab = [&]() {
-    Gate::template load<FT>(as, A.fo, A.lds + ahead, 0, 1);
-    Gate::template load<FT>(bs, A.fo, A.lds + ahead, 1, 2);
-    Gate::template load<TT>(xs, A.to, A.lds + ahead + FT::kBytes);
+  floatx4 ab[4][NJ], dact[2][NJ];
+  mm_zero(ab);
+  mm_zero(dact);
+  uint32_t stage = 0;
+  auto advance = [&]() {
+    const uint32_t here = stage;
+    stage = stage == 2 * kStage ? 0 : stage + kStage;
+    return here;
+  };
+  // Loads of the next chunk, of x w13^T or (OUT) of dy w2, part i of `parts`.
+  struct Chunk {
+    intx4 a, b, t;
+  };
+  auto next_gate = [&]() {
+    Gate::template clip<FT>(as, A.fo);
+    Gate::template clip<TT>(xs, A.to);
+    const Chunk c{as.rsrc(), bs.rsrc(), xs.rsrc()};
     as.next();
     bs.next();
     xs.next();
-    ahead = mm_next_stage(ahead, kStage);
+    return c;
   };
-  auto issue_out = [&]() {
-    B.issue(ss, ys, ahead);
-    ahead = mm_next_stage(ahead, kStage);
+  auto next_out = [&]() {
+    Out::template clip<TT>(ys, B.to);
+    const Chunk c{ss.rsrc(), ss.rsrc(), ys.rsrc()};
+    ss.next();
+    ys.next();
+    return c;
   };
-  // chunk ch of both sums in a row
-  auto issue = [&](int ch) {
-    if (ch < n1) issue_ab();
-    else if (ch < n1 + n2) issue_out();
+  auto load_gate = [&](const Chunk &c, uint32_t at, int i, int parts) {
+#pragma unroll
+    for (int l = 0; l < Gate::kLoads; ++l)
+      if (l >= i * Gate::kLoads / parts && l < (i + 1) * Gate::kLoads / parts)
+        mm_load_lds(l == 0 ? c.a : l == 1 ? c.b : c.t, l < 2 ? A.fo[l] : A.to[l - 2], A.lds + at + l * 4096);
   };
-  floatx4 ab[4][NJ];
-  mm_zero(ab);
-  issue(0);
-  issue(1);
-  uint32_t now = 0;
-  for (int ch = 0; ch < n1; ++ch) {
-    if (ch + 1 < n1) mm_wait_barrier<Gate::kLoads>();
-    else if (n2 > 0) mm_wait_barrier<Out::kLoads>();
-    else mm_wait_barrier<0>();
-    issue(ch + 2);
-    A.compute(now, ab);
-    now = mm_next_stage(now, kStage);
-  }
-  floatx4 dact[2][NJ];
-  mm_zero(dact);
+  auto load_out = [&](const Chunk &c, uint32_t at, int i, int parts) {
+#pragma unroll
+    for (int l = 0; l < Out::kLoads; ++l)
+      if (l >= i * Out::kLoads / parts && l < (i + 1) * Out::kLoads / parts) B.load(l, c.a, c.t, at);
+  };
+
+  // Steps of x w13^T: loading a chunk of the same, or (the last three) of dy w2.
+  auto step = [&](const typename Gate::Frags &cur, typename Gate::Frags &next) {
+    const uint32_t here = advance();
+    const Chunk c = next_gate();
+    Gate::products(cur, ab, [&](int i) { load_gate(c, here, i, 4); }, [&](int i) { A.read_part(next, stage, i); });
+  };
+  auto step_to_out = [&](const typename Gate::Frags &cur, typename Gate::Frags &next) {
+    const uint32_t here = advance();
+    const Chunk c = next_out();
+    Gate::products(cur, ab, [&](int i) { load_out(c, here, i, 4); }, [&](int i) { A.read_part(next, stage, i); });
+  };
+  typename Gate::Frags x, y;
+  load_gate(next_gate(), 0, 0, 1);
+  load_gate(next_gate(), kStage, 0, 1);
+  int left = n1;                          // chunks of x w13^T not yet multiplied, an even number
   if constexpr (GRAD) {
-    for (int ch = 0; ch < n2; ++ch) {
-      if (ch + 1 < n2) mm_wait_barrier<Out::kLoads>();
-      else mm_wait_barrier<0>();
-      if (ch + 2 < n2) issue_out();
-      B.compute(now, dact);
-      now = mm_next_stage(now, kStage);
+    if (n1 > 2) {
+      load_gate(next_gate(), 2 * kStage, 0, 1);
+      mm_wait_barrier<2 * Gate::kLoads>();
+    } else {
+      load_out(next_out(), 2 * kStage, 0, 1);
+      mm_wait_barrier<Gate::kLoads + Out::kLoads>();
+    }
+    A.read(x, 0);
+    for (; left > 4; left -= 2) {
+      mm_wait_barrier<Gate::kLoads>();
+      step(x, y);
+      mm_wait_barrier<Gate::kLoads>();
+      step(y, x);
+    }
+    if (left > 2) {
+      mm_wait_barrier<Gate::kLoads>();
+      step(x, y);
+      mm_wait_barrier<Gate::kLoads>();
+      step_to_out(y, x);
+    }
+    mm_wait_barrier<Out::kLoads>();
+    step_to_out(x, y);
+    mm_wait_barrier<Out::kLoads>();       // what step_to_out reads ahead now is the next sum's, and not used
+    step_to_out(y, x);
+    typename Out::Frags u, v;
+    B.read(u, stage);                     // the first chunk of dy w2, landed by the barrier before
+    auto out_step = [&](const typename Out::Frags &cur, typename Out::Frags &next) {
+      mm_wait_barrier<Out::kLoads>();
+      const uint32_t here = advance();
+      const Chunk c = next_out();
+      Out::products(cur, dact, [&](int i) { load_out(c, here, i, 2); }, [&](int i) { B.read_part(next, stage, i); });
+    };
+    for (int more = n2; more > 0; more -= 2) {
+      out_step(u, v);
+      out_step(v, u);
+    }
+  } else {
+    load_gate(next_gate(), 2 * kStage, 0, 1);
+    mm_wait_barrier<2 * Gate::kLoads>();
+    A.read(x, 0);
+    for (; left > 0; left -= 2) {
+      mm_wait_barrier<Gate::kLoads>();
+      step(x, y);
+      mm_wait_barrier<Gate::kLoads>();
+      step(y, x);
     }
   }
+  __builtin_amdgcn_s_waitcnt(0x0F70);     // no load is on its way into LDS when the workgroup ends
 
   // lane (r, g): features f .. f + 7 of token r of each 16
   const int64_t f = f0 + wf + 8 * g;

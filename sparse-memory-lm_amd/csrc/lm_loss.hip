@@ -83,38 +83,42 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
 
   Loop L;
   L.init(smem, a.ldw, a.ldx, wf, wt);
-  const int nch = (int)((a.d + kMmK - 1) / kMmK);
-  // the loads run two chunks ahead of the products, over the ends of tiles
-  int ahead_tile = first;
-  uint32_t ahead = 0;
+  const int nch = mm_chunks(a.d);
+  // the loads run three chunks ahead of the products, over the ends of tiles (past the last tile they load what is not used)
+  int ahead_tile = first, ahead = 0;
   MmSource<FT> fs;
   MmSource<TT> ts;
-  auto tile_starts = [&]() {
+  auto begin_tile = [&]() {
     fs.init(a.w, a.ldw, a.V, a.d, a.v0 + (int64_t)ahead_tile * kLsCols, 0);
     ts.init(a.x, a.ldx, a.M, a.d, t0, 0);
+    if (a.d % kMmK) L.offsets(a.ldw, a.ldx);             // the last chunks' clipped them
+    ahead = 0;
   };
-  auto issue = [&]() {
-    L.issue(fs, ts, ahead);
-    ahead = mm_next_stage(ahead, Loop::kStage);
-    if (fs.k <= 0) {
+  auto loaded = [&]() {
+    if (++ahead == nch) {
       ++ahead_tile;
-      tile_starts();
+      begin_tile();
     }
   };
-  tile_starts();
   floatx4 acc[NI][NJ];
-  int left = (last - first) * nch;    // chunks not yet multiplied
-  if (left > 0) issue();
-  if (left > 1) issue();
-  uint32_t now = 0;
+  typename Loop::Frags x, y;
+  uint32_t stage = 0;
+  begin_tile();
+  if (first < last) {
+    for (int q = 0; q < 3; ++q) {
+      L.issue(fs, ts, q * Loop::kStage);
+      loaded();
+    }
+    mm_wait_barrier<2 * Loop::kLoads>();
+    L.read(x, 0);
+  }
   for (int tile = first; tile < last; ++tile) {
     mm_zero(acc);
-    for (int ch = 0; ch < nch; ++ch, --left) {
-      if (left > 1) mm_wait_barrier<Loop::kLoads>();
-      else mm_wait_barrier<0>();
-      if (left > 2) issue();
-      L.compute(now, acc);
-      now = mm_next_stage(now, Loop::kStage);
+    for (int ch = 0; ch < nch; ch += 2) {
+      L.step(fs, ts, x, y, stage, acc);
+      loaded();
+      L.step(fs, ts, y, x, stage, acc);
+      loaded();
     }
 
     // lane (r, g): columns c0 .. c0 + 15 of token r of each 16
@@ -169,6 +173,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
     }
   }
 
+  __builtin_amdgcn_s_waitcnt(0x0F70);                    // no load is on its way into LDS when the workgroup ends
   if constexpr (!GRAD) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {

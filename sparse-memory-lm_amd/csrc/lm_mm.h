@@ -6,9 +6,12 @@
 // Workgroup = 4 wavefronts, WF x WT of them over the tile, 16 NI features x 16 NJ tokens each.  At the matrix cores' rate a
 // wavefront's tile of 64 features x 128 tokens reads 96 of the 128 bytes per clock that the LDS has, one of 64 x 64 all
 // of them: hence 128 x 256 tiles where there are enough of them.
-// k streams through three LDS stages of 32, two chunks ahead, loaded straight from memory into LDS (buffer_load ... lds,
-// no registers in between); one barrier per chunk both publishes a chunk and frees the stage that is loaded next.  A
-// stage takes 24 KB for 128 x 256, so that two workgroups fit a CU: one's epilogue runs under the other's products.
+// k streams through three LDS stages of 32, loaded straight from memory into LDS (buffer_load ... lds, no registers in
+// between).  While a chunk is multiplied, the next one's fragments are read into a second set of registers and the chunk
+// three ahead is loaded into the stage that the first came from (which all wavefronts have read by the barrier that opens
+// the step), the reads and loads spread between the products: neither LDS nor memory latency stands between two chunks'
+// products.  The number of chunks is even, so that the two register sets alternate without copies.  A stage takes 24 KB for
+// 128 x 256, so that two workgroups fit a CU: one's epilogue runs under the other's products.
 //
 // LDS layouts (16-byte pieces; banks repeat every 256 bytes):
 //   k contiguous: 64-byte rows, piece c of row R at c ^ swz(R), so that the 16 rows of a fragment read fall on distinct
@@ -106,7 +109,7 @@ struct MmTile {
 };
 
 // Where an operand's next chunk comes from: wave-uniform, stepped from chunk to chunk.  `left` is exact: the bytes from the
-// chunk's first to the operand's last, which the record count of its loads is clipped to.
+// chunk's first to the operand's last, which the record count of its loads is clipped to: past the end they read zeros.
 template <class O>
 struct MmSource {
   const uint16_t *p;
@@ -121,7 +124,8 @@ struct MmSource {
   }
   __device__ __forceinline__ intx4 rsrc() const {
     const uint64_t a = (uint64_t)p;
-    return intx4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(left >> 32 ? 0xFFFFFFF0u : (uint32_t)left), 0x00020000};
+    const uint32_t n = left >> 32 ? 0xFFFFFFF0u : (uint32_t)left;
+    return intx4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(left <= 0 ? 0u : n), 0x00020000};
   }
   __device__ __forceinline__ void next() {
     p += step / 2;
@@ -130,66 +134,113 @@ struct MmSource {
   }
 };
 
+template <int NI, int NJ>
+struct MmFrags {
+  bf16x8 a[NI], b[NJ];
+};
+
 // The loop's state of one thread for an F tile of features and a T tile of tokens: a stage holds F, then T.
 template <class F, class T, int NI, int NJ>
 struct MmLoop {
   static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads;
+  typedef MmFrags<NI, NJ> Frags;
   uint32_t fo[F::kLoads], to[T::kLoads], fa[NI], ta[NJ], lds;
 
+  __device__ __forceinline__ void offsets(int64_t ldf, int64_t ldt) {
+#pragma unroll
+    for (int u = 0; u < F::kLoads; ++u) fo[u] = F::offset(u, threadIdx.x, ldf);
+#pragma unroll
+    for (int u = 0; u < T::kLoads; ++u) to[u] = T::offset(u, threadIdx.x, ldt);
+  }
   // wf, wt: first feature and token row of this wavefront in the tile
   __device__ __forceinline__ void init(const unsigned char *smem, int64_t ldf, int64_t ldt, int wf, int wt) {
-    const int tid = threadIdx.x, lane = tid % kWave, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
     const uint32_t base = (uint32_t)(uintptr_t)(lds_byte *)smem;
-#pragma unroll
-    for (int u = 0; u < F::kLoads; ++u) fo[u] = F::offset(u, tid, ldf);
-#pragma unroll
-    for (int u = 0; u < T::kLoads; ++u) to[u] = T::offset(u, tid, ldt);
+    offsets(ldf, ldt);
 #pragma unroll
     for (int i = 0; i < NI; ++i) fa[i] = base + F::frag_at(wf, i, r, g);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) ta[j] = base + F::kBytes + T::frag_at(wt, j, r, g);
-    lds = base + __builtin_amdgcn_readfirstlane(tid / kWave) * 1024;
+    lds = base + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * 1024;
   }
 
-  // Loads first .. last - 1 of an operand's next chunk into LDS at `at`.
+  // The last chunks of contiguous rows: the pieces from the sum's end on come from outside, as zeros, from now on.
   template <class O>
-  static __device__ __forceinline__ void load(const MmSource<O> &s, const uint32_t *off, uint32_t at, int first = 0,
-                                              int last = O::kLoads) {
-    const intx4 rsrc = s.rsrc();
-    if (O::kContiguous && s.k < kMmK) {                  // wave-uniform, and rare: a path of its own
+  static __device__ __forceinline__ void clip(const MmSource<O> &s, uint32_t *off) {
+    if (O::kContiguous && s.k < kMmK) {                  // wave-uniform
       const bool inside = O::first_k(threadIdx.x) < s.k;
 #pragma unroll
-      for (int u = 0; u < O::kLoads; ++u)
-        if (u >= first && u < last) mm_load_lds(rsrc, inside ? off[u] : kMmOutside, at + u * 4096);
-    } else {
-#pragma unroll
-      for (int u = 0; u < O::kLoads; ++u)
-        if (u >= first && u < last) mm_load_lds(rsrc, off[u], at + u * 4096);
+      for (int u = 0; u < O::kLoads; ++u) off[u] = inside ? off[u] : kMmOutside;
     }
   }
+  // Load l of the sources' next chunk (F's first) into `stage`.
+  __device__ __forceinline__ void load(int l, intx4 frsrc, intx4 trsrc, uint32_t stage) const {
+    mm_load_lds(l < F::kLoads ? frsrc : trsrc, l < F::kLoads ? fo[l] : to[l - F::kLoads], lds + stage + l * 4096);
+  }
   __device__ __forceinline__ void issue(MmSource<F> &f, MmSource<T> &t, uint32_t stage) {
-    load<F>(f, fo, lds + stage);
-    load<T>(t, to, lds + stage + F::kBytes);
+    clip(f, fo);
+    clip(t, to);
+    const intx4 fr = f.rsrc(), tr = t.rsrc();
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) load(l, fr, tr, stage);
     f.next();
     t.next();
   }
-
-  __device__ __forceinline__ void compute(uint32_t stage, floatx4 (&acc)[NI][NJ]) const {
-    bf16x8 a[NI], b[NJ];
+  __device__ __forceinline__ void read(Frags &x, uint32_t stage) const {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) a[i] = F::frag(fa[i] + stage);
+    for (int i = 0; i < NI; ++i) x.a[i] = F::frag(fa[i] + stage);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) b[j] = T::frag(ta[j] + stage);
+    for (int j = 0; j < NJ; ++j) x.b[j] = T::frag(ta[j] + stage);
+  }
+  // The products of `cur`, with load(i) and read(i), i < NI, spread between them.
+  template <class LOAD, class READ>
+  static __device__ __forceinline__ void products(const Frags &cur, floatx4 (&acc)[NI][NJ], LOAD load, READ read) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i) {
+      load(i);
+      read(i);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < NJ; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[i], cur.b[j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __device__ __forceinline__ void read_part(Frags &x, uint32_t stage, int i) const {
+    x.a[i] = F::frag(fa[i] + stage);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j >= i * NJ / NI && j < (i + 1) * NJ / NI) x.b[j] = T::frag(ta[j] + stage);
+  }
+  // One step: the products of `cur` (chunk ch, whose stage is `stage`), while `next` is read from chunk ch + 1's stage and
+  // the sources' chunk ch + 3 is loaded into chunk ch's.  On the way at its start: the loads of chunks ch + 1 and ch + 2.
+  __device__ __forceinline__ void step(MmSource<F> &f, MmSource<T> &t, const Frags &cur, Frags &next, uint32_t &stage,
+                                       floatx4 (&acc)[NI][NJ]) {
+    mm_wait_barrier<kLoads>();
+    const uint32_t here = stage;
+    stage = stage == 2 * kStage ? 0 : stage + kStage;
+    clip(f, fo);
+    clip(t, to);
+    const intx4 fr = f.rsrc(), tr = t.rsrc();
+    products(
+        cur, acc,
+        [&](int i) {
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l)
+            if (l >= i * kLoads / NI && l < (i + 1) * kLoads / NI) load(l, fr, tr, here);
+        },
+        [&](int i) { read_part(next, stage, i); });
+    f.next();
+    t.next();
+  }
+  // Fills the three stages and reads the first chunk's fragments.
+  __device__ __forceinline__ void start(MmSource<F> &f, MmSource<T> &t, Frags &x) {
+    issue(f, t, 0);
+    issue(f, t, kStage);
+    issue(f, t, 2 * kStage);
+    mm_wait_barrier<2 * kLoads>();
+    read(x, 0);
   }
 };
-
-__device__ __forceinline__ uint32_t mm_next_stage(uint32_t stage, uint32_t bytes) {
-  return stage == 2 * bytes ? 0 : stage + bytes;
-}
 
 template <int NI, int NJ>
 __device__ __forceinline__ void mm_zero(floatx4 (&acc)[NI][NJ]) {
@@ -206,12 +257,15 @@ __device__ __forceinline__ int mm_tile_of(unsigned id, unsigned n) {
 }
 inline int64_t mm_grid(int64_t n) { return (n + kMmXcds - 1) / kMmXcds * kMmXcds; }
 
+// Chunks of a sum over k, an even number.
+__device__ __forceinline__ int mm_chunks(int64_t k) { return (int)((k + 2 * kMmK - 1) / (2 * kMmK)) * 2; }
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- plain products (lm_mm.hip) ----------------------------------------------------------------------------------------
 // out[t, f] = sum_k tok[t, k] feat[f, k]; an operand with *_kc = false is stored [k][row].  Rows and strides in elements,
 // rows of 16-byte pieces.  nsplit > 1 or f32: fp32 parts [nsplit][T][F] (with accumulate added to what is there), split s
-// summing k_per (a multiple of 32) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
+// summing k_per (a multiple of 64) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
 // F a multiple of 8; K one too where an operand has k contiguous, that operand's k from the sum's end up to it zeros; a k
 // strided tok has rows of at least T rounded up to 8.  Kf: the k that a k strided feat has (the last of K may lack).
 struct MmArgs {

@@ -26,21 +26,19 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm_kernel(MmArgs a) {
   L.init(smem, a.ldf, a.ldt, wf, wt);
   floatx4 acc[NI][NJ];
   mm_zero(acc);
-  const int nch = k_end > k_begin ? (int)((k_end - k_begin + kMmK - 1) / kMmK) : 0;
   MmSource<FT> fs;
   MmSource<TT> ts;
   fs.init(a.feat, a.ldf, a.F, FKC ? a.K : a.Kf, f0, k_begin);
   ts.init(a.tok, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, t0, k_begin);
-  if (nch > 0) L.issue(fs, ts, 0);
-  if (nch > 1) L.issue(fs, ts, Loop::kStage);
-  uint32_t now = 0, next = 2 * Loop::kStage;
-  for (int ch = 0; ch < nch; ++ch) {
-    if (ch + 1 < nch) mm_wait_barrier<Loop::kLoads>();
-    else mm_wait_barrier<0>();
-    if (ch + 2 < nch) L.issue(fs, ts, next);             // into the stage of chunk ch - 1, which all have read
-    L.compute(now, acc);
-    now = mm_next_stage(now, Loop::kStage);
-    next = mm_next_stage(next, Loop::kStage);
+  if (k_end > k_begin) {  // workgroup-uniform; k_end is K or a whole number of double chunks on
+    typename Loop::Frags x, y;
+    L.start(fs, ts, x);
+    uint32_t stage = 0;
+    for (int left = mm_chunks(k_end - k_begin); left > 0; left -= 2) {
+      L.step(fs, ts, x, y, stage, acc);
+      L.step(fs, ts, y, x, stage, acc);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // no load is on its way into LDS when the workgroup ends
   }
 
   // lane (r, g): features 4 NI g .. (permuted) or 4 g .. of each 16, of token r of each 16
@@ -132,7 +130,7 @@ int64_t mm_splits(int64_t T, int64_t F, int64_t K, int64_t min_k) {
   return std::min(most, std::max<int64_t>(1, 512 / tiles));
 }
 
-int64_t mm_k_per(int64_t K, int64_t nsplit) { return ceil_div(ceil_div(K, nsplit), kMmK) * kMmK; }
+int64_t mm_k_per(int64_t K, int64_t nsplit) { return ceil_div(ceil_div(K, nsplit), 2 * kMmK) * 2 * kMmK; }
 
 int mm_reduce_launch(const float *parts, int64_t nsplit, int64_t T, int64_t F, const float *scale, void *out, int64_t ldo,
                      hipStream_t stream, const char *what) {

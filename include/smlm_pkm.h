@@ -542,7 +542,7 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
  * smlm/model.py:286-293): per token logsumexp(s_n) - s_n[targets[n]], 0 where targets[n] == ignore_index, NaN where it
  * is any other index outside the vocabulary; their mean over the tokens that are not ignored (NaN if none), or sum.
  *   x (M, d) and w (V, d) bf16, rows of x_row_stride / w_row_stride elements (multiples of 8, 16-byte aligned, at most
- *   2^22), d a multiple of 8; targets (M,) int64
+ *   2^21), d a multiple of 8; targets (M,) int64
  *   loss  SMLM_REDUCE_NONE: (M,) fp32; otherwise fp32[2]: the loss, and the number of tokens that are not ignored
  *   lse   (M,) fp32: the tokens' logsumexp, which the gradient needs
  * workspace: smlm_linear_ce_workspace(M, V, d, 0) bytes, 16-byte aligned, free again when the call's work is done.
@@ -569,19 +569,20 @@ int smlm_linear_ce_backward(const float *grad, const float *count, int per_token
 /*
  * The gated feed-forward block y = (silu(a) * b) w2^T, a | b = the halves of x w13^T (smlm/model.py:110-118).
  *   x (M, d), w13 (2 * hidden, d), w2 (n_out, hidden) bf16 with row strides as above, d, hidden and n_out multiples of 8
- *   act (M, hidden) bf16: scratch; y (M, n_out) contiguous bf16
- * a, b and the gate in fp32, act and y rounded once each.
+ *   y (M, n_out) contiguous bf16
+ * workspace: smlm_gated_ffn_workspace(..., 0) bytes, 16-byte aligned.  a, b and the gate in fp32, the activation and y
+ * rounded once each.
  */
+int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out, int grad);
 int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w13, int64_t w13_row_stride, const void *w2,
-                   int64_t w2_row_stride, int64_t M, int64_t d, int64_t hidden, int64_t n_out, void *act, void *y,
-                   void *stream);
+                   int64_t w2_row_stride, int64_t M, int64_t d, int64_t hidden, int64_t n_out, void *y,
+                   void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * Its gradients from dy (M, n_out) and the inputs alone (a and b are formed again): dx (M, d), dw13 (2 * hidden, d), dw2
- * (n_out, hidden), contiguous bf16, each NULL if not wanted.  workspace: smlm_gated_ffn_workspace(...) bytes, 16-byte
+ * (n_out, hidden), contiguous bf16, each NULL if not wanted.  workspace: smlm_gated_ffn_workspace(..., 1) bytes, 16-byte
  * aligned.  fp32 sums in a fixed order; the gradients of a and b are rounded to bf16 as operands of their products.
  */
-int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out);
 int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, const void *x, int64_t x_row_stride, const void *w13,
                             int64_t w13_row_stride, const void *w2, int64_t w2_row_stride, int64_t M, int64_t d,
                             int64_t hidden, int64_t n_out, void *dx, void *dw13, void *dw2, void *workspace,

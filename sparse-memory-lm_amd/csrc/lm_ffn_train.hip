@@ -18,7 +18,6 @@
 namespace smlm {
 namespace {
 
-constexpr int kGateFeat = 64;                             // features per tile: 64 rows of a and 64 of b
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct GateArgs {
@@ -31,187 +30,201 @@ __device__ __forceinline__ float sigmoid(float a) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-a * kLog2e));
 }
 
-template <int NJ, bool GRAD>
-__global__ void __launch_bounds__(kMmThreads, 2) gate_kernel(GateArgs p) {
-  typedef MmTile<2 * kGateFeat, true, 8> FT;              // rows of w13: 64 of a, then 64 of b
-  typedef MmTile<kGateFeat, false, 8> ST;                 // columns of w2
-  typedef MmTile<32 * NJ, true, 0> TT;
-  typedef MmLoop<FT, TT, 4, NJ> Gate;
-  typedef MmLoop<ST, TT, 2, NJ> Out;
+// A tile takes S::kF rows of w13: half of them a's, and b's for the same features; each wavefront 8 NI features of either.
+template <class S>
+struct GateKernel {
+  static constexpr int kFeat = S::kF / 2, kHalf = S::NI / 2, kLane = 2 * S::NI;   // features of a tile; tiles; of a lane
+  typedef MmTile<S::kF, true, kLane, S::kThreads, 64> F;       // rows of w13
+  typedef MmTile<kFeat, false, kLane, S::kThreads, 64> W2;     // columns of w2
+  typedef MmTile<S::kT, true, 0, S::kThreads, 64> T;
+  typedef MmLoop<F, T, S::NI, S::NJ> Gate;
+  typedef MmLoop<W2, T, kHalf, S::NJ> Out;
+};
+
+template <class S, bool GRAD>
+__global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
+  typedef GateKernel<S> K;
+  typedef typename K::Gate Gate;
+  typedef typename K::Out Out;
+  constexpr int NI = S::NI, NJ = S::NJ, kHalf = K::kHalf, kLane = K::kLane;
   constexpr uint32_t kStage = Gate::kStage;               // the larger of the two
   extern __shared__ __align__(16) unsigned char smem[];
-  const unsigned nf = (unsigned)((p.hidden + kGateFeat - 1) / kGateFeat), nt = (unsigned)((p.M + TT::kRows - 1) / TT::kRows);
+  const unsigned nf = (unsigned)((p.hidden + K::kFeat - 1) / K::kFeat), nt = (unsigned)((p.M + S::kT - 1) / S::kT);
   const int tile = mm_tile_of(blockIdx.x, nf * nt);
   if (tile < 0) return;  // workgroup-uniform
   // the feature tiles of a token tile are neighbours: on one XCD its rows are read from memory once
   const unsigned row = tile / nf;
-  const int64_t f0 = (int64_t)(tile - row * nf) * kGateFeat, t0 = (int64_t)row * TT::kRows;
-  const int wave = threadIdx.x / kWave, wf = (wave & 1) * 32, wt = (wave >> 1) * 16 * NJ;
+  const int64_t f0 = (int64_t)(tile - row * nf) * K::kFeat, t0 = (int64_t)row * S::kT;
+  const int wave = threadIdx.x / kWave, wf = S::feature(wave) / 2, wt = S::token(wave);
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
 
   Gate A;
   A.init(smem, p.ldw13, p.ldx, wf, wt);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) A.fa[2 + i] = A.fa[i] + kGateFeat * FT::kRowBytes;   // b's rows: the same swizzle
   Out B;
   if constexpr (GRAD) B.init(smem, p.ldw2, p.lddy, wf, wt);
-  const int n1 = mm_chunks(p.d), n2 = GRAD ? mm_chunks(p.n_out) : 0;
   // rows of a beyond hidden are b's, whose results are not stored; rows of b beyond the weight read as zeros
-  MmSource<FT> as, bs;
-  MmSource<TT> xs, ys;
-  MmSource<ST> ss;
+  MmSource<typename K::F> as, bs;
+  MmSource<typename K::T> xs, ys;
+  MmSource<typename K::W2> ss;
   as.init(p.w13, p.ldw13, 2 * p.hidden, p.d, f0, 0);
-  bs.init(p.w13, p.ldw13, 2 * p.hidden, p.d, p.hidden + f0 - kGateFeat, 0);   // load 1 adds 64 rows
+  bs.init(p.w13, p.ldw13, 2 * p.hidden, p.d, p.hidden + f0 - K::kFeat, 0);   // its loads are those of rows kFeat on
   xs.init(p.x, p.ldx, p.M, p.d, t0, 0);
   if constexpr (GRAD) {
     ss.init(p.w2, p.ldw2, p.hidden, p.n_out, f0, 0);
     ys.init(p.dy, p.lddy, p.M, p.n_out, t0, 0);
   }
-  floatx4 ab[4][NJ], dact[2][NJ];
-  mm_zero(ab);
-  mm_zero(dact);
-  uint32_t stage = 0;
-  auto advance = [&]() {
-    const uint32_t here = stage;
-    stage = stage == 2 * kStage ? 0 : stage + kStage;
-    return here;
-  };
-  // Loads of the next chunk, of x w13^T or (OUT) of dy w2, part i of `parts`.
-  struct Chunk {
+  // Where a stage of x w13^T or dy w2 comes from, and its loads, part i of `parts`
+  struct Stage {
     intx4 a, b, t;
   };
   auto next_gate = [&]() {
-    Gate::template clip<FT>(as, A.fo);
-    Gate::template clip<TT>(xs, A.to);
-    const Chunk c{as.rsrc(), bs.rsrc(), xs.rsrc()};
+    Gate::template clip<typename K::F>(as, A.fo);
+    Gate::template clip<typename K::T>(xs, A.to);
+    const Stage c{as.rsrc(), bs.rsrc(), xs.rsrc()};
     as.next();
     bs.next();
     xs.next();
     return c;
   };
   auto next_out = [&]() {
-    Out::template clip<TT>(ys, B.to);
-    const Chunk c{ss.rsrc(), ss.rsrc(), ys.rsrc()};
+    Out::template clip<typename K::T>(ys, B.to);
+    const Stage c{ss.rsrc(), ss.rsrc(), ys.rsrc()};
     ss.next();
     ys.next();
     return c;
   };
-  auto load_gate = [&](const Chunk &c, uint32_t at, int i, int parts) {
+  auto load_gate = [&](const Stage &c, uint32_t at, int i, int parts) {
+    constexpr int kF = K::F::kLoads;
 #pragma unroll
     for (int l = 0; l < Gate::kLoads; ++l)
       if (l >= i * Gate::kLoads / parts && l < (i + 1) * Gate::kLoads / parts)
-        mm_load_lds(l == 0 ? c.a : l == 1 ? c.b : c.t, l < 2 ? A.fo[l] : A.to[l - 2], A.lds + at + l * 4096);
+        mm_load_lds(l < kF / 2 ? c.a : l < kF ? c.b : c.t, l < kF ? A.fo[l] : A.to[l - kF], A.lds + at + l * K::F::kPerLoad);
   };
-  auto load_out = [&](const Chunk &c, uint32_t at, int i, int parts) {
+  auto load_out = [&](const Stage &c, uint32_t at, int i, int parts) {
 #pragma unroll
     for (int l = 0; l < Out::kLoads; ++l)
       if (l >= i * Out::kLoads / parts && l < (i + 1) * Out::kLoads / parts) B.load(l, c.a, c.t, at);
   };
+  // fragments of a in the first half of the row groups, of b (kFeat rows on, the same swizzle) in the second
+  auto read_gate = [&](typename Gate::Frags &x, uint32_t stage, int h, int i) {
+    x.a[i] = K::F::frag(A.fa, i % kHalf, h, stage + (i < kHalf ? 0 : K::kFeat * K::F::kRowBytes));
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j >= i * NJ / NI && j < (i + 1) * NJ / NI) x.b[j] = K::T::frag(A.ta, j, h, stage);
+  };
 
-  // Steps of x w13^T: loading a chunk of the same, or (the last three) of dy w2.
-  auto step = [&](const typename Gate::Frags &cur, typename Gate::Frags &next) {
-    const uint32_t here = advance();
-    const Chunk c = next_gate();
-    Gate::products(cur, ab, [&](int i) { load_gate(c, here, i, 4); }, [&](int i) { A.read_part(next, stage, i); });
-  };
-  auto step_to_out = [&](const typename Gate::Frags &cur, typename Gate::Frags &next) {
-    const uint32_t here = advance();
-    const Chunk c = next_out();
-    Gate::products(cur, ab, [&](int i) { load_out(c, here, i, 4); }, [&](int i) { A.read_part(next, stage, i); });
-  };
+  floatx4 ab[NI][NJ], dact[kHalf][NJ];
+  mm_zero(ab);
+  mm_zero(dact);
   typename Gate::Frags x, y;
+  const int n1 = mm_units(p.d), n2 = GRAD ? mm_units(p.n_out) : 0;
   load_gate(next_gate(), 0, 0, 1);
-  load_gate(next_gate(), kStage, 0, 1);
-  int left = n1;                          // chunks of x w13^T not yet multiplied, an even number
-  if constexpr (GRAD) {
-    if (n1 > 2) {
-      load_gate(next_gate(), 2 * kStage, 0, 1);
-      mm_wait_barrier<2 * Gate::kLoads>();
-    } else {
-      load_out(next_out(), 2 * kStage, 0, 1);
-      mm_wait_barrier<Gate::kLoads + Out::kLoads>();
-    }
-    A.read(x, 0);
-    for (; left > 4; left -= 2) {
-      mm_wait_barrier<Gate::kLoads>();
-      step(x, y);
-      mm_wait_barrier<Gate::kLoads>();
-      step(y, x);
-    }
-    if (left > 2) {
-      mm_wait_barrier<Gate::kLoads>();
-      step(x, y);
-      mm_wait_barrier<Gate::kLoads>();
-      step_to_out(y, x);
-    }
-    mm_wait_barrier<Out::kLoads>();
-    step_to_out(x, y);
-    mm_wait_barrier<Out::kLoads>();       // what step_to_out reads ahead now is the next sum's, and not used
-    step_to_out(y, x);
-    typename Out::Frags u, v;
-    B.read(u, stage);                     // the first chunk of dy w2, landed by the barrier before
-    auto out_step = [&](const typename Out::Frags &cur, typename Out::Frags &next) {
-      mm_wait_barrier<Out::kLoads>();
-      const uint32_t here = advance();
-      const Chunk c = next_out();
-      Out::products(cur, dact, [&](int i) { load_out(c, here, i, 2); }, [&](int i) { B.read_part(next, stage, i); });
-    };
-    for (int more = n2; more > 0; more -= 2) {
-      out_step(u, v);
-      out_step(v, u);
-    }
+  if (!GRAD || n1 > 1) {                                  // uniform
+    load_gate(next_gate(), kStage, 0, 1);
+    mm_wait_barrier<Gate::kLoads>();
   } else {
-    load_gate(next_gate(), 2 * kStage, 0, 1);
-    mm_wait_barrier<2 * Gate::kLoads>();
-    A.read(x, 0);
-    for (; left > 0; left -= 2) {
-      mm_wait_barrier<Gate::kLoads>();
-      step(x, y);
-      mm_wait_barrier<Gate::kLoads>();
-      step(y, x);
+    load_out(next_out(), kStage, 0, 1);
+    mm_wait_barrier<Out::kLoads>();
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i) read_gate(x, 0, 0, i);
+  uint32_t stage = 0;
+  for (int left = n1; left > 0; --left) {
+    const uint32_t here = stage;
+    stage = kStage - stage;
+    Gate::products(x, ab, [&](int i) { read_gate(y, here, 1, i); });
+    mm_wait_barrier<0>();                                 // the next stage has landed, all have read this one
+    if (!GRAD || left > 2) {
+      const Stage c = next_gate();
+      Gate::products(y, ab, [&](int i) {
+        load_gate(c, here, i, NI);
+        read_gate(x, stage, 0, i);
+      });
+    } else {                                              // the last two stages' places take dy w2's first two
+      const Stage c = next_out();
+      Gate::products(y, ab, [&](int i) {
+        load_out(c, here, i, NI);
+        if (left > 1) read_gate(x, stage, 0, i);
+      });
     }
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);     // no load is on its way into LDS when the workgroup ends
+  if constexpr (GRAD) {
+    typename Out::Frags u, v;
+    B.read(u, stage, 0);                                  // landed by the last barrier
+    for (int left = n2; left > 0; --left) {
+      const uint32_t here = stage;
+      stage = kStage - stage;
+      Out::products(u, dact, [&](int i) { B.read_part(v, here, 1, i); });
+      mm_wait_barrier<0>();
+      const Stage c = next_out();
+      Out::products(v, dact, [&](int i) {
+        load_out(c, here, i, kHalf);
+        B.read_part(u, stage, 0, i);
+      });
+    }
+  }
+  mm_finish();
 
-  // lane (r, g): features f .. f + 7 of token r of each 16
-  const int64_t f = f0 + wf + 8 * g;
-  if (f >= p.hidden) return;                              // hidden is a multiple of 8
+  // lane (r, g): features f .. f + kLane - 1 of token r of each 16
+  const int64_t f = f0 + wf + kLane * g;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int64_t t = t0 + wt + 16 * j + r;
     if (t >= p.M) continue;
-    float h[8], da[8], db[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float a = ab[q / 4][j][q % 4], b = ab[2 + q / 4][j][q % 4], s = sigmoid(a), as = a * s;
-      h[q] = as * b;
-      if constexpr (GRAD) {
-        const float dh = dact[q / 4][j][q % 4];
-        da[q] = dh * b * (s + as * (1.f - s));
-        db[q] = dh * as;
+    for (int o = 0; o < kLane; o += 8) {
+      if (f + o >= p.hidden) continue;                    // hidden is a multiple of 8
+      float h[8], da[8], db[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int i = (o + q) / 4, e = q % 4;
+        const float a = ab[i][j][e], b = ab[kHalf + i][j][e], s = sigmoid(a), as = a * s;
+        h[q] = as * b;
+        if constexpr (GRAD) {
+          const float dh = dact[i][j][e];
+          da[q] = dh * b * (s + as * (1.f - s));
+          db[q] = dh * as;
+        }
       }
-    }
-    auto store = [&](uint16_t *o, const float *v) {
-      *(uint4 *)o = uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    };
-    store(p.act + t * p.hidden + f, h);
-    if constexpr (GRAD) {
-      store(p.dab + t * 2 * p.hidden + f, da);
-      store(p.dab + t * 2 * p.hidden + p.hidden + f, db);
+      auto store = [&](uint16_t *to, const float *v) {
+        *(uint4 *)to = uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                             pack_bf16x2(v[6], v[7])};
+      };
+      store(p.act + t * p.hidden + f + o, h);
+      if constexpr (GRAD) {
+        store(p.dab + t * 2 * p.hidden + f + o, da);
+        store(p.dab + t * 2 * p.hidden + p.hidden + f + o, db);
+      }
     }
   }
 }
 
-template <int NJ, bool GRAD>
+typedef MmShape<2, 4, 8, 4> Gate256;                     // 128 features x 256 tokens
+typedef MmShape<4, 2, 4, 4> Gate128;                     // 128 x 128
+typedef MmShape<2, 2, 4, 4> Gate64;                      // 64 x 128, four wavefronts
+typedef MmShape<2, 2, 4, 2> Gate32;                      // 64 x 64
+
+template <class S, bool GRAD>
 int launch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
-  constexpr int kLds = kMmStages * (2 * kGateFeat + 32 * NJ) * kMmK * 2;
-  const hipError_t e = hipFuncSetAttribute((const void *)gate_kernel<NJ, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
+  constexpr int kLds = GateKernel<S>::Gate::kLds;
+  const hipError_t e = hipFuncSetAttribute((const void *)gate_kernel<S, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                            kLds);
   if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
-  const int64_t n = ceil_div(p.hidden, kGateFeat) * ceil_div(p.M, 32 * NJ);
+  const int64_t n = ceil_div(p.hidden, GateKernel<S>::kFeat) * ceil_div(p.M, S::kT);
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
-  hipLaunchKernelGGL((gate_kernel<NJ, GRAD>), dim3((unsigned)mm_grid(n)), dim3(kMmThreads), kLds, stream, p);
+  hipLaunchKernelGGL((gate_kernel<S, GRAD>), dim3((unsigned)mm_grid(n)), dim3(S::kThreads), kLds, stream, p);
   return launch_status(what);
+}
+
+// The largest tile of which there is one for each CU at least.
+template <bool GRAD>
+int dispatch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
+  const int64_t n128 = ceil_div(p.hidden, 128), n64 = ceil_div(p.hidden, 64), t128 = ceil_div(p.M, 128);
+  if constexpr (!GRAD)
+    if (n128 * ceil_div(p.M, 256) >= 256) return launch_gate<Gate256, GRAD>(p, stream, what);
+  if (n128 * t128 >= 256) return launch_gate<Gate128, GRAD>(p, stream, what);
+  if (n64 * t128 >= 256) return launch_gate<Gate64, GRAD>(p, stream, what);
+  return launch_gate<Gate32, GRAD>(p, stream, what);
 }
 
 int check_ffn(const char *what, const void *x, int64_t ldx, const void *w13, int64_t ldw13, const void *w2, int64_t ldw2,
@@ -228,50 +241,65 @@ int check_ffn(const char *what, const void *x, int64_t ldx, const void *w13, int
     return fail(SMLM_EUNSUPPORTED, "%s: M=%lld d=%lld hidden=%lld n_out=%lld too large", what, (long long)M, (long long)d,
                 (long long)hidden, (long long)n_out);
   if (ldx < d || ldw13 < d || ldw2 < hidden || ldx % 8 || ldw13 % 8 || ldw2 % 8 || std::max(std::max(ldx, ldw13), ldw2) >
-      (1 << 22) || ((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2) % 16)
-    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^22 elements (x %lld, "
+      kMmMaxStride || ((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2) % 16)
+    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^21 elements (x %lld, "
                 "w13 %lld, w2 %lld)", what, (long long)ldx, (long long)ldw13, (long long)ldw2);
   return SMLM_OK;
 }
 
-// out [T][F] = sum over k of tok[k][T] feat[k][F], k split over workgroups
-struct WeightGrad {
-  int64_t T, F, K, splits;
-  int64_t bytes() const { return splits > 1 ? splits * T * F * 4 : 0; }
+// The products besides the gate's: y over hidden, dx over a and b, the weights' gradients over the tokens.
+struct FfnPlan {
+  MmPlan y, dx, dw13, dw2;
+  int64_t act, parts_forward, parts_backward;             // bytes
 };
-WeightGrad weight_grad(int64_t T, int64_t F, int64_t K) { return {T, F, K, mm_splits(T, F, K, 256)}; }
+FfnPlan ffn_plan(int64_t M, int64_t d, int64_t hidden, int64_t n_out) {
+  FfnPlan p;
+  p.y = mm_plan(M, n_out, hidden, true);
+  p.dx = mm_plan(M, d, 2 * hidden, true);
+  p.dw13 = mm_plan(2 * hidden, d, M, true);
+  p.dw2 = mm_plan(n_out, hidden, M, true);
+  p.act = M * hidden * 2;
+  p.parts_forward = p.y.part_bytes(M, n_out);
+  p.parts_backward = std::max(p.dx.part_bytes(M, d), std::max(p.dw13.part_bytes(2 * hidden, d), p.dw2.part_bytes(n_out, hidden)));
+  return p;
+}
 
-int run_weight_grad(const WeightGrad &g, const void *tok, int64_t ldt, const void *feat, int64_t ldf, float *parts, void *out,
-                    hipStream_t s, const char *what) {
+// out [T][F] = sum over k of tok feat, contiguous
+MmArgs product(const void *feat, int64_t ldf, const void *tok, int64_t ldt, int64_t F, int64_t T, int64_t K, void *out) {
   MmArgs m{};
   m.feat = (const uint16_t *)feat;
   m.tok = (const uint16_t *)tok;
   m.ldf = ldf;
   m.ldt = ldt;
-  m.F = g.F;
-  m.T = g.T;
-  m.K = m.Kf = g.K;
-  m.f32 = g.splits > 1;
-  m.out = m.f32 ? (void *)parts : out;
-  m.ldo = g.F;
-  m.nsplit = g.splits;
-  m.k_per = mm_k_per(g.K, g.splits);
-  if (const int rc = mm_launch(m, false, false, s, what)) return rc;
-  return m.f32 ? mm_reduce_launch(parts, g.splits, g.T, g.F, nullptr, out, g.F, s, what) : SMLM_OK;
+  m.F = F;
+  m.T = T;
+  m.K = m.Kf = K;
+  m.out = out;
+  m.ldo = F;
+  return m;
 }
 
 }  // namespace
 }  // namespace smlm
 
+extern "C" int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out, int grad) {
+  using namespace smlm;
+  if (M < 1 || d < 1 || hidden < 1 || n_out < 1) return 0;
+  const FfnPlan p = ffn_plan(M, d, hidden, n_out);
+  return grad ? 3 * p.act + p.parts_backward : p.act + p.parts_forward;
+}
+
 extern "C" int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w13, int64_t w13_row_stride, const void *w2,
-                              int64_t w2_row_stride, int64_t M, int64_t d, int64_t hidden, int64_t n_out, void *act, void *y,
-                              void *stream) {
+                              int64_t w2_row_stride, int64_t M, int64_t d, int64_t hidden, int64_t n_out, void *y,
+                              void *workspace, int64_t workspace_bytes, void *stream) {
   using namespace smlm;
   const char *what = "smlm_gated_ffn";
   if (const int rc = check_ffn(what, x, x_row_stride, w13, w13_row_stride, w2, w2_row_stride, M, d, hidden, n_out)) return rc;
-  if (!act || !y || ((uintptr_t)act | (uintptr_t)y) % 16)
-    return fail(SMLM_EINVAL, "%s: act and y must be 16-byte aligned tensors", what);
+  if (!y || (uintptr_t)y % 16) return fail(SMLM_EINVAL, "%s: y must be a 16-byte aligned tensor", what);
   if (M == 0) return SMLM_OK;
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < smlm_gated_ffn_workspace(M, d, hidden, n_out, 0))
+    return fail(SMLM_EINVAL, "%s: the workspace needs %lld bytes, 16-byte aligned", what,
+                (long long)smlm_gated_ffn_workspace(M, d, hidden, n_out, 0));
   hipStream_t s = (hipStream_t)stream;
   GateArgs p{};
   p.x = (const uint16_t *)x;
@@ -281,31 +309,11 @@ extern "C" int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w
   p.M = M;
   p.d = d;
   p.hidden = hidden;
-  p.act = (uint16_t *)act;
-  const int64_t nf = ceil_div(hidden, kGateFeat);
-  const int rc = nf * ceil_div(M, 256) >= 384 ? launch_gate<8, false>(p, s, what)
-                 : nf * ceil_div(M, 128) >= 256 ? launch_gate<4, false>(p, s, what)
-                                                : launch_gate<2, false>(p, s, what);
-  if (rc) return rc;
-  MmArgs m{};
-  m.feat = (const uint16_t *)w2;
-  m.ldf = w2_row_stride;
-  m.tok = p.act;
-  m.ldt = hidden;
-  m.F = n_out;
-  m.T = M;
-  m.K = m.Kf = hidden;
-  m.out = y;
-  m.ldo = n_out;
-  m.nsplit = 1;
-  m.k_per = mm_k_per(hidden, 1);
-  return mm_launch(m, true, true, s, what);
-}
-
-extern "C" int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out) {
-  using namespace smlm;
-  if (M < 1 || d < 1 || hidden < 1 || n_out < 1) return 0;
-  return M * hidden * 6 + std::max(weight_grad(2 * hidden, d, M).bytes(), weight_grad(n_out, hidden, M).bytes());
+  p.act = (uint16_t *)workspace;
+  const FfnPlan plan = ffn_plan(M, d, hidden, n_out);
+  if (const int rc = dispatch_gate<false>(p, s, what)) return rc;
+  return mm_run(product(w2, w2_row_stride, p.act, hidden, n_out, M, hidden, y), true, true, plan.y,
+                (float *)((char *)workspace + plan.act), s, what);
 }
 
 extern "C" int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, const void *x, int64_t x_row_stride,
@@ -315,15 +323,15 @@ extern "C" int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, co
   using namespace smlm;
   const char *what = "smlm_gated_ffn_backward";
   if (const int rc = check_ffn(what, x, x_row_stride, w13, w13_row_stride, w2, w2_row_stride, M, d, hidden, n_out)) return rc;
-  if (!dy || dy_row_stride < n_out || dy_row_stride % 8 || dy_row_stride > (1 << 22) || (uintptr_t)dy % 16)
-    return fail(SMLM_EINVAL, "%s: dy must have 16-byte aligned rows with a stride from %lld to 2^22 elements", what,
+  if (!dy || dy_row_stride < n_out || dy_row_stride % 8 || dy_row_stride > kMmMaxStride || (uintptr_t)dy % 16)
+    return fail(SMLM_EINVAL, "%s: dy must have 16-byte aligned rows with a stride from %lld to 2^21 elements", what,
                 (long long)n_out);
   if ((!dx && !dw13 && !dw2) || ((uintptr_t)dx | (uintptr_t)dw13 | (uintptr_t)dw2) % 16)
     return fail(SMLM_EINVAL, "%s: dx, dw13 and dw2 must be 16-byte aligned, one of them at least given", what);
   if (M < 1) return fail(SMLM_EINVAL, "%s: no tokens", what);
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < smlm_gated_ffn_workspace(M, d, hidden, n_out))
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < smlm_gated_ffn_workspace(M, d, hidden, n_out, 1))
     return fail(SMLM_EINVAL, "%s: the workspace needs %lld bytes, 16-byte aligned", what,
-                (long long)smlm_gated_ffn_workspace(M, d, hidden, n_out));
+                (long long)smlm_gated_ffn_workspace(M, d, hidden, n_out, 1));
   hipStream_t s = (hipStream_t)stream;
   GateArgs p{};
   p.x = (const uint16_t *)x;
@@ -341,27 +349,17 @@ extern "C" int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, co
   p.act = (uint16_t *)workspace;
   p.dab = p.act + M * hidden;
   float *parts = (float *)(p.dab + 2 * M * hidden);
-  const int64_t nf = ceil_div(hidden, kGateFeat);
-  if (const int rc = nf * ceil_div(M, 128) >= 256 ? launch_gate<4, true>(p, s, what) : launch_gate<2, true>(p, s, what))
-    return rc;
-  if (dx) {
-    MmArgs m{};
-    m.feat = p.w13;
-    m.ldf = p.ldw13;
-    m.tok = p.dab;
-    m.ldt = 2 * hidden;
-    m.F = d;
-    m.T = M;
-    m.K = m.Kf = 2 * hidden;
-    m.out = dx;
-    m.ldo = d;
-    m.nsplit = 1;
-    m.k_per = mm_k_per(m.K, 1);
-    if (const int rc = mm_launch(m, false, true, s, what)) return rc;
-  }
-  if (dw13)
-    if (const int rc = run_weight_grad(weight_grad(2 * hidden, d, M), p.dab, 2 * hidden, x, x_row_stride, parts, dw13, s, what))
+  if (const int rc = dispatch_gate<true>(p, s, what)) return rc;
+  const FfnPlan plan = ffn_plan(M, d, hidden, n_out);
+  if (dx)
+    if (const int rc = mm_run(product(w13, w13_row_stride, p.dab, 2 * hidden, d, M, 2 * hidden, dx), false, true, plan.dx, parts,
+                              s, what))
       return rc;
-  if (dw2) return run_weight_grad(weight_grad(n_out, hidden, M), dy, dy_row_stride, p.act, hidden, parts, dw2, s, what);
+  if (dw13)
+    if (const int rc = mm_run(product(x, x_row_stride, p.dab, 2 * hidden, d, 2 * hidden, M, dw13), false, false, plan.dw13,
+                              parts, s, what))
+      return rc;
+  if (dw2)
+    return mm_run(product(p.act, hidden, dy, dy_row_stride, hidden, n_out, M, dw2), false, false, plan.dw2, parts, s, what);
   return SMLM_OK;
 }

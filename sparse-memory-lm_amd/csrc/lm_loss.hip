@@ -23,7 +23,7 @@
 namespace smlm {
 namespace {
 
-constexpr int kLsCols = 128;                              // vocabulary columns per tile
+constexpr int kLsCols = 256;                              // vocabulary columns per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kLsFinishRows = 16;                         // tokens per workgroup of the joining kernel
 constexpr int64_t kLsPieceBytes = 512LL << 20;            // most bytes of one piece's G
@@ -36,8 +36,8 @@ struct LossArgs {
   int64_t ldx, ldw, M, d, v0, v1, V;                      // vocabulary columns [v0, v1) of V
   const int64_t *targets;
   int64_t ignore;
-  int nsplit, tiles;                                      // ranges of the vocabulary, and its 128-column tiles
-  float2 *parts;                                          // forward: (maximum, sum) [M][2 nsplit]
+  int nsplit, tiles;                                      // ranges of the vocabulary, and its tiles of columns
+  float2 *parts;                                          // forward: (maximum, sum) [M][nsplit][wavefronts over a tile]
   float *picked;                                          // forward: the target's logit [M]
   const float *lse, *coef, *grad, *count;                 // gradient: coef per token, or null; grad and count: see below
   float *scale;                                           // gradient: *grad / *count (count null: *grad), written here
@@ -45,23 +45,37 @@ struct LossArgs {
   int64_t ldg;
 };
 
-template <int NJ, bool GRAD>
-__global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
-  constexpr int NI = 4;
-  typedef MmTile<kLsCols, true, 16> FT;
-  typedef MmTile<32 * NJ, true, 0> TT;
-  typedef MmLoop<FT, TT, NI, NJ> Loop;
+// Eight wavefronts, 256 columns: of 256 tokens, each wavefront 128 x 64 (fewer tokens a lane: fewer running maxima), of 128 or
+// 64, each 64 x 64 or 64 x 32.
+typedef MmShape<2, 4, 8, 4> Tokens256;
+typedef MmShape<4, 2, 4, 4> Tokens128;
+typedef MmShape<4, 2, 4, 2> Tokens64;
+
+template <class S>
+struct LossKernel {
+  typedef MmTile<S::kF, true, 4 * S::NI, S::kThreads, 64> F;
+  typedef MmTile<S::kT, true, 0, S::kThreads, 64> T;
+  typedef MmLoop<F, T, S::NI, S::NJ> Loop;
+};
+
+template <class S, bool GRAD>
+__global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
+  static_assert(S::kF == kLsCols, "columns");
+  constexpr int NI = S::NI, NJ = S::NJ, C = 4 * NI;       // C columns of a token per lane
+  typedef typename LossKernel<S>::F FT;
+  typedef typename LossKernel<S>::T TT;
+  typedef typename LossKernel<S>::Loop Loop;
   extern __shared__ __align__(16) unsigned char smem[];
-  const unsigned nt = (unsigned)((a.M + TT::kRows - 1) / TT::kRows);
+  const unsigned nt = (unsigned)((a.M + S::kT - 1) / S::kT);
   if (GRAD && blockIdx.x == 0 && threadIdx.x == 0 && a.grad)   // for the products that follow
     *a.scale = a.count ? (*a.count > 0.f ? *a.grad / *a.count : 0.f) : *a.grad;
   const int unit = mm_tile_of(blockIdx.x, nt * a.nsplit);
   if (unit < 0) return;  // workgroup-uniform
   // the token tiles of one range are neighbours: an XCD reads its ranges of W from memory once
   const int split = unit / nt;
-  const int64_t t0 = (int64_t)(unit - split * nt) * TT::kRows;
+  const int64_t t0 = (int64_t)(unit - split * nt) * S::kT;
   const int first = (int)((int64_t)a.tiles * split / a.nsplit), last = (int)((int64_t)a.tiles * (split + 1) / a.nsplit);
-  const int wave = threadIdx.x / kWave, wf = (wave & 1) * 16 * NI, wt = (wave >> 1) * 16 * NJ;
+  const int wave = threadIdx.x / kWave, wf = S::feature(wave), wt = S::token(wave);
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
 
   int target[NJ];                     // column in [v0, ..), kNoTarget: not in this piece or none
@@ -72,30 +86,30 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
     const int64_t y = t < a.M ? a.targets[t] : a.ignore;
     const bool valid = y != a.ignore && y >= a.v0 && y < a.v1;
     target[j] = valid ? (int)(y - a.v0) : kNoTarget;
-    m[j] = -__builtin_inff();
+    m[j] = GRAD ? __builtin_inff() : -__builtin_inff();   // gradient, an ignored token: every probability is 0
     l[j] = c[j] = 0.f;
-    if (GRAD && t < a.M) {
-      m[j] = a.lse[t];
+    if (GRAD && t < a.M && y != a.ignore) {
       // an index outside the vocabulary makes its token's gradient NaN, as its loss
-      c[j] = y == a.ignore ? 0.f : y < 0 || y >= a.V ? __builtin_nanf("") : a.coef ? a.coef[t] : 1.f;
+      m[j] = y < 0 || y >= a.V ? __builtin_nanf("") : a.lse[t];
+      if (a.coef) c[j] = a.coef[t];
     }
   }
 
   Loop L;
   L.init(smem, a.ldw, a.ldx, wf, wt);
-  const int nch = mm_chunks(a.d);
-  // the loads run three chunks ahead of the products, over the ends of tiles (past the last tile they load what is not used)
+  // the loads run two stages ahead of the products, over the ends of tiles (past the last tile they load what is not used)
+  const int units = mm_units(a.d);
   int ahead_tile = first, ahead = 0;
   MmSource<FT> fs;
   MmSource<TT> ts;
   auto begin_tile = [&]() {
     fs.init(a.w, a.ldw, a.V, a.d, a.v0 + (int64_t)ahead_tile * kLsCols, 0);
     ts.init(a.x, a.ldx, a.M, a.d, t0, 0);
-    if (a.d % kMmK) L.offsets(a.ldw, a.ldx);             // the last chunks' clipped them
+    if (a.d % kMmUnit) L.offsets(a.ldw, a.ldx);          // the last stage's clipped them
     ahead = 0;
   };
   auto loaded = [&]() {
-    if (++ahead == nch) {
+    if (++ahead == units) {
       ++ahead_tile;
       begin_tile();
     }
@@ -105,24 +119,22 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
   uint32_t stage = 0;
   begin_tile();
   if (first < last) {
-    for (int q = 0; q < 3; ++q) {
-      L.issue(fs, ts, q * Loop::kStage);
-      loaded();
-    }
-    mm_wait_barrier<2 * Loop::kLoads>();
-    L.read(x, 0);
+    L.issue(fs, ts, 0);
+    loaded();
+    L.issue(fs, ts, Loop::kStage);
+    loaded();
+    mm_wait_barrier<Loop::kLoads>();
+    L.read(x, 0, 0);
   }
   for (int tile = first; tile < last; ++tile) {
     mm_zero(acc);
-    for (int ch = 0; ch < nch; ch += 2) {
-      L.step(fs, ts, x, y, stage, acc);
-      loaded();
-      L.step(fs, ts, y, x, stage, acc);
+    for (int u = 0; u < units; ++u) {
+      L.multiply(fs, ts, x, y, stage, acc);
       loaded();
     }
 
-    // lane (r, g): columns c0 .. c0 + 15 of token r of each 16
-    const int c0 = tile * kLsCols + wf + 16 * g;
+    // lane (r, g): columns c0 .. c0 + C - 1 of token r of each 16
+    const int c0 = tile * kLsCols + wf + C * g;
     const int64_t end = (GRAD ? a.v1 : a.V) - a.v0;
     if ((int64_t)(tile + 1) * kLsCols > end) {          // columns past the end count for nothing
       const int valid = (int)(end - c0);
@@ -137,43 +149,50 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
     for (int j = 0; j < NJ; ++j) {
       const unsigned rel = (unsigned)(target[j] - c0);
       if constexpr (!GRAD) {
-        if (__any(rel < 16u)) {                         // about one 16-token group in 50 at 50,304 columns
+        if (__any(rel < (unsigned)C)) {                   // rare: 64 of the vocabulary's columns for 16 tokens
           float v = 0.f;
 #pragma unroll
-          for (int q = 0; q < 16; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
-          if (rel < 16u) a.picked[t0 + wt + 16 * j + r] = v;
+          for (int q = 0; q < C; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
+          if (rel < (unsigned)C) a.picked[t0 + wt + 16 * j + r] = v;
         }
         float top = m[j];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[q / 4][j][q % 4]);
+        for (int q = 0; q < C; ++q) top = fmaxf(top, acc[q / 4][j][q % 4]);
+        // the difference first: a logit that is the maximum counts exactly 1, so that no loss is below 0
         const float ref = top == -__builtin_inff() ? 0.f : top;   // nothing yet: every exponential is 0
-        float sum = l[j] * exp2_hw((m[j] - ref) * kLog2e);
+        float sum = l[j] * exp2_hw((m[j] - ref) * kLog2e), more = 0.f;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) sum += exp2_hw((acc[q / 4][j][q % 4] - ref) * kLog2e);
+        for (int q = 0; q < C; q += 2) {
+          sum += exp2_hw((acc[q / 4][j][q % 4] - ref) * kLog2e);
+          more += exp2_hw((acc[q / 4][j][q % 4 + 1] - ref) * kLog2e);
+        }
         m[j] = top;
-        l[j] = sum;
+        l[j] = sum + more;
       } else {
         const int64_t t = t0 + wt + 16 * j + r;
-        float p[16];
+        float p[C];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) p[q] = exp2_hw((acc[q / 4][j][q % 4] - m[j]) * kLog2e);
-        if (__any(rel < 16u)) {
+        for (int q = 0; q < C; ++q) p[q] = exp2_hw((acc[q / 4][j][q % 4] - m[j]) * kLog2e);
+        if (__any(rel < (unsigned)C)) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q) p[q] = rel == (unsigned)q ? p[q] - 1.f : p[q];
+          for (int q = 0; q < C; ++q) p[q] = rel == (unsigned)q ? p[q] - 1.f : p[q];
         }
-        uint32_t o[8];
+        if (a.coef) {                                     // uniform
 #pragma unroll
-        for (int q = 0; q < 8; ++q) o[q] = c[j] == 0.f ? 0u : pack_bf16x2(p[2 * q] * c[j], p[2 * q + 1] * c[j]);
+          for (int q = 0; q < C; ++q) p[q] *= c[j];
+        }
         if (t < a.M) {
           uint4 *out = (uint4 *)(a.g + t * a.ldg + c0);
-          out[0] = uint4{o[0], o[1], o[2], o[3]};
-          out[1] = uint4{o[4], o[5], o[6], o[7]};
+#pragma unroll
+          for (int q = 0; q < C / 8; ++q)
+            out[q] = uint4{pack_bf16x2(p[8 * q], p[8 * q + 1]), pack_bf16x2(p[8 * q + 2], p[8 * q + 3]),
+                           pack_bf16x2(p[8 * q + 4], p[8 * q + 5]), pack_bf16x2(p[8 * q + 6], p[8 * q + 7])};
         }
       }
     }
   }
 
-  __builtin_amdgcn_s_waitcnt(0x0F70);                    // no load is on its way into LDS when the workgroup ends
+  mm_finish();
   if constexpr (!GRAD) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -185,7 +204,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) loss_kernel(LossArgs a) {
         m[j] = top;
       }
       const int64_t t = t0 + wt + 16 * j + r;
-      if (g == 0 && t < a.M) a.parts[t * 2 * a.nsplit + 2 * split + (wave & 1)] = make_float2(m[j], l[j]);
+      if (g == 0 && t < a.M) a.parts[(t * a.nsplit + split) * S::WF + wave % S::WF] = make_float2(m[j], l[j]);
     }
   }
 }
@@ -262,38 +281,41 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict
   }
 }
 
-template <int NJ, bool GRAD>
+template <class S, bool GRAD>
 int launch_loss(LossArgs a, hipStream_t stream, const char *what) {
-  constexpr int kLds = kMmStages * (kLsCols + 32 * NJ) * kMmK * 2;
-  const hipError_t e = hipFuncSetAttribute((const void *)loss_kernel<NJ, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
+  constexpr int kLds = LossKernel<S>::Loop::kLds;
+  const hipError_t e = hipFuncSetAttribute((const void *)loss_kernel<S, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                            kLds);
   if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
-  const int64_t n = ceil_div(a.M, 32 * NJ) * a.nsplit;
+  const int64_t n = ceil_div(a.M, S::kT) * a.nsplit;
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
-  hipLaunchKernelGGL((loss_kernel<NJ, GRAD>), dim3((unsigned)mm_grid(n)), dim3(kMmThreads), kLds, stream, a);
+  hipLaunchKernelGGL((loss_kernel<S, GRAD>), dim3((unsigned)mm_grid(n)), dim3(S::kThreads), kLds, stream, a);
   return launch_status(what);
 }
 
-// Tokens of a tile: 16 NJ per wavefront.
-int tile_nj(int64_t M) { return M > 128 ? 8 : M > 64 ? 4 : 2; }
+// Tokens of a tile, and its wavefronts over the columns (each leaves its own maximum and sum).
+int tile_tokens(int64_t M) { return M > 128 ? 256 : M > 64 ? 128 : 64; }
+int tile_parts(int64_t M) { return M > 128 ? Tokens256::WF : Tokens128::WF; }
 
 template <bool GRAD>
 int dispatch_loss(const LossArgs &a, hipStream_t stream, const char *what) {
-  switch (tile_nj(a.M)) {
-    case 8: return launch_loss<8, GRAD>(a, stream, what);
-    case 4: return launch_loss<4, GRAD>(a, stream, what);
-    default: return launch_loss<2, GRAD>(a, stream, what);
+  switch (tile_tokens(a.M)) {
+    case 256: return launch_loss<Tokens256, GRAD>(a, stream, what);
+    case 128: return launch_loss<Tokens128, GRAD>(a, stream, what);
+    default: return launch_loss<Tokens64, GRAD>(a, stream, what);
   }
 }
 
-// Ranges of `tiles` vocabulary tiles: two workgroups for each CU, all of them at once on the card.
+// Ranges of `tiles` vocabulary tiles: one workgroup for each CU, all of them at once on the card.
 int range_count(int64_t M, int64_t tiles) {
-  const int64_t nt = ceil_div(M, 32 * tile_nj(M));
-  return (int)std::min<int64_t>(tiles, std::max<int64_t>(1, 512 / nt));
+  const int64_t nt = ceil_div(M, tile_tokens(M));
+  return (int)std::min<int64_t>(tiles, std::max<int64_t>(1, 256 / nt));
 }
+int64_t part_count(int64_t M, int64_t V) { return (int64_t)tile_parts(M) * range_count(M, ceil_div(V, kLsCols)); }
 
 struct GradPlan {
-  int64_t cols, pieces, splits, g_bytes, part_bytes;
+  int64_t cols, pieces, g_bytes, part_bytes;
+  MmPlan dx, dw;
 };
 GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
   GradPlan p;
@@ -301,9 +323,10 @@ GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
   p.pieces = ceil_div(V, most);
   p.cols = ceil_div(ceil_div(V, p.pieces), kLsCols) * kLsCols;
   p.pieces = ceil_div(V, p.cols);
-  p.splits = mm_splits(M, d, p.cols, 512);
+  p.dx = mm_plan(M, d, p.cols, true);
+  p.dw = mm_plan(p.cols, d, M, false);
   p.g_bytes = M * p.cols * 2;
-  p.part_bytes = p.pieces * p.splits > 1 ? p.splits * M * d * 4 : 0;
+  p.part_bytes = p.pieces * p.dx.splits > 1 ? p.dx.splits * M * d * 4 : 0;
   return p;
 }
 
@@ -316,9 +339,9 @@ int check_loss(const char *what, const void *x, int64_t x_stride, const void *w,
   if (V > (1 << 30) || d > (1 << 20) || M > (1LL << 36) / d)
     return fail(SMLM_EUNSUPPORTED, "%s: M=%lld V=%lld d=%lld too large", what, (long long)M, (long long)V, (long long)d);
   // the lanes' 32-bit byte offsets span 256 rows
-  if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > (1 << 22) || w_stride > (1 << 22) ||
+  if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > kMmMaxStride || w_stride > kMmMaxStride ||
       ((uintptr_t)x | (uintptr_t)w) % 16 || (uintptr_t)targets % 8)
-    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^22 elements (x %lld, "
+    return fail(SMLM_EINVAL, "%s: rows must be 16-byte aligned with strides from their widths to 2^21 elements (x %lld, "
                 "weight %lld)", what, (long long)x_stride, (long long)w_stride);
   return SMLM_OK;
 }
@@ -334,7 +357,7 @@ extern "C" int64_t smlm_linear_ce_workspace(int64_t M, int64_t V, int64_t d, int
     return 256 + p.g_bytes + p.part_bytes;
   }
   // (maximum, sum) of every range, the picked logits, and the partial sums of the losses
-  return M * 2 * range_count(M, ceil_div(V, kLsCols)) * 8 + ceil_div(M, 4) * 16 + ceil_div(M, kLsFinishRows) * 16;
+  return M * part_count(M, V) * 8 + 8 + ceil_div(M, 4) * 16 + ceil_div(M, kLsFinishRows) * 16;
 }
 
 extern "C" int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w_row_stride,
@@ -366,13 +389,13 @@ extern "C" int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w
   a.nsplit = range_count(M, a.tiles);
   char *ws = (char *)workspace;
   a.parts = (float2 *)ws;
-  ws += M * 2 * a.nsplit * 8;
+  ws += (M * part_count(M, V) * 8 + 15) / 16 * 16;
   a.picked = (float *)ws;
   double *sums = reduction == SMLM_REDUCE_NONE ? nullptr : (double *)(ws + ceil_div(M, 4) * 16);
   if (const int rc = dispatch_loss<false>(a, s, what)) return rc;
   const int64_t blocks = ceil_div(M, kLsFinishRows);
   if (blocks > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: M=%lld too large", what, (long long)M);
-  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a.parts, 2 * a.nsplit, a.picked, targets,
+  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a.parts, (int)part_count(M, V), a.picked, targets,
                      ignore_index, M, V, lse, reduction == SMLM_REDUCE_NONE ? loss : nullptr, sums);
   if (const int rc = launch_status(what)) return rc;
   if (!sums) return SMLM_OK;
@@ -434,11 +457,9 @@ extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, in
       m.f32 = p.part_bytes > 0;
       m.out = m.f32 ? (void *)parts : dx;
       m.ldo = d;
-      m.nsplit = p.splits;
-      m.k_per = mm_k_per(m.K, p.splits);
       m.scale = scale;
       m.accumulate = piece > 0;
-      if (const int rc = mm_launch(m, false, true, s, what)) return rc;
+      if (const int rc = mm_launch(m, false, true, p.dx, s, what)) return rc;
     }
     if (dw) {   // the sum over the tokens
       MmArgs m{};
@@ -451,12 +472,10 @@ extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, in
       m.T = n;
       m.out = (uint16_t *)dw + a.v0 * d;
       m.ldo = d;
-      m.nsplit = 1;
-      m.k_per = mm_k_per(M, 1);
       m.scale = scale;
-      if (const int rc = mm_launch(m, false, false, s, what)) return rc;
+      if (const int rc = mm_launch(m, false, false, p.dw, s, what)) return rc;
     }
   }
-  if (dx && p.part_bytes > 0) return mm_reduce_launch(parts, p.splits, M, d, scale, dx, d, s, what);
+  if (dx && p.part_bytes > 0) return mm_reduce_launch(parts, p.dx.splits, M, d, scale, dx, d, s, what);
   return SMLM_OK;
 }

@@ -1,24 +1,27 @@
 // The K loop of the training step's products on the matrix cores (v_mfma_f32_16x16x32_bf16, fp32 sums): a tile of
-// TT rows ("tokens") x FT columns ("features") from two bf16 operands, each of which may have the summed dimension k
+// kT rows ("tokens") x kF columns ("features") from two bf16 operands, each of which may have the summed dimension k
 // contiguous (rows of k: a linear layer's input and weight) or strided (rows of tokens or features, k the slow dimension:
 // the operands of a weight's gradient).
 //
-// Workgroup = 4 wavefronts, WF x WT of them over the tile, 16 NI features x 16 NJ tokens each.  At the matrix cores' rate a
-// wavefront's tile of 64 features x 128 tokens reads 96 of the 128 bytes per clock that the LDS has, one of 64 x 64 all
-// of them: hence 128 x 256 tiles where there are enough of them.
-// k streams through three LDS stages of 32, loaded straight from memory into LDS (buffer_load ... lds, no registers in
-// between).  While a chunk is multiplied, the next one's fragments are read into a second set of registers and the chunk
-// three ahead is loaded into the stage that the first came from (which all wavefronts have read by the barrier that opens
-// the step), the reads and loads spread between the products: neither LDS nor memory latency stands between two chunks'
-// products.  The number of chunks is even, so that the two register sets alternate without copies.  A stage takes 24 KB for
-// 128 x 256, so that two workgroups fit a CU: one's epilogue runs under the other's products.
+// Workgroup = WF x WT wavefronts over the tile, 16 NI features x 16 NJ tokens each.  What bounds the loop is the way from
+// the vector cache into LDS, 64 bytes per clock and CU: a chunk of 32 k takes (kF + kT) clocks of it and kF kT / 64 of the
+// matrix cores.  Hence tiles of 256 x 256 or 384 x 128 where there are enough of them (half and two thirds of the products'
+// time; 128 x 128 takes all of it), by eight wavefronts, two per SIMD, one workgroup a CU; and rows of 64 k, whole cache
+// lines, where k is contiguous (rows of 32 k: 900 TFLOP/s on 8,192 cubed with both operands so, 1,260 with neither).
 //
-// LDS layouts (16-byte pieces; banks repeat every 256 bytes):
-//   k contiguous: 64-byte rows, piece c of row R at c ^ swz(R), so that the 16 rows of a fragment read fall on distinct
-//     banks; read with ds_read_b128.  Feature rows are read permuted (lane r of tile i takes row 4 NI (r / 4) + 4 i +
-//     r % 4), which leaves each lane 4 NI consecutive features of a token in its accumulators: 32-byte stores.
-//   k strided: rows of 32 k, piece c of row k at c ^ v(k), read with ds_read_b64_tr_b16, which gives lane r four k of
-//     column r.  Lane group g takes k = 8 g .. 8 g + 7 in both layouts.
+// k streams through LDS, loaded straight from memory (buffer_load ... lds, no registers in between), in stages of 64 k (two
+// of them) or 32 (three, for products without long contiguous rows on both sides), and is multiplied in steps of 32.  While
+// a step's products run, the next step's fragments are read into a second set of registers; behind the barrier before a
+// stage's last step, by which all wavefronts have read the stage, a later one is loaded into it, the loads spread between
+// the step's products.  Neither LDS nor memory latency stands between two steps' products.
+//
+// LDS layouts (16-byte pieces; 64 banks, 256 bytes; ds_read_b128 serves lanes 0-3, 12-15 and 20-27 of each 32 together,
+// then the others):
+//   k contiguous: 128-byte rows, piece c of row R at c ^ swz(R), so that the lanes served together fall on distinct banks.
+//     Feature rows may be read permuted (lane r of tile i takes row 4 NI (r / 4) + 4 i + r % 4), which leaves each lane 4 NI
+//     consecutive features of a token in its accumulators: whole 32-byte stores.
+//   k strided: rows of kF or kT, piece c of row k at c ^ vsw(k), read with ds_read_b64_tr_b16, which gives lane r four k of
+//     column r.  Lane group g takes k = 8 g .. 8 g + 7 of a step in both layouts.
 // Out of range rows and k read as zeros (the buffer's record count; the k beyond the end of contiguous rows by an offset
 // out of range), so tails need no other care than not storing what lies outside.
 #pragma once
@@ -33,10 +36,11 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
-constexpr int kMmThreads = 256, kMmK = 32, kMmStages = 3, kMmXcds = 8;
+constexpr int kMmStep = 32, kMmUnit = 64, kMmXcds = 8;    // k of a step; sums are padded with zeros to whole units
+constexpr int kMmMaxStride = 1 << 21;         // elements: a tile's byte offsets stay below 2^31
 
 // 16 bytes per lane from a buffer straight into LDS at lds + 16 * lane (wave-uniform lds).  Inline assembly, so that the
-// compiler adds no wait for it before every LDS read; the kernels wait themselves (mm_wait).
+// compiler adds no wait for it before every LDS read; the kernels wait themselves (mm_wait_barrier).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void mm_load_lds(intx4 rsrc, uint32_t voff, uint32_t lds) {
@@ -46,7 +50,7 @@ __device__ __forceinline__ void mm_load_lds(intx4 rsrc, uint32_t voff, uint32_t 
 #pragma clang diagnostic pop
 
 // At most N vector memory operations on their way and every LDS read done; then the barrier.  Loads complete in order:
-// with N = the loads issued after a chunk's, that chunk has landed.
+// with N = the loads issued after a stage's, that stage has landed.
 template <int N>
 __device__ __forceinline__ void mm_wait_barrier() {
   asm volatile("" ::: "memory");
@@ -54,62 +58,82 @@ __device__ __forceinline__ void mm_wait_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// No load is on its way into LDS when the workgroup ends.
+__device__ __forceinline__ void mm_finish() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 constexpr uint32_t kMmOutside = 0xFFFFFFF0u;  // an offset that no record count reaches
 
-// One operand's LDS tile of ROWS rows (tokens or features) x 32 k.  PERM: features per lane group (4 NI) of a permuted
+template <int WF_, int WT_, int NI_, int NJ_>
+struct MmShape {
+  static constexpr int WF = WF_, WT = WT_, NI = NI_, NJ = NJ_;
+  static constexpr int kThreads = 64 * WF * WT, kF = 16 * WF * NI, kT = 16 * WT * NJ;
+  // the wavefront's first feature and token in the tile
+  static __device__ __forceinline__ int feature(int wave) { return wave % WF * 16 * NI; }
+  static __device__ __forceinline__ int token(int wave) { return wave / WF * 16 * NJ; }
+};
+
+// One operand's LDS tile of ROWS rows (tokens or features) x K k (32 or 64).  PERM: features per lane group of a permuted
 // fragment, 0 for a plain one.
-template <int ROWS, bool KC, int PERM>
+template <int ROWS, bool KC, int PERM, int THREADS, int K>
 struct MmTile {
   static constexpr bool kContiguous = KC;
-  static constexpr int kRows = ROWS, kBytes = ROWS * kMmK * 2;
-  static constexpr int kLoads = kBytes / 4096;                       // per thread and chunk
-  static constexpr int kRowBytes = KC ? kMmK * 2 : ROWS * 2;
-  static constexpr int kRowsPerLoad = 4096 / kRowBytes;              // LDS rows that one load of the workgroup fills
-  static_assert(kBytes % 4096 == 0, "a whole number of loads");
+  static constexpr int kK = K, kRows = ROWS, kBytes = ROWS * K * 2, kPerLoad = THREADS * 16;
+  static constexpr int kLoads = kBytes / kPerLoad;                   // per thread and stage
+  static constexpr int kRowBytes = KC ? K * 2 : ROWS * 2;
+  static_assert(kBytes % kPerLoad == 0, "a whole number of loads");
 
   static __device__ __forceinline__ int swz(int row) {               // KC
-    return -(PERM ? row / PERM : row / 4) & 3;
+    if constexpr (K == 32) return -(PERM ? row / PERM : row / 4) & 3;
+    else return PERM ? (row >> 1 & 1) | (row / PERM & 3) << 1 : row >> 1 & 7;
   }
   static __device__ __forceinline__ int vsw(int k) {                 // k strided
-    return ROWS >= 128 ? 2 * ((k & 3) | ((k >> 3 & 1) << 2)) : 2 * ((k >> 1 & 1) | ((k >> 3 & 1) << 1));
+    return ROWS % 128 == 0 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 2 * ((k >> 1 & 1) | (k >> 3 & 1) << 1);
   }
 
-  // This thread's byte offset of load u from the chunk's first byte.
+  // This thread's byte offset of load u from the stage's first byte in memory; its first k (KC).
   static __device__ __forceinline__ uint32_t offset(int u, int tid, int64_t ld) {
-    if constexpr (KC) {
-      return (uint32_t)((u * kRowsPerLoad + tid / 4) * ld * 2 + first_k(tid) * 2);
-    } else {
-      const int per = kRowBytes / 16, k = u * kRowsPerLoad + tid / per;
-      return (uint32_t)(k * ld * 2 + (((tid % per) ^ vsw(k)) * 16));
-    }
+    const int at = u * kPerLoad + tid * 16, row = at / kRowBytes, c = at % kRowBytes / 16;
+    if constexpr (KC) return (uint32_t)(row * ld * 2 + (c ^ swz(row)) * 16);
+    else return (uint32_t)(row * ld * 2 + (c ^ vsw(row)) * 16);
   }
-  static __device__ __forceinline__ int first_k(int tid) { return 8 * ((tid % 4) ^ swz(tid / 4)); }   // KC
-  // LDS address (from the tile's base) that lane (r, g) reads the wavefront's row group i from, its rows starting at w0.
-  static __device__ __forceinline__ uint32_t frag_at(int w0, int i, int r, int g) {
-    if constexpr (KC) {                       // w0 a multiple of 4 * PERM or 16: the swizzle is that of i = 0
-      const int R = PERM ? w0 + PERM * (r / 4) + r % 4 : w0 + r;
-      return R * kRowBytes + ((g ^ swz(R)) * 16) + i * (PERM ? 4 : 16) * kRowBytes;
-    } else {
-      const int k = 8 * g + r / 4;
-      const int col = PERM ? w0 + PERM * (r % 4) + 4 * i : w0 + 16 * i + 4 * (r % 4);
-      return k * kRowBytes + (((col / 8) ^ vsw(k)) * 16) + (col % 8) * 2;
-    }
+  static __device__ __forceinline__ int first_k(int u, int tid) {
+    const int at = u * kPerLoad + tid * 16;
+    return 8 * (at % kRowBytes / 16 ^ swz(at / kRowBytes));
   }
-  static __device__ __forceinline__ bf16x8 frag(uint32_t at) {
+
+  // LDS address (from the tile's base) that lane (r, g) reads the wavefront's row group i from, its rows starting at w0,
+  // in step h (0, 1) of the stage.  KC: i only adds to it; k strided: h does.
+  static __device__ __forceinline__ uint32_t at_contiguous(int w0, int h, int r, int g) {
+    const int R = PERM ? w0 + PERM * (r / 4) + r % 4 : w0 + r;       // w0 a multiple of 4 PERM or 16
+    return R * kRowBytes + (((K == 32 ? 0 : 4 * h) + g) ^ swz(R)) * 16;
+  }
+  static __device__ __forceinline__ uint32_t at_strided(int w0, int i, int r, int g) {
+    const int k = 8 * g + r / 4;
+    const int col = PERM ? w0 + PERM * (r % 4) + 4 * i : w0 + 16 * i + 4 * (r % 4);
+    return k * kRowBytes + (col / 8 ^ vsw(k)) * 16 + col % 8 * 2;
+  }
+  template <int N>
+  static __device__ __forceinline__ void addresses(uint32_t (&a)[N], uint32_t base, int w0, int r, int g) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = base + (KC ? at_contiguous(w0, i & 1, r, g) : at_strided(w0, i, r, g));
+  }
+  // Row group i, step h, of the stage at byte `stage`, from the addresses above (KC uses the first two).
+  template <int N>
+  static __device__ __forceinline__ bf16x8 frag(const uint32_t (&a)[N], int i, int h, uint32_t stage) {
     if constexpr (KC) {
-      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)at;
+      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)(a[h] + stage + i * (PERM ? 4 : 16) * kRowBytes);
     } else {
       typedef __attribute__((address_space(3))) bf16x4 *p4;
-      const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)at);
-      const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(at + 4 * kRowBytes));
-      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      const uint32_t at = a[i] + stage + h * 32 * kRowBytes;
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)at);
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((p4)(uintptr_t)(at + 4 * kRowBytes));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 };
 
-// Where an operand's next chunk comes from: wave-uniform, stepped from chunk to chunk.  `left` is exact: the bytes from the
-// chunk's first to the operand's last, which the record count of its loads is clipped to: past the end they read zeros.
+// Where an operand's next stage comes from: wave-uniform, stepped from stage to stage.  `left` is exact: the bytes from the
+// stage's first to the operand's last, which the record count of its loads is clipped to: past the end they read zeros.
 template <class O>
 struct MmSource {
   const uint16_t *p;
@@ -119,7 +143,7 @@ struct MmSource {
     const int64_t major = O::kContiguous ? row0 : k0, minor = O::kContiguous ? k0 : row0;
     p = base + major * ld + minor;
     left = (((O::kContiguous ? rows : K) - 1 - major) * ld + (O::kContiguous ? K : rows) - minor) * 2;
-    step = O::kContiguous ? kMmK * 2 : kMmK * 2 * ld;
+    step = O::kContiguous ? O::kK * 2 : O::kK * 2 * ld;
     k = K - k0;
   }
   __device__ __forceinline__ intx4 rsrc() const {
@@ -130,7 +154,7 @@ struct MmSource {
   __device__ __forceinline__ void next() {
     p += step / 2;
     left -= step;
-    k -= kMmK;
+    k -= O::kK;
   }
 };
 
@@ -139,12 +163,15 @@ struct MmFrags {
   bf16x8 a[NI], b[NJ];
 };
 
-// The loop's state of one thread for an F tile of features and a T tile of tokens: a stage holds F, then T.
+// The loop's state of one thread for a feature tile F and a token tile T: a stage holds F, then T.
 template <class F, class T, int NI, int NJ>
 struct MmLoop {
-  static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads;
+  static_assert(F::kK == T::kK, "one stage");
+  static constexpr int kK = F::kK, kStages = kK == 32 ? 3 : 2;
+  static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads, kLds = kStages * kStage;
+  static constexpr int kFa = F::kContiguous ? 2 : NI, kTa = T::kContiguous ? 2 : NJ;
   typedef MmFrags<NI, NJ> Frags;
-  uint32_t fo[F::kLoads], to[T::kLoads], fa[NI], ta[NJ], lds;
+  uint32_t fo[F::kLoads], to[T::kLoads], fa[kFa], ta[kTa], lds;
 
   __device__ __forceinline__ void offsets(int64_t ldf, int64_t ldt) {
 #pragma unroll
@@ -157,25 +184,22 @@ struct MmLoop {
     const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
     const uint32_t base = (uint32_t)(uintptr_t)(lds_byte *)smem;
     offsets(ldf, ldt);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) fa[i] = base + F::frag_at(wf, i, r, g);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) ta[j] = base + F::kBytes + T::frag_at(wt, j, r, g);
+    F::addresses(fa, base, wf, r, g);
+    T::addresses(ta, base + F::kBytes, wt, r, g);
     lds = base + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * 1024;
   }
 
-  // The last chunks of contiguous rows: the pieces from the sum's end on come from outside, as zeros, from now on.
+  // The last stage of contiguous rows: the pieces from the sum's end on come from outside, as zeros, from now on.
   template <class O>
   static __device__ __forceinline__ void clip(const MmSource<O> &s, uint32_t *off) {
-    if (O::kContiguous && s.k < kMmK) {                  // wave-uniform
-      const bool inside = O::first_k(threadIdx.x) < s.k;
+    if (O::kContiguous && s.k < O::kK) {                 // wave-uniform
 #pragma unroll
-      for (int u = 0; u < O::kLoads; ++u) off[u] = inside ? off[u] : kMmOutside;
+      for (int u = 0; u < O::kLoads; ++u) off[u] = O::first_k(u, threadIdx.x) < s.k ? off[u] : kMmOutside;
     }
   }
-  // Load l of the sources' next chunk (F's first) into `stage`.
+  // Load l of the sources' next stage (F's first) into `stage`.
   __device__ __forceinline__ void load(int l, intx4 frsrc, intx4 trsrc, uint32_t stage) const {
-    mm_load_lds(l < F::kLoads ? frsrc : trsrc, l < F::kLoads ? fo[l] : to[l - F::kLoads], lds + stage + l * 4096);
+    mm_load_lds(l < F::kLoads ? frsrc : trsrc, l < F::kLoads ? fo[l] : to[l - F::kLoads], lds + stage + l * F::kPerLoad);
   }
   __device__ __forceinline__ void issue(MmSource<F> &f, MmSource<T> &t, uint32_t stage) {
     clip(f, fo);
@@ -186,59 +210,69 @@ struct MmLoop {
     f.next();
     t.next();
   }
-  __device__ __forceinline__ void read(Frags &x, uint32_t stage) const {
+  // Part i of NI of step h's fragments.
+  __device__ __forceinline__ void read_part(Frags &x, uint32_t stage, int h, int i) const {
+    x.a[i] = F::frag(fa, i, h, stage);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) x.a[i] = F::frag(fa[i] + stage);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) x.b[j] = T::frag(ta[j] + stage);
+    for (int j = 0; j < NJ; ++j)
+      if (j >= i * NJ / NI && j < (i + 1) * NJ / NI) x.b[j] = T::frag(ta, j, h, stage);
   }
-  // The products of `cur`, with load(i) and read(i), i < NI, spread between them.
-  template <class LOAD, class READ>
-  static __device__ __forceinline__ void products(const Frags &cur, floatx4 (&acc)[NI][NJ], LOAD load, READ read) {
+  __device__ __forceinline__ void read(Frags &x, uint32_t stage, int h) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) read_part(x, stage, h, i);
+  }
+  // The products of `cur`, with between(i), i < NI, spread between them.
+  template <class BETWEEN>
+  static __device__ __forceinline__ void products(const Frags &cur, floatx4 (&acc)[NI][NJ], BETWEEN between) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      load(i);
-      read(i);
+      between(i);
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[i], cur.b[j], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  __device__ __forceinline__ void read_part(Frags &x, uint32_t stage, int i) const {
-    x.a[i] = F::frag(fa[i] + stage);
+  // Fills the stages and reads the first step's fragments.
+  __device__ __forceinline__ void start(MmSource<F> &f, MmSource<T> &t, Frags &x) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (j >= i * NJ / NI && j < (i + 1) * NJ / NI) x.b[j] = T::frag(ta[j] + stage);
+    for (int q = 0; q < kStages; ++q) issue(f, t, q * kStage);
+    mm_wait_barrier<(kStages - 1) * kLoads>();
+    read(x, 0, 0);
   }
-  // One step: the products of `cur` (chunk ch, whose stage is `stage`), while `next` is read from chunk ch + 1's stage and
-  // the sources' chunk ch + 3 is loaded into chunk ch's.  On the way at its start: the loads of chunks ch + 1 and ch + 2.
-  __device__ __forceinline__ void step(MmSource<F> &f, MmSource<T> &t, const Frags &cur, Frags &next, uint32_t &stage,
-                                       floatx4 (&acc)[NI][NJ]) {
-    mm_wait_barrier<kLoads>();
-    const uint32_t here = stage;
-    stage = stage == 2 * kStage ? 0 : stage + kStage;
+  static __device__ __forceinline__ uint32_t after(uint32_t stage) {
+    return stage == (kStages - 1) * kStage ? 0 : stage + kStage;
+  }
+  // The last step of the stage at `here`, its fragments in `cur`: reads the first step of the stage behind it into `next`
+  // and loads the sources' next stage into its own place.
+  __device__ __forceinline__ void last_step(MmSource<F> &f, MmSource<T> &t, const Frags &cur, Frags &next, uint32_t here,
+                                            floatx4 (&acc)[NI][NJ]) {
+    mm_wait_barrier<(kStages - 2) * kLoads>();           // the next stage has landed, all have read this one
     clip(f, fo);
     clip(t, to);
     const intx4 fr = f.rsrc(), tr = t.rsrc();
-    products(
-        cur, acc,
-        [&](int i) {
+    const uint32_t there = after(here);
+    products(cur, acc, [&](int i) {
 #pragma unroll
-          for (int l = 0; l < kLoads; ++l)
-            if (l >= i * kLoads / NI && l < (i + 1) * kLoads / NI) load(l, fr, tr, here);
-        },
-        [&](int i) { read_part(next, stage, i); });
+      for (int l = 0; l < kLoads; ++l)
+        if (l >= i * kLoads / NI && l < (i + 1) * kLoads / NI) load(l, fr, tr, here);
+      read_part(next, there, 0, i);
+    });
     f.next();
     t.next();
   }
-  // Fills the three stages and reads the first chunk's fragments.
-  __device__ __forceinline__ void start(MmSource<F> &f, MmSource<T> &t, Frags &x) {
-    issue(f, t, 0);
-    issue(f, t, kStage);
-    issue(f, t, 2 * kStage);
-    mm_wait_barrier<2 * kLoads>();
-    read(x, 0);
+  // The products of a unit of 64 k from the stage at `stage` on, whose first step's fragments are in x: leaves the next
+  // unit's in x.
+  __device__ __forceinline__ void multiply(MmSource<F> &f, MmSource<T> &t, Frags &x, Frags &y, uint32_t &stage,
+                                           floatx4 (&acc)[NI][NJ]) {
+    if constexpr (kK == 32) {
+      last_step(f, t, x, y, stage, acc);
+      stage = after(stage);
+    } else {
+      products(x, acc, [&](int i) { read_part(y, stage, 1, i); });
+    }
+    last_step(f, t, y, x, stage, acc);
+    stage = after(stage);
   }
 };
 
@@ -257,15 +291,13 @@ __device__ __forceinline__ int mm_tile_of(unsigned id, unsigned n) {
 }
 inline int64_t mm_grid(int64_t n) { return (n + kMmXcds - 1) / kMmXcds * kMmXcds; }
 
-// Chunks of a sum over k, an even number.
-__device__ __forceinline__ int mm_chunks(int64_t k) { return (int)((k + 2 * kMmK - 1) / (2 * kMmK)) * 2; }
-
+__device__ __forceinline__ int mm_units(int64_t k) { return (int)((k + kMmUnit - 1) / kMmUnit); }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- plain products (lm_mm.hip) ----------------------------------------------------------------------------------------
 // out[t, f] = sum_k tok[t, k] feat[f, k]; an operand with *_kc = false is stored [k][row].  Rows and strides in elements,
 // rows of 16-byte pieces.  nsplit > 1 or f32: fp32 parts [nsplit][T][F] (with accumulate added to what is there), split s
-// summing k_per (a multiple of 64) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
+// summing k_per (whole units) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
 // F a multiple of 8; K one too where an operand has k contiguous, that operand's k from the sum's end up to it zeros; a k
 // strided tok has rows of at least T rounded up to 8.  Kf: the k that a k strided feat has (the last of K may lack).
 struct MmArgs {
@@ -277,10 +309,17 @@ struct MmArgs {
   const float *scale;
   int f32, accumulate;
 };
-int mm_launch(const MmArgs &a, bool feat_kc, bool tok_kc, hipStream_t stream, const char *what);
-// Splits of k for T x F outputs over K: as many as fill the card, each of at least min_k.
-int64_t mm_splits(int64_t T, int64_t F, int64_t K, int64_t min_k);
-int64_t mm_k_per(int64_t K, int64_t nsplit);
+// A product's tile shape (an index of lm_mm.hip's) and the splits of its k.
+struct MmPlan {
+  int shape;
+  int64_t splits;
+  int64_t part_bytes(int64_t T, int64_t F) const { return splits > 1 ? splits * T * F * 4 : 0; }
+};
+MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split);
+// One launch of it: the parts (a.f32) or, with one split, the result.  a.nsplit and a.k_per are set from the plan.
+int mm_launch(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, hipStream_t stream, const char *what);
+// The product into bf16 a.out [T][a.ldo]: parts (part_bytes of the plan) and their sum where k is split.
+int mm_run(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, float *parts, hipStream_t stream, const char *what);
 // out bf16 [T][ldo] = scale * sum of `parts` fp32 [nsplit][T][F] in order
 int mm_reduce_launch(const float *parts, int64_t nsplit, int64_t T, int64_t F, const float *scale, void *out, int64_t ldo,
                      hipStream_t stream, const char *what);

@@ -2,43 +2,59 @@
 // tiles alone are too few (a weight's gradient: few outputs, many tokens), the parts added in order by a second kernel (the
 // same bits on every call).
 #include "lm_mm.h"
+#ifndef KS_K
+#define KS_K 32
+#endif
 
 #include <algorithm>
 
 namespace smlm {
 namespace {
 
-template <int NI, int NJ, bool FKC, bool TKC, bool F32>
-__global__ void __launch_bounds__(kMmThreads, 2) mm_kernel(MmArgs a) {
-  typedef MmTile<32 * NI, FKC, FKC ? 4 * NI : 0> FT;
-  typedef MmTile<32 * NJ, TKC, 0> TT;
-  typedef MmLoop<FT, TT, NI, NJ> Loop;
+typedef MmShape<4, 2, 4, 8> Square;                       // 256 features x 256 tokens, 8 wavefronts
+typedef MmShape<4, 2, 6, 4> Wide;                         // 384 x 128, 8 wavefronts
+typedef MmShape<2, 2, 4, 4> Small;                        // 128 x 128, 4 wavefronts, two workgroups a CU
+typedef MmShape<2, 2, 2, 2> Tiny;                         // 64 x 64, 4 wavefronts, six a CU
+
+template <class S, bool FKC, bool TKC>
+struct MmKernel {
+  // permuted fragments where the features are rows of k: 8, 16 or 32 consecutive ones a lane
+  static constexpr int kPerm = FKC && (S::NI & (S::NI - 1)) == 0 ? 4 * S::NI : 0;
+  static constexpr int kK = FKC && TKC ? 64 : KS_K;
+  typedef MmTile<S::kF, FKC, kPerm, S::kThreads, kK> F;
+  typedef MmTile<S::kT, TKC, 0, S::kThreads, kK> T;
+  typedef MmLoop<F, T, S::NI, S::NJ> Loop;
+  static constexpr int kLds = Loop::kLds;
+};
+
+template <class S, bool FKC, bool TKC, bool F32>
+__global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
+  typedef MmKernel<S, FKC, TKC> K;
+  typedef typename K::Loop Loop;
+  constexpr int NI = S::NI, NJ = S::NJ;
   extern __shared__ __align__(16) unsigned char smem[];
-  const unsigned nf = (unsigned)((a.F + FT::kRows - 1) / FT::kRows), nt = (unsigned)((a.T + TT::kRows - 1) / TT::kRows);
+  const unsigned nf = (unsigned)((a.F + S::kF - 1) / S::kF), nt = (unsigned)((a.T + S::kT - 1) / S::kT);
   const int tile = mm_tile_of(blockIdx.x, nf * nt * (unsigned)a.nsplit);   // the host has checked that they are this few
   if (tile < 0) return;  // workgroup-uniform
   // the feature tiles of one token tile are neighbours: on one XCD its rows come from memory once
   const unsigned row = tile / nf, split = row / nt;
-  const int64_t f0 = (int64_t)(tile - row * nf) * FT::kRows, t0 = (int64_t)(row - split * nt) * TT::kRows, s = split;
+  const int64_t f0 = (int64_t)(tile - row * nf) * S::kF, t0 = (int64_t)(row - split * nt) * S::kT, s = split;
   const int64_t k_begin = s * a.k_per, k_end = min(a.K, k_begin + a.k_per);
-  const int wave = threadIdx.x / kWave, wf = (wave & 1) * 16 * NI, wt = (wave >> 1) * 16 * NJ;
+  const int wave = threadIdx.x / kWave, wf = S::feature(wave), wt = S::token(wave);
   Loop L;
   L.init(smem, a.ldf, a.ldt, wf, wt);
   floatx4 acc[NI][NJ];
   mm_zero(acc);
-  MmSource<FT> fs;
-  MmSource<TT> ts;
+  MmSource<typename K::F> fs;
+  MmSource<typename K::T> ts;
   fs.init(a.feat, a.ldf, a.F, FKC ? a.K : a.Kf, f0, k_begin);
   ts.init(a.tok, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, t0, k_begin);
-  if (k_end > k_begin) {  // workgroup-uniform; k_end is K or a whole number of double chunks on
+  if (k_end > k_begin) {  // workgroup-uniform; k_end is K or a whole number of units on
     typename Loop::Frags x, y;
     L.start(fs, ts, x);
     uint32_t stage = 0;
-    for (int left = mm_chunks(k_end - k_begin); left > 0; left -= 2) {
-      L.step(fs, ts, x, y, stage, acc);
-      L.step(fs, ts, y, x, stage, acc);
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // no load is on its way into LDS when the workgroup ends
+    for (int left = mm_units(k_end - k_begin); left > 0; --left) L.multiply(fs, ts, x, y, stage, acc);
+    mm_finish();
   }
 
   // lane (r, g): features 4 NI g .. (permuted) or 4 g .. of each 16, of token r of each 16
@@ -50,7 +66,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm_kernel(MmArgs a) {
     if (t >= a.T) continue;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int64_t f = f0 + wf + (FKC ? 4 * NI * g + 4 * i : 16 * i + 4 * g);
+      const int64_t f = f0 + wf + (K::kPerm ? 4 * NI * g + 4 * i : 16 * i + 4 * g);
       if (f >= a.F) continue;                 // F is a multiple of 8
       floatx4 v = acc[i][j];
       if constexpr (F32) {
@@ -93,44 +109,71 @@ __global__ void __launch_bounds__(256)
   *(uint2 *)(out + t * ldo + f) = uint2{pack_bf16x2(v.x * c, v.y * c), pack_bf16x2(v.z * c, v.w * c)};
 }
 
-template <int NI, int NJ, bool FKC, bool TKC>
+template <class S, bool FKC, bool TKC>
 int launch(const MmArgs &a, hipStream_t stream, const char *what) {
-  typedef MmLoop<MmTile<32 * NI, FKC, FKC ? 4 * NI : 0>, MmTile<32 * NJ, TKC, 0>, NI, NJ> Loop;
-  constexpr int kLds = kMmStages * Loop::kStage;
-  const int64_t n = ceil_div(a.F, 32 * NI) * ceil_div(a.T, 32 * NJ) * a.nsplit;
+  constexpr int kLds = MmKernel<S, FKC, TKC>::kLds;
+  const int64_t n = ceil_div(a.F, S::kF) * ceil_div(a.T, S::kT) * a.nsplit;
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
-  const void *k = a.f32 ? (const void *)mm_kernel<NI, NJ, FKC, TKC, true> : (const void *)mm_kernel<NI, NJ, FKC, TKC, false>;
+  const void *k = a.f32 ? (const void *)mm_kernel<S, FKC, TKC, true> : (const void *)mm_kernel<S, FKC, TKC, false>;
   const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
-  const dim3 grid((unsigned)mm_grid(n)), block(kMmThreads);
-  if (a.f32) hipLaunchKernelGGL((mm_kernel<NI, NJ, FKC, TKC, true>), grid, block, kLds, stream, a);
-  else hipLaunchKernelGGL((mm_kernel<NI, NJ, FKC, TKC, false>), grid, block, kLds, stream, a);
+  const dim3 grid((unsigned)mm_grid(n)), block(S::kThreads);
+  if (a.f32) hipLaunchKernelGGL((mm_kernel<S, FKC, TKC, true>), grid, block, kLds, stream, a);
+  else hipLaunchKernelGGL((mm_kernel<S, FKC, TKC, false>), grid, block, kLds, stream, a);
   return launch_status(what);
 }
 
-// Largest tile of which there are enough for the 256 CUs.
 template <bool FKC, bool TKC>
-int choose(const MmArgs &a, hipStream_t stream, const char *what) {
-  const int64_t big = ceil_div(a.F, 128) * a.nsplit;
-  if (big * ceil_div(a.T, 256) >= 384) return launch<4, 8, FKC, TKC>(a, stream, what);
-  if (big * ceil_div(a.T, 128) >= 256) return launch<4, 4, FKC, TKC>(a, stream, what);
-  return launch<2, 2, FKC, TKC>(a, stream, what);
+int choose(const MmArgs &a, int shape, hipStream_t stream, const char *what) {
+  switch (shape) {
+    case 0: return launch<Square, FKC, TKC>(a, stream, what);
+    case 1: return launch<Wide, FKC, TKC>(a, stream, what);
+    case 2: return launch<Small, FKC, TKC>(a, stream, what);
+    default: return launch<Tiny, FKC, TKC>(a, stream, what);
+  }
 }
 
 }  // namespace
 
-int mm_launch(const MmArgs &a, bool feat_kc, bool tok_kc, hipStream_t stream, const char *what) {
-  if (feat_kc && tok_kc) return choose<true, true>(a, stream, what);
-  if (tok_kc) return choose<false, true>(a, stream, what);
-  return choose<false, false>(a, stream, what);   // feat_kc without tok_kc: no caller
+// The shape and the splits with the least estimated time: rounds of workgroups over the card, each with its units of 64 k
+// and what it takes to begin and end, and for parts their way through memory and a second launch.
+MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split) {
+  struct Tile {
+    int f, t, slots;
+    double unit, fixed;                                   // us
+  };
+  static const Tile tiles[4] = {{256, 256, 256, 1.85, 5.0}, {384, 128, 256, 1.40, 4.5}, {128, 128, 512, 1.25, 4.0}, {64, 64, 1536, 1.5, 3.5}};
+  const int64_t units = ceil_div(K, kMmUnit);
+  MmPlan best{0, 1};
+  double least = 1e30;
+  for (int64_t s = 1; s <= (may_split ? 128 : 1) && (s == 1 || units / s >= 4); s += s < 16 ? 1 : 8)
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = ceil_div(F, tiles[i].f) * ceil_div(T, tiles[i].t) * s;
+      double time = ceil_div(n, tiles[i].slots) * (ceil_div(units, s) * tiles[i].unit + tiles[i].fixed);
+      if (s > 1) time += 6.0 + s * T * F * 8 / 4e6;       // 4 TB/s
+      if (time < least) {
+        least = time;
+        best = {i, s};
+      }
+    }
+  return best;
 }
 
-int64_t mm_splits(int64_t T, int64_t F, int64_t K, int64_t min_k) {
-  const int64_t tiles = ceil_div(F, 128) * ceil_div(T, 128), most = std::max<int64_t>(1, K / min_k);
-  return std::min(most, std::max<int64_t>(1, 512 / tiles));
+int mm_launch(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, hipStream_t stream, const char *what) {
+  a.nsplit = plan.splits;
+  a.k_per = ceil_div(ceil_div(a.K, plan.splits), kMmUnit) * kMmUnit;
+  if (feat_kc && tok_kc) return choose<true, true>(a, plan.shape, stream, what);
+  if (tok_kc) return choose<false, true>(a, plan.shape, stream, what);
+  return choose<false, false>(a, plan.shape, stream, what);   // feat_kc without tok_kc: no caller
 }
 
-int64_t mm_k_per(int64_t K, int64_t nsplit) { return ceil_div(ceil_div(K, nsplit), 2 * kMmK) * 2 * kMmK; }
+int mm_run(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, float *parts, hipStream_t stream, const char *what) {
+  void *out = a.out;
+  a.f32 = plan.splits > 1;
+  if (a.f32) a.out = parts;
+  if (const int rc = mm_launch(a, feat_kc, tok_kc, plan, stream, what)) return rc;
+  return a.f32 ? mm_reduce_launch(parts, plan.splits, a.T, a.F, a.scale, out, a.ldo, stream, what) : SMLM_OK;
+}
 
 int mm_reduce_launch(const float *parts, int64_t nsplit, int64_t T, int64_t F, const float *scale, void *out, int64_t ldo,
                      hipStream_t stream, const char *what) {

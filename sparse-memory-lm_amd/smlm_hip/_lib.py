@@ -82,8 +82,8 @@ EXPORTS = {
     "smlm_linear_ce": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
     "smlm_linear_ce_backward": (_i, [_p, _p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,
                                      _p]),
-    "smlm_gated_ffn": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p]),
-    "smlm_gated_ffn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "smlm_gated_ffn": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p]),
+    "smlm_gated_ffn_workspace": (_i64, [_i64, _i64, _i64, _i64, _i]),
     "smlm_gated_ffn_backward": (_i, [_p, _i64] * 4 + [_i64] * 4 + [_p] * 4 + [_i64, _p]),
     "smlm_rmsnorm_train": (_i, [_p, _i, _p, _i, _p, _i, _f, _i64, _i64, _p, _p, _i, _p, _p]),
     "smlm_rmsnorm_parts": (_i64, [_i64, _i64]),

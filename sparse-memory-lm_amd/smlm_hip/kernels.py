@@ -1163,7 +1163,7 @@ def _one_device(name, first, *others):
             raise ValueError(f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
 
 
-MAX_ROW_STRIDE = 1 << 22      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
+MAX_ROW_STRIDE = 1 << 21      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
 
 
 def _mm_rows(t, rows, cols):
@@ -1284,11 +1284,12 @@ class _GatedFFN(torch.autograd.Function):
         if x.numel() == 0:
             return x.new_empty(*x.shape[:-1], o)
         a, b, c, M, d8, h8, o8 = _GatedFFN._operands(x, w13, w2)
-        act = torch.empty(M, h8, dtype=x.dtype, device=x.device)
+        L = _lib.lib()
+        ws = torch.empty(L.smlm_gated_ffn_workspace(M, d8, h8, o8, 0), dtype=torch.uint8, device=x.device)
         y = torch.empty(M, o8, dtype=x.dtype, device=x.device)
         with torch.cuda.device(x.device):
-            rc = _lib.lib().smlm_gated_ffn(a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0),
-                                           M, d8, h8, o8, act.data_ptr(), y.data_ptr(), _stream(x))
+            rc = L.smlm_gated_ffn(a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0), M, d8,
+                                  h8, o8, y.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
         _lib.check(rc, "smlm_gated_ffn")
         return y[:, :o].reshape(*x.shape[:-1], o)
 
@@ -1310,7 +1311,7 @@ class _GatedFFN(torch.autograd.Function):
         out = [torch.empty(*s, dtype=x.dtype, device=x.device) if want else None
                for s, want in zip(((M, d8), (2, h8, d8), (o8, h8)), wants)]
         L = _lib.lib()
-        ws = torch.empty(L.smlm_gated_ffn_workspace(M, d8, h8, o8), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(L.smlm_gated_ffn_workspace(M, d8, h8, o8, 1), dtype=torch.uint8, device=x.device)
         with torch.cuda.device(x.device):
             rc = L.smlm_gated_ffn_backward(
                 g.data_ptr(), g.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0),

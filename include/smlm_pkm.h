@@ -556,7 +556,7 @@ int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w
 
 /*
  * Its gradient: dx = G W (M, d) and dw = G^T x (V, d), contiguous bf16, either NULL if not wanted, with
- * G[n, v] = c_n (softmax(s_n)[v] - [v == targets[n]]), formed in bf16 in pieces of the vocabulary of at most 512 MB (or 128
+ * G[n, v] = c_n (softmax(s_n)[v] - [v == targets[n]]), formed in bf16 in pieces of the vocabulary of at most 1 GiB (or 256
  * columns).  grad: per_token ? (M,) fp32, c_n = grad[n] : one fp32, c_n = grad[0] / (count ? count[0] : 1), applied in
  * fp32 behind the sums.  c_n = 0 for ignored tokens.  lse from the forward; workspace: smlm_linear_ce_workspace(M, V, d,
  * 1) bytes, 16-byte aligned.  fp32 sums in a fixed order.

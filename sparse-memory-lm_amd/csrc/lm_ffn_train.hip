@@ -33,10 +33,10 @@ __device__ __forceinline__ float sigmoid(float a) {
 // A tile takes S::kF rows of w13: half of them a's, and b's for the same features; each wavefront 8 NI features of either.
 template <class S>
 struct GateKernel {
-  static constexpr int kFeat = S::kF / 2, kHalf = S::NI / 2, kLane = 2 * S::NI;   // features of a tile; tiles; of a lane
-  typedef MmTile<S::kF, true, kLane, S::kThreads, 64> F;       // rows of w13
-  typedef MmTile<kFeat, false, kLane, S::kThreads, 64> W2;     // columns of w2
-  typedef MmTile<S::kT, true, 0, S::kThreads, 64> T;
+  static constexpr int kFeat = S::kF / 2, kHalf = S::NI / 2;   // features of a tile, row groups of either half
+  typedef MmTile<S::kF, true, true, S::kThreads, 64> F;        // rows of w13
+  typedef MmTile<kFeat, false, true, S::kThreads, 64> W2;      // columns of w2
+  typedef MmTile<S::kT, true, false, S::kThreads, 64> T;
   typedef MmLoop<F, T, S::NI, S::NJ> Gate;
   typedef MmLoop<W2, T, kHalf, S::NJ> Out;
 };
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
   typedef GateKernel<S> K;
   typedef typename K::Gate Gate;
   typedef typename K::Out Out;
-  constexpr int NI = S::NI, NJ = S::NJ, kHalf = K::kHalf, kLane = K::kLane;
+  constexpr int NI = S::NI, NJ = S::NJ, kHalf = K::kHalf;
   constexpr uint32_t kStage = Gate::kStage;               // the larger of the two
   extern __shared__ __align__(16) unsigned char smem[];
   const unsigned nf = (unsigned)((p.hidden + K::kFeat - 1) / K::kFeat), nt = (unsigned)((p.M + S::kT - 1) / S::kT);
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
   // the feature tiles of a token tile are neighbours: on one XCD its rows are read from memory once
   const unsigned row = tile / nf;
   const int64_t f0 = (int64_t)(tile - row * nf) * K::kFeat, t0 = (int64_t)row * S::kT;
-  const int wave = threadIdx.x / kWave, wf = S::feature(wave) / 2, wt = S::token(wave);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wf = S::feature(wave) / 2, wt = S::token(wave);
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
 
   Gate A;
@@ -73,37 +73,30 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
     ss.init(p.w2, p.ldw2, p.hidden, p.n_out, f0, 0);
     ys.init(p.dy, p.lddy, p.M, p.n_out, t0, 0);
   }
-  // Where a stage of x w13^T or dy w2 comes from, and its loads, part i of `parts`
-  struct Stage {
-    intx4 a, b, t;
-  };
-  auto next_gate = [&]() {
-    Gate::template clip<typename K::F>(as, A.fo);
-    Gate::template clip<typename K::T>(xs, A.to);
-    const Stage c{as.rsrc(), bs.rsrc(), xs.rsrc()};
-    as.next();
-    bs.next();
-    xs.next();
-    return c;
-  };
-  auto next_out = [&]() {
-    Out::template clip<typename K::T>(ys, B.to);
-    const Stage c{ss.rsrc(), ss.rsrc(), ys.rsrc()};
-    ss.next();
-    ys.next();
-    return c;
-  };
-  auto load_gate = [&](const Stage &c, uint32_t at, int i, int parts) {
+  // The loads of the next stage of x w13^T or dy w2 to `at`, part i of `parts`; then the sources step on.
+  auto load_gate = [&](uint32_t at, int i, int parts) {
     constexpr int kF = K::F::kLoads;
 #pragma unroll
     for (int l = 0; l < Gate::kLoads; ++l)
-      if (l >= i * Gate::kLoads / parts && l < (i + 1) * Gate::kLoads / parts)
-        mm_load_lds(l < kF / 2 ? c.a : l < kF ? c.b : c.t, l < kF ? A.fo[l] : A.to[l - kF], A.lds + at + l * K::F::kPerLoad);
+      if (l >= i * Gate::kLoads / parts && l < (i + 1) * Gate::kLoads / parts) {
+        if (l < kF / 2) Gate::load_one(as, A.fo, l, A.lds + at);
+        else if (l < kF) Gate::load_one(bs, A.fo, l, A.lds + at);
+        else Gate::load_one(xs, A.to, l - kF, A.lds + at + K::F::kBytes);
+      }
   };
-  auto load_out = [&](const Stage &c, uint32_t at, int i, int parts) {
+  auto clip_gate = [&]() {
+    Gate::clip(as, A.fo);
+    Gate::clip(xs, A.to);
+  };
+  auto next_gate = [&]() {
+    as.next();
+    bs.next();
+    xs.next();
+  };
+  auto load_out = [&](uint32_t at, int i, int parts) {
 #pragma unroll
     for (int l = 0; l < Out::kLoads; ++l)
-      if (l >= i * Out::kLoads / parts && l < (i + 1) * Out::kLoads / parts) B.load(l, c.a, c.t, at);
+      if (l >= i * Out::kLoads / parts && l < (i + 1) * Out::kLoads / parts) B.load(l, ss, ys, at);
   };
   // fragments of a in the first half of the row groups, of b (kFeat rows on, the same swizzle) in the second
   auto read_gate = [&](typename Gate::Frags &x, uint32_t stage, int h, int i) {
@@ -118,12 +111,16 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
   mm_zero(dact);
   typename Gate::Frags x, y;
   const int n1 = mm_units(p.d), n2 = GRAD ? mm_units(p.n_out) : 0;
-  load_gate(next_gate(), 0, 0, 1);
+  clip_gate();
+  load_gate(0, 0, 1);
+  next_gate();
   if (!GRAD || n1 > 1) {                                  // uniform
-    load_gate(next_gate(), kStage, 0, 1);
+    clip_gate();
+    load_gate(kStage, 0, 1);
+    next_gate();
     mm_wait_barrier<Gate::kLoads>();
   } else {
-    load_out(next_out(), kStage, 0, 1);
+    B.issue(ss, ys, kStage);
     mm_wait_barrier<Out::kLoads>();
   }
 #pragma unroll
@@ -135,17 +132,20 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
     Gate::products(x, ab, [&](int i) { read_gate(y, here, 1, i); });
     mm_wait_barrier<0>();                                 // the next stage has landed, all have read this one
     if (!GRAD || left > 2) {
-      const Stage c = next_gate();
+      clip_gate();
       Gate::products(y, ab, [&](int i) {
-        load_gate(c, here, i, NI);
+        load_gate(here, i, NI);
         read_gate(x, stage, 0, i);
       });
+      next_gate();
     } else {                                              // the last two stages' places take dy w2's first two
-      const Stage c = next_out();
+      Out::clip(ys, B.to);
       Gate::products(y, ab, [&](int i) {
-        load_out(c, here, i, NI);
+        load_out(here, i, NI);
         if (left > 1) read_gate(x, stage, 0, i);
       });
+      ss.next();
+      ys.next();
     }
   }
   if constexpr (GRAD) {
@@ -156,28 +156,30 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
       stage = kStage - stage;
       Out::products(u, dact, [&](int i) { B.read_part(v, here, 1, i); });
       mm_wait_barrier<0>();
-      const Stage c = next_out();
+      Out::clip(ys, B.to);
       Out::products(v, dact, [&](int i) {
-        load_out(c, here, i, kHalf);
+        load_out(here, i, kHalf);
         B.read_part(u, stage, 0, i);
       });
+      ss.next();
+      ys.next();
     }
   }
   mm_finish();
 
-  // lane (r, g): features f .. f + kLane - 1 of token r of each 16
-  const int64_t f = f0 + wf + kLane * g;
+  // lane (r, g): 8 features from f + 32 p on, p < kHalf / 2, of token r of each 16
+  const int64_t f = f0 + wf + 8 * g;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int64_t t = t0 + wt + 16 * j + r;
     if (t >= p.M) continue;
 #pragma unroll
-    for (int o = 0; o < kLane; o += 8) {
+    for (int o = 0; o < 16 * kHalf; o += 32) {
       if (f + o >= p.hidden) continue;                    // hidden is a multiple of 8
       float h[8], da[8], db[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const int i = (o + q) / 4, e = q % 4;
+        const int i = o / 16 + q / 4, e = q % 4;
         const float a = ab[i][j][e], b = ab[kHalf + i][j][e], s = sigmoid(a), as = a * s;
         h[q] = as * b;
         if constexpr (GRAD) {

@@ -24,9 +24,9 @@ namespace smlm {
 namespace {
 
 constexpr int kLsCols = 256;                              // vocabulary columns per tile
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kLsFinishRows = 16;                         // tokens per workgroup of the joining kernel
-constexpr int64_t kLsPieceBytes = 512LL << 20;            // most bytes of one piece's G
+constexpr int64_t kLsPieceBytes = 1LL << 30;            // most bytes of one piece's G
 constexpr int kNoTarget = -0x40000000;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -37,7 +37,7 @@ struct LossArgs {
   const int64_t *targets;
   int64_t ignore;
   int nsplit, tiles;                                      // ranges of the vocabulary, and its tiles of columns
-  float2 *parts;                                          // forward: (maximum, sum) [M][nsplit][wavefronts over a tile]
+  float2 *parts;                                          // forward: (maximum, sum) to base 2, [M][nsplit][wavefronts over a tile]
   float *picked;                                          // forward: the target's logit [M]
   const float *lse, *coef, *grad, *count;                 // gradient: coef per token, or null; grad and count: see below
   float *scale;                                           // gradient: *grad / *count (count null: *grad), written here
@@ -53,8 +53,8 @@ typedef MmShape<4, 2, 4, 2> Tokens64;
 
 template <class S>
 struct LossKernel {
-  typedef MmTile<S::kF, true, 4 * S::NI, S::kThreads, 64> F;
-  typedef MmTile<S::kT, true, 0, S::kThreads, 64> T;
+  typedef MmTile<S::kF, true, true, S::kThreads, 64> F;
+  typedef MmTile<S::kT, true, false, S::kThreads, 64> T;
   typedef MmLoop<F, T, S::NI, S::NJ> Loop;
 };
 
@@ -75,23 +75,25 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
   const int split = unit / nt;
   const int64_t t0 = (int64_t)(unit - split * nt) * S::kT;
   const int first = (int)((int64_t)a.tiles * split / a.nsplit), last = (int)((int64_t)a.tiles * (split + 1) / a.nsplit);
-  const int wave = threadIdx.x / kWave, wf = S::feature(wave), wt = S::token(wave);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wf = S::feature(wave), wt = S::token(wave);
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
 
-  int target[NJ];                     // column in [v0, ..), kNoTarget: not in this piece or none
-  float m[NJ], l[NJ], c[NJ];          // forward: running maximum and sum; gradient: m = lse, c = the coefficient
+  // the targets' columns in [v0, ..) wait in LDS (registers are short); kNoTarget: not in this piece or none
+  int *targets = (int *)(smem + Loop::kLds);
+  if (threadIdx.x < S::kT) {
+    const int64_t t = t0 + threadIdx.x, y = t < a.M ? a.targets[t] : a.ignore;
+    targets[threadIdx.x] = y != a.ignore && y >= a.v0 && y < a.v1 ? (int)(y - a.v0) : kNoTarget;
+  }
+  float m[NJ], l[NJ];                 // forward: running maximum and sum; gradient: m = lse
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int64_t t = t0 + wt + 16 * j + r;
-    const int64_t y = t < a.M ? a.targets[t] : a.ignore;
-    const bool valid = y != a.ignore && y >= a.v0 && y < a.v1;
-    target[j] = valid ? (int)(y - a.v0) : kNoTarget;
     m[j] = GRAD ? __builtin_inff() : -__builtin_inff();   // gradient, an ignored token: every probability is 0
-    l[j] = c[j] = 0.f;
-    if (GRAD && t < a.M && y != a.ignore) {
+    l[j] = 0.f;
+    if (GRAD && t < a.M) {
       // an index outside the vocabulary makes its token's gradient NaN, as its loss
-      m[j] = y < 0 || y >= a.V ? __builtin_nanf("") : a.lse[t];
-      if (a.coef) c[j] = a.coef[t];
+      const int64_t y = a.targets[t];
+      if (y != a.ignore) m[j] = y < 0 || y >= a.V ? __builtin_nanf("") : a.lse[t];
     }
   }
 
@@ -133,8 +135,8 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
       loaded();
     }
 
-    // lane (r, g): columns c0 .. c0 + C - 1 of token r of each 16
-    const int c0 = tile * kLsCols + wf + C * g;
+    // lane (r, g): columns c0 + 32 (q / 8) + q % 8, q < C, of token r of each 16
+    const int c0 = tile * kLsCols + wf + 8 * g;
     const int64_t end = (GRAD ? a.v1 : a.V) - a.v0;
     if ((int64_t)(tile + 1) * kLsCols > end) {          // columns past the end count for nothing
       const int valid = (int)(end - c0);
@@ -143,28 +145,32 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = 4 * i + e < valid ? acc[i][j][e] : -__builtin_inff();
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = 32 * (i / 2) + 4 * (i % 2) + e < valid ? acc[i][j][e] : -__builtin_inff();
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const unsigned rel = (unsigned)(target[j] - c0);
+      // the target's q in this lane, if it is here
+      const int off = targets[wt + 16 * j + r] - c0;
+      const unsigned rel = (unsigned)off < 8u * NI * 2 && (off & 24) == 0 ? (unsigned)(off / 32 * 8 + off % 8) : ~0u;
       if constexpr (!GRAD) {
-        if (__any(rel < (unsigned)C)) {                   // rare: 64 of the vocabulary's columns for 16 tokens
+        if (__any(rel < (unsigned)C)) {                   // rare: 16 NI of the vocabulary's columns for 16 tokens
           float v = 0.f;
 #pragma unroll
           for (int q = 0; q < C; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
-          if (rel < (unsigned)C) a.picked[t0 + wt + 16 * j + r] = v;
+          if (rel < (unsigned)C) a.picked[t0 + wt + (unsigned)(16 * j + r)] = v;
         }
-        float top = m[j];
+        float top = -__builtin_inff();
 #pragma unroll
         for (int q = 0; q < C; ++q) top = fmaxf(top, acc[q / 4][j][q % 4]);
-        // the difference first: a logit that is the maximum counts exactly 1, so that no loss is below 0
+        // to base 2: the sum is of 2^(s log2(e) - m), m the maximum times log2(e) as rounded, which makes its rounding no error
+        // (one fma per exponent)
+        top = fmaxf(m[j], top * kLog2e);
         const float ref = top == -__builtin_inff() ? 0.f : top;   // nothing yet: every exponential is 0
-        float sum = l[j] * exp2_hw((m[j] - ref) * kLog2e), more = 0.f;
+        float sum = l[j] * exp2_hw(m[j] - ref), more = 0.f;
 #pragma unroll
         for (int q = 0; q < C; q += 2) {
-          sum += exp2_hw((acc[q / 4][j][q % 4] - ref) * kLog2e);
-          more += exp2_hw((acc[q / 4][j][q % 4 + 1] - ref) * kLog2e);
+          sum += exp2_hw(fmaf(acc[q / 4][j][q % 4], kLog2e, -ref));
+          more += exp2_hw(fmaf(acc[q / 4][j][q % 4 + 1], kLog2e, -ref));
         }
         m[j] = top;
         l[j] = sum + more;
@@ -173,20 +179,27 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
         float p[C];
 #pragma unroll
         for (int q = 0; q < C; ++q) p[q] = exp2_hw((acc[q / 4][j][q % 4] - m[j]) * kLog2e);
-        if (__any(rel < (unsigned)C)) {
-#pragma unroll
-          for (int q = 0; q < C; ++q) p[q] = rel == (unsigned)q ? p[q] - 1.f : p[q];
-        }
+        float c = 1.f;
         if (a.coef) {                                     // uniform
+          c = t < a.M ? a.coef[t] : 0.f;
 #pragma unroll
-          for (int q = 0; q < C; ++q) p[q] *= c[j];
+          for (int q = 0; q < C; ++q) p[q] = p[q] == 0.f ? 0.f : p[q] * c;   // (an ignored token's coefficient may be NaN)
         }
         if (t < a.M) {
-          uint4 *out = (uint4 *)(a.g + t * a.ldg + c0);
+          // a wave-uniform base and 32 bits a lane
+          char *out = (char *)(a.g + (t0 + wt + 16 * j) * a.ldg + tile * kLsCols + wf);
+          const uint32_t at = (uint32_t)(r * a.ldg + 8 * g) * 2;
 #pragma unroll
           for (int q = 0; q < C / 8; ++q)
-            out[q] = uint4{pack_bf16x2(p[8 * q], p[8 * q + 1]), pack_bf16x2(p[8 * q + 2], p[8 * q + 3]),
+            *(uint4 *)(out + (at + 64 * q)) = uint4{pack_bf16x2(p[8 * q], p[8 * q + 1]), pack_bf16x2(p[8 * q + 2], p[8 * q + 3]),
                            pack_bf16x2(p[8 * q + 4], p[8 * q + 5]), pack_bf16x2(p[8 * q + 6], p[8 * q + 7])};
+        }
+        if (__any(rel < (unsigned)C)) {                   // rare: the target's, over what its lane has just stored
+          float v = 0.f;
+#pragma unroll
+          for (int q = 0; q < C; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
+          v = (exp2_hw((v - m[j]) * kLog2e) - 1.f) * c;
+          if (rel < (unsigned)C) a.g[t * a.ldg + c0 + off] = (uint16_t)(pack_bf16x2(v, v) & 0xFFFFu);
         }
       }
     }
@@ -200,7 +213,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
       for (int o = 16; o <= 32; o *= 2) {
         const float m2 = __shfl_xor(m[j], o, kWave), l2 = __shfl_xor(l[j], o, kWave);
         const float top = fmaxf(m[j], m2), ref = top == -__builtin_inff() ? 0.f : top;
-        l[j] = l[j] * exp2_hw((m[j] - ref) * kLog2e) + l2 * exp2_hw((m2 - ref) * kLog2e);
+        l[j] = l[j] * exp2_hw(m[j] - ref) + l2 * exp2_hw(m2 - ref);
         m[j] = top;
       }
       const int64_t t = t0 + wt + 16 * j + r;
@@ -226,18 +239,30 @@ __global__ void __launch_bounds__(256)
     for (int p = lane; p < nparts; p += kWave) {
       const float2 v = parts[t * nparts + p];
       const float top = fmaxf(m, v.x), ref = top == -__builtin_inff() ? 0.f : top;
-      l = l * exp2_hw((m - ref) * kLog2e) + v.y * exp2_hw((v.x - ref) * kLog2e);
+      l = l * exp2_hw(m - ref) + v.y * exp2_hw(v.x - ref);
       m = top;
     }
     for (int o = 32; o > 0; o >>= 1) {
       const float m2 = __shfl_xor(m, o, kWave), l2 = __shfl_xor(l, o, kWave);
       const float top = fmaxf(m, m2), ref = top == -__builtin_inff() ? 0.f : top;
-      l = l * exp2_hw((m - ref) * kLog2e) + l2 * exp2_hw((m2 - ref) * kLog2e);
+      l = l * exp2_hw(m - ref) + l2 * exp2_hw(m2 - ref);
       m = top;
     }
-    const float z = m + logf(l);
+    // loss = (m + log2(l) - s log2(e)) / log2(e), the large terms first: m and s log2(e) cancel without a rounding of
+    // their size, so that it does not fall below 0 by more than the logarithm's own rounding; lse = s + loss, so that a
+    // certain token's probability is exactly 1 in the gradient
     const int64_t y = targets[t];
-    const float loss = y == ignore ? 0.f : y < 0 || y >= V ? __builtin_nanf("") : z - picked[t];
+    const bool valid = y != ignore && y >= 0 && y < V;
+    const float log2l = log2f(l);
+    float loss = 0.f, z = (m + log2l) * kLn2;
+    if (valid) {
+      const float s = picked[t];
+      loss = (fmaf(-s, kLog2e, m) + log2l) * kLn2;
+      loss = loss < 0.f ? 0.f : loss;
+      z = s + loss;
+    } else if (y != ignore) {
+      loss = __builtin_nanf("");
+    }
     if (lane == 0) {
       lse[t] = z;
       if (each) each[t] = loss;
@@ -283,7 +308,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict
 
 template <class S, bool GRAD>
 int launch_loss(LossArgs a, hipStream_t stream, const char *what) {
-  constexpr int kLds = LossKernel<S>::Loop::kLds;
+  constexpr int kLds = LossKernel<S>::Loop::kLds + S::kT * 4;
   const hipError_t e = hipFuncSetAttribute((const void *)loss_kernel<S, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                            kLds);
   if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));

@@ -18,8 +18,8 @@
 // LDS layouts (16-byte pieces; 64 banks, 256 bytes; ds_read_b128 serves lanes 0-3, 12-15 and 20-27 of each 32 together,
 // then the others):
 //   k contiguous: 128-byte rows, piece c of row R at c ^ swz(R), so that the lanes served together fall on distinct banks.
-//     Feature rows may be read permuted (lane r of tile i takes row 4 NI (r / 4) + 4 i + r % 4), which leaves each lane 4 NI
-//     consecutive features of a token in its accumulators: whole 32-byte stores.
+//     Feature rows may be read permuted (mm_feature): row groups 2 p and 2 p + 1 then leave each lane 8 consecutive features
+//     of a token in its accumulators, and the four lanes of a token 32: stores of 16 bytes a lane, 64 a token.
 //   k strided: rows of kF or kT, piece c of row k at c ^ vsw(k), read with ds_read_b64_tr_b16, which gives lane r four k of
 //     column r.  Lane group g takes k = 8 g .. 8 g + 7 of a step in both layouts.
 // Out of range rows and k read as zeros (the buffer's record count; the k beyond the end of contiguous rows by an offset
@@ -72,9 +72,14 @@ struct MmShape {
   static __device__ __forceinline__ int token(int wave) { return wave / WF * 16 * NJ; }
 };
 
-// One operand's LDS tile of ROWS rows (tokens or features) x K k (32 or 64).  PERM: features per lane group of a permuted
-// fragment, 0 for a plain one.
-template <int ROWS, bool KC, int PERM, int THREADS, int K>
+// First of the four features of row group i in lane group g's accumulators.
+template <bool PERM>
+__device__ __forceinline__ constexpr int mm_feature(int i, int g) {
+  return PERM ? 32 * (i / 2) + 8 * g + 4 * (i % 2) : 16 * i + 4 * g;
+}
+
+// One operand's LDS tile of ROWS rows (tokens or features) x K k (32 or 64).  PERM: its fragments are permuted.
+template <int ROWS, bool KC, bool PERM, int THREADS, int K>
 struct MmTile {
   static constexpr bool kContiguous = KC;
   static constexpr int kK = K, kRows = ROWS, kBytes = ROWS * K * 2, kPerLoad = THREADS * 16;
@@ -83,33 +88,37 @@ struct MmTile {
   static_assert(kBytes % kPerLoad == 0, "a whole number of loads");
 
   static __device__ __forceinline__ int swz(int row) {               // KC
-    if constexpr (K == 32) return -(PERM ? row / PERM : row / 4) & 3;
-    else return PERM ? (row >> 1 & 1) | (row / PERM & 3) << 1 : row >> 1 & 7;
+    if constexpr (K == 32) return -(PERM ? row / 8 : row / 4) & 3;
+    else return PERM ? (row >> 1 & 1) | (row / 8 & 3) << 1 : row >> 1 & 7;
   }
   static __device__ __forceinline__ int vsw(int k) {                 // k strided
     return ROWS % 128 == 0 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 2 * ((k >> 1 & 1) | (k >> 3 & 1) << 1);
   }
 
-  // This thread's byte offset of load u from the stage's first byte in memory; its first k (KC).
+  // Loads whose offsets are kept: contiguous rows have one, the loads' rows are kRowStep apart with one swizzle, and the
+  // step goes into the (wave-uniform) descriptor.
+  static constexpr int kRowStep = KC ? kPerLoad / kRowBytes : 0, kOffsets = KC ? 1 : kLoads;
+  static_assert(!KC || (kRowStep % 32 == 0), "one swizzle for all loads");
+  // This thread's byte offset of load u (KC: 0) from the stage's (the load's) first byte in memory; its first k (KC).
   static __device__ __forceinline__ uint32_t offset(int u, int tid, int64_t ld) {
     const int at = u * kPerLoad + tid * 16, row = at / kRowBytes, c = at % kRowBytes / 16;
     if constexpr (KC) return (uint32_t)(row * ld * 2 + (c ^ swz(row)) * 16);
     else return (uint32_t)(row * ld * 2 + (c ^ vsw(row)) * 16);
   }
-  static __device__ __forceinline__ int first_k(int u, int tid) {
-    const int at = u * kPerLoad + tid * 16;
+  static __device__ __forceinline__ int first_k(int tid) {
+    const int at = tid * 16;
     return 8 * (at % kRowBytes / 16 ^ swz(at / kRowBytes));
   }
 
   // LDS address (from the tile's base) that lane (r, g) reads the wavefront's row group i from, its rows starting at w0,
   // in step h (0, 1) of the stage.  KC: i only adds to it; k strided: h does.
   static __device__ __forceinline__ uint32_t at_contiguous(int w0, int h, int r, int g) {
-    const int R = PERM ? w0 + PERM * (r / 4) + r % 4 : w0 + r;       // w0 a multiple of 4 PERM or 16
+    const int R = PERM ? w0 + 8 * (r / 4) + r % 4 : w0 + r;          // w0 a multiple of 32 or 16
     return R * kRowBytes + (((K == 32 ? 0 : 4 * h) + g) ^ swz(R)) * 16;
   }
   static __device__ __forceinline__ uint32_t at_strided(int w0, int i, int r, int g) {
     const int k = 8 * g + r / 4;
-    const int col = PERM ? w0 + PERM * (r % 4) + 4 * i : w0 + 16 * i + 4 * (r % 4);
+    const int col = w0 + mm_feature<PERM>(i, r % 4);
     return k * kRowBytes + (col / 8 ^ vsw(k)) * 16 + col % 8 * 2;
   }
   template <int N>
@@ -121,7 +130,7 @@ struct MmTile {
   template <int N>
   static __device__ __forceinline__ bf16x8 frag(const uint32_t (&a)[N], int i, int h, uint32_t stage) {
     if constexpr (KC) {
-      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)(a[h] + stage + i * (PERM ? 4 : 16) * kRowBytes);
+      return *(const __attribute__((address_space(3))) bf16x8 *)(uintptr_t)(a[h] + stage + mm_feature<PERM>(i, 0) * kRowBytes);
     } else {
       typedef __attribute__((address_space(3))) bf16x4 *p4;
       const uint32_t at = a[i] + stage + h * 32 * kRowBytes;
@@ -137,19 +146,22 @@ struct MmTile {
 template <class O>
 struct MmSource {
   const uint16_t *p;
-  int64_t left, step, k;                                 // step in bytes; k: what is left of the sum
+  int64_t left, step, k, rows_step;                      // steps in bytes; k: what is left of the sum
   // rows from row0 (< rows) on and k from k0 (< K) on of an operand of `rows` rows and K
   __device__ __forceinline__ void init(const uint16_t *base, int64_t ld, int64_t rows, int64_t K, int64_t row0, int64_t k0) {
     const int64_t major = O::kContiguous ? row0 : k0, minor = O::kContiguous ? k0 : row0;
     p = base + major * ld + minor;
     left = (((O::kContiguous ? rows : K) - 1 - major) * ld + (O::kContiguous ? K : rows) - minor) * 2;
     step = O::kContiguous ? O::kK * 2 : O::kK * 2 * ld;
+    rows_step = O::kRowStep * ld * 2;
     k = K - k0;
   }
-  __device__ __forceinline__ intx4 rsrc() const {
-    const uint64_t a = (uint64_t)p;
-    const uint32_t n = left >> 32 ? 0xFFFFFFF0u : (uint32_t)left;
-    return intx4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(left <= 0 ? 0u : n), 0x00020000};
+  // Descriptor of load u.
+  __device__ __forceinline__ intx4 rsrc(int u) const {
+    const uint64_t a = (uint64_t)p + u * rows_step;
+    const int64_t more = left - u * rows_step;
+    const uint32_t n = more >> 32 ? 0xFFFFFFF0u : (uint32_t)more;
+    return intx4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(more <= 0 ? 0u : n), 0x00020000};
   }
   __device__ __forceinline__ void next() {
     p += step / 2;
@@ -171,13 +183,13 @@ struct MmLoop {
   static constexpr int kStage = F::kBytes + T::kBytes, kLoads = F::kLoads + T::kLoads, kLds = kStages * kStage;
   static constexpr int kFa = F::kContiguous ? 2 : NI, kTa = T::kContiguous ? 2 : NJ;
   typedef MmFrags<NI, NJ> Frags;
-  uint32_t fo[F::kLoads], to[T::kLoads], fa[kFa], ta[kTa], lds;
+  uint32_t fo[F::kOffsets], to[T::kOffsets], fa[kFa], ta[kTa], lds;
 
   __device__ __forceinline__ void offsets(int64_t ldf, int64_t ldt) {
 #pragma unroll
-    for (int u = 0; u < F::kLoads; ++u) fo[u] = F::offset(u, threadIdx.x, ldf);
+    for (int u = 0; u < F::kOffsets; ++u) fo[u] = F::offset(u, threadIdx.x, ldf);
 #pragma unroll
-    for (int u = 0; u < T::kLoads; ++u) to[u] = T::offset(u, threadIdx.x, ldt);
+    for (int u = 0; u < T::kOffsets; ++u) to[u] = T::offset(u, threadIdx.x, ldt);
   }
   // wf, wt: first feature and token row of this wavefront in the tile
   __device__ __forceinline__ void init(const unsigned char *smem, int64_t ldf, int64_t ldt, int wf, int wt) {
@@ -192,21 +204,24 @@ struct MmLoop {
   // The last stage of contiguous rows: the pieces from the sum's end on come from outside, as zeros, from now on.
   template <class O>
   static __device__ __forceinline__ void clip(const MmSource<O> &s, uint32_t *off) {
-    if (O::kContiguous && s.k < O::kK) {                 // wave-uniform
-#pragma unroll
-      for (int u = 0; u < O::kLoads; ++u) off[u] = O::first_k(u, threadIdx.x) < s.k ? off[u] : kMmOutside;
-    }
+    if (O::kContiguous && s.k < O::kK)                   // wave-uniform
+      off[0] = O::first_k(threadIdx.x) < s.k ? off[0] : kMmOutside;
+  }
+  // Load u of an operand's next stage to `at`, the place of its first.
+  template <class O>
+  static __device__ __forceinline__ void load_one(const MmSource<O> &s, const uint32_t *off, int u, uint32_t at) {
+    mm_load_lds(s.rsrc(u), off[O::kContiguous ? 0 : u], at + u * O::kPerLoad);
   }
   // Load l of the sources' next stage (F's first) into `stage`.
-  __device__ __forceinline__ void load(int l, intx4 frsrc, intx4 trsrc, uint32_t stage) const {
-    mm_load_lds(l < F::kLoads ? frsrc : trsrc, l < F::kLoads ? fo[l] : to[l - F::kLoads], lds + stage + l * F::kPerLoad);
+  __device__ __forceinline__ void load(int l, const MmSource<F> &f, const MmSource<T> &t, uint32_t stage) const {
+    if (l < F::kLoads) load_one(f, fo, l, lds + stage);
+    else load_one(t, to, l - F::kLoads, lds + stage + F::kBytes);
   }
   __device__ __forceinline__ void issue(MmSource<F> &f, MmSource<T> &t, uint32_t stage) {
     clip(f, fo);
     clip(t, to);
-    const intx4 fr = f.rsrc(), tr = t.rsrc();
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) load(l, fr, tr, stage);
+    for (int l = 0; l < kLoads; ++l) load(l, f, t, stage);
     f.next();
     t.next();
   }
@@ -250,12 +265,11 @@ struct MmLoop {
     mm_wait_barrier<(kStages - 2) * kLoads>();           // the next stage has landed, all have read this one
     clip(f, fo);
     clip(t, to);
-    const intx4 fr = f.rsrc(), tr = t.rsrc();
     const uint32_t there = after(here);
     products(cur, acc, [&](int i) {
 #pragma unroll
       for (int l = 0; l < kLoads; ++l)
-        if (l >= i * kLoads / NI && l < (i + 1) * kLoads / NI) load(l, fr, tr, here);
+        if (l >= i * kLoads / NI && l < (i + 1) * kLoads / NI) load(l, f, t, here);
       read_part(next, there, 0, i);
     });
     f.next();

@@ -18,11 +18,10 @@ typedef MmShape<2, 2, 2, 2> Tiny;                         // 64 x 64, 4 wavefron
 
 template <class S, bool FKC, bool TKC>
 struct MmKernel {
-  // permuted fragments where the features are rows of k: 8, 16 or 32 consecutive ones a lane
-  static constexpr int kPerm = FKC && (S::NI & (S::NI - 1)) == 0 ? 4 * S::NI : 0;
+  static constexpr bool kPerm = FKC;                      // (k strided features: the transposing reads would conflict)
   static constexpr int kK = FKC && TKC ? 64 : KS_K;
   typedef MmTile<S::kF, FKC, kPerm, S::kThreads, kK> F;
-  typedef MmTile<S::kT, TKC, 0, S::kThreads, kK> T;
+  typedef MmTile<S::kT, TKC, false, S::kThreads, kK> T;
   typedef MmLoop<F, T, S::NI, S::NJ> Loop;
   static constexpr int kLds = Loop::kLds;
 };
@@ -40,7 +39,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
   const unsigned row = tile / nf, split = row / nt;
   const int64_t f0 = (int64_t)(tile - row * nf) * S::kF, t0 = (int64_t)(row - split * nt) * S::kT, s = split;
   const int64_t k_begin = s * a.k_per, k_end = min(a.K, k_begin + a.k_per);
-  const int wave = threadIdx.x / kWave, wf = S::feature(wave), wt = S::token(wave);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wf = S::feature(wave), wt = S::token(wave);
   Loop L;
   L.init(smem, a.ldf, a.ldt, wf, wt);
   floatx4 acc[NI][NJ];
@@ -57,7 +56,6 @@ __global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
     mm_finish();
   }
 
-  // lane (r, g): features 4 NI g .. (permuted) or 4 g .. of each 16, of token r of each 16
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
   const float scale = !F32 && a.scale ? *a.scale : 1.0f;
 #pragma unroll
@@ -66,7 +64,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
     if (t >= a.T) continue;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int64_t f = f0 + wf + (K::kPerm ? 4 * NI * g + 4 * i : 16 * i + 4 * g);
+      const int64_t f = f0 + wf + mm_feature<K::kPerm>(i, g);
       if (f >= a.F) continue;                 // F is a multiple of 8
       floatx4 v = acc[i][j];
       if constexpr (F32) {
@@ -77,8 +75,16 @@ __global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
         }
         *o = make_float4(v[0], v[1], v[2], v[3]);
       } else {
-        *(uint2 *)((uint16_t *)a.out + t * a.ldo + f) =
-            uint2{pack_bf16x2(v[0] * scale, v[1] * scale), pack_bf16x2(v[2] * scale, v[3] * scale)};
+        auto packed = [&](const floatx4 &u) {
+          return uint2{pack_bf16x2(u[0] * scale, u[1] * scale), pack_bf16x2(u[2] * scale, u[3] * scale)};
+        };
+        uint16_t *o = (uint16_t *)a.out + t * a.ldo + f;
+        if constexpr (K::kPerm) {             // with the next row group: 8 features
+          const uint2 lo = packed(v), hi = packed(acc[i + 1 < NI ? i + 1 : i][j]);
+          if (i % 2 == 0) *(uint4 *)o = uint4{lo.x, lo.y, hi.x, hi.y};
+        } else {
+          *(uint2 *)o = packed(v);
+        }
       }
     }
   }

@@ -209,9 +209,8 @@ typedef MmShape<2, 2, 4, 2> Gate32;                      // 64 x 64
 template <class S, bool GRAD>
 int launch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
   constexpr int kLds = GateKernel<S>::Gate::kLds;
-  const hipError_t e = hipFuncSetAttribute((const void *)gate_kernel<S, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           kLds);
-  if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
+  static std::atomic<uint64_t> done;
+  if (const int rc = mm_allow_lds((const void *)gate_kernel<S, GRAD>, kLds, done, what)) return rc;
   const int64_t n = ceil_div(p.hidden, GateKernel<S>::kFeat) * ceil_div(p.M, S::kT);
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
   hipLaunchKernelGGL((gate_kernel<S, GRAD>), dim3((unsigned)mm_grid(n)), dim3(S::kThreads), kLds, stream, p);

@@ -309,9 +309,8 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict
 template <class S, bool GRAD>
 int launch_loss(LossArgs a, hipStream_t stream, const char *what) {
   constexpr int kLds = LossKernel<S>::Loop::kLds + S::kT * 4;
-  const hipError_t e = hipFuncSetAttribute((const void *)loss_kernel<S, GRAD>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           kLds);
-  if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
+  static std::atomic<uint64_t> done;
+  if (const int rc = mm_allow_lds((const void *)loss_kernel<S, GRAD>, kLds, done, what)) return rc;
   const int64_t n = ceil_div(a.M, S::kT) * a.nsplit;
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
   hipLaunchKernelGGL((loss_kernel<S, GRAD>), dim3((unsigned)mm_grid(n)), dim3(S::kThreads), kLds, stream, a);

@@ -28,6 +28,8 @@
 
 #include "pkm_common.h"
 
+#include <atomic>
+
 namespace smlm {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -307,6 +309,20 @@ inline int64_t mm_grid(int64_t n) { return (n + kMmXcds - 1) / kMmXcds * kMmXcds
 
 __device__ __forceinline__ int mm_units(int64_t k) { return (int)((k + kMmUnit - 1) / kMmUnit); }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Lets a kernel use `bytes` of dynamic LDS, more than the 64 KB that need no permission: once per kernel and device (the
+// call costs as much as a launch).  done: the kernel's own, a bit per device.
+inline int mm_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &done, const char *what) {
+  if (bytes <= 65536) return SMLM_OK;
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (e == hipSuccess && !(device < 64 && (done.load(std::memory_order_relaxed) & bit))) {
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return e == hipSuccess ? SMLM_OK : fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
+}
 
 // ---- plain products (lm_mm.hip) ----------------------------------------------------------------------------------------
 // out[t, f] = sum_k tok[t, k] feat[f, k]; an operand with *_kc = false is stored [k][row].  Rows and strides in elements,

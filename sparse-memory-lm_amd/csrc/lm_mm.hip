@@ -121,8 +121,8 @@ int launch(const MmArgs &a, hipStream_t stream, const char *what) {
   const int64_t n = ceil_div(a.F, S::kF) * ceil_div(a.T, S::kT) * a.nsplit;
   if (mm_grid(n) > 0x7FFFFFFFLL) return fail(SMLM_EUNSUPPORTED, "%s: too many workgroups", what);
   const void *k = a.f32 ? (const void *)mm_kernel<S, FKC, TKC, true> : (const void *)mm_kernel<S, FKC, TKC, false>;
-  const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (e != hipSuccess) return fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
+  static std::atomic<uint64_t> done[2];
+  if (const int rc = mm_allow_lds(k, kLds, done[a.f32 ? 1 : 0], what)) return rc;
   const dim3 grid((unsigned)mm_grid(n)), block(S::kThreads);
   if (a.f32) hipLaunchKernelGGL((mm_kernel<S, FKC, TKC, true>), grid, block, kLds, stream, a);
   else hipLaunchKernelGGL((mm_kernel<S, FKC, TKC, false>), grid, block, kLds, stream, a);

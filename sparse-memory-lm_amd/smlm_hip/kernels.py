@@ -33,6 +33,7 @@ The dense operators of a training step, differentiable (Transformer.loss calls t
     add_rmsnorm_train(x, delta, norm)       (residual add + RMSNorm, smlm/model.py:156-163)
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -1163,6 +1164,30 @@ def _one_device(name, first, *others):
             raise ValueError(f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
 
 
+def _launch(name, t, *args):
+    """The library's entry point `name` on t's device and torch's current stream there.  A backward runs on a thread of
+    autograd's own, where every Python object costs three times as much as here: no device guard where t's device is
+    the current one, and no stream object."""
+    device = t.get_device()
+    if torch._C._cuda_getDevice() == device:
+        rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name, *sizes):
+    """Bytes (or, for a norm's parts, floats) of an entry point's workspace, a function of the sizes alone."""
+    return getattr(_lib.lib(), name)(*sizes)
+
+
+def _workspace(name, like, *sizes):
+    return torch.empty(_workspace_bytes(name, *sizes), dtype=torch.uint8, device=like.device)
+
+
 MAX_ROW_STRIDE = 1 << 21      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
 
 
@@ -1201,13 +1226,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
             return torch.full((), float("nan") if reduction == "mean" else 0.0, dtype=torch.float32, device=x.device)
         loss = torch.empty(M if reduction == "none" else 2, dtype=torch.float32, device=x.device)
         x2, w2 = _mm_rows(x.reshape(M, d), M, d8), _mm_rows(weight, V, d8)
-        L = _lib.lib()
-        ws = torch.empty(L.smlm_linear_ce_workspace(M, V, d8, 0), dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
-            rc = L.smlm_linear_ce(x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), t.data_ptr(), ignore_index,
-                                  _REDUCTIONS[reduction], M, V, d8, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
-                                  ws.numel(), _stream(x))
-        _lib.check(rc, "smlm_linear_ce")
+        ws = _workspace("smlm_linear_ce_workspace", x, M, V, d8, 0)
+        _launch("smlm_linear_ce", x, x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), t.data_ptr(), ignore_index,
+                _REDUCTIONS[reduction], M, V, d8, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel())
         ctx.save_for_backward(x, weight, targets, lse, loss)
         return loss.view(targets.shape) if reduction == "none" else loss[0].clone()
 
@@ -1229,17 +1250,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
         t, g = targets.reshape(-1).contiguous(), g.reshape(-1).float().contiguous()
         dx = torch.empty(M, d8, dtype=x.dtype, device=x.device) if wants[0] else None
         dw = torch.empty(V, d8, dtype=x.dtype, device=x.device) if wants[1] else None
-        L = _lib.lib()
-        ws = torch.empty(L.smlm_linear_ce_workspace(M, V, d8, 1), dtype=torch.uint8, device=x.device)
+        ws = _workspace("smlm_linear_ce_workspace", x, M, V, d8, 1)
         count = loss.data_ptr() + 4 if ctx.reduction == "mean" else None
-        with torch.cuda.device(x.device):
-            rc = L.smlm_linear_ce_backward(
-                g.data_ptr(), count, ctx.reduction == "none", x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0),
-                t.data_ptr(), ctx.ignore_index, lse.data_ptr(), M, V, d8, None if dx is None else dx.data_ptr(),
-                None if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
-        _lib.check(rc, "smlm_linear_ce_backward")
-        return (None if dx is None else dx[:, :d].reshape(x.shape), None if dw is None else dw[:, :d].reshape(V, d),
-                None, None, None)
+        _launch("smlm_linear_ce_backward", x, g.data_ptr(), count, ctx.reduction == "none", x2.data_ptr(), x2.stride(0),
+                w2.data_ptr(), w2.stride(0), t.data_ptr(), ctx.ignore_index, lse.data_ptr(), M, V, d8,
+                None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel())
+        if d8 != d:
+            dx, dw = (t if t is None else t[:, :d].contiguous() for t in (dx, dw))
+        return None if dx is None else dx.view(x.shape), dw, None, None, None
 
 
 def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
@@ -1284,14 +1302,11 @@ class _GatedFFN(torch.autograd.Function):
         if x.numel() == 0:
             return x.new_empty(*x.shape[:-1], o)
         a, b, c, M, d8, h8, o8 = _GatedFFN._operands(x, w13, w2)
-        L = _lib.lib()
-        ws = torch.empty(L.smlm_gated_ffn_workspace(M, d8, h8, o8, 0), dtype=torch.uint8, device=x.device)
+        ws = _workspace("smlm_gated_ffn_workspace", x, M, d8, h8, o8, 0)
         y = torch.empty(M, o8, dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device):
-            rc = L.smlm_gated_ffn(a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0), M, d8,
-                                  h8, o8, y.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
-        _lib.check(rc, "smlm_gated_ffn")
-        return y[:, :o].reshape(*x.shape[:-1], o)
+        _launch("smlm_gated_ffn", x, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0), M, d8,
+                h8, o8, y.data_ptr(), ws.data_ptr(), ws.numel())
+        return (y if o8 == o else y[:, :o].contiguous()).view(*x.shape[:-1], o)
 
     @staticmethod
     def backward(ctx, dy):
@@ -1309,18 +1324,17 @@ class _GatedFFN(torch.autograd.Function):
         a, b, c, M, d8, h8, o8 = _GatedFFN._operands(x, w13, w2)
         g = _mm_rows(dy.reshape(M, o), M, o8)
         out = [torch.empty(*s, dtype=x.dtype, device=x.device) if want else None
-               for s, want in zip(((M, d8), (2, h8, d8), (o8, h8)), wants)]
-        L = _lib.lib()
-        ws = torch.empty(L.smlm_gated_ffn_workspace(M, d8, h8, o8, 1), dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
-            rc = L.smlm_gated_ffn_backward(
-                g.data_ptr(), g.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0),
-                M, d8, h8, o8, *(None if t is None else t.data_ptr() for t in out), ws.data_ptr(), ws.numel(), _stream(x))
-        _lib.check(rc, "smlm_gated_ffn_backward")
+               for s, want in zip(((M, d8), (2 * h8, d8), (o8, h8)), wants)]
+        ws = _workspace("smlm_gated_ffn_workspace", x, M, d8, h8, o8, 1)
         dx, dw13, dw2 = out
-        return (None if dx is None else dx[:, :d].reshape(x.shape),
-                None if dw13 is None else dw13[:, :h, :d].reshape(2 * h, d),
-                None if dw2 is None else dw2[:o, :h].reshape(o, h))
+        _launch("smlm_gated_ffn_backward", x, g.data_ptr(), g.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
+                c.data_ptr(), c.stride(0), M, d8, h8, o8, None if dx is None else dx.data_ptr(),
+                None if dw13 is None else dw13.data_ptr(), None if dw2 is None else dw2.data_ptr(), ws.data_ptr(), ws.numel())
+        if (d8, h8, o8) != (d, h, o):
+            dx = None if dx is None else dx[:, :d].contiguous()
+            dw13 = None if dw13 is None else dw13.view(2, h8, d8)[:, :h, :d].reshape(2 * h, d)
+            dw2 = None if dw2 is None else dw2[:o, :h].contiguous()
+        return None if dx is None else dx.view(x.shape), dw13, dw2
 
 
 def gated_ffn(x, w13, w2):
@@ -1344,67 +1358,59 @@ NORM_TRAIN_MAX_COLS = 16384        # csrc/lm_rmsnorm.hip
 
 
 class _AddRMSNorm(torch.autograd.Function):
-    """add_rmsnorm_train's node: keeps the sum and one fp32 per row.  A backward that is itself recorded differentiates the
-    PyTorch ops."""
+    """add_rmsnorm_train's node: keeps the sum, the weight and one fp32 per row.  A backward that is itself recorded runs
+    as PyTorch ops."""
 
     @staticmethod
     def forward(ctx, x, delta, weight, eps, out_dtype):
         ctx.set_materialize_grads(False)
         C = x.shape[-1]
         M = x.numel() // C
-        ctx.eps = eps
         a, w = x.contiguous(), weight.contiguous()
         d = None if delta is None else delta.contiguous()
-        xs = a if d is None else torch.empty_like(a)
-        h = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        xs = x if d is None else torch.empty_like(a)          # nothing to add: x itself, as an output of this node
+        h = torch.empty_like(a, dtype=out_dtype)
         rstd = torch.empty(M, dtype=torch.float32, device=x.device)
-        if M > 0:
-            with torch.cuda.device(x.device):
-                rc = _lib.lib().smlm_rmsnorm_train(
-                    a.data_ptr(), _DT[x.dtype], None if d is None else d.data_ptr(),
-                    _DT[x.dtype if d is None else d.dtype], w.data_ptr(), _DT[w.dtype], eps, M, C,
-                    None if d is None else xs.data_ptr(), h.data_ptr(), _DT[out_dtype], rstd.data_ptr(), _stream(x))
-            _lib.check(rc, "smlm_rmsnorm_train")
-        out = x if d is None else xs                           # nothing to add: x itself, as an output of this node
-        ctx.save_for_backward(x, delta, weight, out, rstd)
-        ctx.out_dtype = out_dtype
-        return out, h
+        ctx.delta_dtype, ctx.eps = x.dtype if d is None else d.dtype, eps
+        if M:
+            _launch("smlm_rmsnorm_train", x, a.data_ptr(), _DT[x.dtype], None if d is None else d.data_ptr(),
+                    _DT[ctx.delta_dtype], w.data_ptr(), _DT[w.dtype], eps, M, C, None if d is None else xs.data_ptr(),
+                    h.data_ptr(), _DT[out_dtype], rstd.data_ptr())
+        ctx.save_for_backward(xs, weight, rstd)
+        return xs, h
 
     @staticmethod
     def backward(ctx, dxs, dh):
-        x, delta, weight, xs, rstd = ctx.saved_tensors
-        wants = ctx.needs_input_grad[:3]
-        if dxs is None and dh is None:
-            return None, None, None, None, None
-        if torch.is_grad_enabled():
-            pairs = [(t, want) for t, want in zip((x, delta, weight), wants)]
-            s = x if delta is None else (x.float() + delta.float()).to(x.dtype)
-            h = F.rms_norm(s.float(), weight.shape, weight.float(), ctx.eps).to(ctx.out_dtype)
-            outs = [(o, g) for o, g in ((s, dxs), (h, dh)) if g is not None]
-            got = iter(torch.autograd.grad([o for o, _ in outs], [t for t, want in pairs if want], [g for _, g in outs],
-                                           create_graph=True, allow_unused=True))
-            return (*(next(got) if want else None for _, want in pairs), None, None)
-        C = x.shape[-1]
-        M = x.numel() // C
-        dtype = x.dtype if delta is None else delta.dtype
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        ddelta = None if dtype == x.dtype or not wants[1] else torch.empty(x.shape, dtype=dtype, device=x.device)
-        dw = torch.zeros_like(weight, memory_format=torch.contiguous_format) if wants[2] and M == 0 else None
-        if M > 0:
-            s, w = xs.contiguous(), weight.contiguous()
-            dxs, dh = (None if t is None else t.contiguous() for t in (dxs, dh))
-            L = _lib.lib()
-            parts = None
-            if wants[2]:
-                dw = torch.empty(C, dtype=weight.dtype, device=x.device)
-                parts = torch.empty(L.smlm_rmsnorm_parts(M, C), dtype=torch.float32, device=x.device)
-            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            with torch.cuda.device(x.device):
-                rc = L.smlm_rmsnorm_train_backward(ptr(dxs), ptr(dh), _DT[ctx.out_dtype], s.data_ptr(), _DT[x.dtype],
-                                                   w.data_ptr(), _DT[w.dtype], rstd.data_ptr(), M, C, dx.data_ptr(),
-                                                   ptr(ddelta), _DT[dtype], ptr(dw), ptr(parts), _stream(x))
-            _lib.check(rc, "smlm_rmsnorm_train_backward")
-        return (dx if wants[0] else None, None if not wants[1] else dx if ddelta is None else ddelta, dw, None, None)
+        xs, weight, rstd = ctx.saved_tensors
+        want_x, want_delta, want_w = ctx.needs_input_grad[:3]
+        if dh is None:
+            return (dxs if want_x else None, dxs.to(ctx.delta_dtype) if want_delta and dxs is not None else None,
+                    torch.zeros_like(weight) if want_w and dxs is not None else None, None, None)
+        if torch.is_grad_enabled():                           # in terms of xs, an output of this node
+            r = (xs.float().square().mean(-1, keepdim=True) + ctx.eps).rsqrt()
+            hat = xs.float() * r
+            gw = dh.float() * weight.float()
+            dx = (gw - hat * (gw * hat).mean(-1, keepdim=True)) * r
+            dx = (dx if dxs is None else dx + dxs.float()).to(xs.dtype)
+            dw = (dh.float() * hat).reshape(-1, xs.shape[-1]).sum(0).to(weight.dtype) if want_w else None
+            return dx if want_x else None, dx.to(ctx.delta_dtype) if want_delta else None, dw, None, None
+        C = xs.shape[-1]
+        M = xs.numel() // C
+        s, w = xs.contiguous(), weight.contiguous()
+        dx = torch.empty_like(s)
+        ddelta = None if not want_delta or ctx.delta_dtype == s.dtype else torch.empty_like(s, dtype=ctx.delta_dtype)
+        dw = parts = None
+        if want_w:
+            dw = torch.empty_like(w) if M else torch.zeros_like(w)
+        if M:
+            if want_w:
+                parts = torch.empty(_workspace_bytes("smlm_rmsnorm_parts", M, C), dtype=torch.float32, device=s.device)
+            dh, dxs = dh.contiguous(), None if dxs is None else dxs.contiguous()
+            _launch("smlm_rmsnorm_train_backward", s, None if dxs is None else dxs.data_ptr(), dh.data_ptr(), _DT[dh.dtype],
+                    s.data_ptr(), _DT[s.dtype], w.data_ptr(), _DT[w.dtype], rstd.data_ptr(), M, C, dx.data_ptr(),
+                    None if ddelta is None else ddelta.data_ptr(), _DT[ctx.delta_dtype], None if dw is None else dw.data_ptr(),
+                    None if parts is None else parts.data_ptr())
+        return dx if want_x else None, (dx if ddelta is None else ddelta) if want_delta else None, dw, None, None
 
 
 def add_rmsnorm_train(x, delta, norm, out_dtype=None):

@@ -360,7 +360,7 @@ int check_loss(const char *what, const void *x, int64_t x_stride, const void *w,
   if (M < 0 || V < 1 || d < 1)
     return fail(SMLM_EINVAL, "%s: bad shape M=%lld V=%lld d=%lld", what, (long long)M, (long long)V, (long long)d);
   if (d % 8) return fail(SMLM_EUNSUPPORTED, "%s: d=%lld must be a multiple of 8", what, (long long)d);
-  if (V > (1 << 30) || d > (1 << 20) || M > (1LL << 36) / d)
+  if (V > (1 << 30) || d > (1 << 20) || M > (1 << 30) || M > (1LL << 36) / d)
     return fail(SMLM_EUNSUPPORTED, "%s: M=%lld V=%lld d=%lld too large", what, (long long)M, (long long)V, (long long)d);
   // the lanes' 32-bit byte offsets span 256 rows
   if (x_stride < d || w_stride < d || x_stride % 8 || w_stride % 8 || x_stride > kMmMaxStride || w_stride > kMmMaxStride ||

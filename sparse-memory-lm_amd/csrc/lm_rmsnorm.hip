@@ -253,6 +253,7 @@ extern "C" int smlm_rmsnorm_train(const void *x, int x_dtype, const void *delta,
   using namespace smlm;
   const char *what = "smlm_rmsnorm_train";
   if (!x || !w || !h || !rstd || (delta && !xs)) return fail(SMLM_EINVAL, "%s: null pointer argument", what);
+  if (!(eps >= 0.f)) return fail(SMLM_EINVAL, "%s: eps must not be negative", what);
   if (const int rc = check_norm(what, M, C, x_dtype, w_dtype, h_dtype, delta ? delta_dtype : x_dtype)) return rc;
   if (odd(x, x_dtype) | odd(w, w_dtype) | odd(h, h_dtype) | odd(rstd, SMLM_F32) | odd(delta, delta_dtype) | odd(xs, x_dtype))
     return fail(SMLM_EINVAL, "%s: tensors must be aligned to their elements", what);

@@ -328,6 +328,24 @@ class Block(nn.Module):
         return x
 
 
+def _norm_kernels(norm, x):
+    """Whether kernels.add_rmsnorm_train may stand in for this norm of x."""
+    w = norm.weight if type(norm) is nn.RMSNorm else None
+    return (w is not None and unhooked(norm) and w.shape == x.shape[-1:] and w.numel() <= kernels.NORM_TRAIN_MAX_COLS
+            and w.device == x.device and w.dtype in (torch.float32, torch.bfloat16)
+            and x.dtype in (torch.float32, torch.bfloat16) and ordinary(x, w))
+
+
+def _ffn_kernels(ffn, x):
+    """Whether kernels.gated_ffn may stand in for this feed-forward block behind a bf16 norm."""
+    if type(ffn) is not SwiGLU or type(ffn.w13) is not nn.Linear or type(ffn.w2) is not nn.Linear:
+        return False
+    w13, w2 = ffn.w13.weight, ffn.w2.weight
+    return (unhooked(ffn, ffn.w13, ffn.w2) and ffn.w13.bias is None and ffn.w2.bias is None
+            and w13.device == w2.device == x.device and {w13.dtype, w2.dtype} <= {torch.bfloat16, x.dtype}
+            and ordinary(w13, w2))
+
+
 class Transformer(nn.Module):
     def __init__(self, cfg, ngram_canon=None):
         """ngram_canon: the token compression table of the Engram hash ((vocab_size,) int64), needed for Engram
@@ -432,6 +450,66 @@ class Transformer(nn.Module):
             return logits
         loss = F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.reshape(-1))
         return logits, loss
+
+    def loss(self, idx, targets, ignore_index=-100, reduction="mean"):
+        """forward(idx, targets)[1] (smlm/model.py:266-293) without the logits, for training and for scoring text: the
+        cross entropy of the next-token targets (idx's shape, int64), with F.cross_entropy's ignore_index and reduction
+        ("none": idx's shape).  On the GPU in bf16 (bf16 weights or bf16 autocast) the residual adds, norms, feed-forward
+        blocks and the loss run as kernels.add_rmsnorm_train, gated_ffn and linear_cross_entropy, whose logits are not
+        rounded to bf16 as forward()'s are; anything else, and modules that are watched or replaced, runs the modules."""
+        x = self.tok_emb(idx)
+        if not self._loss_kernels(x, targets):
+            logits = self(idx).float()
+            loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1), ignore_index=ignore_index,
+                                   reduction=reduction)
+            return loss.view(targets.shape) if reduction == "none" else loss
+        rows = self._ngram_rows(idx, None) if self.ngram is not None else None
+        h = self._blocks_recorded(x, rows)
+        return kernels.linear_cross_entropy(h, self.lm_head.weight.to(torch.bfloat16), targets, ignore_index, reduction)
+
+    def _loss_kernels(self, x, targets):
+        """Whether loss() may end in linear_cross_entropy: bf16 arithmetic on the GPU, a plain output embedding and final
+        norm, nothing that watches the ops."""
+        head, bf16 = self.lm_head, torch.bfloat16
+        autocast = torch.is_autocast_enabled("cuda")
+        return (x.is_cuda and (torch.get_autocast_dtype("cuda") == bf16 if autocast else x.dtype == bf16)
+                and type(head) is nn.Linear and head.bias is None and unhooked(head)
+                and head.weight.dtype in (bf16, x.dtype) and targets.device == x.device
+                and _norm_kernels(self.norm, x) and ordinary(x, head.weight, targets))
+
+    def _blocks_recorded(self, x, rows):
+        """The blocks of forward() over whole sequences and the final norm, with every residual add in the launch of the
+        norm that follows it: the same sequence x = x + sublayer(norm(x)).  Returns the normed last hidden state, bf16."""
+        bf16 = torch.bfloat16
+        delta = None
+
+        def normed(norm, dtype):
+            nonlocal x, delta
+            if delta is not None and (delta.dtype not in (bf16, x.dtype) or not _norm_kernels(norm, x)):
+                x, delta = x + delta, None
+            if not _norm_kernels(norm, x):
+                return norm(x)
+            x, h = kernels.add_rmsnorm_train(x, delta, norm, out_dtype=dtype)
+            delta = None
+            return h
+
+        for blk in self.layers:
+            if type(blk) is not Block or not unhooked(blk):
+                x = blk(x if delta is None else x + delta, None, 0, rows)
+                delta = None
+                continue
+            if blk.engram is not None:
+                x, delta = x if delta is None else x + delta, None
+                x = x + blk.engram(x, rows, None)
+            delta = blk.attn(normed(blk.attn_norm, bf16), None, 0)
+            if not blk.is_memory and _ffn_kernels(blk.ffn, x):
+                h = normed(blk.ffn_norm, bf16).to(bf16)
+                delta = kernels.gated_ffn(h, blk.ffn.w13.weight.to(bf16), blk.ffn.w2.weight.to(bf16))
+            else:
+                delta = blk.ffn(normed(blk.ffn_norm, x.dtype))
+            if blk.ffn_r2 is not None:
+                delta = blk.ffn_r2(normed(blk.ffn_norm_r2, x.dtype))
+        return normed(self.norm, bf16)
 
     @torch.no_grad()
     def forward_graphed(self, idx):

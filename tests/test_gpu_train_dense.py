@@ -592,3 +592,164 @@ def test_refusals():
                 lambda: kernels.add_rmsnorm_train(x, None, torch.nn.RMSNorm(16, elementwise_affine=False))):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------------------------------------------ Transformer.loss
+def lm(dtype=F32, **kw):
+    from smlm_hip.model import ModelConfig, Transformer
+    torch.manual_seed(5)
+    canon = kw.pop("canon", None)
+    m = Transformer(ModelConfig(**dict(dict(vocab_size=517, d_model=128, n_layers=3, n_heads=2, ffn_hidden=200,
+                                            max_seq_len=64), **kw)), ngram_canon=canon)
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.dim() == 2:
+                p.mul_(4.0)                   # logits that matter
+    return m.to(DEV).to(dtype)
+
+
+def batch(V=517, seed=0, ignored=True):
+    g = torch.Generator().manual_seed(seed)
+    idx = torch.randint(0, V, (3, 33), generator=g)
+    t = torch.roll(idx, -1, 1)
+    if ignored:
+        t[:, -1], t[1, 20:] = -100, -100
+    return idx.to(DEV), t.to(DEV)
+
+
+def named_grads(m, loss):
+    names, ps = zip(*[(n, p) for n, p in m.named_parameters() if p.requires_grad])
+    return dict(zip(names, torch.autograd.grad(loss, ps, allow_unused=True)))
+
+
+def spied(monkeypatch):
+    """How often the three operators ran."""
+    calls = {"linear_cross_entropy": 0, "gated_ffn": 0, "add_rmsnorm_train": 0}
+    for name in calls:
+        fn = getattr(kernels, name)
+
+        def wrapped(*a, _fn=fn, _name=name, **k):
+            calls[_name] += 1
+            return _fn(*a, **k)
+
+        monkeypatch.setattr(kernels, name, wrapped)
+    return calls
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_model_loss_against_64_bits(dtype, monkeypatch):
+    """Loss and gradients as near to a 64-bit model's as the module path's, whose bf16 roundings are more."""
+    m = lm(dtype)
+    idx, t = batch()
+    ref = lm(F32).cpu().double()
+    ref.load_state_dict({k: v.cpu().double() for k, v in m.state_dict().items()})
+    for a, b in zip(ref.layers, m.layers):
+        a.attn.rope.cos, a.attn.rope.sin = b.attn.rope.cos.cpu().double(), b.attn.rope.sin.cpu().double()
+    import smlm_hip.model as model
+    monkeypatch.setattr(model, "_attention", lambda q, k, v, mask: F.scaled_dot_product_attention(q, k, v, attn_mask=mask))
+    logits = ref(idx.cpu())
+    ref_loss = F.cross_entropy(logits.view(-1, 517), t.view(-1).cpu())
+    want = named_grads(ref, ref_loss)
+    calls = spied(monkeypatch)
+    with torch.autocast("cuda", dtype=BF16, enabled=dtype == F32):
+        loss = m.loss(idx, t)
+        assert calls == {"linear_cross_entropy": 1, "gated_ffn": 3, "add_rmsnorm_train": 7}
+        _, plain = m(idx, t)
+    assert loss.dtype == F32 and abs(loss.item() - ref_loss.item()) <= 1.5 * abs(plain.item() - ref_loss.item()) + 4 * HALF
+    got, base = named_grads(m, loss), named_grads(m, plain)
+    for n, r in want.items():
+        err = lambda g: float((g.cpu().double() - r).norm() / r.norm())  # noqa: E731
+        assert got[n].dtype == dtype and err(got[n]) <= 1.25 * err(base[n]) + 2 * HALF, (n, err(got[n]), err(base[n]))
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_model_loss_scores_text_without_gradients(reduction):
+    m = lm(BF16).eval()
+    idx, t = batch()
+    with torch.no_grad():
+        got, logits = m.loss(idx, t, reduction=reduction), m(idx)
+    ref = F.cross_entropy(logits.double().view(-1, 517), t.view(-1), reduction="none").view(t.shape)
+    if reduction == "sum":
+        assert abs(got.item() - ref.sum().item()) <= 0.02 * ref.sum().item()
+        return
+    assert got.shape == t.shape and not got.requires_grad and not got[t == -100].any()
+    # the module path rounds its logits (of size s) to bf16 and both round the hidden state
+    s = logits.double().abs().amax(-1)
+    assert ((got.double() - ref).abs() <= 8 * HALF * (1 + s)).all()
+
+
+def test_model_loss_with_memory_and_engram_layers(monkeypatch):
+    """Memory layers get the stream's type, Engram layers the summed stream; the table's row-sparse gradients arrive."""
+    m = lm(F32, d_model=64, n_heads=2, ffn_hidden=96, n_layers=4, mem_layers=[1, 2], mem_n_keys=16, mem_heads=2, mem_knn=4,
+           mem_k_dim=32, mem_share_values=True, mem_round_layers=[2], eng_layers=[0, 3], eng_heads=2, eng_head_dim=8,
+           eng_rows=101, canon=torch.arange(517)).train()
+    idx, t = batch()
+    calls = spied(monkeypatch)
+    state = {k: v.clone() for k, v in m.state_dict().items()}
+    with torch.autocast("cuda", dtype=BF16):
+        loss = m.loss(idx, t)
+        assert calls == {"linear_cross_entropy": 1, "gated_ffn": 2, "add_rmsnorm_train": 10}
+        got = named_grads(m, loss)
+        m.load_state_dict(state)
+        _, plain = m(idx, t)
+        want = named_grads(m, plain)
+    assert abs(loss.item() - plain.item()) <= 0.03 * plain.item()
+    for n, g in want.items():
+        assert (g is None) == (got[n] is None), n
+
+
+@pytest.mark.parametrize("watch", ["norm", "ffn", "block", "head", "subclass", "final"])
+def test_model_loss_keeps_watched_modules(watch, monkeypatch):
+    m = lm(BF16)
+    idx, t = batch()
+    seen = []
+    target = {"norm": m.layers[1].ffn_norm, "ffn": m.layers[1].ffn.w2, "block": m.layers[1], "head": m.lm_head,
+              "final": m.norm}.get(watch)
+    if target is not None:
+        target.register_forward_hook(lambda *a: seen.append(1))
+    else:
+        class Other(torch.nn.Parameter):
+            pass
+        m.layers[1].ffn.w13.weight = Other(m.layers[1].ffn.w13.weight.detach())
+    calls = spied(monkeypatch)
+    loss = m.loss(idx, t)
+    _, plain = m(idx, t)
+    assert abs(loss.item() - plain.item()) <= 0.03 * plain.item()
+    if target is not None:
+        assert len(seen) == 2                              # once in each
+    expected = {"norm": (1, 3, 6), "ffn": (1, 2, 7), "block": (1, 2, 5), "head": (0, 0, 0), "subclass": (1, 2, 7),
+                "final": (0, 0, 0)}[watch]
+    assert tuple(calls.values()) == expected, calls
+
+
+def test_model_loss_follows_function_transforms():
+    """Under a function mode the modules run, and it sees their ops."""
+    from torch.overrides import TorchFunctionMode
+
+    class Count(TorchFunctionMode):
+        n = 0
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            Count.n += func is F.cross_entropy
+            return func(*args, **(kwargs or {}))
+
+    m = lm(BF16)
+    idx, t = batch()
+    with Count(), torch.no_grad():
+        m.loss(idx, t)
+    assert Count.n == 1
+
+
+def test_model_trains_on_the_loss():
+    """Ten steps on one batch run and change every parameter."""
+    m = lm(F32).train()
+    idx, t = batch()
+    before = {n: p.detach().clone() for n, p in m.named_parameters()}
+    opt = torch.optim.AdamW(m.parameters(), lr=1e-3)
+    for _ in range(10):
+        with torch.autocast("cuda", dtype=BF16):
+            loss = m.loss(idx, t)
+        loss.backward()
+        opt.step()
+        opt.zero_grad()
+    assert torch.isfinite(loss) and all(not torch.equal(p, before[n]) for n, p in m.named_parameters())

@@ -1,0 +1,141 @@
+"""The dense training operators without a GPU: argument checks of the library and the wrappers, before anything is
+launched, and Transformer.loss where it runs the modules."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from smlm_hip import _lib, kernels
+from smlm_hip.model import ModelConfig, Transformer
+
+FAKE = 256                    # a 16-byte aligned address that is never read: the checks fail first
+BIG = 1 << 60
+
+
+def loss_call(**kw):
+    ok = dict(x=FAKE, ldx=64, w=FAKE, ldw=64, t=FAKE, ignore=-100, reduction=_lib.REDUCE_MEAN, M=10, V=100, d=64, loss=FAKE,
+              lse=FAKE, ws=FAKE, bytes=BIG)
+    return _lib.lib().smlm_linear_ce(*dict(ok, **kw).values(), None)
+
+
+def test_linear_ce_refusals():
+    for name in ("x", "w", "t", "loss", "lse"):
+        assert loss_call(**{name: None}) == _lib.EINVAL and "null" in _lib.last_error(), name
+    for name in ("x", "w"):
+        assert loss_call(**{name: FAKE + 8}) == _lib.EINVAL and "aligned" in _lib.last_error(), name
+    assert loss_call(t=FAKE + 4) == _lib.EINVAL
+    assert loss_call(ldx=56) == loss_call(ldw=60) == loss_call(ldx=68) == loss_call(ldw=(1 << 21) + 8) == _lib.EINVAL
+    assert loss_call(M=-1) == loss_call(V=0) == loss_call(d=0) == loss_call(reduction=3) == loss_call(reduction=-1) == _lib.EINVAL
+    assert loss_call(d=60) == loss_call(V=1 << 31) == loss_call(M=1 << 40) == loss_call(M=(1 << 30) + 1, d=8) == _lib.EUNSUPPORTED
+    assert loss_call(ws=None) == loss_call(ws=FAKE + 8) == loss_call(bytes=100) == _lib.EINVAL
+    assert "workspace" in _lib.last_error()
+    assert loss_call(M=0, reduction=_lib.REDUCE_NONE) == _lib.OK and loss_call(M=0) == _lib.EINVAL
+
+
+def test_linear_ce_backward_refusals():
+    ok = dict(g=FAKE, count=None, per_token=0, x=FAKE, ldx=64, w=FAKE, ldw=64, t=FAKE, ignore=-100, lse=FAKE, M=10, V=100, d=64,
+              dx=FAKE, dw=FAKE, ws=FAKE, bytes=BIG)
+
+    def call(**kw):
+        return _lib.lib().smlm_linear_ce_backward(*dict(ok, **kw).values(), None)
+
+    for name in ("g", "x", "w", "t", "lse"):
+        assert call(**{name: None}) == _lib.EINVAL and "null" in _lib.last_error(), name
+    assert call(dx=None, dw=None) == _lib.EINVAL
+    assert call(dx=FAKE + 8) == call(dw=FAKE + 8) == call(M=0) == call(ws=FAKE + 4) == call(bytes=1000) == _lib.EINVAL
+    assert call(d=12) == _lib.EUNSUPPORTED
+
+
+@pytest.mark.parametrize("M,V,d", [(1, 1, 8), (64, 32000, 384), (129, 50304, 384), (16384, 50304, 384), (100000, 65536, 64),
+                                   (1 << 22, 1000, 8)])
+def test_linear_ce_workspaces_are_bounded(M, V, d):
+    """The gradient's pieces stay within 1 GiB (or 256 columns), and its parts within what 128 splits take."""
+    lib = _lib.lib()
+    assert 0 < lib.smlm_linear_ce_workspace(M, V, d, 0) <= M * 8 * 1024 + (M + 64) * 16 + 4096
+    grad = lib.smlm_linear_ce_workspace(M, V, d, 1)
+    assert 0 < grad <= max(1 << 30, M * 512) + 256 + 128 * M * d * 4
+    assert lib.smlm_linear_ce_workspace(0, V, d, 1) == 0
+
+
+def ffn_call(**kw):
+    ok = dict(x=FAKE, ldx=64, w13=FAKE, ld13=64, w2=FAKE, ld2=96, M=10, d=64, hidden=96, o=64, y=FAKE, ws=FAKE, bytes=BIG)
+    return _lib.lib().smlm_gated_ffn(*dict(ok, **kw).values(), None)
+
+
+def test_gated_ffn_refusals():
+    for name in ("x", "w13", "w2", "y"):
+        assert ffn_call(**{name: None}) == _lib.EINVAL, name
+        assert ffn_call(**{name: FAKE + 8}) == _lib.EINVAL, name
+    assert ffn_call(ldx=60) == ffn_call(ld13=56) == ffn_call(ld2=100) == ffn_call(ld2=(1 << 21) + 8) == _lib.EINVAL
+    assert ffn_call(d=60) == ffn_call(hidden=100, ld2=104) == ffn_call(o=4) == ffn_call(M=1 << 34) == _lib.EUNSUPPORTED
+    assert ffn_call(M=-1) == ffn_call(d=0) == ffn_call(hidden=0) == ffn_call(o=0) == _lib.EINVAL
+    assert ffn_call(ws=None) == ffn_call(bytes=64) == _lib.EINVAL
+    assert ffn_call(M=0) == _lib.OK
+    ok = dict(dy=FAKE, ldy=64, x=FAKE, ldx=64, w13=FAKE, ld13=64, w2=FAKE, ld2=96, M=10, d=64, hidden=96, o=64, dx=FAKE,
+              dw13=FAKE, dw2=FAKE, ws=FAKE, bytes=BIG)
+
+    def back(**kw):
+        return _lib.lib().smlm_gated_ffn_backward(*dict(ok, **kw).values(), None)
+
+    for name in ("dy", "x", "w13", "w2"):
+        assert back(**{name: None}) == _lib.EINVAL, name
+    for name in ("dy", "dx", "dw13", "dw2"):
+        assert back(**{name: FAKE + 8}) == _lib.EINVAL, name
+    assert back(dx=None, dw13=None, dw2=None) == back(M=0) == back(ldy=56) == back(bytes=64) == _lib.EINVAL
+
+
+def test_rmsnorm_train_refusals():
+    lib = _lib.lib()
+    ok = dict(x=FAKE, xt=_lib.F32, delta=FAKE, dt=_lib.BF16, w=FAKE, wt=_lib.F32, eps=1e-5, M=10, C=64, xs=FAKE, h=FAKE,
+              ht=_lib.BF16, rstd=FAKE)
+
+    def call(**kw):
+        return lib.smlm_rmsnorm_train(*dict(ok, **kw).values(), None)
+
+    for name in ("x", "w", "xs", "h", "rstd"):
+        assert call(**{name: None}) == _lib.EINVAL, name
+        assert call(**{name: FAKE + 1}) == _lib.EINVAL, name
+    assert call(xt=_lib.F16) == call(wt=_lib.I8) == call(ht=_lib.I64) == call(xt=_lib.BF16, dt=_lib.F32) == _lib.EINVAL
+    assert call(M=-1) == call(C=0) == call(eps=-1.0) == call(eps=float("nan")) == _lib.EINVAL
+    assert call(C=16385) == _lib.EUNSUPPORTED
+    assert call(M=0) == call(M=0, delta=None, xs=None) == _lib.OK
+    ok = dict(dxs=FAKE, dh=FAKE, ht=_lib.BF16, xs=FAKE, xt=_lib.F32, w=FAKE, wt=_lib.F32, rstd=FAKE, M=10, C=64, dx=FAKE,
+              ddelta=FAKE, dt=_lib.BF16, dw=FAKE, parts=FAKE)
+
+    def back(**kw):
+        return lib.smlm_rmsnorm_train_backward(*dict(ok, **kw).values(), None)
+
+    for name in ("xs", "w", "rstd", "dx", "parts"):
+        assert back(**{name: None}) == _lib.EINVAL, name
+    assert back(dxs=None, dh=None) == back(M=0) == back(xt=_lib.BF16, dt=_lib.F32) == back(dw=FAKE + 2) == _lib.EINVAL
+    assert back(C=16385) == _lib.EUNSUPPORTED
+    assert lib.smlm_rmsnorm_parts(1 << 30, 64) <= 1024 * 64 and lib.smlm_rmsnorm_parts(1, 7) == 7
+
+
+def test_the_wrappers_want_a_gpu():
+    x, w, t = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(30, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: kernels.linear_cross_entropy(x, w, t), lambda: kernels.gated_ffn(x, w, w[:, :15].contiguous()),
+                 lambda: kernels.add_rmsnorm_train(x, None, torch.nn.RMSNorm(16))):
+        with pytest.raises(ValueError, match="device"):
+            call()
+
+
+def small(**kw):
+    torch.manual_seed(3)
+    return Transformer(ModelConfig(**dict(dict(vocab_size=67, d_model=32, n_layers=2, n_heads=2, ffn_hidden=48, max_seq_len=16),
+                                          **kw)))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_on_the_cpu_is_the_modules(reduction):
+    m = small()
+    idx = torch.randint(0, 67, (2, 9), generator=torch.Generator().manual_seed(0))
+    t = torch.roll(idx, -1, 1)
+    t[:, -1] = 5
+    logits, mean = m(idx, t)
+    assert torch.equal(m.loss(idx, t), mean)
+    t[0, 3] = -1
+    got = m.loss(idx, t, ignore_index=-1, reduction=reduction)
+    ref = F.cross_entropy(logits.view(-1, 67), t.view(-1), ignore_index=-1, reduction=reduction)
+    assert torch.equal(got.reshape(-1), ref.reshape(-1)) and got.shape == (t.shape if reduction == "none" else ())
+    got.sum().backward()
+    assert m.tok_emb.weight.grad is not None

@@ -543,7 +543,7 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
  * is any other index outside the vocabulary; their mean over the tokens that are not ignored (NaN if none), or sum.
  *   x (M, d) and w (V, d) bf16, rows of x_row_stride / w_row_stride elements (multiples of 8, 16-byte aligned, at most
  *   2^21), d a multiple of 8; targets (M,) int64
- *   loss  SMLM_REDUCE_NONE: (M,) fp32; otherwise fp32[2]: the loss, and the number of tokens that are not ignored
+ *   loss  SMLM_REDUCE_NONE: (M,) fp32, count unused; otherwise one fp32, and count one fp32: the tokens not ignored
  *   lse   (M,) fp32: the tokens' logsumexp, which the gradient needs
  * workspace: smlm_linear_ce_workspace(M, V, d, 0) bytes, 16-byte aligned, free again when the call's work is done.
  * Logits and sums in fp32, the sum over the tokens in fp64; the same result on every call.
@@ -551,8 +551,8 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
 enum smlm_reduction { SMLM_REDUCE_NONE = 0, SMLM_REDUCE_MEAN = 1, SMLM_REDUCE_SUM = 2 };
 int64_t smlm_linear_ce_workspace(int64_t M, int64_t V, int64_t d, int grad);
 int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w_row_stride, const int64_t *targets,
-                   int64_t ignore_index, int reduction, int64_t M, int64_t V, int64_t d, float *loss, float *lse,
-                   void *workspace, int64_t workspace_bytes, void *stream);
+                   int64_t ignore_index, int reduction, int64_t M, int64_t V, int64_t d, float *loss, float *count,
+                   float *lse, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * Its gradient: dx = G W (M, d) and dw = G^T x (V, d), contiguous bf16, either NULL if not wanted, with

@@ -282,8 +282,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// out[0] = the loss, out[1] = the number of tokens that count.
-__global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict__ sums, int64_t n, int mean, float *out) {
+// The loss, and the number of tokens that count.
+__global__ void __launch_bounds__(1024)
+    loss_sum_kernel(const double *__restrict__ sums, int64_t n, int mean, float *loss, float *count) {
   __shared__ double s[2][16];
   double v[2] = {0.0, 0.0};
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
@@ -301,8 +302,8 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const double *__restrict
       a += s[0][i];
       b += s[1][i];
     }
-    out[0] = (float)(mean ? a / b : a);  // no token counts: NaN, as F.cross_entropy
-    out[1] = (float)b;
+    *loss = (float)(mean ? a / b : a);  // no token counts: NaN, as F.cross_entropy
+    *count = (float)b;
   }
 }
 
@@ -386,11 +387,12 @@ extern "C" int64_t smlm_linear_ce_workspace(int64_t M, int64_t V, int64_t d, int
 
 extern "C" int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w_row_stride,
                               const int64_t *targets, int64_t ignore_index, int reduction, int64_t M, int64_t V, int64_t d,
-                              float *loss, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
+                              float *loss, float *count, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
   using namespace smlm;
   const char *what = "smlm_linear_ce";
   if (const int rc = check_loss(what, x, x_row_stride, w, w_row_stride, targets, M, V, d)) return rc;
-  if (!loss || !lse) return fail(SMLM_EINVAL, "%s: null loss or lse pointer", what);
+  if (!loss || !lse || (!count && reduction != SMLM_REDUCE_NONE))
+    return fail(SMLM_EINVAL, "%s: null loss, count or lse pointer", what);
   if (reduction < SMLM_REDUCE_NONE || reduction > SMLM_REDUCE_SUM)
     return fail(SMLM_EINVAL, "%s: unknown reduction %d", what, reduction);
   if (M == 0) return reduction == SMLM_REDUCE_NONE ? SMLM_OK : fail(SMLM_EINVAL, "%s: nothing to reduce", what);
@@ -423,7 +425,8 @@ extern "C" int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w
                      ignore_index, M, V, lse, reduction == SMLM_REDUCE_NONE ? loss : nullptr, sums);
   if (const int rc = launch_status(what)) return rc;
   if (!sums) return SMLM_OK;
-  hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, sums, blocks, reduction == SMLM_REDUCE_MEAN ? 1 : 0, loss);
+  hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, s, sums, blocks, reduction == SMLM_REDUCE_MEAN ? 1 : 0, loss,
+                     count);
   return launch_status(what);
 }
 

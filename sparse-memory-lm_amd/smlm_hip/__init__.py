@@ -4,6 +4,6 @@
                       pk_scores and the int8 table format, backed by libsmlm_pkm.so (include/smlm_pkm.h)
     smlm_hip.pkm      ProductKeyMemory (module API of smlm/pkm.py, impl="hip")
     smlm_hip.model    ModelConfig / Transformer (entry points of smlm/model.py) + whole-step graph decode
-    smlm_hip.build    hipcc build of libsmlm_pkm.so
+    smlm_hip.build    hipcc build of libsmlm_pkm.so, and the autograd nodes _train_ops.so
 """
 __all__ = ["kernels", "pkm", "model"]

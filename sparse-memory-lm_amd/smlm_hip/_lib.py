@@ -11,6 +11,7 @@ import torch  # noqa: F401  (see module docstring)
 
 LIB_NAME = "libsmlm_pkm.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
+TRAIN_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_train_ops.so")
 
 # smlm_dtype / smlm_status values of include/smlm_pkm.h
 F32, BF16, F16, I8, Q4, I32, I64 = range(7)
@@ -79,7 +80,7 @@ EXPORTS = {
     "smlm_engram_mix_parts": (_i64, [_i64, _i64, _i, _i]),
     "smlm_engram_mix_backward": (_i, [_p] * 8 + [_i64, _i64, _i, _i, _i, _f] + [_p] * 9),
     "smlm_linear_ce_workspace": (_i64, [_i64, _i64, _i64, _i]),
-    "smlm_linear_ce": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _p, _p, _p, _i64, _p]),
+    "smlm_linear_ce": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
     "smlm_linear_ce_backward": (_i, [_p, _p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,
                                      _p]),
     "smlm_gated_ffn": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p]),
@@ -118,6 +119,23 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_train = None
+
+
+def train_ops():
+    """The autograd nodes of csrc/torch/train_ops.cpp (loaded once, after the library that they call). Raises if they have
+    not been built."""
+    global _train
+    if _train is None:
+        lib()
+        if not os.path.exists(TRAIN_PATH):
+            raise RuntimeError(f"{TRAIN_PATH} is not built (run `python -m smlm_hip.build` in sparse-memory-lm_amd/ or "
+                               "__graft_entry__.build()); the training operators have no fallback")
+        from . import _train_ops
+        _train = _train_ops
+    return _train
 
 
 def version():

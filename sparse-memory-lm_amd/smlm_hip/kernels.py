@@ -33,11 +33,9 @@ The dense operators of a training step, differentiable (Transformer.loss calls t
     add_rmsnorm_train(x, delta, norm)       (residual add + RMSNorm, smlm/model.py:156-163)
 """
 import ctypes
-import functools
 import math
 
 import torch
-import torch.nn.functional as F
 
 from . import _lib
 
@@ -1157,184 +1155,15 @@ def engram_mix_backward(gy, h, k, v, wh, wk, wv, conv, dilation, eps):
 # ---------------------------------------------------------------------------------------------------------------
 # The dense operators of a training step
 # ---------------------------------------------------------------------------------------------------------------
-def _one_device(name, first, *others):
-    _need_cuda(name, first, *others)
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
-
-
-def _launch(name, t, *args):
-    """The library's entry point `name` on t's device and torch's current stream there.  A backward runs on a thread of
-    autograd's own, where every Python object costs three times as much as here: no device guard where t's device is
-    the current one, and no stream object."""
-    device = t.get_device()
-    if torch._C._cuda_getDevice() == device:
-        rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
-    if rc:
-        _lib.check(rc, name)
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(name, *sizes):
-    """Bytes (or, for a norm's parts, floats) of an entry point's workspace, a function of the sizes alone."""
-    return getattr(_lib.lib(), name)(*sizes)
-
-
-def _workspace(name, like, *sizes):
-    return torch.empty(_workspace_bytes(name, *sizes), dtype=torch.uint8, device=like.device)
-
-
-MAX_ROW_STRIDE = 1 << 21      # elements between the rows of a training product's operand (csrc/lm_loss.hip)
-
-
-def _mm_rows(t, rows, cols):
-    """t (rows', cols') bf16 as the training products read it: rows of 16-byte aligned, 8-element pieces, zeros from
-    rows' and cols' up to rows and cols."""
-    if t.shape != (rows, cols):
-        return F.pad(t, (0, cols - t.shape[1], 0, rows - t.shape[0]))
-    if t.stride(1) != 1 or t.stride(0) % 8 or not cols <= t.stride(0) <= MAX_ROW_STRIDE or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _ceil8(n):
-    return -(-n // 8) * 8
-
-
-_REDUCTIONS = {"none": _lib.REDUCE_NONE, "mean": _lib.REDUCE_MEAN, "sum": _lib.REDUCE_SUM}
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    """linear_cross_entropy's node: keeps its inputs, the tokens' logsumexp and the number of tokens that count.  A
-    backward that is itself recorded (create_graph) differentiates the PyTorch ops."""
-
-    @staticmethod
-    def forward(ctx, x, weight, targets, ignore_index, reduction):
-        d, V = x.shape[-1], weight.shape[0]
-        M, d8 = x.numel() // d, _ceil8(d)
-        t = targets.reshape(-1).contiguous()
-        lse = torch.empty(M, dtype=torch.float32, device=x.device)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        if M == 0:
-            ctx.save_for_backward(x, weight, targets, lse, lse)
-            if reduction == "none":
-                return lse.view(targets.shape)
-            return torch.full((), float("nan") if reduction == "mean" else 0.0, dtype=torch.float32, device=x.device)
-        loss = torch.empty(M if reduction == "none" else 2, dtype=torch.float32, device=x.device)
-        x2, w2 = _mm_rows(x.reshape(M, d), M, d8), _mm_rows(weight, V, d8)
-        ws = _workspace("smlm_linear_ce_workspace", x, M, V, d8, 0)
-        _launch("smlm_linear_ce", x, x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), t.data_ptr(), ignore_index,
-                _REDUCTIONS[reduction], M, V, d8, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel())
-        ctx.save_for_backward(x, weight, targets, lse, loss)
-        return loss.view(targets.shape) if reduction == "none" else loss[0].clone()
-
-    @staticmethod
-    def backward(ctx, g):
-        x, weight, targets, lse, loss = ctx.saved_tensors
-        wants = ctx.needs_input_grad[:2]
-        if torch.is_grad_enabled():
-            inputs = [t for t, want in zip((x, weight), wants) if want]
-            y = F.cross_entropy(x.float().reshape(-1, x.shape[-1]) @ weight.float().T, targets.reshape(-1),
-                                ignore_index=ctx.ignore_index, reduction=ctx.reduction)
-            got = iter(torch.autograd.grad(y.view(g.shape), inputs, g, create_graph=True))
-            return (*(next(got) if want else None for want in wants), None, None, None)
-        d, V = x.shape[-1], weight.shape[0]
-        M, d8 = x.numel() // d, _ceil8(d)
-        if M == 0:
-            return torch.zeros_like(x), torch.zeros_like(weight), None, None, None
-        x2, w2 = _mm_rows(x.reshape(M, d), M, d8), _mm_rows(weight, V, d8)
-        t, g = targets.reshape(-1).contiguous(), g.reshape(-1).float().contiguous()
-        dx = torch.empty(M, d8, dtype=x.dtype, device=x.device) if wants[0] else None
-        dw = torch.empty(V, d8, dtype=x.dtype, device=x.device) if wants[1] else None
-        ws = _workspace("smlm_linear_ce_workspace", x, M, V, d8, 1)
-        count = loss.data_ptr() + 4 if ctx.reduction == "mean" else None
-        _launch("smlm_linear_ce_backward", x, g.data_ptr(), count, ctx.reduction == "none", x2.data_ptr(), x2.stride(0),
-                w2.data_ptr(), w2.stride(0), t.data_ptr(), ctx.ignore_index, lse.data_ptr(), M, V, d8,
-                None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel())
-        if d8 != d:
-            dx, dw = (t if t is None else t[:, :d].contiguous() for t in (dx, dw))
-        return None if dx is None else dx.view(x.shape), dw, None, None, None
-
-
 def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
     """F.cross_entropy(x @ weight.T, targets) on fp32 logits that are never stored (smlm/model.py:286-293; smlm_linear_ce):
     x (..., d) bf16, weight (V, d) bf16 (the output embedding), targets (...) int64.  Tokens whose target is ignore_index
     count for nothing; any other target outside the vocabulary gives a NaN loss and NaN gradients.  reduction "mean" (over
     the tokens that count; NaN if none), "sum" (both 0-d fp32) or "none" (targets' shape, fp32).
     Differentiable in x and weight, both bf16: the gradient forms the logits again, in pieces of the vocabulary, from the
-    inputs and one fp32 per token.  Sums in fp32, softmax and gradient rounded to bf16 once as operands of its products
-    and once as results; the same bits on every call.  A width that is not a multiple of 8, or rows that are not 16-byte
-    aligned, are copied first."""
-    _one_device("linear_cross_entropy", x, weight, targets)
-    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
-        raise ValueError(f"linear_cross_entropy: x and weight must be bf16, got {x.dtype} and {weight.dtype}")
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
-        raise ValueError(f"linear_cross_entropy: expected x (..., d) and weight (V, d), got {tuple(x.shape)} and "
-                         f"{tuple(weight.shape)}")
-    if targets.dtype != torch.int64 or targets.shape != x.shape[:-1]:
-        raise ValueError(f"linear_cross_entropy: targets must be {tuple(x.shape[:-1])} int64, got {targets.dtype} "
-                         f"{tuple(targets.shape)}")
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    return _LinearCrossEntropy.apply(x, weight, targets, int(ignore_index), reduction)
-
-
-class _GatedFFN(torch.autograd.Function):
-    """gated_ffn's node: keeps its inputs only.  A backward that is itself recorded differentiates the PyTorch ops."""
-
-    @staticmethod
-    def _operands(x, w13, w2):
-        d, h, o = x.shape[-1], w2.shape[1], w2.shape[0]
-        M, d8, h8, o8 = x.numel() // d, _ceil8(d), _ceil8(h), _ceil8(o)
-        x2 = _mm_rows(x.reshape(M, d), M, d8)
-        if h8 != h:                                            # the halves end on whole pieces
-            w13 = F.pad(w13.reshape(2, h, d), (0, d8 - d, 0, h8 - h)).view(2 * h8, d8)
-        return x2, _mm_rows(w13, 2 * h8, d8), _mm_rows(w2, o8, h8), M, d8, h8, o8
-
-    @staticmethod
-    def forward(ctx, x, w13, w2):
-        ctx.save_for_backward(x, w13, w2)
-        o = w2.shape[0]
-        if x.numel() == 0:
-            return x.new_empty(*x.shape[:-1], o)
-        a, b, c, M, d8, h8, o8 = _GatedFFN._operands(x, w13, w2)
-        ws = _workspace("smlm_gated_ffn_workspace", x, M, d8, h8, o8, 0)
-        y = torch.empty(M, o8, dtype=x.dtype, device=x.device)
-        _launch("smlm_gated_ffn", x, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0), M, d8,
-                h8, o8, y.data_ptr(), ws.data_ptr(), ws.numel())
-        return (y if o8 == o else y[:, :o].contiguous()).view(*x.shape[:-1], o)
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, w13, w2 = ctx.saved_tensors
-        wants = ctx.needs_input_grad
-        if torch.is_grad_enabled():
-            inputs = [t for t, want in zip((x, w13, w2), wants) if want]
-            a, b = F.linear(x.float(), w13.float()).chunk(2, dim=-1)
-            y = F.linear(F.silu(a) * b, w2.float()).to(dy.dtype)
-            got = iter(torch.autograd.grad(y, inputs, dy, create_graph=True))
-            return tuple(next(got) if want else None for want in wants)
-        if x.numel() == 0:
-            return torch.zeros_like(x), torch.zeros_like(w13), torch.zeros_like(w2)
-        (o, h), d = w2.shape, x.shape[-1]
-        a, b, c, M, d8, h8, o8 = _GatedFFN._operands(x, w13, w2)
-        g = _mm_rows(dy.reshape(M, o), M, o8)
-        out = [torch.empty(*s, dtype=x.dtype, device=x.device) if want else None
-               for s, want in zip(((M, d8), (2 * h8, d8), (o8, h8)), wants)]
-        ws = _workspace("smlm_gated_ffn_workspace", x, M, d8, h8, o8, 1)
-        dx, dw13, dw2 = out
-        _launch("smlm_gated_ffn_backward", x, g.data_ptr(), g.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
-                c.data_ptr(), c.stride(0), M, d8, h8, o8, None if dx is None else dx.data_ptr(),
-                None if dw13 is None else dw13.data_ptr(), None if dw2 is None else dw2.data_ptr(), ws.data_ptr(), ws.numel())
-        if (d8, h8, o8) != (d, h, o):
-            dx = None if dx is None else dx[:, :d].contiguous()
-            dw13 = None if dw13 is None else dw13.view(2, h8, d8)[:, :h, :d].reshape(2 * h, d)
-            dw2 = None if dw2 is None else dw2[:o, :h].contiguous()
-        return None if dx is None else dx.view(x.shape), dw13, dw2
+    inputs and one fp32 per token.  Sums in fp32, the gradient of the logits rounded to bf16 as operand of its products; the
+    same bits on every call.  A width that is not a multiple of 8, or rows that are not 16-byte aligned, are copied first."""
+    return _lib.train_ops().linear_cross_entropy(x, weight, targets, int(ignore_index), reduction)
 
 
 def gated_ffn(x, w13, w2):
@@ -1344,73 +1173,10 @@ def gated_ffn(x, w13, w2):
     inputs is kept for the gradient, which forms a and b again (smlm_gated_ffn_backward); its sums are in fp32, the
     gradients of a and b rounded to bf16 as operands.  The same bits on every call.  Sizes that are not multiples of 8, or
     rows that are not 16-byte aligned, are copied first."""
-    _one_device("gated_ffn", x, w13, w2)
-    if any(t.dtype != torch.bfloat16 for t in (x, w13, w2)):
-        raise ValueError(f"gated_ffn: x, w13 and w2 must be bf16, got {x.dtype}, {w13.dtype} and {w2.dtype}")
-    if x.dim() < 1 or w13.dim() != 2 or w2.dim() != 2 or w13.shape != (2 * w2.shape[1], x.shape[-1]) or 0 in w13.shape \
-            or 0 in w2.shape:
-        raise ValueError(f"gated_ffn: expected x (..., d), w13 (2 * hidden, d) and w2 (n_out, hidden), got "
-                         f"{tuple(x.shape)}, {tuple(w13.shape)} and {tuple(w2.shape)}")
-    return _GatedFFN.apply(x, w13, w2)
+    return _lib.train_ops().gated_ffn(x, w13, w2)
 
 
 NORM_TRAIN_MAX_COLS = 16384        # csrc/lm_rmsnorm.hip
-
-
-class _AddRMSNorm(torch.autograd.Function):
-    """add_rmsnorm_train's node: keeps the sum, the weight and one fp32 per row.  A backward that is itself recorded runs
-    as PyTorch ops."""
-
-    @staticmethod
-    def forward(ctx, x, delta, weight, eps, out_dtype):
-        ctx.set_materialize_grads(False)
-        C = x.shape[-1]
-        M = x.numel() // C
-        a, w = x.contiguous(), weight.contiguous()
-        d = None if delta is None else delta.contiguous()
-        xs = x if d is None else torch.empty_like(a)          # nothing to add: x itself, as an output of this node
-        h = torch.empty_like(a, dtype=out_dtype)
-        rstd = torch.empty(M, dtype=torch.float32, device=x.device)
-        ctx.delta_dtype, ctx.eps = x.dtype if d is None else d.dtype, eps
-        if M:
-            _launch("smlm_rmsnorm_train", x, a.data_ptr(), _DT[x.dtype], None if d is None else d.data_ptr(),
-                    _DT[ctx.delta_dtype], w.data_ptr(), _DT[w.dtype], eps, M, C, None if d is None else xs.data_ptr(),
-                    h.data_ptr(), _DT[out_dtype], rstd.data_ptr())
-        ctx.save_for_backward(xs, weight, rstd)
-        return xs, h
-
-    @staticmethod
-    def backward(ctx, dxs, dh):
-        xs, weight, rstd = ctx.saved_tensors
-        want_x, want_delta, want_w = ctx.needs_input_grad[:3]
-        if dh is None:
-            return (dxs if want_x else None, dxs.to(ctx.delta_dtype) if want_delta and dxs is not None else None,
-                    torch.zeros_like(weight) if want_w and dxs is not None else None, None, None)
-        if torch.is_grad_enabled():                           # in terms of xs, an output of this node
-            r = (xs.float().square().mean(-1, keepdim=True) + ctx.eps).rsqrt()
-            hat = xs.float() * r
-            gw = dh.float() * weight.float()
-            dx = (gw - hat * (gw * hat).mean(-1, keepdim=True)) * r
-            dx = (dx if dxs is None else dx + dxs.float()).to(xs.dtype)
-            dw = (dh.float() * hat).reshape(-1, xs.shape[-1]).sum(0).to(weight.dtype) if want_w else None
-            return dx if want_x else None, dx.to(ctx.delta_dtype) if want_delta else None, dw, None, None
-        C = xs.shape[-1]
-        M = xs.numel() // C
-        s, w = xs.contiguous(), weight.contiguous()
-        dx = torch.empty_like(s)
-        ddelta = None if not want_delta or ctx.delta_dtype == s.dtype else torch.empty_like(s, dtype=ctx.delta_dtype)
-        dw = parts = None
-        if want_w:
-            dw = torch.empty_like(w) if M else torch.zeros_like(w)
-        if M:
-            if want_w:
-                parts = torch.empty(_workspace_bytes("smlm_rmsnorm_parts", M, C), dtype=torch.float32, device=s.device)
-            dh, dxs = dh.contiguous(), None if dxs is None else dxs.contiguous()
-            _launch("smlm_rmsnorm_train_backward", s, None if dxs is None else dxs.data_ptr(), dh.data_ptr(), _DT[dh.dtype],
-                    s.data_ptr(), _DT[s.dtype], w.data_ptr(), _DT[w.dtype], rstd.data_ptr(), M, C, dx.data_ptr(),
-                    None if ddelta is None else ddelta.data_ptr(), _DT[ctx.delta_dtype], None if dw is None else dw.data_ptr(),
-                    None if parts is None else parts.data_ptr())
-        return dx if want_x else None, (dx if ddelta is None else ddelta) if want_delta else None, dw, None, None
 
 
 def add_rmsnorm_train(x, delta, norm, out_dtype=None):
@@ -1419,17 +1185,6 @@ def add_rmsnorm_train(x, delta, norm, out_dtype=None):
     156-163; smlm_rmsnorm_train).  x (..., C) fp32 or bf16, delta of its shape, bf16 or x's type, norm an nn.RMSNorm over C
     with an fp32 or bf16 weight, C <= 16384.  Differentiable in x, delta and the norm's weight, whose gradient is summed in
     fp32 in a fixed order: the same bits on every call."""
-    weight = norm.weight
-    _one_device("add_rmsnorm_train", x, delta, weight)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if x.dtype not in _DT or out_dtype not in _DT or weight is None or weight.dtype not in _DT:
-        raise ValueError(f"add_rmsnorm_train: x, the norm's weight and out_dtype must be fp32 or bf16, got {x.dtype}, "
-                         f"{None if weight is None else weight.dtype} and {out_dtype}")
-    if delta is not None and (delta.shape != x.shape or delta.dtype not in (torch.bfloat16, x.dtype)):
-        raise ValueError(f"add_rmsnorm_train: delta must be {tuple(x.shape)} in bf16 or {x.dtype}, got {tuple(delta.shape)} "
-                         f"{delta.dtype}")
-    if x.dim() < 1 or weight.shape != x.shape[-1:] or not 0 < x.shape[-1] <= NORM_TRAIN_MAX_COLS:
-        raise ValueError(f"add_rmsnorm_train: x {tuple(x.shape)} must end with the norm's {tuple(weight.shape)}, at most "
-                         f"{NORM_TRAIN_MAX_COLS} columns")
-    eps = norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
-    return _AddRMSNorm.apply(x, delta, weight, float(eps), out_dtype)
+    if norm.weight is None:
+        raise ValueError("add_rmsnorm_train: the norm needs a weight")
+    return _lib.train_ops().add_rmsnorm_train(x, delta, norm.weight, norm.eps, out_dtype)

@@ -13,12 +13,12 @@ BIG = 1 << 60
 
 def loss_call(**kw):
     ok = dict(x=FAKE, ldx=64, w=FAKE, ldw=64, t=FAKE, ignore=-100, reduction=_lib.REDUCE_MEAN, M=10, V=100, d=64, loss=FAKE,
-              lse=FAKE, ws=FAKE, bytes=BIG)
+              count=FAKE, lse=FAKE, ws=FAKE, bytes=BIG)
     return _lib.lib().smlm_linear_ce(*dict(ok, **kw).values(), None)
 
 
 def test_linear_ce_refusals():
-    for name in ("x", "w", "t", "loss", "lse"):
+    for name in ("x", "w", "t", "loss", "count", "lse"):
         assert loss_call(**{name: None}) == _lib.EINVAL and "null" in _lib.last_error(), name
     for name in ("x", "w"):
         assert loss_call(**{name: FAKE + 8}) == _lib.EINVAL and "aligned" in _lib.last_error(), name
@@ -28,7 +28,7 @@ def test_linear_ce_refusals():
     assert loss_call(d=60) == loss_call(V=1 << 31) == loss_call(M=1 << 40) == loss_call(M=(1 << 30) + 1, d=8) == _lib.EUNSUPPORTED
     assert loss_call(ws=None) == loss_call(ws=FAKE + 8) == loss_call(bytes=100) == _lib.EINVAL
     assert "workspace" in _lib.last_error()
-    assert loss_call(M=0, reduction=_lib.REDUCE_NONE) == _lib.OK and loss_call(M=0) == _lib.EINVAL
+    assert loss_call(M=0, count=None, reduction=_lib.REDUCE_NONE) == _lib.OK and loss_call(M=0) == _lib.EINVAL
 
 
 def test_linear_ce_backward_refusals():

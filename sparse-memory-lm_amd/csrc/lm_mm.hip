@@ -2,16 +2,15 @@
 // tiles alone are too few (a weight's gradient: few outputs, many tokens), the parts added in order by a second kernel (the
 // same bits on every call).
 #include "lm_mm.h"
-#ifndef KS_K
-#define KS_K 32
-#endif
 
 #include <algorithm>
 
 namespace smlm {
 namespace {
 
-typedef MmShape<4, 2, 4, 8> Square;                       // 256 features x 256 tokens, 8 wavefronts
+constexpr int64_t kCus = 256;
+
+typedef MmShape<2, 4, 8, 4> Square;                       // 256 features x 256 tokens, 8 wavefronts
 typedef MmShape<4, 2, 6, 4> Wide;                         // 384 x 128, 8 wavefronts
 typedef MmShape<2, 2, 4, 4> Small;                        // 128 x 128, 4 wavefronts, two workgroups a CU
 typedef MmShape<2, 2, 2, 2> Tiny;                         // 64 x 64, 4 wavefronts, six a CU
@@ -19,7 +18,8 @@ typedef MmShape<2, 2, 2, 2> Tiny;                         // 64 x 64, 4 wavefron
 template <class S, bool FKC, bool TKC>
 struct MmKernel {
   static constexpr bool kPerm = FKC;                      // (k strided features: the transposing reads would conflict)
-  static constexpr int kK = FKC && TKC ? 64 : KS_K;
+  // k strided: stages of 32 k, three of them; with 64 the same products took 2 to 10% longer (two stages fit, not three)
+  static constexpr int kK = FKC && TKC ? 64 : 32;
   typedef MmTile<S::kF, FKC, kPerm, S::kThreads, kK> F;
   typedef MmTile<S::kT, TKC, false, S::kThreads, kK> T;
   typedef MmLoop<F, T, S::NI, S::NJ> Loop;
@@ -141,22 +141,30 @@ int choose(const MmArgs &a, int shape, hipStream_t stream, const char *what) {
 
 }  // namespace
 
-// The shape and the splits with the least estimated time: rounds of workgroups over the card, each with its units of 64 k
-// and what it takes to begin and end, and for parts their way through memory and a second launch.
+// The shape and the splits with the least estimated time. The workgroups of a CU share its matrix cores and its way into
+// LDS, so a unit of 64 k takes a CU `busy` us for each of its workgroups, and at least `wait` us however few they are (the
+// way from memory and the barriers); `fixed` us are the beginning, the end and the launch; the outputs' way to memory, or
+// the parts' to memory and back and a second launch, comes on top. The figures are a fit to 54 products of 1 to 50,304
+// outputs a side, each timed in every shape with up to 104 splits: the choice is the fastest one or within 5% of it, but
+// for one token's row of 384 outputs of k = 32,000 (14.7 us for 12.0); 0.5% slower in the mean. One shape for all:
+// 4,096 x 384 outputs of k = 1,024 take 10 us in Tiny, 15 in Small and 23 in Wide; 32,768 x 384 of the same k 46, 37
+// and 30; 8,192 x 2,048 of k = 5,632 take 143 in Square, 199 in Small.
 MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split) {
   struct Tile {
-    int f, t, slots;
-    double unit, fixed;                                   // us
+    int f, t;
+    double wait, busy, fixed;                             // us
   };
-  static const Tile tiles[4] = {{256, 256, 256, 1.85, 5.0}, {384, 128, 256, 1.40, 4.5}, {128, 128, 512, 1.25, 4.0}, {64, 64, 1536, 1.5, 3.5}};
+  static const Tile tiles[4] = {
+      {256, 256, 1.27, 1.51, 4.3}, {384, 128, 1.12, 1.16, 5.9}, {128, 128, 0.63, 0.47, 4.4}, {64, 64, 0.29, 0.22, 3.4}};
   const int64_t units = ceil_div(K, kMmUnit);
   MmPlan best{0, 1};
   double least = 1e30;
   for (int64_t s = 1; s <= (may_split ? 128 : 1) && (s == 1 || units / s >= 4); s += s < 16 ? 1 : 8)
     for (int i = 0; i < 4; ++i) {
-      const int64_t n = ceil_div(F, tiles[i].f) * ceil_div(T, tiles[i].t) * s;
-      double time = ceil_div(n, tiles[i].slots) * (ceil_div(units, s) * tiles[i].unit + tiles[i].fixed);
-      if (s > 1) time += 6.0 + s * T * F * 8 / 4e6;       // 4 TB/s
+      const Tile &c = tiles[i];
+      const int64_t per_cu = ceil_div(ceil_div(F, c.f) * ceil_div(T, c.t) * s, kCus);
+      double time = ceil_div(units, s) * std::max(c.wait, per_cu * c.busy) + c.fixed;
+      time += s > 1 ? 2.4 + s * T * F * 8 / 5.8e6 : T * F * 2 / 3.7e6;
       if (time < least) {
         least = time;
         best = {i, s};

@@ -204,7 +204,13 @@ __global__ void __launch_bounds__(1024)
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
   float v = 0.f;
   if (col < C)
-    for (int p = p0; p < nparts; p += 32) v += parts[p * C + col];
+    for (int p = p0; p < nparts; p += 256) {   // 8 loads in flight, added in order (one by one: 10.6 us for 1,024 parts)
+      float u[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) u[q] = p + 32 * q < nparts ? parts[(p + 32 * q) * C + col] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += u[q];
+    }
   s[p0][c] = v;
   __syncthreads();
   if (p0 > 0 || col >= C) return;

@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kLsCols = 256;                              // vocabulary columns per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kLsFinishRows = 16;                         // tokens per workgroup of the joining kernel
+constexpr int kLsFinishRows = 4;                          // tokens per workgroup of the joining kernel, one a wavefront
 constexpr int64_t kLsPieceBytes = 1LL << 30;            // most bytes of one piece's G
 constexpr int kNoTarget = -0x40000000;
 
@@ -222,24 +222,37 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
   }
 }
 
-// Joins the ranges of kLsFinishRows tokens: lse, and the losses (each) or their sum and number (sums, counts).
+// Joins the ranges of kLsFinishRows tokens: lse, and the losses (each) or their sum and number (sums, counts).  64 tokens
+// have 500 parts each: eight loads a lane in flight, 6 us (one after the other, four tokens a wavefront: 14 us).
 __global__ void __launch_bounds__(256)
     loss_join_kernel(const float2 *__restrict__ parts, int nparts, const float *__restrict__ picked,
                      const int64_t *__restrict__ targets, int64_t ignore, int64_t M, int64_t V, float *__restrict__ lse,
                      float *__restrict__ each, double *__restrict__ sums) {
-  __shared__ double sum[4];
-  __shared__ int num[4];
+  __shared__ double sum[kLsFinishRows];
+  __shared__ int num[kLsFinishRows];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int64_t t = (int64_t)blockIdx.x * kLsFinishRows + wave;
   double total = 0.0;
   int count = 0;
-  for (int q = 0; q < kLsFinishRows / 4; ++q) {
-    const int64_t t = (int64_t)blockIdx.x * kLsFinishRows + wave * (kLsFinishRows / 4) + q;
-    if (t >= M) break;
+  if (t < M) {  // wave-uniform
+    const int64_t y = targets[t];
+    const bool valid = y != ignore && y >= 0 && y < V;
+    const float s = valid ? picked[t] : 0.f;
     float m = -__builtin_inff(), l = 0.f;
-    for (int p = lane; p < nparts; p += kWave) {
-      const float2 v = parts[t * nparts + p];
-      const float top = fmaxf(m, v.x), ref = top == -__builtin_inff() ? 0.f : top;
-      l = l * exp2_hw(m - ref) + v.y * exp2_hw(v.x - ref);
+    for (int p0 = 0; p0 < nparts; p0 += 8 * kWave) {
+      float2 v[8];
+      float top = m;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int p = p0 + q * kWave + lane;
+        v[q] = p < nparts ? parts[t * nparts + p] : make_float2(-__builtin_inff(), 0.f);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) top = fmaxf(top, v[q].x);
+      const float ref = top == -__builtin_inff() ? 0.f : top;
+      l *= exp2_hw(m - ref);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) l += v[q].y * exp2_hw(v[q].x - ref);
       m = top;
     }
     for (int o = 32; o > 0; o >>= 1) {
@@ -250,16 +263,13 @@ __global__ void __launch_bounds__(256)
     }
     // loss = (m + log2(l) - s log2(e)) / log2(e), the large terms first: m and s log2(e) cancel without a rounding of
     // their size, so that it does not fall below 0 by more than the logarithm's own rounding; lse = s + loss, so that a
-    // certain token's probability is exactly 1 in the gradient
-    const int64_t y = targets[t];
-    const bool valid = y != ignore && y >= 0 && y < V;
+    // certain token's probability is exactly 1 in the gradient (s may be -inf, lse is finite then)
     const float log2l = log2f(l);
     float loss = 0.f, z = (m + log2l) * kLn2;
     if (valid) {
-      const float s = picked[t];
       loss = (fmaf(-s, kLog2e, m) + log2l) * kLn2;
       loss = loss < 0.f ? 0.f : loss;
-      z = s + loss;
+      z = s == -__builtin_inff() ? z : s + loss;
     } else if (y != ignore) {
       loss = __builtin_nanf("");
     }
@@ -267,8 +277,8 @@ __global__ void __launch_bounds__(256)
       lse[t] = z;
       if (each) each[t] = loss;
     }
-    total += loss;
-    count += y != ignore;
+    total = loss;
+    count = y != ignore;
   }
   if (!sums) return;  // workgroup-uniform
   if (lane == 0) {
@@ -287,9 +297,15 @@ __global__ void __launch_bounds__(1024)
     loss_sum_kernel(const double *__restrict__ sums, int64_t n, int mean, float *loss, float *count) {
   __shared__ double s[2][16];
   double v[2] = {0.0, 0.0};
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    v[0] += sums[2 * i];
-    v[1] += sums[2 * i + 1];
+  for (int64_t i = threadIdx.x; i < n; i += 4 * 1024) {
+    double2 u[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) u[q] = i + q * 1024 < n ? ((const double2 *)sums)[i + q * 1024] : make_double2(0.0, 0.0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[0] += u[q].x;
+      v[1] += u[q].y;
+    }
   }
   for (int o = 32; o > 0; o >>= 1)
     for (int q = 0; q < 2; ++q) v[q] += __shfl_xor(v[q], o, kWave);
@@ -344,7 +360,8 @@ struct GradPlan {
 };
 GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
   GradPlan p;
-  const int64_t most = std::max<int64_t>(kLsPieceBytes / (2 * M) / kLsCols, 1) * kLsCols;
+  // at most the products' widest rows: few tokens would have wider ones
+  const int64_t most = std::min<int64_t>(kMmMaxStride, std::max<int64_t>(kLsPieceBytes / (2 * M) / kLsCols, 1) * kLsCols);
   p.pieces = ceil_div(V, most);
   p.cols = ceil_div(ceil_div(V, p.pieces), kLsCols) * kLsCols;
   p.pieces = ceil_div(V, p.cols);

@@ -147,10 +147,40 @@ def test_loss_strided_operands(layout):
 
 
 def test_loss_in_several_pieces_of_the_vocabulary():
-    """More than 512 MB of one piece's gradient: 33,000 tokens x 10,000 columns in two pieces."""
-    M, V, d = 33000, 10000, 16
+    """More than 1 GiB of logits' gradient: 57,000 tokens x 10,000 columns in two pieces."""
+    M, V, d = 57000, 10000, 16
     note("loss", M, V, d)
     check_loss(randn(M, d), randn(V, d, std=0.5, seed=2), targets(M, V, ignored=0.1))
+
+
+def test_loss_of_few_tokens_over_a_very_large_vocabulary():
+    """Two pieces of at most 2^21 columns: the products take no wider rows."""
+    M, V, d = 3, (1 << 21) + 300, 8
+    note("loss", M, V, d)
+    t = targets(M, V)
+    t[1] = V - 1
+    check_loss(randn(M, d), randn(V, d, std=0.5, seed=2), t)
+
+
+def test_loss_excluded_vocabulary_row():
+    """A row whose logit is -inf for every token counts for nothing; as a target its loss is inf and the gradients of all
+    rows are still finite: softmax - 1 at the target."""
+    M, V, d = 40, 300, 32
+    x, w, t = randn(M, d), randn(V, d, std=0.3, seed=2), targets(M, V)
+    t[t == 5] = 6
+    x[:, 0], w[5, 0] = 1.0, float("-inf")
+    w[5, 1:] = 0
+    t[7] = 5
+    loss, _, dw = run_loss(x, w, t, "none", g=torch.ones(M, device=DEV))
+    kept = torch.arange(V, device=DEV) != 5
+    others = torch.where(t == 5, -100, t - (t > 5).long())
+    (l, lt), _, (rw, wt) = loss_reference(x, w[kept], others, -100, "none", torch.ones(M, device=DEV))
+    assert torch.isposinf(loss[7])
+    close(torch.where(t == 5, 0.0, loss), l, lt, "loss")
+    p = torch.softmax(x[7].double() @ w[kept].double().T, 0)
+    more = p.unsqueeze(1) * x[7].double()              # the excluded target's token: its probabilities, no 1 among the kept
+    close(dw[kept], rw + more, wt + 2 * HALF * (more.abs() + rw.abs()) + 2.0 ** -12 * more.abs() + TINY, "dw")
+    assert torch.equal(dw[5], -x[7])
 
 
 def test_loss_large_logits_and_certain_tokens():

@@ -6,11 +6,14 @@
 // Only the inputs are kept for the gradient: a and b are formed again there, in the launch that forms dact, so that the
 // gate's derivative is taken on fp32 accumulators and neither the projection nor dact touches memory.  (Keeping a | b
 // would save a quarter of the gradient's first launch, and cost 4 hidden bytes a token written and read, and a rounding.)
-//   gate_kernel       x w13^T and the activation: tiles of 64 a- and 64 b-rows, so that a lane holds matching a and b
-//   gate_grad_kernel  the same, then dy w2 on the same tokens and features: writes act and [da | db] in bf16
-//   mm_kernel         y, dx, dw13, dw2 (lm_mm.hip); the weights' sums over the tokens are split over workgroups
-// Bound by the products: 6 M d hidden operations forward, 16 in the gradient.  The gradient's first launch has 32
-// features x 64 tokens per wavefront and operand and is held by its LDS reads (14 KB per 24 products of 16 x 16 x 32).
+//   gate_kernel   x w13^T and the activation; each lane holds matching a and b.  For the gradient (GRAD) dy w2 on the
+//                 same tokens and features through the same stages: writes act and [da | db] in bf16
+//   mm_kernel     y, dx, dw13, dw2 (lm_mm.hip); the weights' sums over the tokens are split over workgroups
+// Bound by the products: 6 M d hidden operations forward, 18 with the recomputed a | b in the gradient, d = 384 of them six
+// units of 64 k, so that a tile's beginning and end weigh as much as a third of its products; the rate while they run is that
+// of the way from cache into LDS (lm_mm.h).  Measured for 32,768 tokens of d = 384, hidden 1,024: the gate 65 to 74 us (750 TFLOP/s),
+// y 32, the gradient's gate 140 (550; its three results are 201 MB written), dx 62, dw13 58, dw2 51 and the joining of
+// their parts 14.
 #include "lm_mm.h"
 
 #include <algorithm>
@@ -203,8 +206,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
 
 typedef MmShape<2, 4, 8, 4> Gate256;                     // 128 features x 256 tokens
 typedef MmShape<4, 2, 4, 4> Gate128;                     // 128 x 128
-typedef MmShape<2, 2, 4, 4> Gate64;                      // 64 x 128, four wavefronts
-typedef MmShape<2, 2, 4, 2> Gate32;                      // 64 x 64
+typedef MmShape<2, 2, 4, 2> Gate64;                      // 64 x 64, four wavefronts
 
 template <class S, bool GRAD>
 int launch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
@@ -217,15 +219,16 @@ int launch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
   return launch_status(what);
 }
 
-// The largest tile of which there is one for each CU at least.
+// The largest tile of which there is one for each CU at least (d = 384, hidden = 1,024; forward with its y product, the
+// gradient with dw2's): 32,768 tokens take 90 us in Gate256, 100 in Gate128, 107 in Gate64; the gradient 174 in Gate128,
+// 194 in Gate64 (in Gate256 its registers do not suffice); 1,024 tokens 22, 17 and 14, the gradient 25 and 21.
 template <bool GRAD>
 int dispatch_gate(const GateArgs &p, hipStream_t stream, const char *what) {
-  const int64_t n128 = ceil_div(p.hidden, 128), n64 = ceil_div(p.hidden, 64), t128 = ceil_div(p.M, 128);
+  const int64_t n128 = ceil_div(p.hidden, 128);
   if constexpr (!GRAD)
     if (n128 * ceil_div(p.M, 256) >= 256) return launch_gate<Gate256, GRAD>(p, stream, what);
-  if (n128 * t128 >= 256) return launch_gate<Gate128, GRAD>(p, stream, what);
-  if (n64 * t128 >= 256) return launch_gate<Gate64, GRAD>(p, stream, what);
-  return launch_gate<Gate32, GRAD>(p, stream, what);
+  if (n128 * ceil_div(p.M, 128) >= 256) return launch_gate<Gate128, GRAD>(p, stream, what);
+  return launch_gate<Gate64, GRAD>(p, stream, what);
 }
 
 int check_ffn(const char *what, const void *x, int64_t ldx, const void *w13, int64_t ldw13, const void *w2, int64_t ldw2,

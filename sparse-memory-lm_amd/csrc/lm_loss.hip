@@ -2,7 +2,7 @@
 // (F.cross_entropy(lm_head(x).float(), targets) of smlm/model.py:286-293), without ever holding the logits:
 //   s_n = x_n W^T, loss_n = logsumexp(s_n) - s_n[t_n], dx = G W, dW = G^T x, G = c_n (softmax(s_n) - 1[t_n]).
 //
-// Forward: a workgroup takes 256 tokens and a range of the vocabulary, forms 128 columns of logits at a time in its
+// Forward: a workgroup takes up to 256 tokens and a range of the vocabulary, forms 256 columns of logits at a time in its
 // accumulators and keeps a running maximum and sum of exponentials per lane, each lane over its own columns (no exchange
 // between lanes until the range ends).  The (maximum, sum) of every range go to a small array, which a second kernel joins,
 // one wavefront per token; the target's logit is picked from the accumulators, so that it is the very value in the sum.
@@ -13,9 +13,12 @@
 // rows of the piece are final, dx gathers over the pieces in fp32.
 //
 // Bound by the products: 2 M V d operations forward, three times that in the gradient (one third for the logits again, which
-// is what not keeping them costs), with d = 384 a short sum: 12 chunks of 32 per 128 x 256 tile, then 128 exponentials a
-// lane.  The chunks of successive tiles run through one pipeline, so that a tile's first loads are on their way during its
-// predecessor's exponentials.
+// is what not keeping them costs).  With d = 384 a tile's sum is short, six units of 64 k, and 128 exponentials a lane follow
+// it: the stages of successive tiles run through one pipeline, so that a tile's first loads are on their way during its
+// predecessor's exponentials.  Measured (d = 384, V = 50,304): 16,384 tokens 600 to 640 us forward (1,030 TFLOP/s; d = 1,024
+// reaches 1,240), in the gradient 900 to 980 for G (its 1.65 GB are written in whole 64-byte lines, which do not overlap its
+// products: 65 us of each 412 MB), 640 to 720 for dx, 600 to 630 for dW.  64 tokens of 32,000 are bound by W's bytes and the
+// launches: 56 us for all.
 #include "lm_mm.h"
 
 #include <algorithm>
@@ -334,9 +337,11 @@ int launch_loss(LossArgs a, hipStream_t stream, const char *what) {
   return launch_status(what);
 }
 
-// Tokens of a tile, and its wavefronts over the columns (each leaves its own maximum and sum).
-int tile_tokens(int64_t M) { return M > 128 ? 256 : M > 64 ? 128 : 64; }
-int tile_parts(int64_t M) { return M > 128 ? Tokens256::WF : Tokens128::WF; }
+// Tokens of a tile, and its wavefronts over the columns (each leaves its own maximum and sum).  Two smaller tiles beat one
+// half empty, as the ranges are short then (32,000 x 384, forward and gradient of x): 128 tokens 40 us in tiles of 64, 45
+// of 128, 52 of 256; 200 tokens 52, 50 and 59; 300 tokens 66, 65 and 64; 1,000 tokens 137, 118 and 111.
+int tile_tokens(int64_t M) { return M > 256 ? 256 : M > 128 ? 128 : 64; }
+int tile_parts(int64_t M) { return M > 256 ? Tokens256::WF : Tokens128::WF; }
 
 template <bool GRAD>
 int dispatch_loss(const LossArgs &a, hipStream_t stream, const char *what) {

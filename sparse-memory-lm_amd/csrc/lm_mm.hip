@@ -155,7 +155,7 @@ MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split) {
     double wait, busy, fixed;                             // us
   };
   static const Tile tiles[4] = {
-      {256, 256, 1.27, 1.51, 4.3}, {384, 128, 1.12, 1.16, 5.9}, {128, 128, 0.63, 0.47, 4.4}, {64, 64, 0.29, 0.22, 3.4}};
+      {256, 256, 1.32, 1.50, 5.0}, {384, 128, 1.10, 1.17, 5.7}, {128, 128, 0.64, 0.48, 4.5}, {64, 64, 0.29, 0.23, 3.4}};
   const int64_t units = ceil_div(K, kMmUnit);
   MmPlan best{0, 1};
   double least = 1e30;
@@ -164,7 +164,7 @@ MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split) {
       const Tile &c = tiles[i];
       const int64_t per_cu = ceil_div(ceil_div(F, c.f) * ceil_div(T, c.t) * s, kCus);
       double time = ceil_div(units, s) * std::max(c.wait, per_cu * c.busy) + c.fixed;
-      time += s > 1 ? 2.4 + s * T * F * 8 / 5.8e6 : T * F * 2 / 3.7e6;
+      time += s > 1 ? 2.4 + s * T * F * 8 / 5.9e6 : T * F * 2 / 3.8e6;
       if (time < least) {
         least = time;
         best = {i, s};

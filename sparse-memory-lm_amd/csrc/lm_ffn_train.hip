@@ -27,6 +27,7 @@ struct GateArgs {
   const uint16_t *x, *w13, *dy, *w2;
   int64_t ldx, ldw13, lddy, ldw2, M, d, hidden, n_out;
   uint16_t *act, *dab;                                    // [M][hidden], [M][2 hidden]
+  int64_t rest;                                           // M hidden: act's second term is so many on, dab's twice; or 0
 };
 
 __device__ __forceinline__ float sigmoid(float a) {
@@ -191,14 +192,18 @@ __global__ void __launch_bounds__(S::kThreads, 2) gate_kernel(GateArgs p) {
           db[q] = dh * as;
         }
       }
-      auto store = [&](uint16_t *to, const float *v) {
-        *(uint4 *)to = uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                             pack_bf16x2(v[6], v[7])};
+      auto store = [&](uint16_t *to, float *v, int64_t rest) {
+        *(uint4 *)to = mm_pack(v);
+        if (p.rest) {                                     // uniform
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = mm_rest(v[q]);
+          *(uint4 *)(to + rest) = mm_pack(v);
+        }
       };
-      store(p.act + t * p.hidden + f + o, h);
+      store(p.act + t * p.hidden + f + o, h, p.rest);
       if constexpr (GRAD) {
-        store(p.dab + t * 2 * p.hidden + f + o, da);
-        store(p.dab + t * 2 * p.hidden + p.hidden + f + o, db);
+        store(p.dab + t * 2 * p.hidden + f + o, da, 2 * p.rest);
+        store(p.dab + t * 2 * p.hidden + p.hidden + f + o, db, 2 * p.rest);
       }
     }
   }
@@ -254,7 +259,7 @@ int check_ffn(const char *what, const void *x, int64_t ldx, const void *w13, int
 // The products besides the gate's: y over hidden, dx over a and b, the weights' gradients over the tokens.
 struct FfnPlan {
   MmPlan y, dx, dw13, dw2;
-  int64_t act, parts_forward, parts_backward;             // bytes
+  int64_t act, parts_forward, parts_backward;             // bytes; da and db take twice act's
 };
 FfnPlan ffn_plan(int64_t M, int64_t d, int64_t hidden, int64_t n_out) {
   FfnPlan p;
@@ -262,15 +267,18 @@ FfnPlan ffn_plan(int64_t M, int64_t d, int64_t hidden, int64_t n_out) {
   p.dx = mm_plan(M, d, 2 * hidden, true);
   p.dw13 = mm_plan(2 * hidden, d, M, true);
   p.dw2 = mm_plan(n_out, hidden, M, true);
-  p.act = M * hidden * 2;
+  p.act = M * hidden * 2 * mm_terms(M);
   p.parts_forward = p.y.part_bytes(M, n_out);
   p.parts_backward = std::max(p.dx.part_bytes(M, d), std::max(p.dw13.part_bytes(2 * hidden, d), p.dw2.part_bytes(n_out, hidden)));
   return p;
 }
 
 // out [T][F] = sum over k of tok feat, contiguous
-MmArgs product(const void *feat, int64_t ldf, const void *tok, int64_t ldt, int64_t F, int64_t T, int64_t K, void *out) {
+MmArgs product(const void *feat, int64_t ldf, int64_t feat_rest, const void *tok, int64_t ldt, int64_t tok_rest, int64_t F,
+               int64_t T, int64_t K, void *out) {
   MmArgs m{};
+  m.feat_rest = feat_rest;
+  m.tok_rest = tok_rest;
   m.feat = (const uint16_t *)feat;
   m.tok = (const uint16_t *)tok;
   m.ldf = ldf;
@@ -314,9 +322,10 @@ extern "C" int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w
   p.d = d;
   p.hidden = hidden;
   p.act = (uint16_t *)workspace;
+  p.rest = mm_terms(M) > 1 ? M * hidden : 0;
   const FfnPlan plan = ffn_plan(M, d, hidden, n_out);
   if (const int rc = dispatch_gate<false>(p, s, what)) return rc;
-  return mm_run(product(w2, w2_row_stride, p.act, hidden, n_out, M, hidden, y), true, true, plan.y,
+  return mm_run(product(w2, w2_row_stride, 0, p.act, hidden, p.rest, n_out, M, hidden, y), true, true, plan.y,
                 (float *)((char *)workspace + plan.act), s, what);
 }
 
@@ -351,19 +360,21 @@ extern "C" int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, co
   p.hidden = hidden;
   p.n_out = n_out;
   p.act = (uint16_t *)workspace;
-  p.dab = p.act + M * hidden;
-  float *parts = (float *)(p.dab + 2 * M * hidden);
+  p.rest = mm_terms(M) > 1 ? M * hidden : 0;
+  p.dab = p.act + M * hidden * mm_terms(M);
+  float *parts = (float *)(p.dab + 2 * M * hidden * mm_terms(M));
   if (const int rc = dispatch_gate<true>(p, s, what)) return rc;
   const FfnPlan plan = ffn_plan(M, d, hidden, n_out);
   if (dx)
-    if (const int rc = mm_run(product(w13, w13_row_stride, p.dab, 2 * hidden, d, M, 2 * hidden, dx), false, true, plan.dx, parts,
-                              s, what))
+    if (const int rc = mm_run(product(w13, w13_row_stride, 0, p.dab, 2 * hidden, 2 * p.rest, d, M, 2 * hidden, dx), false, true,
+                              plan.dx, parts, s, what))
       return rc;
   if (dw13)
-    if (const int rc = mm_run(product(x, x_row_stride, p.dab, 2 * hidden, d, 2 * hidden, M, dw13), false, false, plan.dw13,
-                              parts, s, what))
+    if (const int rc = mm_run(product(x, x_row_stride, 0, p.dab, 2 * hidden, 2 * p.rest, d, 2 * hidden, M, dw13), false, false,
+                              plan.dw13, parts, s, what))
       return rc;
   if (dw2)
-    return mm_run(product(p.act, hidden, dy, dy_row_stride, hidden, n_out, M, dw2), false, false, plan.dw2, parts, s, what);
+    return mm_run(product(p.act, hidden, p.rest, dy, dy_row_stride, 0, hidden, n_out, M, dw2), false, false, plan.dw2, parts, s,
+                  what);
   return SMLM_OK;
 }

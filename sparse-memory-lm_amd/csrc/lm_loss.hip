@@ -8,8 +8,8 @@
 // one wavefront per token; the target's logit is picked from the accumulators, so that it is the very value in the sum.
 // A third launch adds the tokens' losses up (in fp64, in a fixed order).  Only lse (fp32 per token) is kept.
 //
-// Gradient, in pieces of the vocabulary: the logits of a piece again, G of the piece as bf16 (c_n is 0 or 1 where the loss
-// is a mean or sum, so that G needs no scale: 1 / count goes on at the end), then its two products (lm_mm.hip): dW's
+// Gradient, in pieces of the vocabulary: the logits of a piece again, G of the piece as bf16 (of up to 64 tokens as two bf16
+// terms; c_n is 0 or 1 where the loss is a mean or sum, so that G needs no scale: 1 / count goes on at the end), then its two products (lm_mm.hip): dW's
 // rows of the piece are final, dx gathers over the pieces in fp32.
 //
 // Bound by the products: 2 M V d operations forward, three times that in the gradient (one third for the logits again, which
@@ -45,7 +45,7 @@ struct LossArgs {
   const float *lse, *coef, *grad, *count;                 // gradient: coef per token, or null; grad and count: see below
   float *scale;                                           // gradient: *grad / *count (count null: *grad), written here
   uint16_t *g;                                            // gradient: G of the piece [M][ldg]
-  int64_t ldg;
+  int64_t ldg, rest;                                      // where G's second term is, elements on, or 0 (mm_terms)
 };
 
 // Eight wavefronts, 256 columns: of 256 tokens, each wavefront 128 x 64 (fewer tokens a lane: fewer running maxima), of 128 or
@@ -193,16 +193,25 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
           char *out = (char *)(a.g + (t0 + wt + 16 * j) * a.ldg + tile * kLsCols + wf);
           const uint32_t at = (uint32_t)(r * a.ldg + 8 * g) * 2;
 #pragma unroll
-          for (int q = 0; q < C / 8; ++q)
-            *(uint4 *)(out + (at + 64 * q)) = uint4{pack_bf16x2(p[8 * q], p[8 * q + 1]), pack_bf16x2(p[8 * q + 2], p[8 * q + 3]),
-                           pack_bf16x2(p[8 * q + 4], p[8 * q + 5]), pack_bf16x2(p[8 * q + 6], p[8 * q + 7])};
+          for (int q = 0; q < C / 8; ++q) *(uint4 *)(out + (at + 64 * q)) = mm_pack(p + 8 * q);
+          if (a.rest) {                                   // uniform
+#pragma unroll
+            for (int q = 0; q < C; ++q) p[q] = mm_rest(p[q]);
+#pragma unroll
+            for (int q = 0; q < C / 8; ++q) *(uint4 *)(out + 2 * a.rest + (at + 64 * q)) = mm_pack(p + 8 * q);
+          }
         }
         if (__any(rel < (unsigned)C)) {                   // rare: the target's, over what its lane has just stored
           float v = 0.f;
 #pragma unroll
           for (int q = 0; q < C; ++q) v = rel == (unsigned)q ? acc[q / 4][j][q % 4] : v;
           v = (exp2_hw((v - m[j]) * kLog2e) - 1.f) * c;
-          if (rel < (unsigned)C) a.g[t * a.ldg + c0 + off] = (uint16_t)(pack_bf16x2(v, v) & 0xFFFFu);
+          if (rel < (unsigned)C) {
+            const float rest = mm_rest(v);
+            uint16_t *to = a.g + t * a.ldg + c0 + off;
+            *to = (uint16_t)(pack_bf16x2(v, v) & 0xFFFFu);
+            if (a.rest) to[a.rest] = (uint16_t)(pack_bf16x2(rest, rest) & 0xFFFFu);
+          }
         }
       }
     }
@@ -366,13 +375,14 @@ struct GradPlan {
 GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
   GradPlan p;
   // at most the products' widest rows: few tokens would have wider ones
-  const int64_t most = std::min<int64_t>(kMmMaxStride, std::max<int64_t>(kLsPieceBytes / (2 * M) / kLsCols, 1) * kLsCols);
+  const int64_t row = 2 * M * mm_terms(M);                // bytes of a column of G
+  const int64_t most = std::min<int64_t>(kMmMaxStride, std::max<int64_t>(kLsPieceBytes / row / kLsCols, 1) * kLsCols);
   p.pieces = ceil_div(V, most);
   p.cols = ceil_div(ceil_div(V, p.pieces), kLsCols) * kLsCols;
   p.pieces = ceil_div(V, p.cols);
   p.dx = mm_plan(M, d, p.cols, true);
   p.dw = mm_plan(p.cols, d, M, false);
-  p.g_bytes = M * p.cols * 2;
+  p.g_bytes = row * p.cols;
   p.part_bytes = p.pieces * p.dx.splits > 1 ? p.dx.splits * M * d * 4 : 0;
   return p;
 }
@@ -484,6 +494,7 @@ extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, in
   a.scale = (float *)workspace;
   a.g = (uint16_t *)((char *)workspace + 256);
   a.ldg = p.cols;
+  a.rest = mm_terms(M) > 1 ? M * p.cols : 0;
   float *parts = (float *)((char *)workspace + 256 + p.g_bytes);
   const float *scale = per_token ? nullptr : a.scale;
   for (int64_t piece = 0; piece < p.pieces; ++piece) {
@@ -500,6 +511,7 @@ extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, in
       m.Kf = n;
       m.tok = a.g;
       m.ldt = a.ldg;
+      m.tok_rest = a.rest;
       m.F = d;
       m.T = M;
       m.K = (n + 7) / 8 * 8;
@@ -517,6 +529,7 @@ extern "C" int smlm_linear_ce_backward(const float *grad, const float *count, in
       m.Kf = m.K = M;
       m.tok = a.g;
       m.ldt = a.ldg;
+      m.tok_rest = a.rest;
       m.F = d;
       m.T = n;
       m.out = (uint16_t *)dw + a.v0 * d;

@@ -324,14 +324,32 @@ inline int mm_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &do
   return e == hipSuccess ? SMLM_OK : fail(SMLM_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// Terms that an operand formed on the way (the activation, the logits' gradient) is held in: bf16, and for few tokens a
+// second bf16 with what the first leaves, 16 bits of mantissa together.  Over many tokens the first's roundings average out
+// in the sums; of a few tokens single values carry a result, whose error would be up to twice its own rounding's, and the
+// products are bound by the weights' bytes and the launches (the second terms cost the loss of 64 tokens 56 -> 60 us, an FFN
+// block of 48 tokens 36 -> 44, both below what the calls take on the host).
+constexpr int64_t kMmFewTokens = 64;
+inline int mm_terms(int64_t tokens) { return tokens <= kMmFewTokens ? 2 : 1; }
+__device__ __forceinline__ uint4 mm_pack(const float *v) {
+  return uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+// v - bf16(v), exact: the second term.  What is not finite stays in the first alone.
+__device__ __forceinline__ float mm_rest(float v) {
+  const float rest = v - round_bf16_hw(v);
+  return fabsf(rest) < __builtin_inff() ? rest : 0.f;
+}
+
 // ---- plain products (lm_mm.hip) ----------------------------------------------------------------------------------------
 // out[t, f] = sum_k tok[t, k] feat[f, k]; an operand with *_kc = false is stored [k][row].  Rows and strides in elements,
 // rows of 16-byte pieces.  nsplit > 1 or f32: fp32 parts [nsplit][T][F] (with accumulate added to what is there), split s
 // summing k_per (whole units) from s * k_per on; otherwise bf16 out [T][ldo], times *scale where scale is given.
 // F a multiple of 8; K one too where an operand has k contiguous, that operand's k from the sum's end up to it zeros; a k
 // strided tok has rows of at least T rounded up to 8.  Kf: the k that a k strided feat has (the last of K may lack).
+// feat_rest, tok_rest: where not 0, the operand's second term is so many elements on (mm_terms).
 struct MmArgs {
   const uint16_t *feat, *tok;
+  int64_t feat_rest, tok_rest;
   int64_t ldf, ldt, F, T, K, Kf;
   void *out;
   int64_t ldo;

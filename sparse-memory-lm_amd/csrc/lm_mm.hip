@@ -46,14 +46,21 @@ __global__ void __launch_bounds__(S::kThreads, 2) mm_kernel(MmArgs a) {
   mm_zero(acc);
   MmSource<typename K::F> fs;
   MmSource<typename K::T> ts;
-  fs.init(a.feat, a.ldf, a.F, FKC ? a.K : a.Kf, f0, k_begin);
-  ts.init(a.tok, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, t0, k_begin);
-  if (k_end > k_begin) {  // workgroup-uniform; k_end is K or a whole number of units on
-    typename Loop::Frags x, y;
-    L.start(fs, ts, x);
-    uint32_t stage = 0;
-    for (int left = mm_units(k_end - k_begin); left > 0; --left) L.multiply(fs, ts, x, y, stage, acc);
-    mm_finish();
+  const bool two = a.feat_rest | a.tok_rest;
+  for (int term = 0; term <= two; ++term) {               // uniform
+    fs.init(a.feat + term * a.feat_rest, a.ldf, a.F, FKC ? a.K : a.Kf, f0, k_begin);
+    ts.init(a.tok + term * a.tok_rest, a.ldt, TKC ? a.T : (a.T + 7) & ~7LL, a.K, t0, k_begin);
+    if (term) {
+      __syncthreads();                                    // all have read the stages
+      L.offsets(a.ldf, a.ldt);                            // the last stage's clipped them
+    }
+    if (k_end > k_begin) {  // workgroup-uniform; k_end is K or a whole number of units on
+      typename Loop::Frags x, y;
+      L.start(fs, ts, x);
+      uint32_t stage = 0;
+      for (int left = mm_units(k_end - k_begin); left > 0; --left) L.multiply(fs, ts, x, y, stage, acc);
+      mm_finish();
+    }
   }
 
   const int lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;

@@ -21,6 +21,12 @@ U32 = 2.0 ** -24                 # an fp32 one
 TINY = 2.0 ** -126
 
 
+def half_between(tokens):
+    """The rounding of what the products read back: up to 64 tokens as two bf16 terms, the second rounding what the first
+    leaves."""
+    return HALF * HALF if tokens <= 64 else HALF
+
+
 def note(*what):
     print("[case]", *what, flush=True)
 
@@ -58,7 +64,7 @@ def loss_reference(x, w, t, ignore=-100, reduction="mean", g=None):
         c = c / n
     p = torch.exp(logits - lse.unsqueeze(1))
     G = c.unsqueeze(1) * p.scatter_add(1, at, -torch.ones_like(at, dtype=torch.float64))
-    G_tol = TINY + HALF * G.abs() + c.abs().unsqueeze(1) * p * (2 * logit_err.unsqueeze(1) + 32 * U32) * 1.01
+    G_tol = TINY + half_between(x.shape[0]) * G.abs() + c.abs().unsqueeze(1) * p * (2 * logit_err.unsqueeze(1) + 32 * U32) * 1.01
     dx, dw = G @ w, G.T @ x
     k = (w.shape[0] + 64) * U32
     dx_tol = (G_tol + k * G.abs()) @ w.abs() * 1.01 + HALF * dx.abs() * 1.01 + TINY
@@ -286,12 +292,13 @@ def ffn_reference(x, w13, w2, g):
     hid = act * b
     # |silu'| <= 1.1 and |silu''| <= 0.5; 2^-20 for the sigmoid
     act_tol = 1.1 * ea + 2.0 ** -20 * act.abs()
-    hid_tol = HALF * hid.abs() + 1.01 * (act_tol * b.abs() + act.abs() * eb)
+    half = half_between(M)
+    hid_tol = TINY + half * hid.abs() + 1.01 * (act_tol * b.abs() + act.abs() * eb)
     dh = g @ w2
     dh_err = (g.abs() @ w2.abs()) * (w2.shape[0] + 4) * U32
     dab = torch.cat([dh * b * ds, dh * act], 1)
     ds_tol = 0.5 * ea + 2.0 ** -20 * (s + a.abs())
-    dab_tol = HALF * dab.abs() + 1.01 * torch.cat([dh_err * (b * ds).abs() + (dh * b).abs() * ds_tol + (dh * ds).abs() * eb,
+    dab_tol = TINY + half * dab.abs() + 1.01 * torch.cat([dh_err * (b * ds).abs() + (dh * b).abs() * ds_tol + (dh * ds).abs() * eb,
                                                    dh_err * act.abs() + dh.abs() * act_tol], 1)
 
     def product(p, tol, q, n):

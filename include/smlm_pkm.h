@@ -556,10 +556,10 @@ int smlm_linear_ce(const void *x, int64_t x_row_stride, const void *w, int64_t w
 
 /*
  * Its gradient: dx = G W (M, d) and dw = G^T x (V, d), contiguous bf16, either NULL if not wanted, with
- * G[n, v] = c_n (softmax(s_n)[v] - [v == targets[n]]), formed in bf16 (up to 64 tokens: as two bf16 terms) in pieces of the
- * vocabulary of at most 1 GiB (or 256 columns).  grad: per_token ? (M,) fp32, c_n = grad[n] : one fp32, c_n = grad[0] / (count ? count[0] : 1), applied in
- * fp32 behind the sums.  c_n = 0 for ignored tokens.  lse from the forward; workspace: smlm_linear_ce_workspace(M, V, d,
- * 1) bytes, 16-byte aligned.  fp32 sums in a fixed order.
+ * G[n, v] = c_n (softmax(s_n)[v] - [v == targets[n]]), formed in bf16 (up to 128 tokens: as two bf16 terms) in pieces of the
+ * vocabulary of at most 1 GiB (or 256 columns).  grad: per_token ? (M,) fp32, c_n = grad[n] : one fp32, c_n = grad[0] /
+ * (count ? count[0] : 1), applied in fp32 behind the sums.  c_n = 0 for ignored tokens.  lse from the forward; workspace:
+ * smlm_linear_ce_workspace(M, V, d, 1) bytes, 16-byte aligned.  fp32 sums in a fixed order.
  */
 int smlm_linear_ce_backward(const float *grad, const float *count, int per_token, const void *x, int64_t x_row_stride,
                             const void *w, int64_t w_row_stride, const int64_t *targets, int64_t ignore_index,
@@ -570,7 +570,7 @@ int smlm_linear_ce_backward(const float *grad, const float *count, int per_token
  * The gated feed-forward block y = (silu(a) * b) w2^T, a | b = the halves of x w13^T (smlm/model.py:110-118).
  *   x (M, d), w13 (2 * hidden, d), w2 (n_out, hidden) bf16 with row strides as above, d, hidden and n_out multiples of 8
  *   y (M, n_out) contiguous bf16
- * workspace: smlm_gated_ffn_workspace(..., 0) bytes, 16-byte aligned.  a, b and the gate in fp32, the activation (up to 64
+ * workspace: smlm_gated_ffn_workspace(..., 0) bytes, 16-byte aligned.  a, b and the gate in fp32, the activation (up to 128
  * tokens: as two bf16 terms) and y rounded once each.
  */
 int64_t smlm_gated_ffn_workspace(int64_t M, int64_t d, int64_t hidden, int64_t n_out, int grad);
@@ -582,7 +582,7 @@ int smlm_gated_ffn(const void *x, int64_t x_row_stride, const void *w13, int64_t
  * Its gradients from dy (M, n_out) and the inputs alone (a and b are formed again): dx (M, d), dw13 (2 * hidden, d), dw2
  * (n_out, hidden), contiguous bf16, each NULL if not wanted.  workspace: smlm_gated_ffn_workspace(..., 1) bytes, 16-byte
  * aligned.  fp32 sums in a fixed order; the activation and the gradients of a and b are rounded to bf16 as operands of
- * their products (up to 64 tokens: to two bf16 terms each).
+ * their products (up to 128 tokens: to two bf16 terms each).
  */
 int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, const void *x, int64_t x_row_stride, const void *w13,
                             int64_t w13_row_stride, const void *w2, int64_t w2_row_stride, int64_t M, int64_t d,

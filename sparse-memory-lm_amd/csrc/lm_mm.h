@@ -326,10 +326,11 @@ inline int mm_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &do
 
 // Terms that an operand formed on the way (the activation, the logits' gradient) is held in: bf16, and for few tokens a
 // second bf16 with what the first leaves, 16 bits of mantissa together.  Over many tokens the first's roundings average out
-// in the sums; of a few tokens single values carry a result, whose error would be up to twice its own rounding's, and the
-// products are bound by the weights' bytes and the launches (the second terms cost the loss of 64 tokens 56 -> 60 us, an FFN
-// block of 48 tokens 36 -> 44, both below what the calls take on the host).
-constexpr int64_t kMmFewTokens = 64;
+// in the sums (a result's error is 1.4 of its own rounding's); of a few tokens single values carry a result, whose error
+// would be up to twice that, and the products are bound by the weights' bytes and the launches: the second terms cost the
+// loss of 64 tokens 56 -> 61 us and an FFN block of 48 tokens 36 -> 44, both less than the calls take on the host; at 512 tokens
+// the loss' two products would take twice as long.
+constexpr int64_t kMmFewTokens = 128;
 inline int mm_terms(int64_t tokens) { return tokens <= kMmFewTokens ? 2 : 1; }
 __device__ __forceinline__ uint4 mm_pack(const float *v) {
   return uint4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};

@@ -1162,7 +1162,8 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     the tokens that count; NaN if none), "sum" (both 0-d fp32) or "none" (targets' shape, fp32).
     Differentiable in x and weight, both bf16: the gradient forms the logits again, in pieces of the vocabulary, from the
     inputs and one fp32 per token.  Sums in fp32, the gradient of the logits rounded to bf16 as operand of its products (up
-    to 64 tokens: to two bf16 terms); the same bits on every call.  A width that is not a multiple of 8, or rows that are not 16-byte aligned, are copied first."""
+    to 128 tokens: to two bf16 terms); the same bits on every call.  A width that is not a multiple of 8, or rows that are
+    not 16-byte aligned, are copied first."""
     return _lib.train_ops().linear_cross_entropy(x, weight, targets, int(ignore_index), reduction)
 
 
@@ -1171,7 +1172,7 @@ def gated_ffn(x, w13, w2):
     differentiable node (smlm_gated_ffn).  x (..., d), w13 (2 * hidden, d), w2 (n_out, hidden) bf16 -> (..., n_out) bf16.
     The projection stays in fp32 up to the activation, which is rounded to bf16 as the operand of w2.  Nothing but the
     inputs is kept for the gradient, which forms a and b again (smlm_gated_ffn_backward); its sums are in fp32, the
-    gradients of a and b rounded to bf16 as operands.  Up to 64 tokens these operands are two bf16 terms each, so that the
+    gradients of a and b rounded to bf16 as operands.  Up to 128 tokens these operands are two bf16 terms each, so that the
     results' own rounding is all that is lost.  The same bits on every call.  Sizes that are not multiples of 8, or
     rows that are not 16-byte aligned, are copied first."""
     return _lib.train_ops().gated_ffn(x, w13, w2)

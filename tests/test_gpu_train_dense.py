@@ -22,9 +22,9 @@ TINY = 2.0 ** -126
 
 
 def half_between(tokens):
-    """The rounding of what the products read back: up to 64 tokens as two bf16 terms, the second rounding what the first
+    """The rounding of what the products read back: up to 128 tokens as two bf16 terms, the second rounding what the first
     leaves."""
-    return HALF * HALF if tokens <= 64 else HALF
+    return HALF * HALF if tokens <= 128 else HALF
 
 
 def note(*what):

@@ -593,7 +593,7 @@ int smlm_gated_ffn_backward(const void *dy, int64_t dy_row_stride, const void *x
  * Residual add and RMSNorm of a recorded pass (smlm/model.py:124-126, 156-163): xs = x + delta rounded to x's type,
  * h = xs * rstd * w, rstd = rsqrt(mean(xs^2) + eps) in fp32.
  *   x, xs (M, C) of x_dtype; delta (M, C) of delta_dtype or NULL (xs is then not written and may be NULL); w (C,) of
- *   w_dtype; h (M, C) of h_dtype; rstd (M,) fp32.  Types SMLM_F32 or SMLM_BF16; all contiguous.
+ *   w_dtype; h (M, C) of h_dtype; rstd (M,) fp32.  Types SMLM_F32 or SMLM_BF16; all contiguous, no output over an input.
  */
 int smlm_rmsnorm_train(const void *x, int x_dtype, const void *delta, int delta_dtype, const void *w, int w_dtype,
                        float eps, int64_t M, int64_t C, void *xs, void *h, int h_dtype, float *rstd, void *stream);
@@ -602,7 +602,8 @@ int smlm_rmsnorm_train(const void *x, int x_dtype, const void *delta, int delta_
  * Its gradients: dx (M, C) of x_dtype = rstd (gw - hat mean(gw hat)) + dxs with gw = dh w, hat = xs rstd, and, if not
  * NULL, the same in ddelta (delta_dtype); dw (C,) of w_dtype = sum over the rows of dh hat (NULL if not wanted).  dxs
  * (M, C) of x_dtype, the gradient of xs, or NULL; dh or NULL likewise (not both).
- * parts: caller-owned scratch of smlm_rmsnorm_parts(M, C) floats.  The same result on every call.
+ * parts: caller-owned scratch of smlm_rmsnorm_parts(M, C) floats.  No output over an input.  The same result on every
+ * call.
  */
 int64_t smlm_rmsnorm_parts(int64_t M, int64_t C);
 int smlm_rmsnorm_train_backward(const void *dxs, const void *dh, int h_dtype, const void *xs, int x_dtype, const void *w,

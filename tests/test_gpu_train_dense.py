@@ -453,7 +453,8 @@ TYPES = [(F32, BF16, F32, BF16), (F32, F32, F32, F32), (F32, None, BF16, F32), (
 
 @pytest.mark.parametrize("M,C", [(1, 1), (1, 384), (2, 7), (5, 8), (64, 384), (33, 511), (9, 512), (17, 513), (300, 1001),
                                  (11, 1024), (7, 1025), (20, 2048), (6, 2049), (5, 4097), (3, 16384), (4097, 392),
-                                 (20000, 24)])
+                                 (20000, 24), (70, 9), (33, 64), (3, 100), (130, 128), (1000, 129), (9, 255), (41, 257),
+                                 (2, 1500), (5, 4104), (7, 8191), (4, 8200), (3, 16383)])
 def test_norm_sizes(M, C):
     note("norm", M, C)
     for types in TYPES:

@@ -9,6 +9,7 @@
 // A backward that is itself recorded (create_graph) runs as PyTorch ops, so that it can be differentiated again.
 #include <ATen/ATen.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "smlm_pkm.h"
@@ -31,7 +32,11 @@ void check(int rc, const char *what) {
   TORCH_CHECK(rc == SMLM_OK, what, " failed with status ", rc, ": ", smlm_pkm_last_error());
 }
 
+// t with its values in memory as they are (a view may hold a sign that is yet to be applied).
+Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void check_device(const char *name, const Tensor &first, std::initializer_list<const Tensor *> others) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced: a trace would hold its outputs as they were");
   TORCH_CHECK_VALUE(first.is_cuda(), name, ": all tensors must be on a HIP (cuda) device, got ", first.device());
   for (const Tensor *t : others)
     TORCH_CHECK_VALUE(!t->defined() || t->device() == first.device(), name, ": all tensors must be on one device, got ",
@@ -54,6 +59,11 @@ Tensor mm_rows(const Tensor &t, int64_t rows, int64_t cols) {
 Tensor narrowed(const Tensor &t, int64_t rows, int64_t cols) {
   return t.size(0) == rows && t.size(1) == cols ? t : t.narrow(0, 0, rows).narrow(1, 0, cols);
 }
+
+// Within it the ops of a recorded backward keep their fp32 where autocast is on.
+struct NoAutocast {
+  c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset};
+};
 
 // The gradients of `y` with respect to the wanted inputs, recorded.
 variable_list recorded(const Tensor &y, const Tensor &dy, const variable_list &inputs, const std::vector<bool> &wants) {
@@ -102,10 +112,15 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const int64_t d = x.size(-1), V = weight.size(0), M = x.numel() / d, d8 = ceil8(d);
-    Tensor g = grads[0];
+    Tensor g = plain(grads[0]);
     if (at::GradMode::is_enabled()) {
-      const Tensor logits = at::matmul(x.reshape({M, d}).to(at::kFloat), weight.to(at::kFloat).t());
-      const Tensor y = at::cross_entropy_loss(logits, targets.reshape({M}), {}, reduction, ignore);
+      const NoAutocast fp32;
+      // an index outside the vocabulary, which the loss would stop the device for: any other, and NaN
+      const Tensor t = targets.reshape({M}), bad = t.ne(ignore).logical_and(t.lt(0).logical_or(t.ge(V)));
+      const Tensor one = at::ones({}, x.options().dtype(at::kFloat));
+      const Tensor poison = at::where(bad, one * std::numeric_limits<float>::quiet_NaN(), one).unsqueeze(1);
+      const Tensor logits = at::matmul(x.reshape({M, d}).to(at::kFloat), weight.to(at::kFloat).t()) * poison;
+      const Tensor y = at::cross_entropy_loss(logits, t.masked_fill(bad, ignore == 0 && V > 1 ? 1 : 0), {}, reduction, ignore);
       const auto got = recorded(y, g.reshape(y.sizes()), {x, weight}, {want_x, want_w});
       return {got[0], got[1], Tensor(), Tensor(), Tensor()};
     }
@@ -139,7 +154,7 @@ Tensor linear_cross_entropy(const Tensor &x, const Tensor &weight, const Tensor 
   const int64_t how = reduction == "mean" ? SMLM_REDUCE_MEAN : reduction == "sum" ? SMLM_REDUCE_SUM
                       : reduction == "none" ? SMLM_REDUCE_NONE : -1;
   TORCH_CHECK_VALUE(how >= 0, "linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got '", reduction, "'");
-  return LinearCrossEntropy::apply(x, weight, targets, ignore, how);
+  return LinearCrossEntropy::apply(plain(x), plain(weight), targets, ignore, how);
 }
 
 // ---- the feed-forward block --------------------------------------------------------------------------------------------
@@ -168,10 +183,11 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
 
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w13 = saved[1], &w2 = saved[2], &dy = grads[0];
+    const Tensor &x = saved[0], &w13 = saved[1], &w2 = saved[2], dy = plain(grads[0]);
     const bool want_x = ctx->needs_input_grad(0), want_w13 = ctx->needs_input_grad(1), want_w2 = ctx->needs_input_grad(2);
     const int64_t d = x.size(-1), o = w2.size(0), h = w2.size(1), M = x.numel() / d, d8 = ceil8(d), h8 = ceil8(h), o8 = ceil8(o);
     if (at::GradMode::is_enabled()) {
+      const NoAutocast fp32;
       const auto ab = at::matmul(x.to(at::kFloat), w13.to(at::kFloat).t()).chunk(2, -1);
       const Tensor y = at::matmul(at::silu(ab[0]) * ab[1], w2.to(at::kFloat).t()).to(dy.scalar_type());
       return recorded(y, dy, {x, w13, w2}, {want_x, want_w13, want_w2});
@@ -204,7 +220,7 @@ Tensor gated_ffn(const Tensor &x, const Tensor &w13, const Tensor &w2) {
                         w13.size(1) == x.size(-1) && w13.numel() > 0 && w2.numel() > 0,
                     "gated_ffn: expected x (..., d), w13 (2 * hidden, d) and w2 (n_out, hidden), got ", x.sizes(), ", ",
                     w13.sizes(), " and ", w2.sizes());
-  return GatedFFN::apply(x, w13, w2);
+  return GatedFFN::apply(plain(x), plain(w13), plain(w2));
 }
 
 // ---- the norm ----------------------------------------------------------------------------------------------------------
@@ -231,7 +247,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
 
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &xs = saved[0], &weight = saved[1], &rstd = saved[2], &dxs = grads[0], &dh = grads[1];
+    const Tensor &xs = saved[0], &weight = saved[1], &rstd = saved[2], dxs = plain(grads[0]), dh = plain(grads[1]);
     const int64_t kind = ctx->saved_data["delta"].toInt();
     const bool add = kind >= 0;
     const auto delta_dtype = add ? (at::ScalarType)kind : xs.scalar_type();
@@ -299,7 +315,8 @@ std::tuple<Tensor, Tensor> add_rmsnorm_train(const Tensor &x, const std::optiona
                     name, ": x ", x.sizes(), " must end with the norm's ", weight.sizes(), ", at most ", kNormMaxCols, " columns");
   const double e = eps.value_or(x.scalar_type() == at::kFloat ? 0x1p-23 : 0x1p-7);   // torch.finfo(x.dtype).eps
   TORCH_CHECK_VALUE(e >= 0, name, ": the norm's eps must not be negative, got ", e);
-  const auto got = AddRMSNorm::apply(x, delta, weight, e, out);
+  const auto added = delta.has_value() ? std::optional<Tensor>(plain(*delta)) : delta;
+  const auto got = AddRMSNorm::apply(plain(x), added, plain(weight), e, out);
   return {got[0], got[1]};
 }
 

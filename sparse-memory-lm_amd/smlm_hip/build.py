@@ -4,9 +4,9 @@
 
 Every .hip file is compiled to an object in sparse-memory-lm_amd/_build/ (in parallel), then linked into
 smlm_hip/libsmlm_pkm.so next to this file, where smlm_hip._lib loads it.  The autograd nodes of the training operators
-(csrc/torch/*.cpp, host code against torch's headers) become the Python module smlm_hip/_train_ops.so.  The memory-ceiling kernels of bench.py
-(csrc/bench/*.hip: sequential read / write / copy and random-row reads) go into a separate smlm_hip/libsmlm_bench.so,
-so the lookup library holds only the product.
+(csrc/torch/*.cpp, host code against torch's headers) become the Python module smlm_hip/_train_ops.so.  The memory-ceiling
+kernels of bench.py (csrc/bench/*.hip: sequential read / write / copy and random-row reads) go into a separate
+smlm_hip/libsmlm_bench.so, so the lookup library holds only the product.
 """
 import os
 import subprocess

@@ -457,25 +457,27 @@ class Transformer(nn.Module):
         ("none": idx's shape).  On the GPU in bf16 (bf16 weights or bf16 autocast) the residual adds, norms, feed-forward
         blocks and the loss run as kernels.add_rmsnorm_train, gated_ffn and linear_cross_entropy, whose logits are not
         rounded to bf16 as forward()'s are; anything else, and modules that are watched or replaced, runs the modules."""
-        x = self.tok_emb(idx)
-        if not self._loss_kernels(x, targets):
+        if not self._loss_kernels(idx, targets):
             logits = self(idx).float()
             loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)), targets.reshape(-1), ignore_index=ignore_index,
                                    reduction=reduction)
             return loss.view(targets.shape) if reduction == "none" else loss
         rows = self._ngram_rows(idx, None) if self.ngram is not None else None
-        h = self._blocks_recorded(x, rows)
+        h = self._blocks_recorded(self.tok_emb(idx), rows)
         return kernels.linear_cross_entropy(h, self.lm_head.weight.to(torch.bfloat16), targets, ignore_index, reduction)
 
-    def _loss_kernels(self, x, targets):
-        """Whether loss() may end in linear_cross_entropy: bf16 arithmetic on the GPU, a plain output embedding and final
+    def _loss_kernels(self, idx, targets):
+        """Whether loss() may end in linear_cross_entropy: bf16 arithmetic on the GPU, plain embeddings and a plain final
         norm, nothing that watches the ops."""
-        head, bf16 = self.lm_head, torch.bfloat16
+        emb, head, bf16 = self.tok_emb, self.lm_head, torch.bfloat16
+        if (type(self).forward is not Transformer.forward or type(emb) is not nn.Embedding or type(head) is not nn.Linear
+                or not unhooked(self, emb, head)):
+            return False
+        x = emb.weight
         autocast = torch.is_autocast_enabled("cuda")
         return (x.is_cuda and (torch.get_autocast_dtype("cuda") == bf16 if autocast else x.dtype == bf16)
-                and type(head) is nn.Linear and head.bias is None and unhooked(head)
-                and head.weight.dtype in (bf16, x.dtype) and targets.device == x.device
-                and _norm_kernels(self.norm, x) and ordinary(x, head.weight, targets))
+                and head.bias is None and head.weight.dtype in (bf16, x.dtype) and idx.device == targets.device == x.device
+                and _norm_kernels(self.norm, x) and ordinary(idx, head.weight, targets))
 
     def _blocks_recorded(self, x, rows):
         """The blocks of forward() over whole sequences and the final norm, with every residual add in the launch of the
@@ -509,7 +511,7 @@ class Transformer(nn.Module):
                 delta = blk.ffn(normed(blk.ffn_norm, x.dtype))
             if blk.ffn_r2 is not None:
                 delta = blk.ffn_r2(normed(blk.ffn_norm_r2, x.dtype))
-        return normed(self.norm, bf16)
+        return normed(self.norm, bf16).to(bf16)
 
     @torch.no_grad()
     def forward_graphed(self, idx):

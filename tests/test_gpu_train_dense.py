@@ -281,6 +281,26 @@ def test_loss_recorded_gradient():
     assert float((got.double() - ref).norm() / ref.norm()) <= 0.02
 
 
+def test_loss_recorded_gradient_of_targets_outside_the_vocabulary():
+    x, w, t = randn(6, 16).requires_grad_(), randn(20, 16, std=0.3, seed=2).requires_grad_(), targets(6, 20)
+    t[2], t[4] = 20, -7
+    for create in (False, True):
+        dx, = torch.autograd.grad(kernels.linear_cross_entropy(x, w, t, reduction="sum"), x, create_graph=create)
+        assert torch.isnan(dx[[2, 4]]).all() and torch.isfinite(dx[[0, 1, 3, 5]]).all()
+
+
+def test_recorded_gradients_keep_fp32_under_autocast():
+    x, w, t = randn(6, 16).requires_grad_(), randn(20, 16, std=0.3, seed=2).requires_grad_(), targets(6, 20)
+    y, w13, w2, g = ffn_inputs(9, 16, 24, 16)
+    y = y.requires_grad_()
+    got = []
+    for on in (False, True):
+        with torch.autocast("cuda", dtype=BF16, enabled=on):
+            got.append(torch.autograd.grad(kernels.linear_cross_entropy(x, w, t), (x, w), create_graph=True)
+                       + torch.autograd.grad(kernels.gated_ffn(y, w13, w2), y, g, create_graph=True))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ---------------------------------------------------------------------------------------------- the FFN block
 def ffn_reference(x, w13, w2, g):
     x, w13, w2, g = (t.double() for t in (x, w13, w2, g))
@@ -613,6 +633,33 @@ def test_two_graphs_share_nothing():
 
 
 # --------------------------------------------------------------------------------------------------- refusals
+def test_lazily_negated_views():
+    """Views whose sign is yet to be applied (a conjugate's imaginary part is one) count with it, gradients too."""
+    x, w, t = randn(40, 24), randn(60, 24, std=0.3, seed=2), targets(40, 60)
+    neg = torch._neg_view
+    assert all(torch.equal(a, b) for a, b in zip(run_loss(neg(x), neg(w), t, "none", g=neg(randn(40, dtype=F32))),
+                                                 run_loss(-x, -w, t, "none", g=-randn(40, dtype=F32))))
+    ins = ffn_inputs(40, 24, 32, 16)
+    assert all(torch.equal(a, b) for a, b in zip(run_ffn(*map(neg, ins)), run_ffn(*(-i for i in ins))))
+    n = torch.nn.RMSNorm(24, eps=1e-5, device=DEV)
+    z = torch.complex(randn(40, 24, dtype=F32), randn(40, 24, seed=3, dtype=F32)).conj().imag
+    assert z.is_neg()
+    a, b = kernels.add_rmsnorm_train(z, z, n), kernels.add_rmsnorm_train(z.clone().resolve_neg(), z.resolve_neg(), n)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_no_traces():
+    x, w, t = randn(8, 16), randn(20, 16), targets(8, 20)
+    _, w13, w2, _ = ffn_inputs(8, 16, 16, 16)
+    n = torch.nn.RMSNorm(16, device=DEV)
+    for f in (lambda x: kernels.linear_cross_entropy(x, w, t), lambda x: kernels.gated_ffn(x, w13, w2),
+              lambda x: kernels.add_rmsnorm_train(x, None, n)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.func.vmap(f)(torch.stack([x, x]))
+
+
 def test_refusals():
     x, w, t = randn(4, 16), randn(30, 16), targets(4, 30)
     for bad in (lambda: kernels.linear_cross_entropy(x.float(), w, t), lambda: kernels.linear_cross_entropy(x, w.float(), t),
@@ -736,13 +783,13 @@ def test_model_loss_with_memory_and_engram_layers(monkeypatch):
         assert (g is None) == (got[n] is None), n
 
 
-@pytest.mark.parametrize("watch", ["norm", "ffn", "block", "head", "subclass", "final"])
+@pytest.mark.parametrize("watch", ["norm", "ffn", "block", "head", "subclass", "final", "embedding", "model"])
 def test_model_loss_keeps_watched_modules(watch, monkeypatch):
     m = lm(BF16)
     idx, t = batch()
     seen = []
     target = {"norm": m.layers[1].ffn_norm, "ffn": m.layers[1].ffn.w2, "block": m.layers[1], "head": m.lm_head,
-              "final": m.norm}.get(watch)
+              "final": m.norm, "embedding": m.tok_emb, "model": m}.get(watch)
     if target is not None:
         target.register_forward_hook(lambda *a: seen.append(1))
     else:
@@ -756,7 +803,7 @@ def test_model_loss_keeps_watched_modules(watch, monkeypatch):
     if target is not None:
         assert len(seen) == 2                              # once in each
     expected = {"norm": (1, 3, 6), "ffn": (1, 2, 7), "block": (1, 2, 5), "head": (0, 0, 0), "subclass": (1, 2, 7),
-                "final": (0, 0, 0)}[watch]
+                "final": (0, 0, 0), "embedding": (0, 0, 0), "model": (0, 0, 0)}[watch]
     assert tuple(calls.values()) == expected, calls
 
 

@@ -139,3 +139,11 @@ def test_loss_on_the_cpu_is_the_modules(reduction):
     assert torch.equal(got.reshape(-1), ref.reshape(-1)) and got.shape == (t.shape if reduction == "none" else ())
     got.sum().backward()
     assert m.tok_emb.weight.grad is not None
+
+
+def test_loss_calls_a_watched_embedding_once():
+    m, seen = small(), []
+    m.tok_emb.register_forward_hook(lambda *a: seen.append(1))
+    m.register_forward_hook(lambda *a: seen.append(2))
+    m.loss(torch.zeros(1, 4, dtype=torch.int64), torch.ones(1, 4, dtype=torch.int64))
+    assert seen == [1, 2]

@@ -263,10 +263,11 @@ struct FfnPlan {
 };
 FfnPlan ffn_plan(int64_t M, int64_t d, int64_t hidden, int64_t n_out) {
   FfnPlan p;
-  p.y = mm_plan(M, n_out, hidden, true);
-  p.dx = mm_plan(M, d, 2 * hidden, true);
-  p.dw13 = mm_plan(2 * hidden, d, M, true);
-  p.dw2 = mm_plan(n_out, hidden, M, true);
+  const int terms = mm_terms(M);
+  p.y = mm_plan(M, n_out, hidden * terms, true);
+  p.dx = mm_plan(M, d, 2 * hidden * terms, true);
+  p.dw13 = mm_plan(2 * hidden, d, M * terms, true);
+  p.dw2 = mm_plan(n_out, hidden, M * terms, true);
   p.act = M * hidden * 2 * mm_terms(M);
   p.parts_forward = p.y.part_bytes(M, n_out);
   p.parts_backward = std::max(p.dx.part_bytes(M, d), std::max(p.dw13.part_bytes(2 * hidden, d), p.dw2.part_bytes(n_out, hidden)));

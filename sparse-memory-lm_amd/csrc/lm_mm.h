@@ -328,7 +328,7 @@ inline int mm_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &do
 // second bf16 with what the first leaves, 16 bits of mantissa together.  Over many tokens the first's roundings average out
 // in the sums (a result's error is 1.4 of its own rounding's); of a few tokens single values carry a result, whose error
 // would be up to twice that, and the products are bound by the weights' bytes and the launches: the second terms cost the
-// loss of 64 tokens 56 -> 61 us and an FFN block of 48 tokens 36 -> 44, both less than the calls take on the host; at 512 tokens
+// loss of 64 tokens 56 -> 61 us and an FFN block of 48 tokens 36 -> 41, both less than the calls take on the host; at 512 tokens
 // the loss' two products would take twice as long.
 constexpr int64_t kMmFewTokens = 128;
 inline int mm_terms(int64_t tokens) { return tokens <= kMmFewTokens ? 2 : 1; }

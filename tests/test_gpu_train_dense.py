@@ -633,6 +633,54 @@ def test_two_graphs_share_nothing():
 
 
 # --------------------------------------------------------------------------------------------------- refusals
+def bulk(rows, cols, std=1.0, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.empty(rows, cols, dtype=BF16, device=DEV).normal_(0, std, generator=g)
+
+
+def test_ffn_past_2_31_elements():
+    """1,100,000 x 2,048 gradients of a and b: the last rows against the reference; of the others dy is 0, so that the
+    weights' gradients are those of the last rows alone."""
+    M, d, h, o, n = 1100000, 16, 1024, 16, 700
+    note("ffn", M, d, h, o)
+    x, (_, w13, w2, _) = bulk(M, d), ffn_inputs(1, d, h, o)
+    g = torch.zeros(M, o, dtype=BF16, device=DEV)
+    g[-n:] = randn(n, o, std=0.1, seed=3)
+    y, dx, dw13, dw2 = run_ffn(x, w13, w2, g)
+    ref = ffn_reference(x[-n:], w13, w2, g[-n:])
+    assert not dx[:-n].any()
+    for name, t, (r, tol) in zip(("y", "dx", "dw13", "dw2"), (y[-n:], dx[-n:], dw13, dw2), ref):
+        close(t, r, tol, name)
+
+
+def test_loss_past_2_31_elements():
+    """2,200,000 x 1,000 states, of which the last few count, over a small vocabulary."""
+    M, V, d, n = 2200000, 300, 1000, 500
+    note("loss", M, V, d)
+    x, w = bulk(M, d), randn(V, d, std=0.1, seed=2)
+    t = torch.full((M,), -100, device=DEV)
+    t[-n:] = targets(n, V)
+    loss, dx, dw = run_loss(x, w, t, "sum")
+    (l, lt), (rx, xt), (rw, wt) = loss_reference(x[-n:], w, t[-n:], -100, "sum")
+    assert not dx[:-n].any()
+    for name, got, r, tol in (("loss", loss, l, lt), ("dx", dx[-n:], rx, xt), ("dw", dw, rw, wt)):
+        close(got, r, tol, name)
+
+
+def test_norm_past_2_31_elements():
+    M, C, n = 2200000, 1001, 300
+    note("norm", M, C)
+    norm = norm_of(C, F32)
+    x, gh = bulk(M, C), torch.zeros(M, C, dtype=BF16, device=DEV)
+    gh[-n:] = randn(n, C, seed=5)
+    xs, h, (dx, dw) = run_norm(x, None, norm, BF16, None, gh)
+    small = run_norm(x[-n:], None, norm, BF16, None, gh[-n:])
+    assert torch.equal(h[-n:], small[1]) and torch.equal(dx[-n:], small[2][0]) and not dx[:-n].any()
+    # the same terms in another order: n sums of fp32
+    hat = small[1].double() / norm.weight.detach().double()
+    close(dw, small[2][1].double(), 2 * (n + 64) * U32 * (gh[-n:].double() * hat).abs().sum(0) + TINY, "dw")
+
+
 def test_lazily_negated_views():
     """Views whose sign is yet to be applied (a conjugate's imaginary part is one) count with it, gradients too."""
     x, w, t = randn(40, 24), randn(60, 24, std=0.3, seed=2), targets(40, 60)

@@ -9,11 +9,10 @@
 //   gate_kernel   x w13^T and the activation; each lane holds matching a and b.  For the gradient (GRAD) dy w2 on the
 //                 same tokens and features through the same stages: writes act and [da | db] in bf16
 //   mm_kernel     y, dx, dw13, dw2 (lm_mm.hip); the weights' sums over the tokens are split over workgroups
-// Bound by the products: 6 M d hidden operations forward, 18 with the recomputed a | b in the gradient, d = 384 of them six
-// units of 64 k, so that a tile's beginning and end weigh as much as a third of its products; the rate while they run is that
-// of the way from cache into LDS (lm_mm.h).  Measured for 32,768 tokens of d = 384, hidden 1,024: the gate 65 to 74 us (750 TFLOP/s),
-// y 32, the gradient's gate 140 (550; its three results are 201 MB written), dx 62, dw13 58, dw2 51 and the joining of
-// their parts 14.
+// Bound by the products: 6 M d hidden operations forward, 18 with the recomputed a | b in the gradient; their rate is that of
+// the way from cache into LDS (lm_mm.h), and d = 384 of them are only six units of 64 k a tile.  Measured for 32,768 tokens
+// of d = 384, hidden 1,024: the gate 65 to 74 us (750 TFLOP/s), y 32, the gradient's gate 120 to 140 (its three results are
+// 201 MB, and take 60 us of it: they do not overlap its products), dx 62, dw13 58, dw2 51 and the joining of their parts 14.
 #include "lm_mm.h"
 
 #include <algorithm>

@@ -8,9 +8,9 @@
 // one wavefront per token; the target's logit is picked from the accumulators, so that it is the very value in the sum.
 // A third launch adds the tokens' losses up (in fp64, in a fixed order).  Only lse (fp32 per token) is kept.
 //
-// Gradient, in pieces of the vocabulary: the logits of a piece again, G of the piece as bf16 (of up to 128 tokens as two bf16
-// terms; c_n is 0 or 1 where the loss is a mean or sum, so that G needs no scale: 1 / count goes on at the end), then its two products (lm_mm.hip): dW's
-// rows of the piece are final, dx gathers over the pieces in fp32.
+// Gradient, in pieces of the vocabulary: the logits of a piece again, G of the piece as bf16 (of up to 128 tokens as two
+// bf16 terms; c_n is 0 or 1 where the loss is a mean or sum, so that G needs no scale: 1 / count goes on at the end), then
+// its two products (lm_mm.hip): dW's rows of the piece are final, dx gathers over the pieces in fp32.
 //
 // Bound by the products: 2 M V d operations forward, three times that in the gradient (one third for the logits again, which
 // is what not keeping them costs).  With d = 384 a tile's sum is short, six units of 64 k, and 128 exponentials a lane follow

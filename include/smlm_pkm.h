@@ -538,6 +538,14 @@ int smlm_engram_mix_backward(const float *gy, const float *h, const void *k, con
                              float *dconv, float *parts, void *stream);
 
 /*
+ * Rows of 16-bit elements with zeros behind them, as the training products read their operands: `blocks` groups of `rows` rows
+ * of `cols`, row_stride elements apart, into groups of rows_out >= rows rows of cols_out >= cols (a multiple of 8),
+ * contiguous and 16-byte aligned.
+ */
+int smlm_pad_rows(const void *src, int64_t row_stride, int64_t blocks, int64_t rows, int64_t cols, void *dst,
+                  int64_t rows_out, int64_t cols_out, void *stream);
+
+/*
  * Cross entropy of the logits s = x W^T without storing them (F.cross_entropy(lm_head(x).float(), targets),
  * smlm/model.py:286-293): per token logsumexp(s_n) - s_n[targets[n]], 0 where targets[n] == ignore_index, NaN where it
  * is any other index outside the vocabulary; their mean over the tokens that are not ignored (NaN if none), or sum.

@@ -122,6 +122,33 @@ __global__ void __launch_bounds__(256)
   *(uint2 *)(out + t * ldo + f) = uint2{pack_bf16x2(v.x * c, v.y * c), pack_bf16x2(v.z * c, v.w * c)};
 }
 
+struct __attribute__((packed, aligned(2))) Piece {
+  uint32_t v[4];
+};
+
+// One thread per 8 elements of the copy; bound by memory and, for what is padded most often, by its launch.
+__global__ void __launch_bounds__(256)
+    pad_rows_kernel(const uint16_t *__restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
+                    int64_t rows_out, int64_t cols_out, int64_t total) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= total) return;
+  const int64_t at = i / (cols_out / 8), c = 8 * (i - at * (cols_out / 8)), block = at / rows_out, r = at - block * rows_out;
+  const int64_t n = r < rows ? cols - c : 0;
+  const uint16_t *p = src + (block * rows + r) * ld + c;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (n >= 8) {
+    const Piece w = *(const Piece *)p;
+    v = make_uint4(w.v[0], w.v[1], w.v[2], w.v[3]);
+  } else if (n > 0) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) w[e / 2] |= (uint32_t)p[e] << 16 * (e % 2);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  *(uint4 *)(dst + at * cols_out + c) = v;
+}
+
 template <class S, bool FKC, bool TKC>
 int launch(const MmArgs &a, hipStream_t stream, const char *what) {
   constexpr int kLds = MmKernel<S, FKC, TKC>::kLds;
@@ -206,3 +233,19 @@ int mm_reduce_launch(const float *parts, int64_t nsplit, int64_t T, int64_t F, c
 }
 
 }  // namespace smlm
+
+extern "C" int smlm_pad_rows(const void *src, int64_t row_stride, int64_t blocks, int64_t rows, int64_t cols, void *dst,
+                             int64_t rows_out, int64_t cols_out, void *stream) {
+  using namespace smlm;
+  const char *what = "smlm_pad_rows";
+  if (!src || !dst) return fail(SMLM_EINVAL, "%s: null pointer argument", what);
+  if (blocks < 1 || rows < 0 || cols < 0 || rows_out < rows || cols_out < cols || rows_out < 1 || cols_out < 8 || cols_out % 8 ||
+      row_stride < cols || (uintptr_t)dst % 16 || (uintptr_t)src % 2)
+    return fail(SMLM_EINVAL, "%s: bad shape, or dst not in 16-byte aligned rows", what);
+  if (blocks > (1 << 20) || rows_out > (1LL << 40) || cols_out > (1LL << 30) || rows_out > (1LL << 38) / cols_out / blocks)
+    return fail(SMLM_EUNSUPPORTED, "%s: too large", what);
+  const int64_t total = blocks * rows_out * (cols_out / 8);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, (hipStream_t)stream,
+                     (const uint16_t *)src, row_stride, rows, cols, (uint16_t *)dst, rows_out, cols_out, total);
+  return launch_status(what);
+}

@@ -79,6 +79,7 @@ EXPORTS = {
     "smlm_engram_mix": (_i, [_p] * 7 + [_i, _p, _p, _i64, _i64, _i, _i, _i, _f, _p, _p]),
     "smlm_engram_mix_parts": (_i64, [_i64, _i64, _i, _i]),
     "smlm_engram_mix_backward": (_i, [_p] * 8 + [_i64, _i64, _i, _i, _i, _f] + [_p] * 9),
+    "smlm_pad_rows": (_i, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p]),
     "smlm_linear_ce_workspace": (_i64, [_i64, _i64, _i64, _i]),
     "smlm_linear_ce": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
     "smlm_linear_ce_backward": (_i, [_p, _p, _i, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,

@@ -83,6 +83,15 @@ def test_gated_ffn_refusals():
     assert back(dx=None, dw13=None, dw2=None) == back(M=0) == back(ldy=56) == back(bytes=64) == _lib.EINVAL
 
 
+def test_pad_rows_refusals():
+    def call(**kw):
+        ok = dict(src=FAKE, ld=65, blocks=2, rows=5, cols=65, dst=FAKE, rows_out=8, cols_out=72)
+        return _lib.lib().smlm_pad_rows(*dict(ok, **kw).values(), None)
+    assert call(src=None) == call(dst=None) == call(dst=FAKE + 8) == call(src=FAKE + 1) == _lib.EINVAL
+    assert call(ld=64) == call(blocks=0) == call(rows=9) == call(rows=-1) == call(cols=73) == call(cols_out=68) == _lib.EINVAL
+    assert call(rows_out=1 << 41) == call(cols_out=1 << 31) == call(blocks=1 << 21) == call(rows_out=1 << 36) == _lib.EUNSUPPORTED
+
+
 def test_rmsnorm_train_refusals():
     lib = _lib.lib()
     ok = dict(x=FAKE, xt=_lib.F32, delta=FAKE, dt=_lib.BF16, w=FAKE, wt=_lib.F32, eps=1e-5, M=10, C=64, xs=FAKE, h=FAKE,

@@ -322,7 +322,7 @@ std::tuple<Tensor, Tensor> add_rmsnorm_train(const Tensor &x, const std::optiona
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 1 && weight.size(0) == x.size(-1) && x.size(-1) > 0 &&
                         x.size(-1) <= kNormMaxCols,
                     name, ": x ", x.sizes(), " must end with the norm's ", weight.sizes(), ", at most ", kNormMaxCols, " columns");
-  const double e = eps.value_or(x.scalar_type() == at::kFloat ? 0x1p-23 : 0x1p-7);   // torch.finfo(x.dtype).eps
+  const double e = eps.value_or(0x1p-23);   // nn.RMSNorm's default: of fp32, which it computes in, whatever x's type
   TORCH_CHECK_VALUE(e >= 0, name, ": the norm's eps must not be negative, got ", e);
   const auto added = delta.has_value() ? std::optional<Tensor>(plain(*delta)) : delta;
   const auto got = AddRMSNorm::apply(plain(x), added, plain(weight), e, out);

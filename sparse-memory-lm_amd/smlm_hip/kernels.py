@@ -616,18 +616,18 @@ def add_rmsnorm(x, delta, norm):
         raise ValueError("add_rmsnorm: the norm needs a bf16 weight of size C")
     x = x.contiguous()
     delta = delta.contiguous() if delta is not None else None
-    eps = norm.eps if norm.eps is not None else torch.finfo(torch.bfloat16).eps
     h = torch.empty_like(x)
     x_out = torch.empty_like(x) if delta is not None else x
     rc = _lib.lib().smlm_add_rmsnorm(x.data_ptr(), delta.data_ptr() if delta is not None else None,
-                                     norm.weight.data_ptr(), float(eps), x.numel() // C, C,
+                                     norm.weight.data_ptr(), float(_rms_eps(norm)), x.numel() // C, C,
                                      x_out.data_ptr() if delta is not None else None, h.data_ptr(), _stream(x))
     _lib.check(rc, "smlm_add_rmsnorm")
     return x_out, h
 
 
 def _rms_eps(norm):
-    return norm.eps if norm.eps is not None else torch.finfo(torch.bfloat16).eps
+    """The norm's epsilon; without one, as F.rms_norm, that of fp32, which the statistics are in."""
+    return norm.eps if norm.eps is not None else torch.finfo(torch.float32).eps
 
 
 def decode_linear(weight, x=None, *, delta=None, norm=None, tok=None, emb=None, write_x=False, bias=None,

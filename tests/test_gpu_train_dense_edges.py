@@ -1,0 +1,50 @@
+"""Edges of the dense training operators on the GPU: default arguments, operands of one row, inputs that depend on each
+other, what a backward gets back, replaced and watched sublayers, and every tile of the products.  Tolerances as in
+test_gpu_train_dense.py."""
+import ctypes
+import itertools
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from smlm_hip import _lib, kernels
+from test_gpu_train_dense import (BF16, DEV, F32, HALF, U32, batch, check_ffn, check_loss, close, ffn_inputs, lm, note, randn,
+                                  rounding, run_ffn, run_loss, spied, targets)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- default epsilons
+@pytest.mark.parametrize("xt,wt", itertools.product([F32, BF16], repeat=2))
+def test_norm_default_eps(xt, wt):
+    """nn.RMSNorm(C) without eps adds the epsilon of fp32, the type it computes in, whatever its input's: rows whose mean
+    square is about as small tell it from any other."""
+    M, C = 9, 40
+    norm = torch.nn.RMSNorm(C, device=DEV, dtype=wt)
+    x = randn(M, C, std=2.0 ** -11, dtype=xt).requires_grad_()
+    g = randn(M, C, seed=4, dtype=xt)
+    _, h = kernels.add_rmsnorm_train(x, None, norm)
+    dx, dw = torch.autograd.grad(h, (x, norm.weight), g)
+    s, w = x.detach().double(), norm.weight.detach().double()
+    r = (s.square().mean(1, keepdim=True) + 2.0 ** -23).rsqrt()
+    hat, k = s * r, (C + 16) * U32
+    close(h.detach(), hat * w, (hat * w).abs() * (rounding(xt) + k) * 1.01, "h")
+    close(F.rms_norm(x.detach(), (C,), norm.weight.detach()), hat * w, (hat * w).abs() * (2 * rounding(xt) + k) * 1.01, "torch's")
+    gw = g.double() * w
+    mean, mean_abs = (gw * hat).mean(1, keepdim=True), (gw * hat).abs().mean(1, keepdim=True)
+    ref = (gw - hat * mean) * r
+    close(dx, ref, (2 * k * r * (gw.abs() + hat.abs() * mean_abs) + rounding(xt) * ref.abs()) * 1.01, "dx")
+    ref = (g.double() * hat).sum(0)
+    close(dw, ref, ((g.double() * hat).abs().sum(0) * (M + C + 64) * U32 + rounding(wt) * ref.abs()) * 1.01, "dw")
+
+
+def test_forward_norms_default_eps():
+    """The forward-only norm and the decode linear's: the same bits as with that epsilon given."""
+    C = 64
+    norm, same = (torch.nn.RMSNorm(C, eps=e, device=DEV, dtype=BF16) for e in (None, 2.0 ** -23))
+    x, w = randn(9, C, std=2.0 ** -11), randn(48, C, std=0.1, seed=2)
+    assert torch.equal(kernels.add_rmsnorm(x, None, norm)[1], kernels.add_rmsnorm(x, None, same)[1])
+    assert torch.equal(kernels.decode_linear(w, x, norm=norm), kernels.decode_linear(w, x, norm=same))
+    close(kernels.add_rmsnorm(x, None, norm)[1], F.rms_norm(x.double(), (C,), None, 2.0 ** -23),
+          2.0 * HALF * F.rms_norm(x.double(), (C,), None, 2.0 ** -23).abs(), "h")

@@ -156,3 +156,11 @@ def test_loss_calls_a_watched_embedding_once():
     m.register_forward_hook(lambda *a: seen.append(2))
     m.loss(torch.zeros(1, 4, dtype=torch.int64), torch.ones(1, 4, dtype=torch.int64))
     assert seen == [1, 2]
+
+
+def test_default_eps_is_that_of_fp32():
+    """F.rms_norm's without one, for bf16 inputs too."""
+    norm, x = torch.nn.RMSNorm(16), (torch.randn(5, 16, generator=torch.Generator().manual_seed(0)) * 2.0 ** -11).bfloat16()
+    assert kernels._rms_eps(norm) == 2.0 ** -23 and kernels._rms_eps(torch.nn.RMSNorm(16, eps=1e-5)) == 1e-5
+    got, ref = F.rms_norm(x, (16,)).double(), F.rms_norm(x.double(), (16,), eps=kernels._rms_eps(norm))
+    assert ((got - ref).abs() <= 2 * 2.0 ** -8 * ref.abs()).all()

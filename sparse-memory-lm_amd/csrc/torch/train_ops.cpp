@@ -49,7 +49,8 @@ Tensor workspace(const Tensor &like, int64_t bytes) { return at::empty({bytes}, 
 // t, `blocks` groups of rows, with zeros behind each group's rows and behind the columns.  (Fill and copy, as constant_pad_nd
 // does it, are two launches: forward and gradient of an FFN block of 48 x 65, hidden 130, took 85 us instead of 68.)
 Tensor padded(const Tensor &t, int64_t blocks, int64_t rows, int64_t cols) {
-  const Tensor s = t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
+  // (contiguous() would leave a single row its stride, which may be any)
+  const Tensor s = t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.clone(at::MemoryFormat::Contiguous);
   const Tensor out = at::empty({blocks * rows, cols}, t.options());
   check(smlm_pad_rows(s.data_ptr(), s.stride(0), blocks, s.size(0) / blocks, s.size(1), out.data_ptr(), rows, cols, stream_of(t)),
         "smlm_pad_rows");

@@ -48,3 +48,24 @@ def test_forward_norms_default_eps():
     assert torch.equal(kernels.decode_linear(w, x, norm=norm), kernels.decode_linear(w, x, norm=same))
     close(kernels.add_rmsnorm(x, None, norm)[1], F.rms_norm(x.double(), (C,), None, 2.0 ** -23),
           2.0 * HALF * F.rms_norm(x.double(), (C,), None, 2.0 ** -23).abs(), "h")
+
+
+# ------------------------------------------------------------------------------------------- operands of one row
+def row(t):
+    """The one row of t as a transposed column: strides (1, 1)."""
+    t = t.reshape(-1, 1).contiguous().t()
+    assert t.stride() == (1, 1)
+    return t
+
+
+def test_operands_of_one_row_have_any_row_stride():
+    """Odd widths, so that the operands are padded: a weight of one row that is a transposed column, and the gradient of a
+    sum, whose strides are 0."""
+    x, w13, w2, g = ffn_inputs(1, 33, 65, 1)
+    assert all(torch.equal(a, b) for a, b in zip(run_ffn(x, w13, w2, g), run_ffn(row(x), w13, row(w2), g)))
+    ins = [t.detach().requires_grad_() for t in (x, w13, w2)]
+    kernels.gated_ffn(*ins).sum().backward()
+    want = run_ffn(x, w13, w2, torch.ones_like(g))[1:]
+    assert all(torch.equal(t.grad, b) for t, b in zip(ins, want))
+    x, w, t = randn(5, 33), randn(1, 33, std=0.3, seed=2), torch.zeros(5, dtype=torch.int64, device=DEV)
+    assert all(torch.equal(a, b) for a, b in zip(run_loss(x, w, t), run_loss(x, row(w), t)))

@@ -76,7 +76,15 @@ struct NoAutocast {
   c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset};
 };
 
-// The gradients of `y` with respect to the wanted inputs, recorded.
+// The inputs as a recorded backward differentiates them: aliases, so that the gradient of one is not also what reaches it by
+// way of another that was computed from it (tied embeddings), which the graph around this node adds by itself.
+variable_list aliases(const variable_list &inputs) {
+  variable_list out;
+  for (const Tensor &t : inputs) out.push_back(t.view_as(t));
+  return out;
+}
+
+// The gradients of `y` with respect to the wanted inputs (aliases), recorded.
 variable_list recorded(const Tensor &y, const Tensor &dy, const variable_list &inputs, const std::vector<bool> &wants) {
   variable_list asked;
   for (size_t i = 0; i < inputs.size(); ++i)
@@ -130,9 +138,10 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       const Tensor t = targets.reshape({M}), bad = t.ne(ignore).logical_and(t.lt(0).logical_or(t.ge(V)));
       const Tensor one = at::ones({}, x.options().dtype(at::kFloat));
       const Tensor poison = at::where(bad, one * std::numeric_limits<float>::quiet_NaN(), one).unsqueeze(1);
-      const Tensor logits = at::matmul(x.reshape({M, d}).to(at::kFloat), weight.to(at::kFloat).t()) * poison;
+      const auto in = aliases({x, weight});
+      const Tensor logits = at::matmul(in[0].reshape({M, d}).to(at::kFloat), in[1].to(at::kFloat).t()) * poison;
       const Tensor y = at::cross_entropy_loss(logits, t.masked_fill(bad, ignore == 0 && V > 1 ? 1 : 0), {}, reduction, ignore);
-      const auto got = recorded(y, g.reshape(y.sizes()), {x, weight}, {want_x, want_w});
+      const auto got = recorded(y, g.reshape(y.sizes()), in, {want_x, want_w});
       return {got[0], got[1], Tensor(), Tensor(), Tensor()};
     }
     if (M == 0) return {at::zeros_like(x), at::zeros_like(weight), Tensor(), Tensor(), Tensor()};
@@ -198,9 +207,10 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
     const int64_t d = x.size(-1), o = w2.size(0), h = w2.size(1), M = x.numel() / d, d8 = ceil8(d), h8 = ceil8(h), o8 = ceil8(o);
     if (at::GradMode::is_enabled()) {
       const NoAutocast fp32;
-      const auto ab = at::matmul(x.to(at::kFloat), w13.to(at::kFloat).t()).chunk(2, -1);
-      const Tensor y = at::matmul(at::silu(ab[0]) * ab[1], w2.to(at::kFloat).t()).to(dy.scalar_type());
-      return recorded(y, dy, {x, w13, w2}, {want_x, want_w13, want_w2});
+      const auto in = aliases({x, w13, w2});
+      const auto ab = at::matmul(in[0].to(at::kFloat), in[1].to(at::kFloat).t()).chunk(2, -1);
+      const Tensor y = at::matmul(at::silu(ab[0]) * ab[1], in[2].to(at::kFloat).t()).to(dy.scalar_type());
+      return recorded(y, dy, in, {want_x, want_w13, want_w2});
     }
     if (M == 0) return {at::zeros_like(x), at::zeros_like(w13), at::zeros_like(w2)};
     const c10::DeviceGuard guard(x.device());

@@ -69,3 +69,31 @@ def test_operands_of_one_row_have_any_row_stride():
     assert all(torch.equal(t.grad, b) for t, b in zip(ins, want))
     x, w, t = randn(5, 33), randn(1, 33, std=0.3, seed=2), torch.zeros(5, dtype=torch.int64, device=DEV)
     assert all(torch.equal(a, b) for a, b in zip(run_loss(x, w, t), run_loss(x, row(w), t)))
+
+
+# --------------------------------------------------------------------------- inputs that depend on each other
+@pytest.mark.parametrize("create", [False, True])
+def test_loss_gradient_of_hidden_states_that_depend_on_the_weight(create):
+    """Tied embeddings: the recorded gradient counts the way through the hidden states once, as the other does."""
+    w = randn(20, 16, std=0.3, seed=2).requires_grad_()
+    t, pick = targets(9, 20), targets(9, 20, seed=7)
+    got, = torch.autograd.grad(kernels.linear_cross_entropy(2 * w[pick], w, t), w, create_graph=create)
+    wd = w.detach().double().requires_grad_()
+    ref, = torch.autograd.grad(F.cross_entropy(2 * wd[pick] @ wd.T, t), wd, create_graph=True)
+    # bf16 roundings of dx, dw, their sum and of the rows that are picked more than once, each at most 2^-8
+    assert float((got.double() - ref).norm() / ref.norm()) <= 8 * HALF
+    if create:
+        got, = torch.autograd.grad(got.float().square().sum(), w)
+        ref, = torch.autograd.grad(ref.square().sum(), wd)
+        assert float((got.double() - ref).norm() / ref.norm()) <= 16 * HALF
+
+
+@pytest.mark.parametrize("create", [False, True])
+def test_ffn_gradient_of_inputs_that_depend_on_each_other(create):
+    """Input and second weight from the first one."""
+    w13, g = randn(48, 16, std=0.3, seed=1).requires_grad_(), randn(9, 16, std=0.1, seed=3)
+    got, = torch.autograd.grad(kernels.gated_ffn(4 * w13[:9], w13, w13[:24].t()), w13, g, create_graph=create)
+    wd = w13.detach().double().requires_grad_()
+    a, b = (4 * wd[:9] @ wd.T).chunk(2, 1)
+    ref, = torch.autograd.grad((F.silu(a) * b) @ wd[:24], wd, g.double())
+    assert float((got.double() - ref).norm() / ref.norm()) <= 8 * HALF

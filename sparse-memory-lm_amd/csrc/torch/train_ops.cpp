@@ -71,6 +71,13 @@ Tensor narrowed(const Tensor &t, int64_t rows, int64_t cols) {
   return t.size(0) == rows && t.size(1) == cols ? t : t.narrow(0, 0, rows).narrow(1, 0, cols);
 }
 
+// What a backward gets back need not be what forward saved (a saved-tensor hook gives what it likes, and a leaf's .data can be
+// replaced meanwhile): the kernels read only tensors of the type, device and sizes that they take them for.
+void check_saved(const char *name, const Tensor &t, at::ScalarType type, at::Device device, at::IntArrayRef sizes) {
+  TORCH_CHECK(t.defined() && t.scalar_type() == type && t.device() == device && t.sizes() == sizes && !t.is_neg(), name,
+              ": a saved tensor came back changed, expected ", type, " ", sizes, " on ", device);
+}
+
 // Within it the ops of a recorded backward keep their fp32 where autocast is on.
 struct NoAutocast {
   c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset};
@@ -129,9 +136,22 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &targets = saved[2];
     const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
-    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
-    const int64_t d = x.size(-1), V = weight.size(0), M = x.numel() / d, d8 = ceil8(d);
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), none = reduction == SMLM_REDUCE_NONE;
     Tensor g = plain(grads[0]);
+    const char *name = "linear_cross_entropy's gradient";
+    const auto device = g.device();
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && weight.dim() == 2, name, ": a saved tensor came back changed");
+    const int64_t d = x.size(-1), V = weight.size(0), M = x.numel() / d, d8 = ceil8(d);
+    check_saved(name, x, at::kBFloat16, device, x.sizes());
+    check_saved(name, weight, at::kBFloat16, device, {V, d});
+    check_saved(name, targets, at::kLong, device, x.sizes().slice(0, x.dim() - 1));
+    TORCH_CHECK(V > 0 && (!none || g.sizes() == targets.sizes()), name, ": a saved tensor came back changed");
+    if (M > 0) {
+      check_saved(name, saved[3], at::kFloat, device, {M});
+      if (reduction == SMLM_REDUCE_MEAN) check_saved(name, saved[4], at::kFloat, device, {});
+      if (saved[5].defined()) check_saved(name, saved[5], at::kBFloat16, device, {M, d8});
+      if (saved[6].defined()) check_saved(name, saved[6], at::kBFloat16, device, {V, d8});
+    }
     if (at::GradMode::is_enabled()) {
       const NoAutocast fp32;
       // an index outside the vocabulary, which the loss would stop the device for: any other, and NaN
@@ -146,14 +166,15 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     }
     if (M == 0) return {at::zeros_like(x), at::zeros_like(weight), Tensor(), Tensor(), Tensor()};
     const c10::DeviceGuard guard(x.device());
-    const Tensor xr = saved[5].defined() ? saved[5] : x.reshape({M, d}), wr = saved[6].defined() ? saved[6] : weight;
-    const Tensor t = targets.reshape({M}).contiguous();
+    const Tensor xr = mm_rows(saved[5].defined() ? saved[5] : x.reshape({M, d}), M, d8);
+    const Tensor wr = mm_rows(saved[6].defined() ? saved[6] : weight, V, d8);
+    const Tensor t = targets.reshape({M}).contiguous(), lse = saved[3].contiguous();
     g = g.reshape({-1}).contiguous();
     const Tensor dx = want_x ? at::empty({M, d8}, x.options()) : Tensor(), dw = want_w ? at::empty({V, d8}, x.options()) : Tensor();
     const Tensor ws = workspace(x, smlm_linear_ce_workspace(M, V, d8, 1));
     check(smlm_linear_ce_backward(g.data_ptr<float>(), reduction == SMLM_REDUCE_MEAN ? saved[4].data_ptr<float>() : nullptr,
-                                  reduction == SMLM_REDUCE_NONE, xr.data_ptr(), xr.stride(0), wr.data_ptr(), wr.stride(0),
-                                  t.data_ptr<int64_t>(), ignore, saved[3].data_ptr<float>(), M, V, d8, ptr(dx), ptr(dw),
+                                  none, xr.data_ptr(), xr.stride(0), wr.data_ptr(), wr.stride(0),
+                                  t.data_ptr<int64_t>(), ignore, lse.data_ptr<float>(), M, V, d8, ptr(dx), ptr(dw),
                                   ws.data_ptr(), ws.numel(), stream_of(x)),
           "smlm_linear_ce_backward");
     return {want_x ? narrowed(dx, M, d).view(x.sizes()) : Tensor(), want_w ? narrowed(dw, V, d) : Tensor(), Tensor(), Tensor(),
@@ -178,6 +199,11 @@ Tensor linear_cross_entropy(const Tensor &x, const Tensor &weight, const Tensor 
 }
 
 // ---- the feed-forward block --------------------------------------------------------------------------------------------
+// w13 with halves that end on whole pieces.
+Tensor halves(const Tensor &w13, int64_t h, int64_t h8, int64_t d8) {
+  return h8 == h ? mm_rows(w13, 2 * h, d8) : padded(w13, 2, h8, d8);
+}
+
 struct GatedFFN : torch::autograd::Function<GatedFFN> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w13, const Tensor &w2) {
     const int64_t d = x.size(-1), o = w2.size(0), h = w2.size(1), M = x.numel() / d, d8 = ceil8(d), h8 = ceil8(h), o8 = ceil8(o);
@@ -188,9 +214,7 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
       return at::empty(shape, x.options());
     }
     const c10::DeviceGuard guard(x.device());
-    const Tensor x2 = x.reshape({M, d}), a = mm_rows(x2, M, d8), c = mm_rows(w2, o8, h8);
-    // the halves of w13 end on whole pieces
-    const Tensor b = h8 == h ? mm_rows(w13, 2 * h, d8) : padded(w13, 2, h8, d8);
+    const Tensor x2 = x.reshape({M, d}), a = mm_rows(x2, M, d8), b = halves(w13, h, h8, d8), c = mm_rows(w2, o8, h8);
     const Tensor ws = workspace(x, smlm_gated_ffn_workspace(M, d8, h8, o8, 0));
     const Tensor y = at::empty({M, o8}, x.options());
     check(smlm_gated_ffn(a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), c.data_ptr(), c.stride(0), M, d8, h8, o8,
@@ -204,7 +228,19 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w13 = saved[1], &w2 = saved[2], dy = plain(grads[0]);
     const bool want_x = ctx->needs_input_grad(0), want_w13 = ctx->needs_input_grad(1), want_w2 = ctx->needs_input_grad(2);
+    const char *name = "gated_ffn's gradient";
+    const auto device = dy.device();
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && w2.dim() == 2 && w2.numel() > 0, name, ": a saved tensor came back changed");
     const int64_t d = x.size(-1), o = w2.size(0), h = w2.size(1), M = x.numel() / d, d8 = ceil8(d), h8 = ceil8(h), o8 = ceil8(o);
+    auto shape = x.sizes().vec();
+    shape.back() = o;
+    check_saved(name, x, at::kBFloat16, device, x.sizes());
+    check_saved(name, w13, at::kBFloat16, device, {2 * h, d});
+    check_saved(name, w2, at::kBFloat16, device, {o, h});
+    TORCH_CHECK(dy.sizes() == at::IntArrayRef(shape), name, ": a saved tensor came back changed");
+    if (saved[3].defined()) check_saved(name, saved[3], at::kBFloat16, device, {M, d8});
+    if (saved[4].defined()) check_saved(name, saved[4], at::kBFloat16, device, {2 * h8, d8});
+    if (saved[5].defined()) check_saved(name, saved[5], at::kBFloat16, device, {o8, h8});
     if (at::GradMode::is_enabled()) {
       const NoAutocast fp32;
       const auto in = aliases({x, w13, w2});
@@ -214,8 +250,9 @@ struct GatedFFN : torch::autograd::Function<GatedFFN> {
     }
     if (M == 0) return {at::zeros_like(x), at::zeros_like(w13), at::zeros_like(w2)};
     const c10::DeviceGuard guard(x.device());
-    const Tensor a = saved[3].defined() ? saved[3] : x.reshape({M, d}), b = saved[4].defined() ? saved[4] : w13,
-                 c = saved[5].defined() ? saved[5] : w2, g = mm_rows(dy.reshape({M, o}), M, o8);
+    const Tensor a = mm_rows(saved[3].defined() ? saved[3] : x.reshape({M, d}), M, d8);
+    const Tensor b = saved[4].defined() ? mm_rows(saved[4], 2 * h8, d8) : halves(w13, h, h8, d8);
+    const Tensor c = mm_rows(saved[5].defined() ? saved[5] : w2, o8, h8), g = mm_rows(dy.reshape({M, o}), M, o8);
     const Tensor dx = want_x ? at::empty({M, d8}, x.options()) : Tensor();
     const Tensor dw13 = want_w13 ? at::empty({2 * h8, d8}, x.options()) : Tensor();
     const Tensor dw2 = want_w2 ? at::empty({o8, h8}, x.options()) : Tensor();
@@ -281,6 +318,14 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
       if (want_w) out[2] = at::zeros_like(weight);
       return out;
     }
+    const char *name = "add_rmsnorm_train's gradient";
+    const auto device = dh.device();
+    check_saved(name, xs, xs.scalar_type(), device, dh.sizes());
+    const int64_t C = xs.size(-1), M = xs.numel() / C;
+    check_saved(name, weight, weight.scalar_type(), device, {C});
+    check_saved(name, rstd, at::kFloat, device, {M});
+    TORCH_CHECK(is_float_type(xs.scalar_type()) && is_float_type(weight.scalar_type()), name, ": a saved tensor came back changed");
+    if (dxs.defined()) check_saved(name, dxs, xs.scalar_type(), device, xs.sizes());
     if (at::GradMode::is_enabled()) {                            // in terms of xs, an output of this node
       const Tensor x = xs.to(at::kFloat), g = dh.to(at::kFloat);
       const Tensor r = (x.square().mean(-1, true) + ctx->saved_data["eps"].toDouble()).rsqrt(), hat = x * r;
@@ -293,9 +338,9 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
       if (want_w) out[2] = (g * hat).reshape({-1, xs.size(-1)}).sum(0).to(weight.scalar_type());
       return out;
     }
-    const int64_t C = xs.size(-1), M = xs.numel() / C;
-    const c10::DeviceGuard guard(xs.device());
+    const c10::DeviceGuard guard(device);
     const Tensor s = xs.contiguous(), w = weight.contiguous(), gh = dh.contiguous(), gx = dxs.defined() ? dxs.contiguous() : dxs;
+    const Tensor r = rstd.contiguous();
     const Tensor dx = at::empty(xs.sizes(), xs.options());
     const bool cast = want_delta && delta_dtype != xs.scalar_type();
     const Tensor ddelta = cast ? at::empty(xs.sizes(), xs.options().dtype(delta_dtype)) : Tensor();
@@ -307,7 +352,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
     if (M > 0)
       check(smlm_rmsnorm_train_backward(ptr(gx), gh.data_ptr(), dtype_of(gh.scalar_type()), s.data_ptr(),
                                         dtype_of(s.scalar_type()), w.data_ptr(), dtype_of(w.scalar_type()),
-                                        rstd.data_ptr<float>(), M, C, dx.data_ptr(), ptr(ddelta), dtype_of(delta_dtype),
+                                        r.data_ptr<float>(), M, C, dx.data_ptr(), ptr(ddelta), dtype_of(delta_dtype),
                                         ptr(dw), (float *)ptr(parts), stream_of(xs)),
             "smlm_rmsnorm_train_backward");
     if (want_x) out[0] = dx;

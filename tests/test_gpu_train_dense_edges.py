@@ -97,3 +97,67 @@ def test_ffn_gradient_of_inputs_that_depend_on_each_other(create):
     a, b = (4 * wd[:9] @ wd.T).chunk(2, 1)
     ref, = torch.autograd.grad((F.silu(a) * b) @ wd[:24], wd, g.double())
     assert float((got.double() - ref).norm() / ref.norm()) <= 8 * HALF
+
+
+# -------------------------------------------------------------------------------------- what a backward gets back
+def operators(odd):
+    """Each operator with leaves and a gradient of its output; odd: sizes whose copies are saved too."""
+    n = 33 if odd else 32
+    x, w, t = randn(9, n), randn(40, n, std=0.3, seed=2), targets(9, 40)
+    y, w13, w2, g = ffn_inputs(9, n, 25 if odd else 24, n)
+    s, norm = randn(9, n, dtype=F32), torch.nn.RMSNorm(n, eps=1e-5, device=DEV)
+    made = {"mean": ([x, w], lambda a: kernels.linear_cross_entropy(*a, t), torch.tensor(1.5, device=DEV)),
+            "none": ([x, w], lambda a: kernels.linear_cross_entropy(*a, t, reduction="none"), randn(9, dtype=F32)),
+            "ffn": ([y, w13, w2], lambda a: kernels.gated_ffn(*a), g),
+            "norm": ([s, norm.weight], lambda a: kernels.add_rmsnorm_train(a[0], a[0], norm)[1], randn(9, n, seed=7, dtype=F32))}
+    return {k: ([i.detach().requires_grad_() if i is not norm.weight else i for i in ins], f, g) for k, (ins, f, g) in made.items()}
+
+
+CHANGES = {"host": lambda t: t.cpu(), "type": lambda t: t.double() if t.dtype == F32 else t.float(),
+           "fewer": lambda t: t[:-1] if t.dim() else t[None], "flat": lambda t: t.reshape(-1)[None]}
+
+
+@pytest.mark.parametrize("name,odd,change,create", itertools.product(["mean", "none", "ffn", "norm"], [False, True], CHANGES,
+                                                                     [False, True]))
+def test_saved_tensors_that_come_back_changed_are_refused(name, odd, change, create):
+    """One saved tensor after the other comes back on the host, in another type or with other sizes."""
+    note(name, odd, change, create)
+    for k in itertools.count():
+        count = itertools.count()
+        ins, f, g = operators(odd)[name]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (next(count), t.detach()),
+                                                      lambda p: CHANGES[change](p[1]) if p[0] == k else p[1]):
+            out = f(ins)
+        if k >= next(count):
+            assert k > 0
+            break
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.autograd.grad(out, ins, g, create_graph=create)
+
+
+@pytest.mark.parametrize("name,odd", itertools.product(["mean", "none", "ffn", "norm"], [False, True]))
+def test_saved_tensors_that_come_back_elsewhere(name, odd):
+    """From host memory, or in other strides: the same bits."""
+    ins, f, g = operators(odd)[name]
+    want = torch.autograd.grad(f(ins), ins, g)
+
+    def turned(t):
+        return t if t.dim() < 2 else t.repeat_interleave(2, 1)[:, ::2]
+
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), turned)):
+        with hooks:
+            out = f(ins)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, ins, g), want))
+
+
+def test_leaves_replaced_between_the_passes_are_refused():
+    """A model moved to another type, or weights freed, after the forward pass."""
+    for name, (ins, f, g) in operators(False).items():
+        for i, new in itertools.product(range(len(ins)), (lambda t: t.to(BF16 if t.dtype == F32 else F32), lambda t: t[:0])):
+            ins, f, g = operators(False)[name]
+            out = f(ins)
+            if name == "norm" and (i == 0 or new(ins[1]).numel()):
+                continue                                 # the stream is kept as it was formed; weights of either type are read
+            ins[i].data = new(ins[i].data)
+            with pytest.raises((RuntimeError, ValueError)):
+                torch.autograd.grad(out, ins, g)

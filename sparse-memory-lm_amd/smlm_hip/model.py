@@ -346,6 +346,13 @@ def _ffn_kernels(ffn, x):
             and ordinary(w13, w2))
 
 
+def _attention_casts(attn):
+    """Whether this attention block only casts its input to bf16 (autocast's cast before its own projection), so that the
+    norm before it may give bf16 at once."""
+    return (type(attn) is Attention and type(attn.wqkv) is nn.Linear and unhooked(attn, attn.wqkv)
+            and ordinary(attn.wqkv.weight))
+
+
 class Transformer(nn.Module):
     def __init__(self, cfg, ngram_canon=None):
         """ngram_canon: the token compression table of the Engram hash ((vocab_size,) int64), needed for Engram
@@ -503,7 +510,7 @@ class Transformer(nn.Module):
             if blk.engram is not None:
                 x, delta = x if delta is None else x + delta, None
                 x = x + blk.engram(x, rows, None)
-            delta = blk.attn(normed(blk.attn_norm, bf16), None, 0)
+            delta = blk.attn(normed(blk.attn_norm, bf16 if _attention_casts(blk.attn) else x.dtype), None, 0)
             if not blk.is_memory and _ffn_kernels(blk.ffn, x):
                 h = normed(blk.ffn_norm, bf16).to(bf16)
                 delta = kernels.gated_ffn(h, blk.ffn.w13.weight.to(bf16), blk.ffn.w2.weight.to(bf16))

@@ -161,3 +161,47 @@ def test_leaves_replaced_between_the_passes_are_refused():
             ins[i].data = new(ins[i].data)
             with pytest.raises((RuntimeError, ValueError)):
                 torch.autograd.grad(out, ins, g)
+
+
+# ------------------------------------------------------------------------- Transformer.loss and its sublayers
+class Seen(torch.nn.Module):
+    """A sublayer put in another's place, which notes its input's type."""
+
+    def __init__(self, inner, types):
+        super().__init__()
+        self.inner, self.types = inner, types
+
+    def forward(self, x, *rest):
+        self.types.append(x.dtype)
+        return self.inner(x, *rest)
+
+
+class SeenLinear(torch.nn.Linear):
+    def forward(self, x):
+        self.types.append(x.dtype)
+        return super().forward(x)
+
+
+@pytest.mark.parametrize("how", ["watched", "projection watched", "replaced", "projection replaced"])
+def test_model_loss_gives_other_attention_the_streams_type(how):
+    """Under autocast the stream is fp32: what watches the attention's input or takes its place sees what forward gives."""
+    m, types = lm(F32), []
+    idx, t = batch()
+    blk = m.layers[1]
+
+    def see(module, args):
+        types.append(args[0].dtype)
+
+    if how == "watched":
+        blk.attn.register_forward_pre_hook(see)
+    elif how == "projection watched":
+        blk.attn.wqkv.register_forward_pre_hook(see)
+    elif how == "replaced":
+        blk.attn = Seen(blk.attn, types)
+    else:
+        blk.attn.wqkv.__class__, blk.attn.wqkv.types = SeenLinear, types
+    with torch.autocast("cuda", dtype=BF16):
+        loss = m.loss(idx, t)
+        _, plain = m(idx, t)
+    assert types == [F32, F32]
+    assert abs(loss.item() - plain.item()) <= 0.03 * plain.item()

@@ -460,8 +460,8 @@ class Transformer(nn.Module):
 
     def loss(self, idx, targets, ignore_index=-100, reduction="mean"):
         """forward(idx, targets)[1] (smlm/model.py:266-293) without the logits, for training and for scoring text: the
-        cross entropy of the next-token targets (idx's shape, int64), with F.cross_entropy's ignore_index and reduction
-        ("none": idx's shape).  On the GPU in bf16 (bf16 weights or bf16 autocast) the residual adds, norms, feed-forward
+        cross entropy of the next-token targets (int64, idx's shape or, as forward() takes them, as many in any other),
+        with F.cross_entropy's ignore_index and reduction ("none": the targets' shape).  On the GPU in bf16 (bf16 weights or bf16 autocast) the residual adds, norms, feed-forward
         blocks and the loss run as kernels.add_rmsnorm_train, gated_ffn and linear_cross_entropy, whose logits are not
         rounded to bf16 as forward()'s are; anything else, and modules that are watched or replaced, runs the modules."""
         if not self._loss_kernels(idx, targets):
@@ -471,7 +471,9 @@ class Transformer(nn.Module):
             return loss.view(targets.shape) if reduction == "none" else loss
         rows = self._ngram_rows(idx, None) if self.ngram is not None else None
         h = self._blocks_recorded(self.tok_emb(idx), rows)
-        return kernels.linear_cross_entropy(h, self.lm_head.weight.to(torch.bfloat16), targets, ignore_index, reduction)
+        loss = kernels.linear_cross_entropy(h, self.lm_head.weight.to(torch.bfloat16), targets.reshape(idx.shape),
+                                            ignore_index, reduction)
+        return loss.view(targets.shape) if reduction == "none" else loss
 
     def _loss_kernels(self, idx, targets):
         """Whether loss() may end in linear_cross_entropy: bf16 arithmetic on the GPU, plain embeddings and a plain final
@@ -484,6 +486,7 @@ class Transformer(nn.Module):
         autocast = torch.is_autocast_enabled("cuda")
         return (x.is_cuda and (torch.get_autocast_dtype("cuda") == bf16 if autocast else x.dtype == bf16)
                 and head.bias is None and head.weight.dtype in (bf16, x.dtype) and idx.device == targets.device == x.device
+                and targets.dtype == torch.int64 and targets.numel() == idx.numel()
                 and _norm_kernels(self.norm, x) and ordinary(idx, head.weight, targets))
 
     def _blocks_recorded(self, x, rows):

@@ -205,3 +205,21 @@ def test_model_loss_gives_other_attention_the_streams_type(how):
         _, plain = m(idx, t)
     assert types == [F32, F32]
     assert abs(loss.item() - plain.item()) <= 0.03 * plain.item()
+
+
+def test_model_loss_targets_of_other_shapes_and_types(monkeypatch):
+    """Targets as forward takes them: flat ones count for the tokens in order, and losses come in the targets' shape; what
+    is not int64 goes the modules' way."""
+    m = lm(BF16)
+    idx, t = batch()
+    calls = spied(monkeypatch)
+    each = m.loss(idx, t, reduction="none")
+    flat = m.loss(idx, t.view(-1), reduction="none")
+    assert flat.shape == (t.numel(),) and torch.equal(flat, each.view(-1))
+    assert torch.equal(m.loss(idx, t.view(-1)), m.loss(idx, t))
+    assert calls["linear_cross_entropy"] == 4
+    small = t.clamp(0, 255).to(torch.uint8)
+    assert torch.equal(m.loss(idx, small), m(idx, small)[1])
+    for bad in (t[:2], t.int()):
+        with pytest.raises((ValueError, RuntimeError)):
+            m.loss(idx, bad)

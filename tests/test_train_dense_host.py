@@ -164,3 +164,12 @@ def test_default_eps_is_that_of_fp32():
     assert kernels._rms_eps(norm) == 2.0 ** -23 and kernels._rms_eps(torch.nn.RMSNorm(16, eps=1e-5)) == 1e-5
     got, ref = F.rms_norm(x, (16,)).double(), F.rms_norm(x.double(), (16,), eps=kernels._rms_eps(norm))
     assert ((got - ref).abs() <= 2 * 2.0 ** -8 * ref.abs()).all()
+
+
+def test_loss_of_flat_targets_on_the_cpu():
+    """Losses in the targets' shape."""
+    m = small()
+    idx = torch.randint(0, 67, (2, 9), generator=torch.Generator().manual_seed(0))
+    t = torch.roll(idx, -1, 1)
+    flat, each = m.loss(idx, t.view(-1), reduction="none"), m.loss(idx, t, reduction="none")
+    assert flat.shape == (18,) and torch.equal(flat, each.view(-1)) and torch.equal(m.loss(idx, t.view(-1)), m.loss(idx, t))

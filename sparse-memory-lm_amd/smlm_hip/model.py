@@ -495,32 +495,42 @@ class Transformer(nn.Module):
         bf16 = torch.bfloat16
         delta = None
 
-        def normed(norm, dtype):
+        def add(y):
+            """x = x + y, left to the launch of the next norm where y is a plain tensor of the stream's shape."""
             nonlocal x, delta
-            if delta is not None and (delta.dtype not in (bf16, x.dtype) or not _norm_kernels(norm, x)):
-                x, delta = x + delta, None
+            if type(y) is torch.Tensor and y.shape == x.shape and y.dtype in (bf16, x.dtype) and y.device == x.device:
+                delta = y
+            else:
+                x = x + y
+
+        def settled():
+            nonlocal x, delta
+            x, delta = x if delta is None else x + delta, None
+            return x
+
+        def normed(norm, dtype=None):
+            """norm(x) in this type, the stream's by default."""
+            nonlocal x, delta
             if not _norm_kernels(norm, x):
-                return norm(x)
+                return norm(settled())
             x, h = kernels.add_rmsnorm_train(x, delta, norm, out_dtype=dtype)
             delta = None
             return h
 
         for blk in self.layers:
             if type(blk) is not Block or not unhooked(blk):
-                x = blk(x if delta is None else x + delta, None, 0, rows)
-                delta = None
+                x = blk(settled(), None, 0, rows)
                 continue
             if blk.engram is not None:
-                x, delta = x if delta is None else x + delta, None
-                x = x + blk.engram(x, rows, None)
-            delta = blk.attn(normed(blk.attn_norm, bf16 if _attention_casts(blk.attn) else x.dtype), None, 0)
+                x = settled() + blk.engram(x, rows, None)
+            add(blk.attn(normed(blk.attn_norm, bf16 if _attention_casts(blk.attn) else None), None, 0))
             if not blk.is_memory and _ffn_kernels(blk.ffn, x):
                 h = normed(blk.ffn_norm, bf16).to(bf16)
-                delta = kernels.gated_ffn(h, blk.ffn.w13.weight.to(bf16), blk.ffn.w2.weight.to(bf16))
+                add(kernels.gated_ffn(h, blk.ffn.w13.weight.to(bf16), blk.ffn.w2.weight.to(bf16)))
             else:
-                delta = blk.ffn(normed(blk.ffn_norm, x.dtype))
+                add(blk.ffn(normed(blk.ffn_norm)))
             if blk.ffn_r2 is not None:
-                delta = blk.ffn_r2(normed(blk.ffn_norm_r2, x.dtype))
+                add(blk.ffn_r2(normed(blk.ffn_norm_r2)))
         return normed(self.norm, bf16).to(bf16)
 
     @torch.no_grad()

@@ -223,3 +223,27 @@ def test_model_loss_targets_of_other_shapes_and_types(monkeypatch):
     for bad in (t[:2], t.int()):
         with pytest.raises((ValueError, RuntimeError)):
             m.loss(idx, bad)
+
+
+class Gives(torch.nn.Module):
+    def __init__(self, value):
+        super().__init__()
+        self.value = torch.nn.Parameter(value) if torch.is_tensor(value) else value
+
+    def forward(self, x, *rest):
+        return self.value
+
+
+def test_model_loss_with_sublayers_that_give_less_than_the_stream():
+    """A sublayer that is switched off (0), or gives one row for all tokens: added as forward adds it."""
+    m = lm(BF16)
+    idx, t = batch()
+    m.layers[0].attn, m.layers[1].ffn = Gives(0.0), Gives(randn(128))
+    m.layers[2].ffn = Gives(randn(1, 33, 128, seed=3))
+    loss, (_, plain) = m.loss(idx, t), m(idx, t)
+    assert abs(loss.item() - plain.item()) <= 0.03 * plain.item()
+    for blk in m.layers[1:]:
+        v = blk.ffn.value
+        got, want = (torch.autograd.grad(x, v, retain_graph=True)[0].double() for x in (loss, plain))
+        # either path within the bf16 roundings of two layers and the loss, forward and back
+        assert float((got - want).norm() / want.norm()) <= 32 * HALF

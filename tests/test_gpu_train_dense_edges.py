@@ -247,3 +247,80 @@ def test_model_loss_with_sublayers_that_give_less_than_the_stream():
         got, want = (torch.autograd.grad(x, v, retain_graph=True)[0].double() for x in (loss, plain))
         # either path within the bf16 roundings of two layers and the loss, forward and back
         assert float((got - want).norm() / want.norm()) <= 32 * HALF
+
+
+# --------------------------------------------------------------------------------- every tile of the products
+class Plan(ctypes.Structure):
+    _fields_ = [("shape", ctypes.c_int), ("splits", ctypes.c_int64)]
+
+
+def plan(T, F, K, may_split):
+    """The library's own choice (smlm::mm_plan of csrc/lm_mm.h)."""
+    f = getattr(_lib.lib(), "_ZN4smlm7mm_planElllb")
+    f.restype, f.argtypes = Plan, [ctypes.c_int64] * 3 + [ctypes.c_bool]
+    p = f(T, F, K, may_split)
+    return ("256 x 256", "384 x 128", "128 x 128", "64 x 64")[p.shape], p.splits > 1
+
+
+def up(n, to=8):
+    return -(-n // to) * to
+
+
+def terms(M):
+    return 2 if M <= 128 else 1
+
+
+def loss_tiles(M, V, d):
+    """(operands with contiguous k, tile, whether k is split, terms) of the loss' two products."""
+    cols, d = up(V, 256), up(d)
+    return {("tokens", *plan(M, d, cols, True), terms(M)), ("none", *plan(cols, d, M, False), terms(M))}
+
+
+def ffn_tiles(M, d, h, o):
+    """Of the block's four."""
+    n, (d, h, o) = terms(M), map(up, (d, h, o))
+    return {("both", *plan(M, o, h * n, True), n), ("tokens", *plan(M, d, 2 * h * n, True), n),
+            ("none", *plan(2 * h, d, M * n, True), n), ("none", *plan(o, h, M * n, True), n)}
+
+
+LOSS_TILES = [(64, 32000, 384), (2031, 32003, 201), (4096, 20011, 392), (2, 24157, 3393)]
+FFN_TILES = [(2, 35, 36, 46), (70, 42, 2594, 2701), (76, 1794, 3641, 40), (312, 2128, 2885, 3336), (870, 73, 409, 50),
+             (1347, 43, 3419, 1979), (7591, 524, 1643, 42), (14074, 33, 3882, 130), (14077, 392, 1001, 392),
+             (15192, 535, 145, 779), (16318, 897, 286, 614), (32801, 384, 1024, 384)]
+
+
+def test_the_sizes_below_take_every_tile():
+    """Every tile in every form of operands with a bf16 result and, where a plan may split k, with fp32 parts; with two terms
+    those that so few tokens take."""
+    seen = set().union(*(loss_tiles(*s) for s in LOSS_TILES), *(ffn_tiles(*s) for s in FFN_TILES))
+    tiles = ("256 x 256", "384 x 128", "128 x 128", "64 x 64")
+    missing = set(itertools.product(("both", "tokens", "none"), tiles, (False, True), (1,))) - seen
+    assert not missing
+    two = {("both", "64 x 64", False), ("both", "64 x 64", True), ("both", "128 x 128", True), ("tokens", "64 x 64", False),
+           ("tokens", "64 x 64", True), ("tokens", "128 x 128", True), ("tokens", "384 x 128", True),
+           *(("none", t, False) for t in tiles)}
+    assert {k[:3] for k in seen if k[3] == 2} >= two
+
+
+@pytest.mark.parametrize("M,V,d", LOSS_TILES)
+def test_loss_tiles(M, V, d):
+    note("loss", M, V, d)
+    check_loss(randn(M, d), randn(V, d, std=4.0 / d ** 0.5, seed=2), targets(M, V, ignored=0.1))
+
+
+@pytest.mark.parametrize("M,d,h,o", FFN_TILES)
+def test_ffn_tiles(M, d, h, o):
+    note("ffn", M, d, h, o)
+    check_ffn(*ffn_inputs(M, d, h, o))
+
+
+@pytest.mark.parametrize("M", [200, 300, 1111])
+def test_loss_weights_of_single_tokens(M):
+    """A coefficient per token in the loss' tiles of 128 and 256 tokens; an ignored token's may be NaN."""
+    V, d = 1500, 136
+    note("loss", M, V, d)
+    t, g = targets(M, V, ignored=0.2), randn(M, seed=5, dtype=F32)
+    want = check_loss(randn(M, d), randn(V, d, std=0.3, seed=2), t, "none", g=g)
+    g[t == -100] = float("nan")
+    got = run_loss(randn(M, d), randn(V, d, std=0.3, seed=2), t, "none", g=g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

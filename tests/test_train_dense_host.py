@@ -173,3 +173,80 @@ def test_loss_of_flat_targets_on_the_cpu():
     t = torch.roll(idx, -1, 1)
     flat, each = m.loss(idx, t.view(-1), reduction="none"), m.loss(idx, t, reduction="none")
     assert flat.shape == (18,) and torch.equal(flat, each.view(-1)) and torch.equal(m.loss(idx, t.view(-1)), m.loss(idx, t))
+
+
+class _DoubleAsBf16:
+    """torch, with 64 bits where the model asks for bf16."""
+    bfloat16 = torch.float64
+
+    def __getattr__(self, name):
+        return getattr(torch, name)
+
+
+def _in_64_bits(monkeypatch):
+    """Transformer.loss takes its kernels' way on the CPU in 64 bits, with the operators' formulas in their place; counts them."""
+    import smlm_hip.model as model
+    calls = {"loss": 0, "ffn": 0, "norm": 0}
+
+    def loss(x, w, t, ignore_index, reduction):
+        calls["loss"] += 1
+        return F.cross_entropy((x @ w.T).flatten(0, -2), t.flatten(), ignore_index=ignore_index, reduction=reduction)
+
+    def ffn(x, w13, w2):
+        calls["ffn"] += 1
+        a, b = (x @ w13.T).chunk(2, -1)
+        return (F.silu(a) * b) @ w2.T
+
+    def norm(x, delta, norm, out_dtype=None):
+        calls["norm"] += 1
+        x = x if delta is None else x + delta
+        return x, F.rms_norm(x, norm.weight.shape, norm.weight, norm.eps)
+
+    monkeypatch.setattr(model, "torch", _DoubleAsBf16())
+    monkeypatch.setattr(Transformer, "_loss_kernels", lambda *a: True)
+    for name, f in (("linear_cross_entropy", loss), ("gated_ffn", ffn), ("add_rmsnorm_train", norm)):
+        monkeypatch.setattr(kernels, name, f)
+    return calls
+
+
+class _Sublayer(torch.nn.Module):
+    """Something nonlinear in a memory or Engram layer's place (whose kernels need a GPU)."""
+
+    def __init__(self, d):
+        super().__init__()
+        self.w = torch.nn.Parameter(torch.randn(d, d) * 0.4)
+
+    def forward(self, x, *rest):
+        return torch.sin(x @ self.w.T)
+
+
+@pytest.mark.parametrize("memory,second,engram,counts", [((), (), (), (4, 9)), ((1, 2), (2,), (), (2, 10)), ((), (), (0, 3), (4, 9)),
+                                                         ((0, 2, 3), (0, 3), (0, 1, 3), (1, 11))])
+def test_loss_sums_and_norms_in_forwards_order(memory, second, engram, counts, monkeypatch):
+    """Every residual add, norm and sublayer of the kernels' way, with sublayers where memory layers, second reads and Engram
+    layers are: the loss and all gradients of forward, in 64 bits (a few thousand roundings of 2^-53 each)."""
+    torch.manual_seed(3)
+    m = Transformer(ModelConfig(vocab_size=67, d_model=32, n_layers=4, n_heads=2, ffn_hidden=48, max_seq_len=16))
+    for i, blk in enumerate(m.layers):
+        if i in memory:
+            blk.is_memory, blk.ffn = True, _Sublayer(32)
+        if i in second:
+            blk.ffn_norm_r2, blk.ffn_r2 = torch.nn.RMSNorm(32, eps=1e-5), _Sublayer(32)
+        if i in engram:
+            blk.engram = _Sublayer(32)
+    m.double().train()
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            p.copy_(p * 4.0 if p.dim() == 2 else p + 0.1 * torch.randn_like(p))
+    idx = torch.randint(0, 67, (2, 9), generator=torch.Generator().manual_seed(0))
+    t = torch.roll(idx, -1, 1)
+    names, params = zip(*m.named_parameters())
+    plain = F.cross_entropy(m(idx).view(-1, 67), t.view(-1))
+    want = torch.autograd.grad(plain, params)
+    calls = _in_64_bits(monkeypatch)
+    loss = m.loss(idx, t)
+    got = torch.autograd.grad(loss, params)
+    assert calls == {"loss": 1, "ffn": counts[0], "norm": counts[1]}
+    assert abs(loss.item() - plain.item()) <= 1e-11 * plain.item()
+    for n, a, b in zip(names, got, want):
+        assert 0 < float(b.norm()) and float((a - b).norm()) <= 1e-9 * float(b.norm()), n

@@ -366,6 +366,7 @@ struct MmPlan {
 };
 MmPlan mm_plan(int64_t T, int64_t F, int64_t K, bool may_split);
 // One launch of it: the parts (a.f32) or, with one split, the result.  a.nsplit and a.k_per are set from the plan.
+// Refuses feat_kc without tok_kc, which no operator needs.
 int mm_launch(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, hipStream_t stream, const char *what);
 // The product into bf16 a.out [T][a.ldo]: parts (part_bytes of the plan) and their sum where k is split.
 int mm_run(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, float *parts, hipStream_t stream, const char *what);

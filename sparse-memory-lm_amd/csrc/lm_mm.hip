@@ -212,7 +212,8 @@ int mm_launch(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, hipStream
   a.k_per = ceil_div(ceil_div(a.K, plan.splits), kMmUnit) * kMmUnit;
   if (feat_kc && tok_kc) return choose<true, true>(a, plan.shape, stream, what);
   if (tok_kc) return choose<false, true>(a, plan.shape, stream, what);
-  return choose<false, false>(a, plan.shape, stream, what);   // feat_kc without tok_kc: no caller
+  if (!feat_kc) return choose<false, false>(a, plan.shape, stream, what);
+  return fail(SMLM_EUNSUPPORTED, "%s: no product of contiguous features with strided tokens", what);
 }
 
 int mm_run(MmArgs a, bool feat_kc, bool tok_kc, const MmPlan &plan, float *parts, hipStream_t stream, const char *what) {

@@ -250,3 +250,20 @@ def test_loss_sums_and_norms_in_forwards_order(memory, second, engram, counts, m
     assert abs(loss.item() - plain.item()) <= 1e-11 * plain.item()
     for n, a, b in zip(names, got, want):
         assert 0 < float(b.norm()) and float((a - b).norm()) <= 1e-9 * float(b.norm()), n
+
+
+def test_products_of_an_operand_form_that_is_not_there():
+    """Contiguous features with strided tokens are refused, not run as another form (smlm::mm_launch of csrc/lm_mm.h)."""
+    import ctypes
+
+    class Args(ctypes.Structure):                     # MmArgs, by value on the stack: at least its size
+        _fields_ = [("bytes", ctypes.c_int64 * 32)]
+
+    class Plan(ctypes.Structure):
+        _fields_ = [("shape", ctypes.c_int), ("splits", ctypes.c_int64)]
+
+    launch = getattr(_lib.lib(), "_ZN4smlm9mm_launchENS_6MmArgsEbbRKNS_6MmPlanEP12ihipStream_tPKc")
+    launch.restype = ctypes.c_int
+    launch.argtypes = [Args, ctypes.c_bool, ctypes.c_bool, ctypes.POINTER(Plan), ctypes.c_void_p, ctypes.c_char_p]
+    assert launch(Args(), True, False, ctypes.byref(Plan(3, 1)), None, b"product") == _lib.EUNSUPPORTED
+    assert "strided tokens" in _lib.last_error()

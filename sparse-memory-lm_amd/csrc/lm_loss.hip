@@ -32,6 +32,8 @@ constexpr int kLsFinishRows = 4;                          // tokens per workgrou
 constexpr int64_t kLsPieceBytes = 1LL << 30;            // most bytes of one piece's G
 constexpr int kNoTarget = -0x40000000;
 
+typedef uint16_t __attribute__((may_alias)) Overlaid;     // a value stored over a part of a wider store, behind it
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct LossArgs {
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(S::kThreads, 2) loss_kernel(LossArgs a) {
           v = (exp2_hw((v - m[j]) * kLog2e) - 1.f) * c;
           if (rel < (unsigned)C) {
             const float rest = mm_rest(v);
-            uint16_t *to = a.g + t * a.ldg + c0 + off;
+            Overlaid *to = (Overlaid *)(a.g + t * a.ldg + c0 + off);
             *to = (uint16_t)(pack_bf16x2(v, v) & 0xFFFFu);
             if (a.rest) to[a.rest] = (uint16_t)(pack_bf16x2(rest, rest) & 0xFFFFu);
           }

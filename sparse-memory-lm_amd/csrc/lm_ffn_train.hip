@@ -11,8 +11,8 @@
 //   mm_kernel     y, dx, dw13, dw2 (lm_mm.hip); the weights' sums over the tokens are split over workgroups
 // Bound by the products: 6 M d hidden operations forward, 18 with the recomputed a | b in the gradient; their rate is that of
 // the way from cache into LDS (lm_mm.h), and d = 384 of them are only six units of 64 k a tile.  Measured for 32,768 tokens
-// of d = 384, hidden 1,024: the gate 65 to 74 us (750 TFLOP/s), y 32, the gradient's gate 120 to 140 (its three results are
-// 201 MB, and take 60 us of it: they do not overlap its products), dx 62, dw13 58, dw2 51 and the joining of their parts 14.
+// of d = 384, hidden 1,024: the gate 63 us (820 TFLOP/s), y 35, the gradient's gate 129 (its three results are 201 MB, and
+// take 60 us of it: they do not overlap its products), dx 61, dw13 51, dw2 48 and the joining of their parts 14.
 #include "lm_mm.h"
 
 #include <algorithm>

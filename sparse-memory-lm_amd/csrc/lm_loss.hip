@@ -17,8 +17,8 @@
 // it: the stages of successive tiles run through one pipeline, so that a tile's first loads are on their way during its
 // predecessor's exponentials.  Measured (d = 384, V = 50,304): 16,384 tokens 600 to 640 us forward (1,030 TFLOP/s; d = 1,024
 // reaches 1,240), in the gradient 900 to 980 for G (its 1.65 GB are written in whole 64-byte lines, which do not overlap its
-// products: 65 us of each 412 MB), 640 to 720 for dx, 600 to 630 for dW.  64 tokens of 32,000 are bound by W's bytes and the
-// launches: 56 us for all.
+// products: 65 us of each 412 MB), 640 to 720 for dx, 590 to 630 for dW.  64 tokens of 32,000 are bound by W's bytes and the
+// launches: 60 us for all.
 #include "lm_mm.h"
 
 #include <algorithm>
@@ -383,6 +383,9 @@ GradPlan grad_plan(int64_t M, int64_t V, int64_t d) {
   p.cols = ceil_div(ceil_div(V, p.pieces), kLsCols) * kLsCols;
   p.pieces = ceil_div(V, p.cols);
   p.dx = mm_plan(M, d, p.cols, true);
+  // Never split over the tokens, so that its rows of bf16 are final: from some 20,000 columns on its tiles fill the card.  Below
+  // they do not, and it takes longer than dx, which is split (16,384 tokens, d = 384): 98 us for 22 of 1,000 columns, 185 for
+  // 122 of 8,192, 290 for 279 of 20,000.
   p.dw = mm_plan(p.cols, d, M, false);
   p.g_bytes = row * p.cols;
   p.part_bytes = p.pieces * p.dx.splits > 1 ? p.dx.splits * M * d * 4 : 0;

@@ -268,8 +268,8 @@ int row_lanes(int64_t C) {
   while (lanes < 1024 && 8 * lanes < C) lanes *= 2;
   return lanes;
 }
-// Workgroups of the gradient: each leaves a row of parts; 4,096 wavefronts at most, of at least 4 rows each (8 by one
-// wavefront).
+// Workgroups of the gradient: each leaves a row of parts; at most 4,096 wavefronts up to 2,048 columns, then 1,024 workgroups
+// (8,192 wavefronts up to 4,096 columns, 16,384 beyond), of at least 4 rows each (8 by one wavefront).
 int64_t grad_blocks(int64_t M, int64_t C) {
   const int lanes = row_lanes(C);
   const int64_t per = lanes <= 64 ? 512 / lanes : 4, most = lanes == 128 ? 2048 : 1024;

@@ -618,6 +618,84 @@ int smlm_rmsnorm_train_backward(const void *dxs, const void *dh, int h_dtype, co
                                 int w_dtype, const float *rstd, int64_t M, int64_t C, void *dx, void *ddelta,
                                 int delta_dtype, void *dw, float *parts, void *stream);
 
+/*
+ * The key-value cache of one attention layer in pages of page_size tokens (a power of two from 16 to 4096), for sequences of
+ * different lengths: a token lies in slot page id * page_size + offset of every kv head.  All dense, 16-byte aligned.
+ *   kind SMLM_BF16: k, v (num_pages, kv_heads, page_size, head_dim) bf16; the scales NULL
+ *   kind SMLM_Q4:   k, v (num_pages, kv_heads, page_size, head_dim / 2) bytes, dim 2 i in the low half of byte i; k_scale,
+ *                   v_scale (num_pages, kv_heads, page_size, 2) bf16, a row's step and lowest value: dim d stands for
+ *                   lowest + step * code[d]
+ * head_dim in {32, 64, 128}.
+ */
+typedef struct smlm_kv_pages {
+  void *k, *v, *k_scale, *v_scale;
+  int64_t num_pages;
+  int kind, page_size, kv_heads, head_dim;
+} smlm_kv_pages;
+
+/*
+ * Appends N tokens to the cache, with the position rotation on the way (smlm/model.py:63-78, 92-97 for tokens anywhere):
+ *   qkv (N, (H + 2 * kv_heads) * head_dim) bf16, row n at qkv + n * qkv_row_stride: H query heads, then keys, then values
+ *   rope_cos, rope_sin (rope_len, rot / 2) of rope_dtype (SMLM_F32 or SMLM_BF16); the first rot dims of a query or key head are
+ *     rotated (rot a multiple of 16, at most head_dim), pairs (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1):
+ *     a' = a cos - b sin, b' = b cos + a sin in fp32, every operation rounded
+ *   positions, slots (N,) int64: the token's row of the tables, and where it goes; distinct slots, any slot outside the pages
+ *     is not written.  A position outside the tables gives NaN and is not written.
+ *   q_out (N, H, head_dim), k_out (N, kv_heads, head_dim) or NULL: the rotated queries and keys, bf16
+ * 4-bit pages: lowest = bf16(min), step = bf16((max - lowest) / 15) (times the fp32 nearest to 1 / 15), code =
+ * clamp(rint((x - lowest) / step), 0, 15), 0 where step is not positive, of the fp32 rotated keys and the values; a row that
+ * is not finite throughout reads back as NaN.  Strides multiples of 8 elements, pointers 16-byte aligned.
+ */
+int smlm_paged_append(const void *qkv, int64_t qkv_row_stride, const void *rope_cos, const void *rope_sin, int rope_dtype,
+                      int64_t rope_len, int rot, int interleaved, const int64_t *positions, const int64_t *slots,
+                      const smlm_kv_pages *pages, int64_t N, int H, void *q_out, void *k_out, void *stream);
+
+/* The rows of slots (N,) int64 as k_out, v_out (N, kv_heads, head_dim) bf16 (zeros for a slot outside the pages). */
+int smlm_paged_gather(const smlm_kv_pages *pages, const int64_t *slots, int64_t N, void *k_out, void *v_out, void *stream);
+
+/*
+ * Causal attention over packed prompts of different lengths, with grouped heads (smlm/model.py:97-105 per sequence):
+ * sequence b has query rows cu_q[b] .. cu_q[b + 1] - 1 of q (N, H, head_dim) and key rows cu_k[b] .. cu_k[b + 1] - 1 of k, v
+ * (S, kv_heads, head_dim); its T queries are the last of its S_b positions, query t sees its keys 0 .. S_b - T + t:
+ *   y[t, h] = sum_s softmax_s(scale q[t, h] . k[s, h / (H / kv_heads)]) v[s, ...],  zeros where it sees none.
+ * Elements (row, head, d) at base + row * strides[0] + head * strides[1] + d.  cu_q, cu_k (B + 1,) int32, ascending (others
+ * give unspecified results within the buffers).  Rows of no sequence are left as they are, or zeroed (zero_rest).  bf16 in
+ * and out, fp32 scores, statistics and sums, probabilities rounded to bf16; masked keys and values count for nothing,
+ * whatever they hold.  head_dim in {32, 64, 128}; q, k, v 16-byte aligned with strides that are multiples of 8 up to 2^22; y
+ * 8-byte aligned, strides multiples of 4.
+ */
+int smlm_packed_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                          const int64_t *v_strides, const int *cu_q, const int *cu_k, int64_t B, int64_t N, int64_t S, int H,
+                          int kv_heads, int head_dim, float scale, void *y, const int64_t *y_strides, int zero_rest,
+                          void *stream);
+
+/*
+ * Attention of one query token per sequence over the cache (smlm/model.py:90-107 for T = 1): q (B, H, head_dim) bf16, row b at
+ * q + b * q_row_stride; sequence b has lengths[b] (int32) tokens, token t in row t % page_size of page
+ * block_table[b * table_row_stride + t / page_size] (int32, max_pages a sequence); lengths beyond the table count as its size.
+ * A page id outside the pages holds no tokens.  y (B, H, head_dim) dense; zeros for a sequence without tokens.  fp32 scores,
+ * statistics and sums, probabilities (4 bits: times the row's step) rounded to bf16.  What lies behind a sequence's last token
+ * counts for nothing.  workspace: smlm_paged_attention_workspace bytes (may be 0), 16-byte aligned.
+ */
+int64_t smlm_paged_attention_workspace(int64_t B, int H, int kv_heads, int head_dim, int page_size, int64_t max_pages);
+int smlm_paged_attention(const void *q, int64_t q_row_stride, const smlm_kv_pages *pages, const int *block_table,
+                         int64_t table_row_stride, int64_t max_pages, const int *lengths, int64_t B, int H, float scale,
+                         void *y, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Sampling from logits (B, V) of dtype (SMLM_BF16 or SMLM_F32, row stride in elements, any alignment) with the random numbers
+ * u (B,) fp32 in [0, 1): weights exp((x - max) / temperature); kept are the top_k largest (all for top_k <= 0), of these the
+ * smallest run of largest whose mass reaches top_p of theirs (all for top_p >= 1, at least one), and of these those that are
+ * at least min_p of the largest; equal logits rank by index.  token[b]: the first token in the order of the vocabulary whose
+ * running kept mass exceeds u times the kept mass.  temperature <= 0 (or NaN): the largest logit's lowest index.  NaN logits
+ * count as the lowest; a row of lowest values alone gives each token the same weight.  Each setting is an array (B,) or, where
+ * that is NULL, one value for all rows.  Masses in whole multiples of 2^-45 of the largest weight: the same token on every
+ * call.  V <= 2^18.
+ */
+int smlm_sample(const void *logits, int dtype, int64_t row_stride, const float *u, const float *temperature,
+                float temperature_all, const int *top_k, int top_k_all, const float *top_p, float top_p_all,
+                const float *min_p, float min_p_all, int64_t B, int64_t V, int64_t *token, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

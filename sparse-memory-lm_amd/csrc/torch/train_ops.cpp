@@ -7,16 +7,10 @@
 // tokens 146, against 40 us for a node that does nothing.
 //
 // A backward that is itself recorded (create_graph) runs as PyTorch ops, so that it can be differentiated again.
-#include <ATen/ATen.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/extension.h>
-
-#include "smlm_pkm.h"
+#include "common.h"
 
 namespace {
 
-using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -24,27 +18,6 @@ constexpr int64_t kMaxRowStride = 1 << 21;   // elements (csrc/lm_mm.h)
 constexpr int64_t kNormMaxCols = 16384;      // csrc/lm_rmsnorm.hip
 
 int64_t ceil8(int64_t n) { return (n + 7) / 8 * 8; }
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-int dtype_of(at::ScalarType t) { return t == at::kFloat ? SMLM_F32 : SMLM_BF16; }
-bool is_float_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
-
-void check(int rc, const char *what) {
-  TORCH_CHECK(rc == SMLM_OK, what, " failed with status ", rc, ": ", smlm_pkm_last_error());
-}
-
-// t with its values in memory as they are (a view may hold a sign that is yet to be applied).
-Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
-
-void check_device(const char *name, const Tensor &first, std::initializer_list<const Tensor *> others) {
-  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced: a trace would hold its outputs as they were");
-  TORCH_CHECK_VALUE(first.is_cuda(), name, ": all tensors must be on a HIP (cuda) device, got ", first.device());
-  for (const Tensor *t : others)
-    TORCH_CHECK_VALUE(!t->defined() || t->device() == first.device(), name, ": all tensors must be on one device, got ",
-                      first.device(), " and ", t->device());
-}
-
-void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-Tensor workspace(const Tensor &like, int64_t bytes) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
 
 // t, `blocks` groups of rows, with zeros behind each group's rows and behind the columns.  (Fill and copy, as constant_pad_nd
 // does it, are two launches: forward and gradient of an FFN block of 48 x 65, hidden 130, took 85 us instead of 68.)

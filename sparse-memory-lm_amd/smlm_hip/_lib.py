@@ -5,6 +5,7 @@ libsmlm_pkm.so makes the library bind to that same HIP runtime, so the stream ha
 valid in our launches.  There is no fallback: if the library is missing, every op raises.
 """
 import ctypes
+import importlib
 import os
 
 import torch  # noqa: F401  (see module docstring)
@@ -12,6 +13,7 @@ import torch  # noqa: F401  (see module docstring)
 LIB_NAME = "libsmlm_pkm.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 TRAIN_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_train_ops.so")
+SERVE_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_serve_ops.so")
 
 # smlm_dtype / smlm_status values of include/smlm_pkm.h
 F32, BF16, F16, I8, Q4, I32, I64 = range(7)
@@ -35,6 +37,12 @@ class LinearArgs(ctypes.Structure):
         ("tok_partial", _p), ("tok_partial_stride", _i64), ("tok_blocks", _i), ("tok_out", _p), ("hist", _p),
         ("hist_stride", _i64), ("hist_len", _i64), ("pos", _p), ("pos_advance", _p),
     ]
+
+class KVPages(ctypes.Structure):
+    """struct smlm_kv_pages of include/smlm_pkm.h, field for field."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("num_pages", _i64), ("kind", _i), ("page_size", _i),
+                ("kv_heads", _i), ("head_dim", _i)]
+
 
 # name -> (restype, argtypes); every function declared in include/smlm_pkm.h
 EXPORTS = {
@@ -90,6 +98,12 @@ EXPORTS = {
     "smlm_rmsnorm_train": (_i, [_p, _i, _p, _i, _p, _i, _f, _i64, _i64, _p, _p, _i, _p, _p]),
     "smlm_rmsnorm_parts": (_i64, [_i64, _i64]),
     "smlm_rmsnorm_train_backward": (_i, [_p, _p, _i, _p, _i, _p, _i, _p, _i64, _i64, _p, _p, _i, _p, _p, _p]),
+    "smlm_paged_append": (_i, [_p, _i64, _p, _p, _i, _i64, _i, _i, _p, _p, ctypes.POINTER(KVPages), _i64, _i, _p, _p, _p]),
+    "smlm_paged_gather": (_i, [ctypes.POINTER(KVPages), _p, _i64, _p, _p, _p]),
+    "smlm_packed_attention": (_i, [_p] * 8 + [_i64] * 3 + [_i] * 3 + [_f, _p, _p, _i, _p]),
+    "smlm_paged_attention_workspace": (_i64, [_i64, _i, _i, _i, _i, _i64]),
+    "smlm_paged_attention": (_i, [_p, _i64, ctypes.POINTER(KVPages), _p, _i64, _i64, _p, _i64, _i, _f, _p, _p, _i64, _p]),
+    "smlm_sample": (_i, [_p, _i, _i64, _p, _p, _f, _p, _i, _p, _f, _p, _f, _i64, _i64, _p, _p]),
     "smlm_row_gather": (_i, [_p, _i64, _p, _i, _i64, _i, _p, _p]),
 }
 ADAM_F32, ADAM_BF16, ADAM_INT8 = 0, 1, 2
@@ -122,21 +136,29 @@ def lib():
     return _lib
 
 
-_train = None
+_modules = {}
+
+
+def _torch_module(name, path, what):
+    module = _modules.get(name)
+    if module is None:
+        lib()
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built (run `python -m smlm_hip.build` in sparse-memory-lm_amd/ or "
+                               f"__graft_entry__.build()); {what} have no fallback")
+        module = _modules[name] = importlib.import_module("." + name, __package__)
+    return module
 
 
 def train_ops():
     """The autograd nodes of csrc/torch/train_ops.cpp (loaded once, after the library that they call). Raises if they have
     not been built."""
-    global _train
-    if _train is None:
-        lib()
-        if not os.path.exists(TRAIN_PATH):
-            raise RuntimeError(f"{TRAIN_PATH} is not built (run `python -m smlm_hip.build` in sparse-memory-lm_amd/ or "
-                               "__graft_entry__.build()); the training operators have no fallback")
-        from . import _train_ops
-        _train = _train_ops
-    return _train
+    return _torch_module("_train_ops", TRAIN_PATH, "the training operators")
+
+
+def serve_ops():
+    """The wrappers of csrc/torch/serve_ops.cpp, loaded likewise."""
+    return _torch_module("_serve_ops", SERVE_PATH, "the ragged-serving operators")
 
 
 def version():

@@ -1190,3 +1190,77 @@ def add_rmsnorm_train(x, delta, norm, out_dtype=None):
     if norm.weight is None:
         raise ValueError("add_rmsnorm_train: the norm needs a weight")
     return _lib.train_ops().add_rmsnorm_train(x, delta, norm.weight, norm.eps, out_dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Serving sequences of different lengths (model.Transformer.generate_ragged): a key-value cache in pages, packed prompts,
+# tokens drawn from the distribution.  Forward only.
+# ---------------------------------------------------------------------------------------------------------------
+def kv_pages(num_pages, n_kv_heads, page_size, head_dim, kind="bf16", device="cuda"):
+    """Empty pages of one attention layer's cache, as the functions below take them: a token lies in slot page id *
+    page_size + offset.  kind "bf16": (k, v), each (num_pages, n_kv_heads, page_size, head_dim) bf16.  "q4": (k, v, k_scale,
+    v_scale), k and v (num_pages, n_kv_heads, page_size, head_dim / 2) uint8, dim 2 i in the low half of byte i, and per row its
+    step and lowest value (..., 2) bf16: a dim stands for lowest + step * code, 4.25 to 5 bits in all."""
+    if kind not in ("bf16", "q4"):
+        raise ValueError(f"kv_pages: kind must be 'bf16' or 'q4', got {kind!r}")
+    if head_dim not in (32, 64, 128):
+        raise ValueError(f"kv_pages: head_dim {head_dim} not in (32, 64, 128)")
+    if page_size < 16 or page_size > 4096 or page_size & (page_size - 1) or num_pages < 1 or n_kv_heads < 1:
+        raise ValueError(f"kv_pages: {num_pages} pages of {page_size} tokens, {n_kv_heads} heads: pages hold a power of two "
+                         "from 16 to 4096 tokens")
+    shape = (num_pages, n_kv_heads, page_size)
+    dtype, row = (torch.bfloat16, head_dim) if kind == "bf16" else (torch.uint8, head_dim // 2)
+    pages = [torch.zeros(*shape, row, dtype=dtype, device=device) for _ in range(2)]
+    if kind == "q4":
+        pages += [torch.zeros(*shape, 2, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    return tuple(pages)
+
+
+def paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, interleaved=False, keys=False):
+    """Rotates the queries and keys of N tokens by their positions and writes keys and values into their slots of the pages
+    (kv_pages) in one launch (smlm/model.py:63-78, 92-97 for tokens of any sequences; smlm_paged_append).  qkv (..., (n_heads +
+    2 * n_kv_heads) * head_dim) bf16, N rows of queries, keys and values; rope tables (positions, rotated dims / 2) fp32 or bf16,
+    rotating the first dims of a head (a multiple of 16) in pairs (i, i + half) or, interleaved, (2 i, 2 i + 1); positions and
+    slots (N,) int64, the slots distinct.  Returns q (N, n_heads, head_dim) and, with keys=True, the rotated keys (N,
+    n_kv_heads, head_dim), else None.  A slot outside the pages (-1) is not written; a position outside the tables gives NaN
+    and is not written.  Rotation in fp32, rounded once; 4-bit pages take the unrounded keys, and a row that is not finite
+    throughout reads back as NaN."""
+    return _lib.serve_ops().paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, interleaved, keys)
+
+
+def paged_gather(pages, slots):
+    """The keys and values of slots (N,) int64 as (N, n_kv_heads, head_dim) bf16 each: what packed_attention reads where a
+    prompt goes on behind a cached beginning.  Zeros for a slot outside the pages.  (smlm_paged_gather)"""
+    return _lib.serve_ops().paged_gather(pages, slots)
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, scale=None, out=None):
+    """Causal attention over packed prompts of different lengths, with grouped heads (smlm/model.py:97-105 for each sequence;
+    smlm_packed_attention): sequence b has the rows cu_q[b] .. cu_q[b + 1] - 1 of q (N, H, hd) and cu_k[b] .. cu_k[b + 1] - 1
+    of k, v (S, n_kv_heads, hd) (cu_k None: the queries' rows), bf16, hd in (32, 64, 128), any strides over rows and heads
+    (views of the qkv projection work as they are where rows are 16-byte aligned); cu_q, cu_k (sequences + 1,) int32 on the
+    device, ascending.  Its queries are the last of its positions, each sees the keys up to its own; query head h reads kv head
+    h // (H / n_kv_heads).  scale: head_dim ** -0.5 by default.  Returns (N, H, hd) bf16, zeros for queries that see nothing and
+    for rows of no sequence; an `out` of that shape (not over an input) keeps the rows of no sequence as they are.  Masked keys
+    and values count for nothing, whatever they hold."""
+    return _lib.serve_ops().packed_attention(q, k, v, cu_q, cu_k, scale, out)
+
+
+def paged_attention(q, pages, block_table, lengths, scale=None):
+    """Attention of one query token per sequence over its cached tokens (smlm/model.py:90-107 for T = 1;
+    smlm_paged_attention): q (B, H, hd) bf16; pages as paged_append fills them; block_table (B, pages of a sequence) int32 page
+    ids; lengths (B,) int32, the new token included (beyond the table: its size).  H a multiple of the pages' kv heads.
+    Returns (B, H, hd) bf16, zeros for a sequence without tokens; ids outside the pages hold no tokens, and what lies behind a
+    sequence's last token counts for nothing."""
+    return _lib.serve_ops().paged_attention(q, pages, block_table, lengths, scale)
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Tokens (B,) int64 drawn from logits (B, V) bf16 or fp32, V <= 2^18, by the random numbers u (B,) fp32 in [0, 1)
+    (smlm_sample): weights exp((x - max) / temperature); kept are the top_k largest (0: all), of these the smallest run of
+    largest with top_p of their mass (1: all; at least one), of these those of at least min_p (at most 1) times the largest
+    weight; equal logits rank by index.  The token is the first in the vocabulary's order whose running kept mass exceeds u times the kept
+    mass.  temperature 0: the largest logit's lowest index.  Each setting is a number or a tensor (B,) (fp32, top_k int32).
+    NaN logits count as the lowest.  Masses are exact sums of fp64 weights rounded to 2^-45 of the largest: the same token on
+    every call."""
+    return _lib.serve_ops().sample_tokens(logits, u, temperature, top_k, top_p, min_p)

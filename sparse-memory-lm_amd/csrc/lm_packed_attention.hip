@@ -3,14 +3,20 @@
 // last of its S positions, so query t sees its keys 0 .. S - T + t:  y = softmax(scale q k^T) v, zeros where it sees none.
 // Query head h reads key head h / (H / Hkv).
 //
+// Bound by the matrix and vector instructions together: per tile of 64 keys and 32 queries a wavefront has 36 matrix instructions
+// of 16 clocks (68 with a head dim of 128) and 32 exponentials of 16 clocks beside some 70 other vector instructions of 4, so
+// the two or three wavefronts of a SIMD overlap one kind with the other, matrix work first (s_setprio).  Measured on 8,192
+// tokens, 32 heads: 1,105 TFLOP/s with a head dim of 128 and 968 with 64; a library product of 8,192 cubed reaches 1,395.
+//
 // A workgroup owns 128 consecutive query rows of one head, whichever sequences they belong to, and walks the key rows from
 // the first one that any of them sees to the last: both ranges grow with the row, so they join up, and the grid follows from
-// the number of rows alone, without the lengths on the host.  A lane finds its own query's range of keys by binary search in
+// the number of rows alone, without the lengths on the host; the last rows start first, and heads that share keys on one XCD (835 ->
+// 1,020 TFLOP/s on 6,001 and 5,000 tokens).  A lane finds its own query's range of keys by binary search in
 // cu_q; tiles that hold keys outside some query's range are masked, per query.  (Tiles of their own for every sequence need
 // the running sum of their tiles, and leave a part-filled tile per sequence.)
 //
 // Products as in a causal prompt pass: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 with the keys as M, so a lane (r, g) holds keys
-// 4 g .. 4 g + 3 of each 16-key tile for ONE query (r), and the running maximum and the rescaling are per lane; O^T = V^T P^T
+// 4 g .. 4 g + 3 of each 16-key tile for ONE query (r), and the softmax is per lane; O^T = V^T P^T
 // with the lane's own probabilities (rounded to bf16) as operand, V^T through transposing LDS reads.  Statistics, scores and
 // output sums in fp32, the probabilities' sum of the same rounded values on the matrix cores.
 //
@@ -19,16 +25,16 @@
 // for the queries that see the key.  So a query's result depends, to the bit, on nothing but what it sees.
 #include <algorithm>
 
-#include "pkm_common.h"
+#include "lm_mm.h"
 
 namespace smlm {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kBM = 128;        // query rows per workgroup
+constexpr int kNW = 4;          // wavefronts per workgroup,
+constexpr int kQJ = 2;          // with kQJ * 16 query rows each
+constexpr int kBM = 16 * kQJ * kNW;
 constexpr int kBN = 64;         // keys per tile
 constexpr int kCuLds = 512;     // entries of cu_q and cu_k kept in LDS
 
@@ -45,16 +51,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 template <int J>
 __device__ __forceinline__ float xor_lane_f(float v) { return __uint_as_float(xor_lane<J>(__float_as_uint(v))); }
 
-// 16-byte loads from a range of n bf16 values straight into LDS, zeros at and past its end
-struct BufferLds {
-  __amdgpu_buffer_rsrc_t r;
-  __device__ __forceinline__ BufferLds(const uint16_t *base, int64_t n)
-      : r(__builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)(n * 2), 0x00020000)) {}
-  __device__ __forceinline__ void load(char *lds, int offset) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, offset, 0, 0, 0);
-  }
-};
-
 struct PackedArgs {
   const uint16_t *q, *k, *v;
   uint16_t *y;
@@ -66,22 +62,25 @@ struct PackedArgs {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) packed_attention_kernel(PackedArgs A) {
-  constexpr int KS = HD / 32, MT = HD / 16, CPR = HD / 8, LPT = kBN * CPR / 256, RB = CPR * 16, SW = CPR < 8 ? CPR : 8;
+__global__ void __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 3 : 2)))
+    packed_attention_kernel(PackedArgs A) {
+  constexpr int KS = HD / 32, MT = HD / 16, CPR = HD / 8, LPT = kBN * CPR / (64 * kNW), RB = CPR * 16, SW = CPR < 8 ? CPR : 8;
   __shared__ __align__(16) uint16_t sK[2][kBN * HD];
   __shared__ __align__(16) uint16_t sV[2][kBN * HD];
   __shared__ int s_cu[2][kCuLds];
-  __shared__ int s_range[2][4];
+  __shared__ int s_range[2][kNW];
 
-  const int h = blockIdx.x % A.H, qt = blockIdx.x / A.H;
+  // the last rows first (of a long sequence the longest walks); heads that share keys on one XCD where they divide evenly
+  const int slot = blockIdx.x % A.H, h = A.H % kMmXcds ? slot : slot % kMmXcds * (A.H / kMmXcds) + slot / kMmXcds;
+  const int qt = (A.N + kBM - 1) / kBM - 1 - blockIdx.x / A.H;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, g = lane >> 4;
-  const int q0 = qt * kBM, qw = q0 + wave * 32;
+  const int q0 = qt * kBM, qw = q0 + wave * 16 * kQJ;
   const uint16_t *qb = A.q + h * A.qsh, *kb = A.k + h / A.G * A.ksh, *vb = A.v + h / A.G * A.vsh;
 
   // this wavefront's queries as B fragments: query row qw + 16 j + r, dims 32 s + 8 g .. +7
-  bf16x8 bq[2][KS];
+  bf16x8 bq[kQJ][KS];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < kQJ; ++j) {
     const int t = min(qw + 16 * j + r, A.N - 1);
 #pragma unroll
     for (int s = 0; s < KS; ++s) bq[j][s] = *(const bf16x8 *)(qb + t * A.qsn + 32 * s + 8 * g);
@@ -90,12 +89,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   // the keys [lo, hi) that query j of this lane sees; lo = hi where it sees none; owned: whether a sequence has its row
   const bool in_lds = A.B < kCuLds;
   if (in_lds)
-    for (int i = tid; i <= A.B; i += 256) s_cu[0][i] = A.cu_q[i], s_cu[1][i] = A.cu_k[i];
+    for (int i = tid; i <= A.B; i += 64 * kNW) s_cu[0][i] = A.cu_q[i], s_cu[1][i] = A.cu_k[i];
   __syncthreads();
-  int lo[2], hi[2];
-  bool owned[2];
+  int lo[kQJ], hi[kQJ];
+  bool owned[kQJ];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < kQJ; ++j) {
     const int i = qw + 16 * j + r;
     int b = 0, e = A.B + 1;          // entries of cu_q not above i
     while (b < e) {
@@ -114,10 +113,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     }
   }
   // over the wavefront's queries, and the workgroup's: the first key that one sees, the end of the last
-  auto first_of = [&](int j) { return hi[j] > lo[j] ? lo[j] : 0x7FFFFFFF; };
-  int w_lo = min(first_of(0), first_of(1)), w_hi = max(hi[0] > lo[0] ? hi[0] : 0, hi[1] > lo[1] ? hi[1] : 0);
-  // ... and the keys that all of them see
-  int all_lo = max(lo[0], lo[1]), all_hi = min(hi[0], hi[1]);
+  int w_lo = 0x7FFFFFFF, w_hi = 0, all_lo = 0, all_hi = 0x7FFFFFFF;
+#pragma unroll
+  for (int j = 0; j < kQJ; ++j) {
+    if (hi[j] > lo[j]) w_lo = min(w_lo, lo[j]), w_hi = max(w_hi, hi[j]);
+    all_lo = max(all_lo, lo[j]), all_hi = min(all_hi, hi[j]);      // the keys that all of them see
+  }
   auto over_rows = [&](int v, bool most) {
 #define SMLM_STEP(J) { const int o = (int)xor_lane<J>((uint32_t)v); v = most ? max(v, o) : min(v, o); }
     SMLM_STEP(1) SMLM_STEP(2) SMLM_STEP(4) SMLM_STEP(8)
@@ -128,53 +129,72 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   all_lo = over_rows(all_lo, true), all_hi = over_rows(all_hi, false);
   if (lane == 0) s_range[0][wave] = w_lo, s_range[1][wave] = w_hi;
   __syncthreads();
-  const int begin = min(min(s_range[0][0], s_range[0][1]), min(s_range[0][2], s_range[0][3]));
-  const int end = max(max(s_range[1][0], s_range[1][1]), max(s_range[1][2], s_range[1][3]));
-  const int ntk = end > begin ? (end - begin + kBN - 1) / kBN : 0;
-
-  float m[2] = {-3.0e38f, -3.0e38f};     // finite: a query may see nothing of the first tiles
-  const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
-  floatx4 lacc[2] = {zero4, zero4};
-  const bf16x8 ones = __builtin_bit_cast(bf16x8, uint4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-  floatx4 oacc[MT][2];
+  int begin = s_range[0][0], end = s_range[1][0];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) oacc[mt][0] = oacc[mt][1] = zero4;
+  for (int i = 1; i < kNW; ++i) begin = min(begin, s_range[0][i]), end = max(end, s_range[1][i]);
+  const int ntk = __builtin_amdgcn_readfirstlane(end > begin ? (end - begin + kBN - 1) / kBN : 0);
+  begin = __builtin_amdgcn_readfirstlane(ntk ? begin : 0);
+
+  float m[kQJ];     // finite: a query may see nothing of the first tiles
+  const floatx4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  floatx4 lacc[kQJ];
+#pragma unroll
+  for (int j = 0; j < kQJ; ++j) m[j] = -3.0e38f, lacc[j] = zero4;
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, uint4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+  floatx4 oacc[MT][kQJ];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int j = 0; j < kQJ; ++j) oacc[mt][j] = zero4;
 
   // A tile goes straight into LDS (lane i of a wavefront's load writes bytes 16 i .. +15 of its 1 KB piece): LDS chunk
   // id = tid + 256 u is slot id % CPR of row id / CPR, which holds the row's chunk slot ^ (row % SW).  The descriptors
   // start at the tile's first row (64-bit) and end with row S - 1, behind which rows read as zeros.
-  int koff[LPT], voff[LPT];
+  uint32_t koff[LPT], voff[LPT];
 #pragma unroll
   for (int u = 0; u < LPT; ++u) {
-    const int id = tid + 256 * u, row = id / CPR, c = (id % CPR) ^ (row % SW);
-    koff[u] = (int)((row * A.ksn + 8 * c) * 2);
-    voff[u] = (int)((row * A.vsn + 8 * c) * 2);
+    const int id = tid + 64 * kNW * u, row = id / CPR, c = (id % CPR) ^ (row % SW);
+    koff[u] = (uint32_t)((row * A.ksn + 8 * c) * 2);
+    voff[u] = (uint32_t)((row * A.vsn + 8 * c) * 2);
   }
-  auto load_tile = [&](int kv0, int buf) {
-    const int rows = min(kBN, A.S - kv0);
-    const BufferLds kr(kb + kv0 * A.ksn, (rows - 1) * A.ksn + HD), vr(vb + kv0 * A.vsn, (rows - 1) * A.vsn + HD);
+  const uint32_t k_lds = (uint32_t)(uintptr_t)(lds_byte *)sK + wave * 1024, v_lds = (uint32_t)(uintptr_t)(lds_byte *)sV + wave * 1024;
+  const uint16_t *kp = kb + begin * A.ksn, *vp = vb + begin * A.vsn;     // of the next tile
+  const int64_t k_step = kBN * A.ksn, v_step = kBN * A.vsn;
+  const int k_full = (int)(((kBN - 1) * A.ksn + HD) * 2), v_full = (int)(((kBN - 1) * A.vsn + HD) * 2);
+  int left = ntk > 0 ? A.S - begin : 0, tiles_left = ntk;                // rows from there to the last; 0 behind the last tile
+  // (Loads in inline assembly: behind the builtin's the compiler waits for them before every LDS read, so that they overlap
+  // nothing.  Three tiles in LDS, a pipeline over half tiles, and 64 or 256 rows a workgroup were slower.)
+  auto load_tile = [&](int buf) __attribute__((always_inline)) {
+    intx4 krs{(int)(uint32_t)(uintptr_t)kp, (int)((uint64_t)(uintptr_t)kp >> 32), k_full, 0x00020000};
+    intx4 vrs{(int)(uint32_t)(uintptr_t)vp, (int)((uint64_t)(uintptr_t)vp >> 32), v_full, 0x00020000};
+    if (left < kBN) {
+      krs[2] = left > 0 ? (int)(((left - 1) * A.ksn + HD) * 2) : 0;
+      vrs[2] = left > 0 ? (int)(((left - 1) * A.vsn + HD) * 2) : 0;
+    }
+    kp += k_step, vp += v_step, left = --tiles_left > 0 ? left - kBN : 0;
 #pragma unroll
     for (int u = 0; u < LPT; ++u) {
-      const int piece = (256 * u + wave * kWave) * 16;
-      kr.load((char *)sK[buf] + piece, koff[u]);
-      vr.load((char *)sV[buf] + piece, voff[u]);
+      mm_load_lds(krs, koff[u], k_lds + buf * (kBN * HD * 2) + u * (64 * kNW * 16));
+      mm_load_lds(vrs, voff[u], v_lds + buf * (kBN * HD * 2) + u * (64 * kNW * 16));
     }
   };
-  if (ntk > 0) load_tile(begin, 0);
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
+  load_tile(0);
 
   for (int tk = 0; tk < ntk; ++tk) {
     const int kv0 = begin + tk * kBN, buf = tk & 1;
-    if (tk + 1 < ntk) load_tile(kv0 + kBN, buf ^ 1);
+    mm_wait_barrier<0>();     // this tile has landed, and all have read the one before
+    load_tile(buf ^ 1);
 
     if (kv0 < w_hi && kv0 + kBN > w_lo) {
       const bool masked = kv0 < all_lo || kv0 + kBN > all_hi;
 
+      __builtin_amdgcn_s_setprio(1);
       // S^T: sacc[kt][j][i] = q(query 16 j + r) . k(key kv0 + 16 kt + 4 g + i)
-      floatx4 sacc[4][2];
+      floatx4 sacc[4][kQJ];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) sacc[kt][0] = sacc[kt][1] = zero4;
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int j = 0; j < kQJ; ++j) sacc[kt][j] = zero4;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         bf16x8 a[4];
@@ -186,58 +206,70 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < kQJ; ++j)
             sacc[kt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[kt], bq[j][s], sacc[kt][j], 0, 0, 0);
       }
 
-      // online softmax per query (lane), in the log2 domain; the reference point m is raised only when a tile's maximum is
-      // more than 2^8 above it, until then the exponentials stay below 256
-      float mx[2];
+      __builtin_amdgcn_s_setprio(0);
+      if (masked) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (masked) {
+        for (int j = 0; j < kQJ; ++j)
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int key = kv0 + 16 * kt + 4 * g + i;
-              if (key < lo[j] || key >= hi[j]) sacc[kt][j][i] = -__builtin_inff();
+              if ((uint32_t)(key - lo[j]) >= (uint32_t)(hi[j] - lo[j])) sacc[kt][j][i] = -__builtin_inff();
             }
-        }
-        float a = fmaxf(fmaxf(sacc[0][j][0], sacc[0][j][1]), fmaxf(sacc[0][j][2], sacc[0][j][3]));
-#pragma unroll
-        for (int kt = 1; kt < 4; ++kt)
-          a = fmaxf(a, fmaxf(fmaxf(sacc[kt][j][0], sacc[kt][j][1]), fmaxf(sacc[kt][j][2], sacc[kt][j][3])));
-        a = fmaxf(a, xor_lane_f<16>(a));
-        mx[j] = fmaxf(a, xor_lane_f<32>(a)) * A.scale_log2;
       }
-      if (__builtin_amdgcn_ballot_w64(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+      // P^T as B fragments: 32-key step ks = key tiles 2 ks and 2 ks + 1, slots 4 g .. and 16 + 4 g .. of them.  Returns the or
+      // of their bits, in which 0x40004000 is set where one is 2 or more (an infinity or a NaN too).
+      bf16x8 bp[kQJ][2];
+      auto probabilities = [&]() __attribute__((always_inline)) {
+        uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float mnew = mx[j] > m[j] + 8.f ? mx[j] : m[j];       // (each query by itself, whatever its neighbours do)
+        for (int j = 0; j < kQJ; ++j)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float p[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                p[i] = __builtin_amdgcn_exp2f(sacc[2 * ks + e / 2][j][2 * (e % 2) + i] * A.scale_log2 - m[j]);
+              u[e] = pack_bf16x2(p[0], p[1]);
+              bits |= u[e];
+            }
+            bp[j][ks] = __builtin_bit_cast(bf16x8, uint4{u[0], u[1], u[2], u[3]});
+          }
+        return bits;
+      };
+      // Online softmax per query (lane), in the log2 domain, with a reference point m that starts 2^8 above the first tile's
+      // maximum and moves, to 2^8 above a tile's, only when an exponential reaches 2: a test of the operands' bits stands in
+      // for the maximum of every tile (head dim 64: 753 -> 800 TFLOP/s).  Each query by itself, whatever its neighbours do.
+      if (__builtin_amdgcn_ballot_w64((probabilities() & 0x40004000u) != 0)) {
+#pragma unroll
+        for (int j = 0; j < kQJ; ++j) {
+          float a = -__builtin_inff();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) a = fmaxf(a, sacc[i / 4][j][i % 4]);
+          a = fmaxf(a, xor_lane_f<16>(a));
+          a = fmaxf(a, xor_lane_f<32>(a)) * A.scale_log2;
+          const float mnew = a - m[j] > 0.99f ? a + 8.f : m[j];
           const float alpha = __builtin_amdgcn_exp2f(m[j] - mnew);
           lacc[j] *= alpha;
           m[j] = mnew;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) oacc[mt][j] *= alpha;
         }
+        probabilities();
       }
-      bf16x8 bp[2][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < kQJ; ++j)
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sacc[kt][j][i] = __builtin_amdgcn_exp2f(sacc[kt][j][i] * A.scale_log2 - m[j]);
-        // P^T as B fragments: 32-key step ks = key tiles 2 ks and 2 ks + 1, slots 4 g .. and 16 + 4 g .. of them
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const floatx4 a = sacc[2 * ks][j], b = sacc[2 * ks + 1][j];
-          bp[j][ks] = __builtin_bit_cast(bf16x8, uint4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]),
-                                                       pack_bf16x2(b[2], b[3])});
+        for (int ks = 0; ks < 2; ++ks)
           lacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp[j][ks], lacc[j], 0, 0, 0);
-        }
-      }
 
       // V^T fragment of dims 16 mt + r at the 32-key step's keys in the same slots, by transposing reads
       auto values = [&](int ks, int mt) {
@@ -263,18 +295,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
           for (int i = 0; i < 4; ++i) fine = fine && fabsf(sums[mt][i]) < __builtin_inff();
         odd = __builtin_amdgcn_ballot_w64(!fine) != 0;
       }
+      if (!odd) {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint4 w = values(ks, mt);
-          if (odd) w = uint4{w.x & ~not_finite(w.x), w.y & ~not_finite(w.y), w.z & ~not_finite(w.z), w.w & ~not_finite(w.w)};
-          const bf16x8 a = __builtin_bit_cast(bf16x8, w);
+          for (int mt = 0; mt < MT; ++mt) {
+            const bf16x8 a = __builtin_bit_cast(bf16x8, values(ks, mt));
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            oacc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bp[j][ks], oacc[mt][j], 0, 0, 0);
-        }
-      if (odd) {
+            for (int j = 0; j < kQJ; ++j)
+              oacc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bp[j][ks], oacc[mt][j], 0, 0, 0);
+          }
+        __builtin_amdgcn_s_setprio(0);
+      } else {
+#pragma unroll 1
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const uint4 w = values(ks, mt);
+            const bf16x8 a = __builtin_bit_cast(bf16x8, uint4{w.x & ~not_finite(w.x), w.y & ~not_finite(w.y), w.z & ~not_finite(w.z),
+                                                              w.w & ~not_finite(w.w)});
+#pragma unroll
+            for (int j = 0; j < kQJ; ++j)
+              oacc[mt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ks ? bp[j][1] : bp[j][0], oacc[mt][j], 0, 0, 0);
+          }
 #pragma unroll 1
         for (int at = 0; at < kBN; ++at) {
           // the operand slot that holds key `at` of the tile: 16-bit half `slot % 2` of register slot / 2, in lane group `group`
@@ -289,7 +333,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             a = uint4{a.x & keep.x & not_finite(a.x), a.y & keep.y & not_finite(a.y), a.z & keep.z & not_finite(a.z),
                       a.w & keep.w & not_finite(a.w)};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < kQJ; ++j) {
               const uint4 p = __builtin_bit_cast(uint4, ks ? bp[j][1] : bp[j][0]);
               const bf16x8 b = __builtin_bit_cast(bf16x8, uint4{p.x & keep.x, p.y & keep.y, p.z & keep.z, p.w & keep.w});
               const floatx4 one = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), b, zero4, 0, 0, 0);
@@ -301,13 +345,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         }
       }
     }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
   }
+  mm_finish();
 
   // y: lane (r, g) holds dims 16 mt + 4 g .. +3 of query row qw + 16 j + r
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < kQJ; ++j) {
     const int t = qw + 16 * j + r;
     if (t >= A.N || (!owned[j] && !A.zero_rest)) continue;
     const float inv = hi[j] > lo[j] ? 1.0f / lacc[j][0] : 0.f;
@@ -319,6 +362,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
       *(uint2 *)(yr + 16 * mt + 4 * g) = out;
     }
   }
+}
+
+template <int HD>
+void launch(const PackedArgs &A, hipStream_t s) {
+  constexpr int rows = kBM;
+  hipLaunchKernelGGL((packed_attention_kernel<HD>), dim3((unsigned)((A.N + rows - 1) / rows * A.H)), dim3(64 * kNW), 0, s, A);
 }
 
 }  // namespace
@@ -338,7 +387,7 @@ extern "C" int smlm_packed_attention(const void *q, const int64_t *q_strides, co
   if (head_dim != 32 && head_dim != 64 && head_dim != 128)
     return fail(SMLM_EUNSUPPORTED, "%s: head_dim %d not in {32, 64, 128}", name, head_dim);
   // rows are numbered, and a tile's rows addressed, in 32 bits
-  if (B > (1 << 30) || N > (1 << 30) || S > (1 << 30) || (N + kBM - 1) / kBM * H > 0x7FFFFFFFLL)
+  if (B > (1 << 30) || N > (1 << 30) || S > (1 << 30) || (N + 63) / 64 * H > 0x7FFFFFFFLL)
     return fail(SMLM_EUNSUPPORTED, "%s: more than 2^30 rows, or 2^31 workgroups", name);
   const int64_t *st[4] = {q_strides, k_strides, v_strides, y_strides};
   for (int a = 0; a < 4; ++a)
@@ -353,11 +402,10 @@ extern "C" int smlm_packed_attention(const void *q, const int64_t *q_strides, co
   const PackedArgs A{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, (uint16_t *)y, q_strides[0], q_strides[1],
                      k_strides[0], k_strides[1], v_strides[0], v_strides[1], y_strides[0], y_strides[1], cu_q, cu_k, (int)N,
                      (int)S, (int)B, H, H / kv_heads, zero_rest, scale * 1.4426950408889634f};
-  const dim3 grid((unsigned)((N + kBM - 1) / kBM * H));
   switch (head_dim) {
-    case 32: hipLaunchKernelGGL((packed_attention_kernel<32>), grid, dim3(256), 0, (hipStream_t)stream, A); break;
-    case 64: hipLaunchKernelGGL((packed_attention_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, A); break;
-    default: hipLaunchKernelGGL((packed_attention_kernel<128>), grid, dim3(256), 0, (hipStream_t)stream, A); break;
+    case 32: launch<32>(A, (hipStream_t)stream); break;
+    case 64: launch<64>(A, (hipStream_t)stream); break;
+    default: launch<128>(A, (hipStream_t)stream); break;
   }
   return launch_status(name);
 }

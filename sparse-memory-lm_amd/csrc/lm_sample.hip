@@ -6,20 +6,22 @@
 //
 // Masses are whole numbers of 2^-45 of the largest weight, from weights in fp64: a sum is exact whatever its order, so every
 // call gives the same token, and one that lies within rounding of its neighbour's border is as rare as in fp64 (fp32 sums over
-// 50,000 tokens would give another token once in some hundred calls).  exp2 by a table of 2^(i / 256) and a polynomial of degree
-// 4: with |r| <= ln 2 / 512 the next term is r^5 / 120 < 4e-17.
+// 50,000 tokens would give another token once in some hundred calls).  exp2 by a table of 2^(i / 16), which the banks serve
+// without conflicts, and a polynomial of degree 7: with |r| <= ln 2 / 32 the next term is r^8 / 40320 < 2e-18.
 //
-// One workgroup of 1,024 a row, the row in LDS where it fits (a wavefront has a run of the vocabulary of its own, so that the running
-// mass is a sum over wavefronts, then over the found wavefront's vectors).  A cut -- the top_k-th token, or the one at which
-// the mass reaches top_p -- is found by histograms: 1,024 bins of count (and mass) between the largest and smallest logit,
-// a scan over the bins, then the bin that holds the cut as the next range, until it has at most 512 tokens, which are ranked
-// against each other in LDS.
+// One workgroup of 1,024 a row, the row in LDS where it fits (a wavefront has a run of the vocabulary of its own, so that the
+// running mass is a sum over wavefronts, then over the found wavefront's vectors).  Bound by the passes over the row, vector
+// instructions all: a pass over 50,304 tokens costs 1.5 to 2 us, one with every token's weight 6, one that also adds it to a
+// histogram 10.  So the tokens that may be kept are listed first, where a bound on them is cheap -- top_k of at most 512: at
+// least that many tokens lie above the bin that holds the k-th largest of the threads' own maxima; min_p: a bound on the
+// logit -- and everything else is done on the list, of at most 512 tokens, by ranking each against all.  Else a cut, the
+// top_k-th token or the one at which the mass reaches top_p, is found by a histogram of 1,024 bins, then within its bin.
 #include "pkm_common.h"
 
 namespace smlm {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 1024, kList = 512;
+constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 1024, kList = 512, kPowerBits = 6, kPowers = 1 << kPowerBits;
 constexpr float kLowest = -3.3895313892515355e38f;   // the lowest bf16: masked logits and NaN
 constexpr double kUnit = 0x1p45;
 
@@ -35,25 +37,26 @@ struct SampleArgs {
 };
 
 struct Shared {
-  double exp2[256];
+  double power[kPowers];
   uint64_t mass[kBins];
   uint32_t count[kBins];
   float list_x[kList];
   int list_i[kList];
-  uint64_t list_w[kList];
+  uint64_t list_w[kList], list_before[kList];
+  uint32_t list_rank[kList];
   uint64_t wave_mass[kWaves];
+  uint64_t wave_kept[kWaves];
   uint32_t wave_count[kWaves];
   float wave_f[2][kWaves];
   // what one thread found for all
   uint64_t mass_above, total;
-  uint32_t count_above, n, lo, hi;
-  int bin, index, cut_rank;
-  uint32_t fill;
+  uint32_t count_above, n, lo, hi, fill;
+  int bin, index;
 };
 constexpr int kSharedVecs = (sizeof(Shared) + 15) / 16;
 constexpr int kLdsVecs = 160 * 1024 / 16 - kSharedVecs;      // vectors of a row that LDS holds
 
-__device__ __forceinline__ uint32_t code_of(float x) { return order32(__float_as_uint(x)); }
+__device__ __forceinline__ uint32_t code_of(float x) { return order32(__float_as_uint(x + 0.f)); }      // (-0 as 0)
 __device__ __forceinline__ float value_of(uint32_t c) { return __uint_as_float(unorder32(c)); }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
@@ -79,11 +82,12 @@ struct Row {
   int V, first, vecs;                 // first vector of this lane, vectors of its run
   bool aligned;
 
-  __device__ __forceinline__ static float fix(float x) { return x > kLowest ? fminf(x, -kLowest) + 0.f : kLowest; }
+  // (med3 of a NaN is the lowest of the others)
+  __device__ __forceinline__ static float fix(float x) { return __builtin_amdgcn_fmed3f(x, kLowest, -kLowest); }
 
-  // vector j of the lane: masked logits and NaN as the lowest value, -0 as 0, -infinity behind the row's end
-  __device__ __forceinline__ uint4 fetch(int j) const {
-    const int at = (first + 64 * j) * W;
+  // vector j of the lane: masked logits and NaN as the lowest value, -infinity behind the row's end
+  __device__ __forceinline__ uint4 fetch(int j) const { return fetch_at((first + 64 * j) * W); }
+  __device__ __forceinline__ uint4 fetch_at(int at) const {
     float x[W];
     if (aligned && at + W <= V) {
       const uint4 raw = *(const uint4 *)(base + (int64_t)at * (BF16 ? 2 : 4));
@@ -110,9 +114,15 @@ struct Row {
   __device__ __forceinline__ Row(const void *p, int64_t row, int64_t stride, int n, int wave, int lane, int vecs_, uint4 *lds)
       : base((const char *)p + row * stride * (BF16 ? 2 : 4)), kept(lds), V(n), first(wave * vecs_ * 64 + lane), vecs(vecs_),
         aligned((uintptr_t)base % 16 == 0) {
-    if constexpr (LDS) {
-#pragma unroll 4
-      for (int j = 0; j < vecs; ++j) kept[first + 64 * j] = fetch(j);
+  }
+  // the first pass: f(x, index) for every element, and the row into LDS
+  template <class F>
+  __device__ __forceinline__ void load(F &&f) const {
+#pragma unroll 8
+    for (int j = 0; j < vecs; ++j) {
+      const uint4 raw = fetch(j);
+      if constexpr (LDS) kept[first + 64 * j] = raw;
+      vec(j, raw, f);
     }
   }
 
@@ -122,9 +132,20 @@ struct Row {
   }
   // f(x, index) for every element of vector j
   template <class F>
-  __device__ __forceinline__ void vec(int j, const uint4 &raw, F &&f) const {
+  __device__ __forceinline__ void vec(int j, const uint4 &raw, F &&f) const { each_of((first + 64 * j) * W, raw, f); }
+  // the same of wavefront w's run
+  __device__ __forceinline__ uint4 of_run(int w, int j) const {
+    const int v = (w * vecs + j) * 64 + (int)(threadIdx.x % kWave);
+    if constexpr (LDS) return kept[v];
+    else return fetch_at(v * W);
+  }
+  template <class F>
+  __device__ __forceinline__ void vec_of_run(int w, int j, const uint4 &raw, F &&f) const {
+    each_of(((w * vecs + j) * 64 + (int)(threadIdx.x % kWave)) * W, raw, f);
+  }
+  template <class F>
+  __device__ __forceinline__ void each_of(int at, const uint4 &raw, F &&f) const {
     const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
-    const int at = (first + 64 * j) * W;
 #pragma unroll
     for (int e = 0; e < W; ++e)
       f(BF16 ? __uint_as_float(e % 2 ? r[e / 2] & 0xFFFF0000u : r[e / 2] << 16) : __uint_as_float(r[e % 4]), at + e);
@@ -134,25 +155,53 @@ struct Row {
 #pragma unroll 2
     for (int j = 0; j < vecs; ++j) vec(j, vector(j), f);
   }
+  // f(x, index, whether the cut keeps it) for every element of vector j, or, where no lane has more than three that it keeps,
+  // for those alone
+  template <class P, class F>
+  __device__ __forceinline__ void vec_where(int j, const uint4 &raw, const P &takes, F &&f) const {
+    const int at = (first + 64 * j) * W;
+    if (takes.all) {
+      vec(j, raw, [&](float x, int i) { f(x, i, true); });
+      return;
+    }
+    uint32_t bits = 0;
+    vec(j, raw, [&](float x, int i) { bits |= takes.keeps(x, i) ? 1u << (i - at) : 0u; });
+    if (__builtin_amdgcn_ballot_w64(__builtin_popcount(bits) > 3)) {
+      vec(j, raw, [&](float x, int i) { f(x, i, (bits >> (i - at) & 1) != 0); });
+      return;
+    }
+    while (__builtin_amdgcn_ballot_w64(bits != 0)) {
+      const int e = bits ? __builtin_ctz(bits) : 0, word = BF16 ? e >> 1 : e;
+      uint32_t w = raw.x;
+      w = word == 1 ? raw.y : w;
+      w = word == 2 ? raw.z : w;
+      w = word == 3 ? raw.w : w;
+      f(__uint_as_float(!BF16 ? w : e & 1 ? w & 0xFFFF0000u : w << 16), at + e, bits != 0);
+      bits &= bits - 1;
+    }
+  }
 };
 
 struct Weight {
-  const double *table;
-  double scale;                       // log2(e) / temperature
-  float top, min_p;
+  const double *power;                // 2^(i / 64)
+  double scale;                       // 64 log2(e) / temperature
+  float top;
+  double min_p;
 
-  // 2^((x - top) scale)
+  // 2^((x - top) scale / 64), from 2^-47 on, below which a mass is 0 either way.  No branches, so that the chains of a vector's
+  // elements overlap, and rounding and scaling by additions (conversions and ldexp take four times as long).
   __device__ __forceinline__ double weight(float x) const {
-    const double t = ((double)x - (double)top) * scale;
-    if (!(t > -46.0)) return 0.0;
-    const double k = __builtin_rint(t * 256.0);
-    const double r = __builtin_fma(k, -1.0 / 256.0, t) * 0.693147180559945309417;
-    const int ki = (int)k;
-    double p = __builtin_fma(r, 1.0 / 24.0, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
+    const double t = __builtin_fmax(((double)x - (double)top) * scale, -47.0 * kPowers);
+    const double m = t + 0x1.8p52, r = t - (m - 0x1.8p52);             // t rounded, in m's low bits
+    const int k = (int)(uint32_t)__double_as_longlong(m);
+    constexpr double c = 0.693147180559945309417 / kPowers;
+    double p = __builtin_fma(r, c * c * c * c * c / 120, c * c * c * c / 24);
+    p = __builtin_fma(p, r, c * c * c / 6);
+    p = __builtin_fma(p, r, c * c / 2);
+    p = __builtin_fma(p, r, c);
     p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return ldexp(p * table[ki & 255], ki >> 8);
+    const uint64_t w = (uint64_t)__double_as_longlong(p * power[k & (kPowers - 1)]);
+    return __longlong_as_double((long long)(w + ((uint64_t)(uint32_t)(k >> kPowerBits) << 52)));
   }
   __device__ __forceinline__ uint64_t mass_of(double w) const {
     return (uint64_t)__double_as_longlong(__builtin_fma(w, kUnit, 0x1p52)) & 0xFFFFFFFFFFFFFull;
@@ -160,7 +209,7 @@ struct Weight {
   __device__ __forceinline__ uint64_t mass(float x) const { return mass_of(weight(x)); }
   __device__ __forceinline__ uint64_t kept_mass(float x) const {
     const double w = weight(x);
-    return w >= (double)min_p ? mass_of(w) : 0;
+    return w >= min_p ? mass_of(w) : 0;
   }
 };
 
@@ -169,139 +218,295 @@ struct Cut {
   float value;
   int index;
   uint32_t n;
-  __device__ __forceinline__ bool keeps(float x, int i) const { return x > value || (x == value && i <= index); }
+  bool all;                            // it keeps every token (and what stands behind the row's end weighs nothing)
+  __device__ __forceinline__ bool keeps(float x, int i) const { return all | (x > value) | ((x == value) & (i <= index)); }
+};
+
+// The bins of a range of logits, from its top down: of equal width in value, or (always possible) in code.
+struct Bins {
+  float hi, inv;
+  uint32_t hi_code;
+  int shift;
+  bool linear;
+  __device__ __forceinline__ Bins(uint32_t lo_code, uint32_t hi_code_, bool by_value) : hi_code(hi_code_) {
+    hi = value_of(hi_code);
+    const float span = hi * 0.5f - value_of(lo_code) * 0.5f;
+    linear = by_value && span > 1e-30f && span < 1e30f;
+    inv = linear ? 511.5f / span : 0.f;
+    shift = max(0, 32 - __builtin_clz((hi_code - lo_code) | 1) - 10);
+  }
+  __device__ __forceinline__ int of(float x) const {
+    // (never past the last bin: what stands behind the row's end is below the range)
+    return linear ? min((int)((hi - x) * inv), kBins - 1) : (int)min((hi_code - code_of(x)) >> shift, (uint32_t)(kBins - 1));
+  }
+};
+
+// The running sum of v over the workgroup's threads up to this one; `total` of all.
+template <class T>
+__device__ __forceinline__ T running(T v, T *wave_sums, T &total) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    T b;
+    if constexpr (sizeof(T) == 8) b = shfl_up64(v, o);
+    else b = __shfl_up(v, o, kWave);
+    if (lane >= o) v += b;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) wave_sums[wave] = v;
+  __syncthreads();
+  total = 0;
+  T before = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    before += i < wave ? wave_sums[i] : 0;
+    total += wave_sums[i];
+  }
+  return v + before;
+}
+
+// Lists the tokens that f takes, in any order; returns how many there are (those beyond kList are not listed).
+template <class R, class F>
+__device__ __forceinline__ uint32_t list(const R &row, Shared &S, F &&f) {
+  __syncthreads();
+  if (threadIdx.x == 0) S.fill = 0;
+  __syncthreads();
+  row.each([&](float x, int i) {
+    if (f(x, i)) {
+      const uint32_t at = atomicAdd(&S.fill, 1u);
+      if (at < kList) S.list_x[at] = x, S.list_i[at] = i;
+    }
+  });
+  __syncthreads();
+  return S.fill;
+}
+
+// Per listed token (n of them): list_rank of the tokens ahead and list_before of their mass, ahead(x, i, y, j) whether the token
+// j of logit y is ahead of the token i of logit x.  Every token is compared with all by several threads, each with a part of
+// them.
+template <class F>
+__device__ __forceinline__ void rank(Shared &S, int n, F &&ahead) {
+  const int tid = threadIdx.x;
+  if (tid < n) S.list_rank[tid] = 0, S.list_before[tid] = 0;
+  __syncthreads();
+  const int parts = kThreads / n, part = tid / n, at = tid - part * n;
+  if (part < parts) {
+    const float x = S.list_x[at];
+    const int i = S.list_i[at];
+    uint32_t c = 0;
+    uint64_t w = 0;
+#pragma unroll 4
+    for (int o = part; o < n; o += parts) {
+      const float y = S.list_x[o];
+      const int j = S.list_i[o];
+      const uint64_t m = S.list_w[o];
+      const bool is = ahead(x, i, y, j);
+      c += is;
+      w += is ? m : 0;
+    }
+    if (c) {
+      atomicAdd(&S.list_rank[at], c);
+      atomicAdd((unsigned long long *)&S.list_before[at], (unsigned long long)w);
+    }
+  }
+  __syncthreads();
+}
+// the order of the logits, and of the vocabulary
+struct ByLogit {
+  __device__ __forceinline__ bool operator()(float x, int i, float y, int j) const { return (y > x) | ((y == x) & (j < i)); }
+};
+struct ByIndex {
+  __device__ __forceinline__ bool operator()(float, int i, float, int j) const { return j < i; }
 };
 
 // The cut after the k-th kept token (MASS false), or after the one at which the mass reaches `share` of the kept mass.
 template <bool MASS, class R>
 __device__ Cut select(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom, uint32_t k, double share) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-  uint32_t lo = code_of(fmaxf(bottom, cut.value)), hi = code_of(top), n = cut.n, above = 0;
+  uint32_t lo = code_of(fmaxf(bottom, cut.value)), hi = code_of(top), above = 0;
   uint64_t mass_above = 0;
   double target = 0.0;                 // of the mass, once the total is known
-  bool first = true;
   // every pass leaves the cut's bin as the range lo .. hi of codes, both of tokens in it: fewer tokens, or one value alone
-  while (n > kList && lo < hi) {
+  for (bool first = true;; first = false) {
+    __syncthreads();
     S.mass[tid] = 0;
     S.count[tid] = 0;
     __syncthreads();
-    const float fhi = value_of(hi), flo = value_of(lo), span = fhi * 0.5f - flo * 0.5f;
-    const bool linear = first && span > 1e-30f && span < 1e30f;   // bins of equal width in value, later in code
-    const float inv = linear ? 511.5f / span : 0.f;
-    const int shift = max(0, 32 - __builtin_clz(hi - lo) - 10);
-    auto bin_of = [&](float x) {
-      return linear ? min((int)((fhi - x) * inv), kBins - 1) : (int)((hi - code_of(x)) >> shift);
-    };
+    const Bins bins(lo, hi, first);
+    const float flo = value_of(lo), fhi = value_of(hi);
     row.each([&](float x, int i) {
       if (x >= flo && x <= fhi && cut.keeps(x, i)) {
-        const int b = bin_of(x);
-        atomicAdd(&S.count[b], 1u);
+        const int b = bins.of(x);
         if constexpr (MASS) atomicAdd((unsigned long long *)&S.mass[b], (unsigned long long)weight.mass(x));
+        else atomicAdd(&S.count[b], 1u);
       }
     });
     __syncthreads();
-    // running count and mass up to this thread's bin
-    const uint32_t c = S.count[tid];
-    const uint64_t w = MASS ? S.mass[tid] : 0;
-    uint32_t cs = c;
-    uint64_t ws = w;
-#pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-      const uint32_t a = __shfl_up(cs, o, kWave);
-      const uint64_t b = MASS ? shfl_up64(ws, o) : 0;
-      if (lane >= o) cs += a, ws += b;
+    // running count or mass up to this thread's bin
+    bool here;
+    if constexpr (MASS) {
+      const uint64_t w = S.mass[tid];
+      uint64_t total;
+      const uint64_t upto = mass_above + running(w, S.wave_mass, total);
+      if (first) target = fmax(share * (double)total, 1.0);
+      here = (double)(upto - w) < target && target <= (double)upto;
+      if (here) S.bin = tid, S.mass_above = upto - w;
+    } else {
+      const uint32_t c = S.count[tid];
+      uint32_t total;
+      const uint32_t upto = above + running(c, S.wave_count, total);
+      here = upto - c < k && k <= upto;
+      if (here) S.bin = tid, S.count_above = upto - c;
     }
-    if (lane == kWave - 1) S.wave_count[wave] = cs, S.wave_mass[wave] = ws;
-    __syncthreads();
-    uint64_t total = mass_above;
-    cs += above, ws += mass_above;
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) cs += S.wave_count[i], ws += S.wave_mass[i];
-      total += S.wave_mass[i];
-    }
-    if (MASS && first) target = fmax(share * (double)total, 1.0);
-    const bool here = MASS ? (double)(ws - w) < target && target <= (double)ws : cs - c < k && k <= cs;
-    if (here) S.bin = tid, S.n = c, S.count_above = cs - c, S.mass_above = ws - w;
     if (tid == 0) S.lo = 0xFFFFFFFFu, S.hi = 0;
     __syncthreads();
     const int bin = S.bin;
-    n = S.n, above = S.count_above, mass_above = S.mass_above;
+    if constexpr (MASS) mass_above = S.mass_above;
+    else above = S.count_above;
+    const uint32_t n = list(row, S, [&](float x, int i) { return x >= flo && x <= fhi && cut.keeps(x, i) && bins.of(x) == bin; });
+    if (n <= kList) {
+      // the bin's tokens ranked against each other
+      if (tid < (int)n) S.list_w[tid] = MASS ? weight.mass(S.list_x[tid]) : 0;
+      __syncthreads();
+      rank(S, (int)n, ByLogit());
+      const bool keep = tid < (int)n && (MASS ? (double)(mass_above + S.list_before[tid]) < target : above + S.list_rank[tid] < k);
+      if (tid == 0) S.n = 0;
+      __syncthreads();
+      if (keep) atomicMax(&S.n, S.list_rank[tid]);       // the last kept token's rank
+      __syncthreads();
+      const uint32_t last = S.n;
+      if (keep && S.list_rank[tid] == last) S.index = tid;
+      __syncthreads();
+      const Cut got{S.list_x[S.index], S.list_i[S.index], above + last + 1, false};
+      __syncthreads();
+      return got;
+    }
     uint32_t bl = 0xFFFFFFFFu, bh = 0;
     row.each([&](float x, int i) {
-      if (x >= flo && x <= fhi && cut.keeps(x, i) && bin_of(x) == bin) bl = min(bl, code_of(x)), bh = max(bh, code_of(x));
+      if (x >= flo && x <= fhi && cut.keeps(x, i) && bins.of(x) == bin) bl = min(bl, code_of(x)), bh = max(bh, code_of(x));
     });
     if (bh) atomicMin(&S.lo, bl), atomicMax(&S.hi, bh);
     __syncthreads();
     lo = S.lo, hi = S.hi;
-    first = false;
-  }
+    if (lo < hi) continue;
 
-  const float flo = value_of(lo), fhi = value_of(hi);
-  if (n <= kList) {
-    // the range's tokens ranked against each other
-    if (tid == 0) S.fill = 0, S.cut_rank = -1;
-    __syncthreads();
-    row.each([&](float x, int i) {
-      if (x >= flo && x <= fhi && cut.keeps(x, i)) {
-        const uint32_t at = atomicAdd(&S.fill, 1u);
-        if (at < kList) S.list_x[at] = x, S.list_i[at] = i;
-      }
-    });
-    __syncthreads();
-    n = min(n, S.fill);
-    if (MASS && tid < (int)n) S.list_w[tid] = weight.mass(S.list_x[tid]);
-    __syncthreads();
-    float x = 0.f;
-    int index = 0, before = 0;
-    bool keep = false;
-    if (tid < (int)n) {
-      x = S.list_x[tid], index = S.list_i[tid];
-      uint64_t mass = mass_above, total = mass_above;
-      for (int i = 0; i < (int)n; ++i) {
-        const float y = S.list_x[i];
-        const bool ahead = y > x || (y == x && S.list_i[i] < index);
-        before += ahead;
-        if constexpr (MASS) {
-          mass += ahead ? S.list_w[i] : 0;
-          total += S.list_w[i];
-        }
-      }
-      if (MASS && first) target = fmax(share * (double)total, 1.0);
-      keep = MASS ? (double)mass < target : above + before < k;
-      if (keep) atomicMax(&S.cut_rank, before);
+    // more equal tokens than the list holds: the first c of them, the last of which is found by bisection of the index
+    uint64_t c = k - above;
+    const float value = value_of(hi);
+    if constexpr (MASS) {
+      const uint64_t one = weight.mass(value);
+      const double more = ceil(target) - (double)mass_above;      // the least whole mass beyond what lies above
+      c = one ? ((uint64_t)fmax(more, 1.0) - 1) / one + 1 : n;
+    }
+    c = c < 1 ? 1 : c > n ? n : c;
+    int a = 0, b = row.V - 1;
+    while (a < b) {
+      const int mid = a + (b - a) / 2;
+      uint32_t upto = 0;
+      row.each([&](float x, int i) { upto += x == value && i <= mid && cut.keeps(x, i); });
+      for (int o = 32; o > 0; o >>= 1) upto += __shfl_xor(upto, o, kWave);
+      __syncthreads();
+      if (lane == 0) S.wave_count[wave] = upto;
+      __syncthreads();
+      uint32_t all = 0;
+      for (int i = 0; i < kWaves; ++i) all += S.wave_count[i];
+      if (all >= c) b = mid;
+      else a = mid + 1;
     }
     __syncthreads();
-    if (keep && before == S.cut_rank) S.list_x[0] = x, S.index = index;   // (read by nobody else any more)
-    __syncthreads();
-    const Cut got{S.list_x[0], S.index, above + (uint32_t)S.cut_rank + 1};
-    __syncthreads();
-    return got;
+    return Cut{value, a, above + (uint32_t)c, false};
   }
-  // more equal tokens than the list holds: the first c of them, the last of which is found by bisection of the index
-  uint64_t c = k - above;
-  if constexpr (MASS) {
-    const uint64_t one = weight.mass(fhi);
-    if (first) target = fmax(share * ((double)n * (double)one), 1.0);
-    const double more = ceil(target) - (double)mass_above;      // the least whole mass beyond what lies above
-    c = one ? ((uint64_t)fmax(more, 1.0) - 1) / one + 1 : n;
-  }
-  c = c < 1 ? 1 : c > n ? n : c;
-  int a = 0, b = row.V - 1;
-  while (a < b) {
-    const int mid = a + (b - a) / 2;
-    uint32_t here = 0;
-    row.each([&](float x, int i) { here += x == fhi && i <= mid && cut.keeps(x, i); });
-    for (int o = 32; o > 0; o >>= 1) here += __shfl_xor(here, o, kWave);
-    __syncthreads();
-    if (lane == 0) S.wave_count[wave] = here;
-    __syncthreads();
-    uint32_t all = 0;
-    for (int i = 0; i < kWaves; ++i) all += S.wave_count[i];
-    if (all >= c) b = mid;
-    else a = mid + 1;
+}
+
+// The cut at which the mass reaches `share` of the kept mass, and the mass that the cut and min_p keep: `sum`, of this thread's
+// tokens above the cut's bin, and S.wave_kept, by wavefront, of those in it.  The bin is found from weights in fp32, and then
+// its borders' masses are checked exactly: false where they do not hold the cut, or the bin holds more than the list.
+template <class R>
+__device__ bool reach(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom, double share, double scale,
+                      Cut &got, uint64_t &sum) {
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const Bins bins(code_of(fmaxf(bottom, cut.value)), code_of(top), true);
+  const float s32 = (float)scale;
+  auto rough = [&](float x) { return __builtin_amdgcn_exp2f((x - top) * s32); };
+  float part = 0.f;
+  row.each([&](float x, int i) { part += cut.keeps(x, i) ? rough(x) : 0.f; });
+  part = wave_sum(part);
+  __syncthreads();
+  S.count[tid] = 0;
+  if (lane == 0) S.wave_f[0][wave] = part;
+  if (tid == 0) S.bin = -1, S.fill = 0;
+  if (tid < kWaves) S.wave_kept[tid] = 0;
+  __syncthreads();
+  part = 0.f;
+  for (int i = 0; i < kWaves; ++i) part += S.wave_f[0][i];
+  const float unit = 0x1p30f / part;       // whole numbers, for an atomic addition of which the LDS takes 24 clocks (fp32: 240)
+  row.each([&](float x, int i) {
+    if (cut.keeps(x, i)) atomicAdd(&S.count[bins.of(x)], (uint32_t)(rough(x) * unit + 0.5f));
+  });
+  __syncthreads();
+  const uint32_t mine = S.count[tid];
+  uint32_t sums;
+  const uint32_t upto = running(mine, S.wave_count, sums);
+  const uint32_t reach = (uint32_t)fmaxf((float)share * (float)sums, 1.f);
+  if (upto - mine < reach && reach <= upto) S.bin = tid;
+  __syncthreads();
+  const int bin = S.bin;
+  if (bin < 0) return false;
+  const bool some = weight.min_p > 0.0;      // min_p drops some of what top_p keeps
+  uint64_t all = 0, above = 0;
+  sum = 0;
+  for (int j = 0; j < row.vecs; ++j)
+    row.vec_where(j, row.vector(j), cut,
+                  [&](float x, int i, bool keep) {
+                    const double w = weight.weight(x);
+                    const uint64_t m = keep ? weight.mass_of(w) : 0;
+                    const int b = bins.of(x);
+                    all += m;
+                    above += b < bin ? m : 0;
+                    if (some) sum += b < bin && w >= weight.min_p ? m : 0;
+                    if (keep && b == bin && x >= kLowest) {
+                      const uint32_t at = atomicAdd(&S.fill, 1u);
+                      if (at < kList) S.list_x[at] = x, S.list_i[at] = i;
+                    }
+                  });
+  sum = some ? sum : above;
+  all = wave_sum64(all), above = wave_sum64(above);
+  if (lane == 0) S.wave_mass[wave] = all;
+  __syncthreads();
+  uint64_t total = 0, over = 0;
+  for (int i = 0; i < kWaves; ++i) total += S.wave_mass[i];
+  const uint32_t n = S.fill;
+  __syncthreads();
+  if (lane == 0) S.wave_mass[wave] = above;
+  if (n > kList || n == 0) return false;
+  double w = 0.0;
+  uint64_t mass = 0;
+  if (tid < (int)n) w = weight.weight(S.list_x[tid]), S.list_w[tid] = mass = weight.mass_of(w);
+  if (tid == 0) S.n = 0, S.total = 0;
+  __syncthreads();
+  for (int i = 0; i < kWaves; ++i) over += S.wave_mass[i];
+  rank(S, (int)n, ByLogit());
+  const double target = fmax(share * (double)total, 1.0);
+  if (mass) atomicAdd((unsigned long long *)&S.total, (unsigned long long)mass);
+  const bool keep = tid < (int)n && (double)(over + S.list_before[tid]) < target;
+  if (keep) {
+    atomicMax(&S.n, S.list_rank[tid]);
+    if (w >= weight.min_p) atomicAdd((unsigned long long *)&S.wave_kept[S.list_i[tid] / (64 * R::W * row.vecs)], (unsigned long long)mass);
   }
   __syncthreads();
-  return Cut{fhi, a, above + (uint32_t)c};
+  if (!((double)over < target && target <= (double)(over + S.total))) return false;
+  const uint32_t last = S.n;
+  if (keep && S.list_rank[tid] == last) S.index = tid;
+  __syncthreads();
+  got = Cut{S.list_x[S.index], S.list_i[S.index], 0, false};      // (how many it keeps is not asked any more)
+  return true;
+}
+
+// The mass that the token's running mass has to exceed.
+__device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
+  const double aim = u * (double)total;
+  const uint64_t target = aim > 0.0 ? (uint64_t)fmin(aim, 9.2e18) : 0;
+  return target < total ? target : total - 1;
 }
 
 template <bool BF16, bool LDS>
@@ -313,15 +518,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
   const Row<BF16, LDS> row(A.logits, at, A.row_stride, A.V, wave, lane, A.vecs, smem + kSharedVecs);
   const float temperature = A.temperature ? A.temperature[at] : A.temperature1;
   const float top_p = A.top_p ? A.top_p[at] : A.top_p1, min_p = A.min_p ? A.min_p[at] : A.min_p1;
-  const int top_k = A.top_k ? A.top_k[at] : A.top_k1;
+  int top_k = A.top_k ? A.top_k[at] : A.top_k1;
   const double u = A.u[at];
-  if (tid < 256) S.exp2[tid] = exp2(tid * (1.0 / 256.0));
+  top_k = top_k > 0 && top_k < A.V ? top_k : 0;
+  if (tid < kPowers) S.power[tid] = exp2(tid * (1.0 / kPowers));
+  S.count[tid] = 0;
 
-  float top = kLowest, bottom = -kLowest;
-  row.each([&](float x, int) {
-    top = fmaxf(top, x);
+  float mine = -__builtin_inff(), top, bottom = -kLowest;        // this thread's largest
+  row.load([&](float x, int) {
+    mine = fmaxf(mine, x);
     bottom = x >= kLowest ? fminf(bottom, x) : bottom;
   });
+  top = mine;
   for (int o = 32; o > 0; o >>= 1) {
     top = fmaxf(top, __shfl_xor(top, o, kWave));
     bottom = fminf(bottom, __shfl_xor(bottom, o, kWave));
@@ -341,52 +549,134 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
     return;
   }
 
-  const Weight weight{S.exp2, 1.4426950408889634074 / (double)temperature, top, fminf(min_p, 1.f)};
-  Cut cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V};
-  if (top_k > 0 && top_k < A.V) cut = select<false>(row, weight, S, cut, top, bottom, (uint32_t)top_k, 0.0);
-  if (top_p < 1.f) cut = select<true>(row, weight, S, cut, top, bottom, 0u, (double)top_p);
+  const double scale = 1.4426950408889634074 / (double)temperature;
+  const Weight weight{S.power, kPowers * scale, top, fmin((double)min_p, 1.0)};
 
-  uint64_t sum = 0;
-  row.each([&](float x, int i) {
-    if (cut.keeps(x, i)) sum += weight.kept_mass(x);
-  });
+  // 1. What may be kept as a list, where that is cheap and short.
+  float least = -__builtin_inff();                   // no token below it is kept
+  if (top_k == 0 && min_p > 0.f) {                   // w >= min_p, with a margin for the logarithm's and this sum's rounding
+    least = (float)fmax((double)kLowest, (double)top + log2(weight.min_p) / scale * 1.000001) - 1e-6f * fabsf(top);
+  } else if (top_k > 0 && top_k <= kList) {
+    const Bins bins(code_of(bottom), code_of(top), true);
+    if (mine >= kLowest) atomicAdd(&S.count[bins.of(mine)], 1u);
+    if (tid == 0) S.bin = kBins;
+    __syncthreads();
+    const uint32_t c = S.count[tid];
+    uint32_t total;
+    const uint32_t upto = running(c, S.wave_count, total);
+    if (upto - c < (uint32_t)top_k && (uint32_t)top_k <= upto) S.bin = tid;
+    if (tid == 0) S.lo = 0xFFFFFFFFu;
+    __syncthreads();
+    // the least of the maxima down to that bin: as many tokens as there are maxima lie at or above it
+    if (mine >= kLowest && bins.of(mine) <= S.bin) atomicMin(&S.lo, code_of(mine));
+    __syncthreads();
+    if (S.bin < kBins) least = fmaxf(least, value_of(S.lo));
+  }
+  const bool lists = (least > -__builtin_inff() || A.V <= kList) && top_k <= kList;
+  const uint32_t n = lists ? list(row, S, [&](float x, int) { return x >= least && x >= kLowest; }) : kList + 1;
+  if (n <= kList) {
+    uint64_t kept = 0;                               // the mass that top_p is a share of
+    if (top_k == 0 && top_p < 1.f) {
+      uint64_t sum = 0;
+      for (int j = 0; j < row.vecs; ++j)             // (nothing behind the row's end)
+        row.vec(j, row.vector(j), [&](float x, int) { sum += weight.mass(x); });
+      sum = wave_sum64(sum);
+      if (lane == 0) S.wave_mass[wave] = sum;
+      __syncthreads();
+      for (int i = 0; i < kWaves; ++i) kept += S.wave_mass[i];
+    }
+    double w = 0.0;
+    if (tid < (int)n) w = weight.weight(S.list_x[tid]), S.list_w[tid] = weight.mass_of(w);
+    __syncthreads();
+    rank(S, (int)n, ByLogit());
+    const uint32_t place = tid < (int)n ? S.list_rank[tid] : kList;
+    const uint64_t mass = tid < (int)n ? S.list_w[tid] : 0, ahead = tid < (int)n ? S.list_before[tid] : 0;
+    bool keep = tid < (int)n && (top_k == 0 || place < (uint32_t)top_k);
+    if (top_k > 0 && top_p < 1.f) {
+      if (tid < (int)n && place == min((uint32_t)top_k, n) - 1) S.total = ahead + mass;
+      __syncthreads();
+      kept = S.total;
+    }
+    if (top_p < 1.f) keep = keep && (double)ahead < fmax((double)top_p * (double)kept, 1.0);
+    keep = keep && w >= weight.min_p;
+    if (tid < (int)n) S.list_w[tid] = keep ? mass : 0;
+    __syncthreads();
+    rank(S, (int)n, ByIndex());
+    if (tid < (int)n && place == 0) S.total = 0;
+    __syncthreads();
+    if (keep) atomicAdd((unsigned long long *)&S.total, (unsigned long long)mass);
+    __syncthreads();
+    const uint64_t target = target_of(u, S.total);
+    if (keep && S.list_before[tid] <= target && S.list_before[tid] + mass > target) A.token[at] = S.list_i[tid];
+    return;
+  }
+
+  // 2. Cuts by histograms.
+  Cut cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V, true};
+  if (top_k > 0) cut = select<false>(row, weight, S, cut, top, bottom, (uint32_t)top_k, 0.0);
+  uint64_t sum = 0;                                  // kept, of this thread
+  bool summed = false;
+  if (top_p < 1.f) {
+    Cut got;
+    summed = reach(row, weight, S, cut, top, bottom, (double)top_p, scale, got, sum);
+    cut = summed ? got : select<true>(row, weight, S, cut, top, bottom, 0u, (double)top_p);
+  }
+  sum = summed ? sum : 0;
+  if (!summed)
+    for (int j = 0; j < row.vecs; ++j)
+      row.vec_where(j, row.vector(j), cut,
+                    [&](float x, int, bool keep) {
+                      const uint64_t m = weight.kept_mass(x);
+                      sum += keep ? m : 0;
+                    });
   sum = wave_sum64(sum);
-  if (lane == 0) S.wave_mass[wave] = sum;
+  __syncthreads();
+  if (lane == 0) S.wave_mass[wave] = sum + (summed ? S.wave_kept[wave] : 0);
   __syncthreads();
   uint64_t total = 0, before = 0;
   for (int i = 0; i < kWaves; ++i) total += S.wave_mass[i];
-  const double aim = u * (double)total;
-  uint64_t target = aim > 0.0 ? (uint64_t)fmin(aim, 9.2e18) : 0;      // the token's running mass is above it
-  if (target >= total) target = total - 1;
-  for (int i = 0; i < wave; ++i) before += S.wave_mass[i];
-  if (before > target || before + sum <= target) return;               // one wavefront goes on
-  for (int j = 0; j < row.vecs; ++j) {
-    const uint4 raw = row.vector(j);
+  const uint64_t target = target_of(u, total);
+  int found = -1;
+  // the found wavefront's vectors, by all of them
+  for (int i = 0; i < kWaves && found < 0; ++i) {
+    if (before + S.wave_mass[i] > target) found = i;
+    else before += S.wave_mass[i];
+  }
+  for (int j0 = 0; j0 < row.vecs; j0 += kWaves) {
+    const int j = j0 + wave;
+    const bool in = j < row.vecs;
+    uint4 raw{0, 0, 0, 0};
     uint64_t mine = 0;
-    row.vec(j, raw, [&](float x, int i) {
-      if (cut.keeps(x, i)) mine += weight.kept_mass(x);
-    });
+    if (in) {
+      raw = row.of_run(found, j);
+      row.vec_of_run(found, j, raw, [&](float x, int i) {
+        const uint64_t m = weight.kept_mass(x);
+        mine += cut.keeps(x, i) ? m : 0;
+      });
+    }
     uint64_t run = mine;
 #pragma unroll
     for (int o = 1; o < kWave; o *= 2) {
       const uint64_t b = shfl_up64(run, o);
       if (lane >= o) run += b;
     }
-    const uint64_t all = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)run, 63) |
-                         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(run >> 32), 63) << 32;
-    if (before + all > target) {
-      uint64_t mass = before + run - mine;
-      if (mass <= target && before + run > target) {
-        int64_t found = -1;
-        row.vec(j, raw, [&](float x, int i) {
-          if (cut.keeps(x, i)) mass += weight.kept_mass(x);
-          if (found < 0 && mass > target) found = i;
-        });
-        A.token[at] = found;
-      }
-      return;
+    __syncthreads();
+    if (lane == kWave - 1) S.wave_kept[wave] = run;
+    __syncthreads();
+    uint64_t upto = before;
+    for (int i = 0; i < wave; ++i) upto += S.wave_kept[i];
+    for (int i = 0; i < kWaves; ++i) before += S.wave_kept[i];
+    uint64_t mass = upto + run - mine;
+    if (in && mass <= target && upto + run > target) {
+      int64_t token = -1;
+      row.vec_of_run(found, j, raw, [&](float x, int i) {
+        const uint64_t m = weight.kept_mass(x);
+        mass += cut.keeps(x, i) ? m : 0;
+        if (token < 0 && mass > target) token = i;
+      });
+      A.token[at] = token;
     }
-    before += all;
+    if (before > target) return;
   }
 }
 

@@ -19,6 +19,7 @@ from torch import nn
 from . import kernels
 from .capture import capture
 from .engram import EngramMemory, NgramHash
+from .paged import PagedKVCache, PagedLayer, StepPlan
 from .pkm import ProductKeyMemory, inference_tables, state_tag, state_tensors
 from .recording import ordinary, records, unhooked
 
@@ -121,6 +122,8 @@ class Attention(nn.Module):
 
     def forward(self, x, kv_cache=None, pos0=0):
         B, T, C = x.shape
+        if isinstance(kv_cache, PagedLayer):
+            return kernels.linear(self.wo, self._paged(kernels.linear(self.wqkv, x), kv_cache).view(B, T, C).to(x.dtype))
         if (T == 1 and torch.is_tensor(pos0) and isinstance(kv_cache, StaticKVCache) and x.is_cuda
                 and kv_cache.k.dtype == torch.bfloat16 and self.head_dim in (16, 32, 64, 128)):
             # one decode step: RoPE, cache write and attention in one kernel (smlm_hip.kernels.decode_attention)
@@ -179,6 +182,21 @@ class Attention(nn.Module):
                 v = torch.cat([kv_cache["v"], v], dim=2)
             kv_cache["k"], kv_cache["v"] = k, v
         return kernels.prefill_attention(q, k, v)
+
+    def _paged(self, qkv, layer):
+        """Attention of the tokens that the cache's plan says these rows of the projection are: appended to the pages, then
+        each behind its own sequence's."""
+        plan, H = layer.plan, self.n_heads
+        qkv = qkv.to(torch.bfloat16)
+        step = isinstance(plan, StepPlan)
+        q, k = kernels.paged_append(qkv, self.rope.cos, self.rope.sin, plan.positions, plan.slots, layer.pages, H,
+                                    keys=not step and plan.cu_k is None)
+        if step:
+            return kernels.paged_attention(q, layer.pages, plan.block_table, plan.lengths)
+        if plan.cu_k is None:
+            return kernels.packed_attention(q, k, qkv.view(-1, 3, H, self.head_dim)[:, 2], plan.cu_q)
+        k, v = kernels.paged_gather(layer.pages, plan.all_slots)
+        return kernels.packed_attention(q, k, v, plan.cu_q, plan.cu_k)
 
     def _static(self, q, k, v, cache, pos0):
         T = q.shape[2]
@@ -373,6 +391,7 @@ class Transformer(nn.Module):
         self._fwd_graphs = {}
         self._fwd_graphs_tag = None
         self._state = None              # state_tensors(self), kept for the graphs' state_tag
+        self._replaced = 0              # how often the memory tables or the kept parameter list were replaced
         self._init_weights()
 
     @torch.no_grad()
@@ -441,22 +460,26 @@ class Transformer(nn.Module):
                 raise ValueError(kind)
         self._decoders.clear()
         self._fwd_graphs.clear()
+        self._replaced += 1
 
     def forward(self, idx, targets=None, kv_caches=None, pos0=0):
         """Logits (B, T, vocab), or (logits, loss) with targets (smlm/model.py:266-293)."""
-        x = self.tok_emb(idx)
-        rows = self._ngram_rows(idx, kv_caches) if self.ngram is not None else None
-        if (x.is_cuda and x.dtype == torch.bfloat16 and not torch.is_autocast_enabled("cuda")
-                and self.ngram is None and not (torch.is_grad_enabled() and records(x, *self.parameters()))):
-            logits = self.lm_head(self._blocks_fused_norms(x, kv_caches, pos0))
-        else:
-            for i, blk in enumerate(self.layers):
-                x = blk(x, None if kv_caches is None else kv_caches[i], pos0, rows)
-            logits = self.lm_head(self.norm(x))
+        logits = self.lm_head(self._hidden(idx, kv_caches, pos0))
         if targets is None:
             return logits
         loss = F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.reshape(-1))
         return logits, loss
+
+    def _hidden(self, idx, kv_caches, pos0):
+        """forward() up to the lm_head: the normed last hidden state."""
+        x = self.tok_emb(idx)
+        rows = self._ngram_rows(idx, kv_caches) if self.ngram is not None else None
+        if (x.is_cuda and x.dtype == torch.bfloat16 and not torch.is_autocast_enabled("cuda")
+                and self.ngram is None and not (torch.is_grad_enabled() and records(x, *self.parameters()))):
+            return self._blocks_fused_norms(x, kv_caches, pos0)
+        for i, blk in enumerate(self.layers):
+            x = blk(x, None if kv_caches is None else kv_caches[i], pos0, rows)
+        return self.norm(x)
 
     def loss(self, idx, targets, ignore_index=-100, reduction="mean"):
         """forward(idx, targets)[1] (smlm/model.py:266-293) without the logits, for training and for scoring text: the
@@ -581,6 +604,7 @@ class Transformer(nn.Module):
         self._fwd_graphs.clear()
         self._fwd_graphs_tag = None
         self._state = None
+        self._replaced += 1
         self._decoders.clear()
         for m in self.memory_layers():
             m._graph = None
@@ -628,6 +652,141 @@ class Transformer(nn.Module):
         dec = self._decoder(B, P + new_tokens + 1, prompt.device)
         tokens = dec.run(prompt, new_tokens, use_graph, sync_every_step)
         return tokens
+
+    # ---- sequences of different lengths ------------------------------------------------------------------------
+    def paged_cache(self, n_seqs, max_len=None, kind="bf16", page_size=64, num_pages=None):
+        """An empty PagedKVCache for n_seqs sequences of up to max_len tokens (the model's longest by default)."""
+        cfg = self.cfg
+        if self.ngram is not None:
+            raise ValueError("paged_cache: Engram layers keep histories of equally long sequences")
+        max_len = cfg.max_seq_len if max_len is None else max_len
+        if not 1 <= max_len <= cfg.max_seq_len:
+            raise ValueError(f"paged_cache: max_len {max_len} is not from 1 to max_seq_len = {cfg.max_seq_len}")
+        return PagedKVCache(cfg.n_layers, n_seqs, max_len, cfg.n_heads, cfg.d_model // cfg.n_heads, page_size, kind, num_pages,
+                            self.tok_emb.weight.device)
+
+    @torch.no_grad()
+    def prefill(self, cache, prompts):
+        """One pass over prompts[b], 1-D token tensors of any lengths (none: an empty one), behind what the cache holds of
+        sequence b: logits (n_seqs, vocab) of each one's last new token (NaN for a sequence without one).  In bf16 (weights
+        or autocast)."""
+        self._check_paged(cache)
+        prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
+        if len(prompts) != cache.n_seqs:
+            raise ValueError(f"prefill: {len(prompts)} prompts for a cache of {cache.n_seqs} sequences")
+        new = [p.numel() for p in prompts]
+        cache.reserve(new)
+        dev = cache.device
+        last = torch.tensor([n > 0 for n in new])
+        if sum(new) == 0:
+            return torch.full((cache.n_seqs, self.cfg.vocab_size), float("nan"), device=dev, dtype=self.lm_head.weight.dtype)
+        cache.plan = cache.plan_prompts(new)
+        try:
+            hidden = self._hidden(torch.cat([p.to(dev, torch.long) for p in prompts]).unsqueeze(0), cache.layers, 0)
+        finally:
+            cache.plan = None
+        cache.advance(new)
+        at = (torch.tensor(new).cumsum(0) - 1).clamp_(min=0).to(dev)
+        logits = self.lm_head(hidden[0].index_select(0, at))
+        return logits if last.all() else logits.masked_fill(~last.to(dev).unsqueeze(1), float("nan"))
+
+    def _check_paged(self, cache):
+        w = self.tok_emb.weight
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
+        if not w.is_cuda or dtype != torch.bfloat16 or cache.device != w.device:
+            raise ValueError(f"the paged cache is for bf16 models (or bf16 autocast) on its own GPU, got {dtype} on {w.device}")
+        if len(cache.layers) != len(self.layers):
+            raise ValueError(f"a cache of {len(cache.layers)} layers for a model of {len(self.layers)}")
+
+    @torch.no_grad()
+    def generate_ragged(self, prompts, new_tokens, cache=None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None,
+                        use_graph=True):
+        """Decoding of sequences of different lengths, greedy or sampled: prefill(cache, prompts), then new_tokens steps of one
+        token each for all sequences, drawn by kernels.sample_tokens with these settings (numbers, or one per sequence:
+        tensors (n_seqs,), fp32, top_k int32) from random numbers of `generator`; temperature 0 is greedy, as generate() is.
+        Returns the ids (n_seqs, new_tokens + 1): the prompts' next tokens, then one per step; all but the last are in the
+        cache afterwards, which a later call may go on from.  Every sequence needs a prompt.  With use_graph a step is one
+        replay of a captured graph, kept by the cache."""
+        prompts = list(prompts)
+        if cache is None:
+            longest = max((len(p) for p in prompts), default=0) + new_tokens
+            cache = self.paged_cache(max(1, len(prompts)), max(1, longest))
+        if len(prompts) != cache.n_seqs or any(len(p) == 0 for p in prompts) or new_tokens < 0:
+            raise ValueError(f"generate_ragged: {cache.n_seqs} prompts of at least one token are needed, and new_tokens >= 0")
+        B, dev = cache.n_seqs, cache.device
+        self._check_paged(cache)
+        if any(inference_tables(m.values) is None for m in self.memory_layers()):
+            use_graph = False               # a staged table tier synchronises in every call: no capture
+        each = lambda v, dtype: v.to(dev, dtype).expand(B) if torch.is_tensor(v) else torch.full((B,), v, dtype=dtype, device=dev)  # noqa: E731
+        f32 = torch.float32
+        settings = (each(temperature, f32), each(top_k, torch.int32), each(top_p, f32), each(min_p, f32))
+        u = torch.rand(new_tokens + 1, B, generator=generator, device=dev if generator is None else generator.device).to(dev)
+        cache.reserve([len(p) + new_tokens for p in prompts])
+        first = kernels.sample_tokens(self.prefill(cache, prompts), u[0], *settings)
+        state = self._ragged_state(cache)
+        for buffer, value in zip(state["settings"], settings):
+            buffer.copy_(value)
+        state["u"][:new_tokens + 1].copy_(u)
+        state["tok"].copy_(first.unsqueeze(1))
+        state["at"].fill_(1)
+        if use_graph and new_tokens:
+            graph = self._ragged_graph(cache, state)
+            for _ in range(new_tokens):
+                graph.replay()
+        else:
+            for _ in range(new_tokens):
+                self._ragged_step(cache, state)
+        cache.seq_lens = [n + new_tokens for n in cache.seq_lens]
+        return torch.cat([first.unsqueeze(1), state["out"][:, 1:new_tokens + 1]], 1)
+
+    def _ragged_state(self, cache):
+        """The buffers of generate_ragged's steps, kept by the cache."""
+        if "tok" not in cache.decoding:
+            B, n, dev = cache.n_seqs, cache.max_len + 1, cache.device
+            new = lambda *shape, dtype: torch.zeros(*shape, dtype=dtype, device=dev)  # noqa: E731
+            cache.decoding.update(tok=new(B, 1, dtype=torch.long), out=new(B, n, dtype=torch.long), at=new(1, dtype=torch.long),
+                                  u=new(n, B, dtype=torch.float32),
+                                  settings=tuple(new(B, dtype=t) for t in (torch.float32, torch.int32, torch.float32, torch.float32)))
+        return cache.decoding
+
+    def _ragged_step(self, cache, state):
+        """One token for every sequence, from and to the device's state."""
+        cache.plan = cache.plan_step()
+        try:
+            logits = self.lm_head(self._hidden(state["tok"], cache.layers, 0))[:, 0]
+        finally:
+            cache.plan = None
+        cache.lengths.add_(1)
+        token = kernels.sample_tokens(logits, state["u"].index_select(0, state["at"]).view(-1), *state["settings"])
+        state["tok"].copy_(token.unsqueeze(1))
+        state["out"].index_copy_(1, state["at"], token.unsqueeze(1))
+        state["at"].add_(1)
+
+    def _ragged_graph(self, cache, state):
+        """The captured step of this cache, captured again where the model has changed since; the cache is left as it was."""
+        ac = torch.is_autocast_enabled("cuda")
+        key = (self._replaced, state_tag(self.state_tensors()), ac)
+        if state.get("graph_of", lambda: None)() is not self or state["graph_key"] != key:
+            ctx = (torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False) if ac
+                   else torch.autocast("cuda", enabled=False))
+            state["graph"] = None
+            table = cache.block_table.clone()
+            saved = [t.clone() for t in (cache.lengths, state["tok"], state["out"], state["at"])]
+            cache.block_table.fill_(-1)          # the steps before the capture (library loads, derived weights) write no page
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side), ctx:
+                for _ in range(2):
+                    self._ragged_step(cache, state)
+            torch.cuda.current_stream().wait_stream(side)
+            cache.block_table.copy_(table)
+            for t, value in zip((cache.lengths, state["tok"], state["out"], state["at"]), saved):
+                t.copy_(value)
+            graph = torch.cuda.CUDAGraph()
+            with capture(graph), ctx:
+                self._ragged_step(cache, state)
+            state["graph"], state["graph_of"], state["graph_key"] = graph, weakref.ref(self), key
+        return state["graph"]
 
     def _decoder(self, B, max_len, device):
         key = (B, max_len, str(device), torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"))

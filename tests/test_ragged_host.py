@@ -185,3 +185,76 @@ def test_the_plain_sampling_counts_out_the_distribution():
         w = torch.zeros(5)
         w[keep] = (x[keep] / T).exp()
         assert torch.allclose(got.double(), (w / w.sum()).double(), atol=1.5 / n), (T, k, p, m)
+
+
+# ---- the cache's bookkeeping ---------------------------------------------------------------------------------------------
+def cache(n=3, max_len=40, page=16, **kw):
+    from smlm_hip.paged import PagedKVCache
+    return PagedKVCache(2, n, max_len, 1, 32, page, device="cpu", **kw)
+
+
+def slots_of(c, b, n):
+    """Where the first n tokens of sequence b lie, from the block table."""
+    t = torch.arange(n)
+    return c.block_table[b, t // c.page_size].long() * c.page_size + t % c.page_size
+
+
+def test_a_cache_plans_prompts_and_steps():
+    c = cache()
+    new = [17, 0, 1]
+    c.reserve(new)
+    plan = c.plan_prompts(new)
+    assert plan.positions.tolist() == list(range(17)) + [0] and plan.cu_q.tolist() == [0, 17, 17, 18] and plan.cu_k is None
+    assert torch.equal(plan.slots, torch.cat([slots_of(c, 0, 17), slots_of(c, 2, 1)]))
+    assert len(set(plan.slots.tolist())) == 18 and plan.slots.max() < c.num_pages * 16
+    c.advance(new)
+    assert c.seq_lens == [17, 0, 1] == c.lengths.tolist()
+    again = [2, 5, 0]
+    c.reserve(again)
+    plan = c.plan_prompts(again)
+    assert plan.positions.tolist() == [17, 18, 0, 1, 2, 3, 4] and plan.cu_q.tolist() == [0, 2, 7, 7]
+    assert plan.cu_k.tolist() == [0, 19, 24, 24]                # sequence 2 is not attended to
+    assert torch.equal(plan.all_slots, torch.cat([slots_of(c, 0, 19), slots_of(c, 1, 5)]))
+    assert torch.equal(plan.slots, torch.cat([slots_of(c, 0, 19)[17:], slots_of(c, 1, 5)]))
+    c.advance(again)
+    c.reserve([1, 1, 1])
+    step = c.plan_step()
+    assert step.positions.tolist() == [19, 5, 1] and step.lengths.tolist() == [20, 6, 2]
+    assert step.slots.tolist() == [int(slots_of(c, b, n)[-1]) for b, n in enumerate((20, 6, 2))]
+
+
+def test_a_full_sequence_has_no_slot_for_a_step():
+    c = cache(2, 16)
+    c.reserve([16, 3])
+    c.advance([16, 3])
+    assert c.plan_step().slots[0] == -1 and c.plan_step().slots[1] >= 0
+    c.block_table.fill_(-1)                                   # no pages: nothing is written
+    assert c.plan_step().slots.tolist() == [-1, -1]
+
+
+def test_a_cache_refuses_what_does_not_fit_and_takes_pages_back():
+    c = cache(3, 40, num_pages=4)
+    for bad in ([41, 0, 0], [1, 1], [-1, 0, 0], [17, 17, 16]):
+        with pytest.raises(ValueError, match="PagedKVCache"):
+            c.reserve(bad)
+        assert len(c._free) == 4 and (c.block_table == -1).all()
+    c.reserve([17, 16, 1])
+    c.advance([17, 16, 1])
+    assert not c._free
+    with pytest.raises(ValueError, match="are free"):
+        c.reserve([0, 1, 0])
+    held = set(c.block_table[0, :2].tolist())
+    c.clear(0)
+    assert set(c._free) == held and c.seq_lens == [0, 16, 1] == c.lengths.tolist() and (c.block_table[0] == -1).all()
+    c.reserve([0, 1, 0])
+    c.clear()
+    assert sorted(c._free) == [0, 1, 2, 3] and c.seq_lens == [0, 0, 0]
+
+
+def test_models_that_a_paged_cache_does_not_fit():
+    from smlm_hip.model import ModelConfig, Transformer
+    m = Transformer(ModelConfig(vocab_size=64, d_model=64, n_layers=1, n_heads=2, ffn_hidden=64, max_seq_len=32))
+    with pytest.raises(ValueError, match="bf16"):             # on the CPU
+        m.prefill(m.paged_cache(1), [torch.tensor([1, 2])])
+    with pytest.raises(ValueError, match="max_len"):
+        m.paged_cache(1, 33)

@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs A, KVPages P) {
     if (store) *(uint4 *)((uint16_t *)(is_v ? P.v : P.k) + at * HD + 8 * c) = packed;
   } else {
 #pragma clang fp contract(off)
+    if (is_q) return;   // whole heads: the lanes of a row stay together
     float lo = x[0], hi = x[0];
     bool finite = true;
 #pragma unroll
@@ -146,11 +147,24 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs A, KVPages P) {
     hi = group_extreme<L, true>(finite ? hi : __builtin_inff());
     lo = round_bf16_hw(lo);
     const float step = round_bf16_hw((hi - lo) * (1.0f / 15.0f));
+    // A reciprocal gives a quotient of up to 16 within 2^-18: it rounds to another code than the quotient
+    // itself only within 2^-16 of halfway, and there the division is done.
     uint32_t codes = 0;
     if (step > 0.f) {
+      const float inv = 1.0f / step;
+      float away = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        codes |= (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) << (4 * i);
+      for (int i = 0; i < 8; ++i) {
+        const float t = (x[i] - lo) * inv, near = rintf(t);
+        away = fmaxf(away, fabsf(t - near));
+        codes |= (uint32_t)fminf(fmaxf(near, 0.f), 15.f) << (4 * i);
+      }
+      if (!(away < 0.5f - 0x1p-16f && inv > 0x1p-125f && inv < 0x1p125f)) {
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          codes |= (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / step), 0.f), 15.f) << (4 * i);
+      }
     }
     if (store) {
       ((uint32_t *)(is_v ? P.v : P.k))[at * L + c] = codes;

@@ -650,6 +650,14 @@ int smlm_paged_append(const void *qkv, int64_t qkv_row_stride, const void *rope_
                       int64_t rope_len, int rot, int interleaved, const int64_t *positions, const int64_t *slots,
                       const smlm_kv_pages *pages, int64_t N, int H, void *q_out, void *k_out, void *stream);
 
+/*
+ * Where the next token of each of B sequences goes: position lengths[b], slot block_table[b, lengths[b] / page_size] * page_size
+ * + lengths[b] % page_size (-1 where that page's id is negative, at max_len and beyond the M pages), and lengths[b] + 1 tokens
+ * with it; lengths (B,) int32 as they were.  block_table row b at block_table + b * row_stride.
+ */
+int smlm_paged_step(const int *block_table, int64_t row_stride, int64_t M, const int *lengths, int64_t B, int page_size,
+                    int64_t max_len, int64_t *positions, int64_t *slots, int *next, void *stream);
+
 /* The rows of slots (N,) int64 as k_out, v_out (N, kv_heads, head_dim) bf16 (zeros for a slot outside the pages). */
 int smlm_paged_gather(const smlm_kv_pages *pages, const int64_t *slots, int64_t N, void *k_out, void *v_out, void *stream);
 

@@ -204,6 +204,17 @@ __global__ void __launch_bounds__(256) gather_kernel(KVPages P, const int64_t *s
   *(uint4 *)(v_out + (int64_t)row * HD + 8 * c) = v;
 }
 
+__global__ void __launch_bounds__(256) step_kernel(const int *table, int64_t row_stride, int64_t M, const int *lengths, int64_t B,
+                                                   int shift, int64_t max_len, int64_t *positions, int64_t *slots, int *next) {
+  const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int n = lengths[b], at = n >> shift;
+  const int page = n >= 0 && n < max_len && at < M ? table[b * row_stride + at] : -1;
+  positions[b] = n;
+  slots[b] = page < 0 ? -1 : ((int64_t)page << shift) + (n & ((1 << shift) - 1));
+  next[b] = n < 0x7FFFFFFF ? n + 1 : n;
+}
+
 }  // namespace
 
 int kv_pages(const char *name, const smlm_kv_pages *p, KVPages *out) {
@@ -268,6 +279,26 @@ extern "C" int smlm_paged_append(const void *qkv, int64_t qkv_row_stride, const 
   else if (hd == 64) { SMLM_APPEND(64); }
   else { SMLM_APPEND(128); }
 #undef SMLM_APPEND
+  return launch_status(name);
+}
+
+extern "C" int smlm_paged_step(const int *block_table, int64_t row_stride, int64_t M, const int *lengths, int64_t B, int page_size,
+                               int64_t max_len, int64_t *positions, int64_t *slots, int *next, void *stream) {
+  using namespace smlm;
+  const char *name = "smlm_paged_step";
+  if (!block_table || !lengths || !positions || !slots || !next) return fail(SMLM_EINVAL, "%s: null pointer argument", name);
+  if (!is_pow2(page_size) || page_size < 16 || page_size > 4096)
+    return fail(SMLM_EUNSUPPORTED, "%s: page size %d is not a power of two from 16 to 4096", name, page_size);
+  if (B < 0 || B > 0x7FFFFFFF || M < 1 || row_stride < M || max_len < 0)
+    return fail(SMLM_EINVAL, "%s: bad shape B=%lld M=%lld row_stride=%lld max_len=%lld", name, (long long)B, (long long)M,
+                (long long)row_stride, (long long)max_len);
+  if (((uintptr_t)block_table | (uintptr_t)lengths | (uintptr_t)next) % 4 || ((uintptr_t)positions | (uintptr_t)slots) % 8)
+    return fail(SMLM_EINVAL, "%s: misaligned pointer", name);
+  if (B == 0) return SMLM_OK;
+  int shift = 0;
+  while (1 << shift < page_size) ++shift;
+  hipLaunchKernelGGL(step_kernel, dim3((unsigned)((B + 255) / 256)), dim3(256), 0, (hipStream_t)stream, block_table, row_stride, M,
+                     lengths, B, shift, max_len, positions, slots, next);
   return launch_status(name);
 }
 

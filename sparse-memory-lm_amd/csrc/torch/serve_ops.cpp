@@ -1,4 +1,4 @@
-// The operators of serving sequences of different lengths (smlm_hip.kernels.paged_append, paged_gather, packed_attention,
+// The operators of serving sequences of different lengths (smlm_hip.kernels.paged_append, paged_step, paged_gather, packed_attention,
 // paged_attention and sample_tokens): argument checks, outputs and workspaces from torch's allocator, and the C entry points of
 // include/smlm_pkm.h on torch's current stream of the inputs' device.  Forward only.
 //
@@ -87,6 +87,27 @@ std::tuple<Tensor, std::optional<Tensor>> paged_append(const Tensor &qkv, const 
                           (int)n_heads, q.data_ptr(), keys ? k->data_ptr() : nullptr, stream_of(qkv)),
         "smlm_paged_append");
   return {q, k};
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_step(const Tensor &block_table, const Tensor &lengths, int64_t page_size,
+                                              int64_t max_len) {
+  const char *name = "paged_step";
+  check_device(name, block_table, {&lengths});
+  const c10::DeviceGuard guard(block_table.device());
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && block_table.scalar_type() == at::kInt && lengths.dim() == 1 &&
+                        lengths.scalar_type() == at::kInt && lengths.size(0) == block_table.size(0) && block_table.size(1) >= 1,
+                    name, ": expected block_table (sequences, pages) and lengths (sequences,) int32, got ", block_table.sizes(), " ",
+                    block_table.scalar_type(), " and ", lengths.sizes(), " ", lengths.scalar_type());
+  TORCH_CHECK_VALUE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0 && max_len >= 0, name,
+                    ": a page holds a power of two from 16 to 4096 tokens, got ", page_size, ", and max_len ", max_len);
+  const Tensor table = block_table.contiguous(), len = lengths.contiguous();
+  const int64_t B = table.size(0);
+  Tensor positions = at::empty({B}, len.options().dtype(at::kLong)), slots = at::empty_like(positions), next = at::empty_like(len);
+  if (B)
+    check(smlm_paged_step(table.data_ptr<int>(), table.size(1), table.size(1), len.data_ptr<int>(), B, (int)page_size, max_len,
+                          positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(), next.data_ptr<int>(), stream_of(block_table)),
+          "smlm_paged_step");
+  return {positions, slots, next};
 }
 
 std::tuple<Tensor, Tensor> paged_gather(const std::vector<Tensor> &pages, const Tensor &slots) {
@@ -232,6 +253,7 @@ Tensor sample_tokens(const Tensor &logits, const Tensor &u, const py::object &te
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_append", &paged_append);
+  m.def("paged_step", &paged_step);
   m.def("paged_gather", &paged_gather);
   m.def("packed_attention", &packed_attention);
   m.def("paged_attention", &paged_attention);

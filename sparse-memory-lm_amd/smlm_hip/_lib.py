@@ -99,6 +99,7 @@ EXPORTS = {
     "smlm_rmsnorm_parts": (_i64, [_i64, _i64]),
     "smlm_rmsnorm_train_backward": (_i, [_p, _p, _i, _p, _i, _p, _i, _p, _i64, _i64, _p, _p, _i, _p, _p, _p]),
     "smlm_paged_append": (_i, [_p, _i64, _p, _p, _i, _i64, _i, _i, _p, _p, ctypes.POINTER(KVPages), _i64, _i, _p, _p, _p]),
+    "smlm_paged_step": (_i, [_p, _i64, _i64, _p, _i64, _i, _i64, _p, _p, _p, _p]),
     "smlm_paged_gather": (_i, [ctypes.POINTER(KVPages), _p, _i64, _p, _p, _p]),
     "smlm_packed_attention": (_i, [_p] * 8 + [_i64] * 3 + [_i] * 3 + [_f, _p, _p, _i, _p]),
     "smlm_paged_attention_workspace": (_i64, [_i64, _i, _i, _i, _i, _i64]),

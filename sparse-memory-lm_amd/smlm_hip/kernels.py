@@ -1228,6 +1228,13 @@ def paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, inte
     return _lib.serve_ops().paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, interleaved, keys)
 
 
+def paged_step(block_table, lengths, page_size, max_len):
+    """Where the next token of every sequence goes, in one launch (smlm_paged_step): positions (B,) int64 = lengths, slots (B,)
+    int64 in pages of page_size tokens through block_table (B, pages of a sequence) int32 (-1 where the page's id is negative
+    and from max_len on), and lengths + 1 (B,) int32.  lengths (B,) int32 stay as they are."""
+    return _lib.serve_ops().paged_step(block_table, lengths, page_size, max_len)
+
+
 def paged_gather(pages, slots):
     """The keys and values of slots (N,) int64 as (N, n_kv_heads, head_dim) bf16 each: what packed_attention reads where a
     prompt goes on behind a cached beginning.  Zeros for a slot outside the pages.  (smlm_paged_gather)"""

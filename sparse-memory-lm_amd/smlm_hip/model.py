@@ -729,6 +729,10 @@ class Transformer(nn.Module):
         state["u"][:new_tokens + 1].copy_(u)
         state["tok"].copy_(first.unsqueeze(1))
         state["at"].fill_(1)
+        if not _FusedDecodeStep.supported(self, torch.bfloat16):
+            state["fused"] = None
+        elif state["fused"] is None or state["fused"]._model() is not self:
+            state["fused"] = _FusedDecodeStep(self)
         if use_graph and new_tokens:
             graph = self._ragged_graph(cache, state)
             for _ in range(new_tokens):
@@ -744,8 +748,8 @@ class Transformer(nn.Module):
         if "tok" not in cache.decoding:
             B, n, dev = cache.n_seqs, cache.max_len + 1, cache.device
             new = lambda *shape, dtype: torch.zeros(*shape, dtype=dtype, device=dev)  # noqa: E731
-            cache.decoding.update(tok=new(B, 1, dtype=torch.long), out=new(B, n, dtype=torch.long), at=new(1, dtype=torch.long),
-                                  u=new(n, B, dtype=torch.float32),
+            cache.decoding.update(fused=None, tok=new(B, 1, dtype=torch.long), out=new(B, n, dtype=torch.long),
+                                  at=new(1, dtype=torch.long), u=new(n, B, dtype=torch.float32),
                                   settings=tuple(new(B, dtype=t) for t in (torch.float32, torch.int32, torch.float32, torch.float32)))
         return cache.decoding
 
@@ -753,7 +757,11 @@ class Transformer(nn.Module):
         """One token for every sequence, from and to the device's state."""
         cache.plan = cache.plan_step()
         try:
-            logits = self.lm_head(self._hidden(state["tok"], cache.layers, 0))[:, 0]
+            if state["fused"] is not None:
+                attend = lambda i, qkv: self.layers[i].attn._paged(qkv, cache.layers[i]).flatten(1)  # noqa: E731
+                logits = state["fused"].run(state["tok"], None, None, None, logits=True, attend=attend)
+            else:
+                logits = self.lm_head(self._hidden(state["tok"], cache.layers, 0))[:, 0]
         finally:
             cache.plan = None
         cache.lengths.add_(1)
@@ -765,7 +773,7 @@ class Transformer(nn.Module):
     def _ragged_graph(self, cache, state):
         """The captured step of this cache, captured again where the model has changed since; the cache is left as it was."""
         ac = torch.is_autocast_enabled("cuda")
-        key = (self._replaced, state_tag(self.state_tensors()), ac)
+        key = (self._replaced, state_tag(self.state_tensors()), ac, state["fused"])      # the step itself: it owns weights that the graph reads
         if state.get("graph_of", lambda: None)() is not self or state["graph_key"] != key:
             ctx = (torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False) if ac
                    else torch.autocast("cuda", enabled=False))
@@ -901,7 +909,7 @@ class _FusedDecodeStep(_KeptByModel):
                 self.mem[i] = (w, b)
         self._tag = self._params_tag()
 
-    def run(self, tok, pos, caches, hist, logits=False, record=None, chain=None):
+    def run(self, tok, pos, caches, hist, logits=False, record=None, chain=None, attend=None):
         """The step for tok (B, 1) at device position pos: writes the next token to tok and hist[:, pos + 1] and
         advances pos.  With logits=True it returns the (B, vocab) bf16 logits instead and changes none of tok,
         hist and pos (the KV caches get the same slot written).  With a dict `record`, record[layer] holds each
@@ -912,7 +920,12 @@ class _FusedDecodeStep(_KeptByModel):
         With `chain` ((B, >= argmax blocks) int64 argmax keys, even row stride; not with logits) the step's token
         is the greedy choice from the keys the previous chained step left in chain (or that _StepDecoder seeded):
         the first launch writes it to tok and hist[:, pos]; the step then leaves its own keys in chain and advances
-        pos.  The next token reaches tok and hist in the next chained step (or in _StepDecoder.finish)."""
+        pos.  The next token reaches tok and hist in the next chained step (or in _StepDecoder.finish).
+
+        With `attend`, attend(layer, qkv) is the attention of each layer (B, d_model) over a cache of its own, and pos, caches
+        and hist are not used (with logits only)."""
+        if attend is not None and not logits:
+            raise ValueError("run: a step with its own attention ends with logits")
         if chain is not None and logits:
             raise ValueError("run: a chained step ends with argmax keys, not logits")
         model = self.model
@@ -931,7 +944,9 @@ class _FusedDecodeStep(_KeptByModel):
                                                norm=blk.attn_norm, write_x=True)
             else:
                 x, qkv = kernels.decode_linear(at.wqkv.weight, x, delta=delta, norm=blk.attn_norm, write_x=True)
-            if proj:
+            if attend is not None:
+                delta = kernels.decode_linear(at.wo.weight, attend(i, qkv))
+            elif proj:
                 delta = kernels.decode_attention_proj(qkv, at.rope.cos, at.rope.sin, pos, caches[i].k, caches[i].v,
                                                       at.wo.weight)
             else:

@@ -106,6 +106,9 @@ class PagedKVCache:
 
     def plan_step(self):
         """The plan of a pass over one more token of every sequence, from the device's lengths (which a captured step advances)."""
+        if self.lengths.is_cuda:
+            positions, slots, lengths = kernels.paged_step(self.block_table, self.lengths, self.page_size, self.max_len)
+            return StepPlan(positions, slots, self.block_table, lengths)
         pos = self.lengths.long()
         page = self.block_table.gather(1, (pos // self.page_size).clamp_(max=self.block_table.shape[1] - 1).unsqueeze(1)).squeeze(1)
         # a sequence at its end has no slot: nothing is written

@@ -140,6 +140,24 @@ def test_append_of_rows_without_spread_or_not_finite_in_4_bits():
     assert torch.isfinite(v[5]).all()
 
 
+@pytest.mark.parametrize("B", [1, 300])
+def test_where_the_next_tokens_go(B):
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, 90, (B,), generator=g, dtype=torch.int32)
+    lengths[0], lengths[-1] = 0, 79
+    table = torch.randint(0, 1 << 30, (B, 7), generator=g, dtype=torch.int32)[:, :5]
+    table[::3, 2] = -1
+    before = lengths.clone()
+    got = K.paged_step(table.to(DEV), lengths.to(DEV), 16, 75)
+    pos = lengths.long()
+    page = table.long().gather(1, (pos // 16).clamp(max=4).unsqueeze(1)).squeeze(1)
+    want = torch.where((page >= 0) & (pos < 75), page * 16 + pos % 16, -1)
+    for a, b in zip(got, (pos, want, before + 1)):
+        assert a.dtype == b.dtype and torch.equal(a.cpu(), b)
+    edge = torch.tensor([-1, 2 ** 31 - 1], dtype=torch.int32, device=DEV)       # no tokens there are: no slot
+    assert K.paged_step(torch.zeros(2, 4, dtype=torch.int32, device=DEV), edge, 16, 2 ** 40)[1].tolist() == [-1, -1]
+
+
 # --------------------------------------------------------------------------------------------- packed prompt attention
 def packed(g, Tq, Sk, H, Hk, D, tail=0, head=0):
     """Packed inputs on the CPU, `head` and `tail` rows of no sequence around them."""

@@ -163,6 +163,34 @@ def test_graphs_follow_the_model():
     same(m)
 
 
+def test_another_models_steps_in_between_leave_the_graph_its_weights():
+    """A run of another model over the same cache without a graph, then the first one's graph again."""
+    m, n = model(), model(seed=9)
+    seqs = prompts([5, 17])
+    cache = m.paged_cache(2, 100)
+    want = m.generate_ragged(seqs, 8, cache)
+    cache.clear()
+    n.generate_ragged(seqs, 8, cache, use_graph=False)
+    torch.empty(1 << 20, device=DEV).fill_(float("nan"))
+    cache.clear()
+    assert torch.equal(m.generate_ragged(seqs, 8, cache), want)
+
+
+def test_a_model_that_the_fused_step_does_not_cover():
+    """A width above the fused step's; the tokens are the same with and without a graph, and the largest logits."""
+    m = model(mem=False, d_model=512, n_heads=8)
+    ref = copy.deepcopy(m).float()
+    seqs = prompts([5, 40])
+    out = m.generate_ragged(seqs, 6)
+    assert torch.equal(out, m.generate_ragged(seqs, 6, use_graph=False))
+    with torch.no_grad():
+        for p, tokens in zip(seqs, out.cpu()):
+            logits = whole(ref, torch.cat([p, tokens[:-1]]))[len(p) - 1:].cpu()
+            took = logits.gather(1, tokens.unsqueeze(1)).squeeze(1)
+            slack = 2 * NEAR["bf16"] * logits.norm(dim=1) / logits.shape[1] ** 0.5 * 4
+            assert (logits.max(1).values - took <= slack).all()
+
+
 def test_autocast():
     m = model(torch.float32)
     seqs = prompts([30, 3])

@@ -58,6 +58,19 @@ def test_paged_gather_refusals():
     assert call(N=-1) == _lib.EINVAL and call(N=1 << 28) == _lib.EUNSUPPORTED and call(N=0) == _lib.OK
 
 
+def test_paged_step_refusals():
+    def call(**kw):
+        return _lib.lib().smlm_paged_step(*dict(dict(table=FAKE, stride=7, M=5, lengths=FAKE, B=3, page=16, max_len=75, pos=FAKE,
+                                                     slots=FAKE, next=FAKE), **kw).values(), None)
+
+    for name in ("table", "lengths", "pos", "slots", "next"):
+        assert call(**{name: None}) == call(**{name: FAKE + 2}) == _lib.EINVAL, name
+    assert call(page=8) == call(page=24) == call(page=8192) == _lib.EUNSUPPORTED
+    assert call(stride=4) == call(M=0) == call(B=-1) == call(max_len=-1) == call(B=1 << 31) == _lib.EINVAL and call(B=0) == _lib.OK
+    with pytest.raises(ValueError, match="must be on a HIP"):
+        kernels.paged_step(torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 16, 32)
+
+
 def two(a, b):
     return (ctypes.c_int64 * 2)(a, b)
 

@@ -670,7 +670,7 @@ int smlm_paged_gather(const smlm_kv_pages *pages, const int64_t *slots, int64_t 
  * give unspecified results within the buffers).  Rows of no sequence are left as they are, or zeroed (zero_rest).  bf16 in
  * and out, fp32 scores, statistics and sums, probabilities rounded to bf16; masked keys and values count for nothing,
  * whatever they hold.  head_dim in {32, 64, 128}; q, k, v 16-byte aligned with strides that are multiples of 8 up to 2^22; y
- * 8-byte aligned, strides multiples of 4.
+ * 8-byte aligned, strides multiples of 4.  0 < scale <= 1e38.
  */
 int smlm_packed_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
                           const int64_t *v_strides, const int *cu_q, const int *cu_k, int64_t B, int64_t N, int64_t S, int H,
@@ -683,7 +683,8 @@ int smlm_packed_attention(const void *q, const int64_t *q_strides, const void *k
  * block_table[b * table_row_stride + t / page_size] (int32, max_pages a sequence); lengths beyond the table count as its size.
  * A page id outside the pages holds no tokens.  y (B, H, head_dim) dense; zeros for a sequence without tokens.  fp32 scores,
  * statistics and sums, probabilities (4 bits: times the row's step) rounded to bf16.  What lies behind a sequence's last token
- * counts for nothing.  workspace: smlm_paged_attention_workspace bytes (may be 0), 16-byte aligned.
+ * counts for nothing.  0 < scale <= 1e38; over 4-bit pages the queries are below 2^100.  workspace:
+ * smlm_paged_attention_workspace bytes (may be 0), 16-byte aligned.
  */
 int64_t smlm_paged_attention_workspace(int64_t B, int H, int kv_heads, int head_dim, int page_size, int64_t max_pages);
 int smlm_paged_attention(const void *q, int64_t q_row_stride, const smlm_kv_pages *pages, const int *block_table,

@@ -23,8 +23,6 @@
 // A masked key weighs exactly nothing, also where its value is an infinity or a NaN (0 times which is NaN): masked tiles sum
 // their values' columns, and where a sum is not finite the values that are not are left out of the products and added key by key,
 // for the queries that see the key.  So a query's result depends, to the bit, on nothing but what it sees.
-#include <algorithm>
-
 #include "lm_mm.h"
 
 namespace smlm {
@@ -397,7 +395,7 @@ extern "C" int smlm_packed_attention(const void *q, const int64_t *q_strides, co
                     (long long)st[a][i]);
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || (uintptr_t)y % 8 || ((uintptr_t)cu_q | (uintptr_t)cu_k) % 4)
     return fail(SMLM_EINVAL, "%s: q, k, v must be 16-byte and y 8-byte aligned", name);
-  if (!(scale > 0.f) || scale > 3e38f) return fail(SMLM_EINVAL, "%s: the scale must be positive and finite", name);
+  if (!(scale > 0.f) || scale > 1e38f) return fail(SMLM_EINVAL, "%s: the scale must be positive, at most 1e38", name);
   if (N == 0 || (B == 0 && !zero_rest)) return SMLM_OK;
   const PackedArgs A{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, (uint16_t *)y, q_strides[0], q_strides[1],
                      k_strides[0], k_strides[1], v_strides[0], v_strides[1], y_strides[0], y_strides[1], cu_q, cu_k, (int)N,

@@ -11,8 +11,6 @@
 // read consecutive 16-byte pieces of the projection's row.  In the half layout a lane also loads its partner's piece, which the
 // partner loads too (the second read hits the L1); so no lane exchange is needed, and a row's minimum and maximum are a
 // reduction over HD / 8 lanes.
-#include <algorithm>
-
 #include "lm_paged.h"
 
 namespace smlm {

@@ -487,7 +487,7 @@ extern "C" int smlm_paged_attention(const void *q, int64_t q_row_stride, const s
   if (q_row_stride < (int64_t)H * hd || q_row_stride % 8 || ((uintptr_t)q | (uintptr_t)y) % 16 ||
       ((uintptr_t)block_table | (uintptr_t)lengths) % 4)
     return fail(SMLM_EINVAL, "%s: q and y must be 16-byte aligned, q's row stride >= H * head_dim and a multiple of 8", name);
-  if (!(scale > 0.f) || scale > 3e38f) return fail(SMLM_EINVAL, "%s: the scale must be positive and finite", name);
+  if (!(scale > 0.f) || scale > 1e38f) return fail(SMLM_EINVAL, "%s: the scale must be positive, at most 1e38", name);
   if (max_pages * pages->page_size > 0x7FFFFF00LL)
     return fail(SMLM_EUNSUPPORTED, "%s: a block table of %lld pages is more than 2^31 tokens", name, (long long)max_pages);
   const int G = H / pages->kv_heads, groups = (G + 15) / 16;

@@ -695,7 +695,7 @@ class Transformer(nn.Module):
         dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
         if not w.is_cuda or dtype != torch.bfloat16 or cache.device != w.device:
             raise ValueError(f"the paged cache is for bf16 models (or bf16 autocast) on its own GPU, got {dtype} on {w.device}")
-        if len(cache.layers) != len(self.layers):
+        if self.ngram is not None or len(cache.layers) != len(self.layers):
             raise ValueError(f"a cache of {len(cache.layers)} layers for a model of {len(self.layers)}")
 
     @torch.no_grad()
@@ -707,7 +707,7 @@ class Transformer(nn.Module):
         Returns the ids (n_seqs, new_tokens + 1): the prompts' next tokens, then one per step; all but the last are in the
         cache afterwards, which a later call may go on from.  Every sequence needs a prompt.  With use_graph a step is one
         replay of a captured graph, kept by the cache."""
-        prompts = list(prompts)
+        prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
         if cache is None:
             longest = max((len(p) for p in prompts), default=0) + new_tokens
             cache = self.paged_cache(max(1, len(prompts)), max(1, longest))
@@ -723,23 +723,24 @@ class Transformer(nn.Module):
         u = torch.rand(new_tokens + 1, B, generator=generator, device=dev if generator is None else generator.device).to(dev)
         cache.reserve([len(p) + new_tokens for p in prompts])
         first = kernels.sample_tokens(self.prefill(cache, prompts), u[0], *settings)
-        state = self._ragged_state(cache)
-        for buffer, value in zip(state["settings"], settings):
-            buffer.copy_(value)
-        state["u"][:new_tokens + 1].copy_(u)
-        state["tok"].copy_(first.unsqueeze(1))
-        state["at"].fill_(1)
-        if not _FusedDecodeStep.supported(self, torch.bfloat16):
-            state["fused"] = None
-        elif state["fused"] is None or state["fused"]._model() is not self:
-            state["fused"] = _FusedDecodeStep(self)
-        if use_graph and new_tokens:
-            graph = self._ragged_graph(cache, state)
-            for _ in range(new_tokens):
-                graph.replay()
-        else:
-            for _ in range(new_tokens):
-                self._ragged_step(cache, state)
+        with torch.cuda.device(dev):
+            state = self._ragged_state(cache)
+            for buffer, value in zip(state["settings"], settings):
+                buffer.copy_(value)
+            state["u"][:new_tokens + 1].copy_(u)
+            state["tok"].copy_(first.unsqueeze(1))
+            state["at"].fill_(1)
+            if not _FusedDecodeStep.supported(self, torch.bfloat16):
+                state["fused"] = None
+            elif state["fused"] is None or state["fused"]._model() is not self:
+                state["fused"] = _FusedDecodeStep(self)
+            if use_graph and new_tokens:
+                graph = self._ragged_graph(cache, state)
+                for _ in range(new_tokens):
+                    graph.replay()
+            else:
+                for _ in range(new_tokens):
+                    self._ragged_step(cache, state)
         cache.seq_lens = [n + new_tokens for n in cache.seq_lens]
         return torch.cat([first.unsqueeze(1), state["out"][:, 1:new_tokens + 1]], 1)
 

@@ -194,6 +194,33 @@ def test_packed_attention(Tq, Sk, H, Hk, D):
     close(y, want, R.bound_of(want, bound))
 
 
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 64), (16, 16, 32), (8, 1, 128)])
+def test_packed_attention_of_very_many_sequences(H, Hk, D):
+    """More sequences than their beginnings are kept for beside the tiles, and heads that are spread over the chip's parts."""
+    g = gen(H + D)
+    Tq = torch.randint(0, 4, (700,), generator=g).tolist() + [150, 1]
+    Sk = [n + more for n, more in zip(Tq, torch.randint(0, 3, (702,), generator=g).tolist())]
+    q, k, v, cu_q, cu_k = packed(g, Tq, Sk, H, Hk, D)
+    y = K.packed_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu_q.to(DEV), cu_k.to(DEV))
+    want, bound = packed_reference(q, k, v, cu_q, cu_k, D ** -0.5)
+    close(y, want, R.bound_of(want, bound))
+
+
+def test_packed_attention_of_rows_far_apart():
+    """Rows 2^22 elements apart, the last 2^31 and more from the first."""
+    g = gen(77)
+    D, stride = 64, 1 << 22
+    q, k, v, cu_q, cu_k = packed(g, [300, 220], [300, 220], 2, 1, D)
+    room = torch.empty(len(q) * stride, dtype=bf16, device=DEV)
+    far = []
+    for at, t in ((0, q), (256, k), (512, v)):
+        view = room.as_strided((len(t), t.shape[1], D), (stride, D, 1), at)
+        far.append(view.copy_(t))
+    y = room.as_strided(q.shape, (stride, D, 1), 1024).zero_()
+    assert K.packed_attention(*far, cu_q.to(DEV), out=y).data_ptr() == y.data_ptr()
+    assert torch.equal(y, K.packed_attention(*[t.to(DEV) for t in (q, k, v, cu_q)], out=torch.zeros_like(q, device=DEV)))
+
+
 def test_packed_attention_of_projection_rows_scaled_with_rows_of_no_sequence():
     """Values as a view of the projection's rows, keys with padded rows, a scale of its own, rows around the sequences."""
     g = gen(5)
@@ -338,6 +365,26 @@ def test_paged_attention_of_long_sequences(kind, lengths, H, Hk, D, page):
     y = K.paged_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.2)
     want, bound = paged_reference(q, pages, slots, 0.2)
     close(y, want, R.bound_of(want, bound))
+
+
+@pytest.mark.parametrize("kind,total", [("bf16", 4200), ("q4", 33800)])
+def test_pages_far_into_a_large_pool(kind, total):
+    """Tokens in the last pages of a pool whose values are 2^31 elements from its first, and those of a small pool."""
+    g = gen(total)
+    D, page, N = 128, 4096, 5000
+    cos, sin = (t.to(DEV) for t in tables(N, D))
+    qkv = randn(g, N, 4 * D).to(DEV)
+    pos = torch.arange(N, device=DEV)
+    got = []
+    for pool, ids in ((K.kv_pages(total, 1, page, D, kind, DEV), [total - 1, total - 2]), (K.kv_pages(2, 1, page, D, kind, DEV), [1, 0])):
+        table = torch.tensor([ids], dtype=torch.int32, device=DEV)
+        slots = table[0].long().repeat_interleave(page)[:N] * page + pos % page
+        q, _ = K.paged_append(qkv, cos, sin, pos, slots, pool, 2)
+        y = K.paged_attention(q[-1:], pool, table, torch.tensor([N], dtype=torch.int32, device=DEV))
+        got.append((q, y, *K.paged_gather(pool, slots)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert got[0][2].any() and got[0][1].any()
 
 
 @pytest.mark.parametrize("kind", ["bf16", "q4"])

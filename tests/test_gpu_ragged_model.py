@@ -202,6 +202,15 @@ def test_autocast():
         m.generate_ragged(seqs, 6)
 
 
+def test_prompts_of_any_shape():
+    """Lists and (1, tokens) tensors are the sequences that they hold."""
+    m = model()
+    seqs = prompts([70, 17])
+    want = m.generate_ragged(seqs, 5)
+    assert torch.equal(want, m.generate_ragged([p.unsqueeze(0) for p in seqs], 5))
+    assert torch.equal(want, m.generate_ragged([p.tolist() for p in seqs], 5))
+
+
 def test_refusals():
     m = model()
     seqs = prompts([5, 17])

@@ -6,14 +6,15 @@
 // Bound by the matrix and vector instructions together: per tile of 64 keys and 32 queries a wavefront has 36 matrix instructions
 // of 16 clocks (68 with a head dim of 128) and 32 exponentials of 16 clocks beside some 70 other vector instructions of 4, so
 // the two or three wavefronts of a SIMD overlap one kind with the other, matrix work first (s_setprio).  Measured on 8,192
-// tokens, 32 heads: 1,105 TFLOP/s with a head dim of 128 and 968 with 64; a library product of 8,192 cubed reaches 1,395.
+// tokens, 32 heads: 1,049 TFLOP/s with a head dim of 128 and 911 with 64; a library product of 8,192 cubed reaches 1,385.
 //
 // A workgroup owns 128 consecutive query rows of one head, whichever sequences they belong to, and walks the key rows from
 // the first one that any of them sees to the last: both ranges grow with the row, so they join up, and the grid follows from
-// the number of rows alone, without the lengths on the host; the last rows start first, and heads that share keys on one XCD (835 ->
-// 1,020 TFLOP/s on 6,001 and 5,000 tokens).  A lane finds its own query's range of keys by binary search in
-// cu_q; tiles that hold keys outside some query's range are masked, per query.  (Tiles of their own for every sequence need
-// the running sum of their tiles, and leave a part-filled tile per sequence.)
+// the number of rows alone, without the lengths on the host; the last rows start first, and heads that share keys on one XCD
+// (835 -> 1,020 TFLOP/s on 6,001 and 5,000 tokens).  A lane finds its own query's range of keys by binary search in cu_q; tiles
+// that hold keys outside some query's range are masked, per query.  (Tiles of their own for every sequence need the running sum
+// of their tiles, and leave a part-filled tile per sequence.  Rows taken by the length of their walks, for compute units that all
+// have long and short ones: 32 ragged prompts of 6 heads 62 -> 59 us, others 36 -> 37.)
 //
 // Products as in a causal prompt pass: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 with the keys as M, so a lane (r, g) holds keys
 // 4 g .. 4 g + 3 of each 16-key tile for ONE query (r), and the softmax is per lane; O^T = V^T P^T

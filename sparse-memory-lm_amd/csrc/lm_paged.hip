@@ -10,7 +10,9 @@
 // Bound by memory (every value read and written once).  One lane takes 8 dims of one row, 16 bytes of bf16: consecutive lanes
 // read consecutive 16-byte pieces of the projection's row.  In the half layout a lane also loads its partner's piece, which the
 // partner loads too (the second read hits the L1); so no lane exchange is needed, and a row's minimum and maximum are a
-// reduction over HD / 8 lanes.
+// reduction over HD / 8 lanes.  Measured, 6 heads of 64: 16 tokens 3 us (6 the whole call), 11,540 tokens 12 (4.6 TB/s).  32 and
+// 2 x 8 heads of 128 into 4 bits, 2,036 tokens: 12 us (query heads leave before the rounding to codes, whose quotients come
+// from a reciprocal: 15.6 without either); reading 17,134 tokens of them back as bf16 (gather) 17.7, 5.0 TB/s.
 #include "lm_paged.h"
 
 namespace smlm {

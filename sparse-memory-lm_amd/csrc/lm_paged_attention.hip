@@ -424,6 +424,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const float *parts, con
 // possible sequence: into 768 workgroups, three for each of the 256 compute units, all of them running at once (2 x 131,072
 // tokens in 4 bits: 65 us; 1,024 workgroups 77, 2,304 74), or, from 8 sequences on, whose lengths differ, into three times as
 // many, which even out (48 of up to 8,191: 768 workgroups 73 us, 2,304 68).
+// (Shares of equally many tiles, cut from the lengths on the device: 72 -> 70 us for these 48, 65 -> 61 for equal ones, but 10.5
+// -> 14.2 for 16 of 2,000 tokens, whose prefix sums and divisions take as long as their walk.)
 struct Plan {
   int waves, splits;
 };

@@ -11,11 +11,15 @@
 //
 // One workgroup of 1,024 a row, the row in LDS where it fits (a wavefront has a run of the vocabulary of its own, so that the
 // running mass is a sum over wavefronts, then over the found wavefront's vectors).  Bound by the passes over the row, vector
-// instructions all: a pass over 50,304 tokens costs 1.5 to 2 us, one with every token's weight 6, one that also adds it to a
-// histogram 10.  So the tokens that may be kept are listed first, where a bound on them is cheap -- top_k of at most 512: at
-// least that many tokens lie above the bin that holds the k-th largest of the threads' own maxima; min_p: a bound on the
-// logit -- and everything else is done on the list, of at most 512 tokens, by ranking each against all.  Else a cut, the
-// top_k-th token or the one at which the mass reaches top_p, is found by a histogram of 1,024 bins, then within its bin.
+// instructions all: of a bf16 row of 50,304, reading it and finding its maximum takes 7 us, a pass that compares 1.5 to 2, one
+// with every token's exact weight 12 (20 where it parts them at a cut), one that adds rough ones to a histogram 12.  So the tokens
+// that may be kept are listed first, where a bound on them is cheap -- top_k of at most 512: at least that many tokens lie above the bin that holds the k-th
+// largest of the threads' own maxima; min_p: a bound on the logit -- and everything else is done on the list, of at most 512
+// tokens, by ranking each against all.  Else a cut, the top_k-th token or the one at which the mass reaches top_p, is found by a
+// histogram of 1,024 bins, then within its bin.  One row, whole calls: the largest 10 us, no cut 23, top_k 50 with top_p 16,
+// min_p 0.1 13, top_p 0.9 alone 55 (reach), top_k 2,000 37; 256 rows 5 to 10% more, rows in memory that is not 16-byte aligned
+// 15 us more.  (Forming the weights' rough sum while the row is read took top_p alone from 59 to 54 us and top_p with min_p from
+// 25 to 27.)
 #include "pkm_common.h"
 
 namespace smlm {

@@ -31,6 +31,15 @@ The dense operators of a training step, differentiable (Transformer.loss calls t
                                              smlm/model.py:286-293 without logits)
     gated_ffn(x, w13, w2)                   (SwiGLU.forward, smlm/model.py:110-118)
     add_rmsnorm_train(x, delta, norm)       (residual add + RMSNorm, smlm/model.py:156-163)
+
+Serving sequences of different lengths (Transformer.prefill and generate_ragged call them; all new):
+    kv_pages(num_pages, n_kv_heads, page_size, head_dim, kind)    empty cache pages in bf16 or 4 bits
+    paged_append(qkv, cos, sin, positions, slots, pages, n_heads) rotation, keys and values into their pages
+    paged_step(block_table, lengths, page_size, max_len)          where the next token of every sequence goes
+    paged_gather(pages, slots)                                    keys and values read back
+    packed_attention(q, k, v, cu_q, cu_k)   causal attention of prompts in a row, grouped heads (smlm/model.py:97-105)
+    paged_attention(q, pages, block_table, lengths)               one query token per sequence over its pages
+    sample_tokens(logits, u, temperature, top_k, top_p, min_p)    tokens drawn by given random numbers
 """
 import ctypes
 import math

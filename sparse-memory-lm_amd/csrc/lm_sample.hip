@@ -6,20 +6,24 @@
 //
 // Masses are whole numbers of 2^-45 of the largest weight, from weights in fp64: a sum is exact whatever its order, so every
 // call gives the same token, and one that lies within rounding of its neighbour's border is as rare as in fp64 (fp32 sums over
-// 50,000 tokens would give another token once in some hundred calls).  exp2 by a table of 2^(i / 16), which the banks serve
-// without conflicts, and a polynomial of degree 7: with |r| <= ln 2 / 32 the next term is r^8 / 40320 < 2e-18.
+// 50,000 tokens would give another token once in some hundred calls).  exp2 by a table of 2^(i / 64) and a
+// polynomial of degree 5: with |r| <= ln 2 / 128 the next term is r^6 / 720 < 4e-17.
 //
 // One workgroup of 1,024 a row, the row in LDS where it fits (a wavefront has a run of the vocabulary of its own, so that the
 // running mass is a sum over wavefronts, then over the found wavefront's vectors).  Bound by the passes over the row, vector
 // instructions all: of a bf16 row of 50,304, reading it and finding its maximum takes 7 us, a pass that compares 1.5 to 2, one
 // with every token's exact weight 12 (20 where it parts them at a cut), one that adds rough ones to a histogram 12.  So the tokens
-// that may be kept are listed first, where a bound on them is cheap -- top_k of at most 512: at least that many tokens lie above the bin that holds the k-th
-// largest of the threads' own maxima; min_p: a bound on the logit -- and everything else is done on the list, of at most 512
-// tokens, by ranking each against all.  Else a cut, the top_k-th token or the one at which the mass reaches top_p, is found by a
-// histogram of 1,024 bins, then within its bin.  One row, whole calls: the largest 10 us, no cut 23, top_k 50 with top_p 16,
-// min_p 0.1 13, top_p 0.9 alone 55 (reach), top_k 2,000 37; 256 rows 5 to 10% more, rows in memory that is not 16-byte aligned
-// 15 us more.  (Forming the weights' rough sum while the row is read took top_p alone from 59 to 54 us and top_p with min_p from
-// 25 to 27.)
+// that may be kept are listed first, where a bound on them is cheap -- top_k: at least that many tokens lie above the bin that
+// holds the k-th largest of the threads' own maxima; min_p: a bound on the logit -- and everything else is done on the list, by ranking
+// each of its 512 tokens at most against all (256 of a bf16 row: 256 rows with min_p 0.01 and top_p 46 us with more, 42 so).
+// Else a cut, the top_k-th token or the one at which the mass reaches top_p, is found in a bf16 row by counting its distinct
+// values, in an fp32 row by a histogram of 1,024 bins, then within its bin.  One row, whole calls: the largest 10 us, no cut 23,
+// top_k 50 with top_p 16, min_p 0.1 13, top_p 0.9 alone 37 by distinct values (55 by the histogram, as in fp32), top_k 2,000 with
+// top_p 36 (57); 256 rows 5 to 15% more, rows in memory that is not 16-byte aligned 15 us more.  (Forming the weights' rough sum
+// while the row is read took top_p alone from 59 to 54 us and top_p with min_p from 25 to 27; masses looked up per distinct value
+// instead of formed per token, 23 to 33 us without a cut.)
+#include <cstddef>
+
 #include "pkm_common.h"
 
 namespace smlm {
@@ -174,6 +178,12 @@ struct Row {
       vec(j, raw, [&](float x, int i) { f(x, i, (bits >> (i - at) & 1) != 0); });
       return;
     }
+    each_bit(j, raw, bits, f);
+  }
+  // f(x, index, whether it is one) for the elements of vector j that have a bit
+  template <class F>
+  __device__ __forceinline__ void each_bit(int j, const uint4 &raw, uint32_t bits, F &&f) const {
+    const int at = (first + 64 * j) * W;
     while (__builtin_amdgcn_ballot_w64(bits != 0)) {
       const int e = bits ? __builtin_ctz(bits) : 0, word = BF16 ? e >> 1 : e;
       uint32_t w = raw.x;
@@ -325,7 +335,8 @@ struct ByIndex {
 
 // The cut after the k-th kept token (MASS false), or after the one at which the mass reaches `share` of the kept mass.
 template <bool MASS, class R>
-__device__ Cut select(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom, uint32_t k, double share) {
+__device__ __forceinline__ Cut select(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom,
+                                          uint32_t k, double share) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   uint32_t lo = code_of(fmaxf(bottom, cut.value)), hi = code_of(top), above = 0;
   uint64_t mass_above = 0;
@@ -426,8 +437,8 @@ __device__ Cut select(const R &row, const Weight &weight, Shared &S, const Cut c
 // tokens above the cut's bin, and S.wave_kept, by wavefront, of those in it.  The bin is found from weights in fp32, and then
 // its borders' masses are checked exactly: false where they do not hold the cut, or the bin holds more than the list.
 template <class R>
-__device__ bool reach(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom, double share, double scale,
-                      Cut &got, uint64_t &sum) {
+__device__ __forceinline__ bool reach(const R &row, const Weight &weight, Shared &S, const Cut cut, float top, float bottom,
+                                      double share, double scale, Cut &got, uint64_t &sum) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const Bins bins(code_of(fmaxf(bottom, cut.value)), code_of(top), true);
   const float s32 = (float)scale;
@@ -513,6 +524,134 @@ __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
   return target < total ? target : total - 1;
 }
 
+// The distinct values of a bf16 row, from the largest down: kSide magnitudes below the largest one of either sign, and all that is
+// nearer to zero as one in the middle (at 3,200, 25 binades, mostly zeros; at 1,088 a cut fell there in one row of 20).
+constexpr int kSide = 3200, kCodes = 2 * kSide + 1;
+struct Codes {
+  uint32_t most;                       // the largest magnitude's bits, of the tokens from `low` on
+  float low;                           // no token below it has a mass
+  __device__ __forceinline__ Codes(float top, float low_) : low(low_) {
+    most = max(__float_as_uint(fabsf(top)) >> 16, (__float_as_uint(fabsf(low_)) + 0xFFFFu) >> 16);
+  }
+  // (of a value outside low .. top: some code)
+  __device__ __forceinline__ int of(float x) const {
+    const uint32_t h = __float_as_uint(x) >> 16, d = most - (h & 0x7FFFu);
+    return d < (uint32_t)kSide ? (int)(h > 0x8000u ? kCodes - 1 - d : d) : kSide;
+  }
+  __device__ __forceinline__ float value(int code) const {
+    const uint32_t d = code < kSide ? code : kCodes - 1 - code, mag = most - d;
+    return d > most || code == kSide ? -__builtin_inff() : __uint_as_float(mag << 16 | (code > kSide ? 0x80000000u : 0u));
+  }
+};
+
+// The cut of top_k and top_p in a bf16 row: weights are formed once per distinct value, of which a row of 50,000 tokens has some
+// 2,000, and summed by counts.  Tokens in the middle, a hundredth of them, have theirs formed one by one.  False where a cut lies
+// among these, or more tokens than a list holds have the cut's value.
+template <class R>
+__device__ __forceinline__ bool cut_by_codes(const R &row, const Weight &weight, Shared &S, float top, float bottom,
+                                             uint32_t top_k, double share, double scale, Cut &got) {
+  static_assert(offsetof(Shared, wave_mass) - offsetof(Shared, mass) >= kCodes * sizeof(uint32_t));
+  uint32_t *count = (uint32_t *)S.mass;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  constexpr int W = R::W, EACH = (kCodes + kThreads - 1) / kThreads;
+  const Codes codes(top, fmaxf(bottom, (float)fmax((double)kLowest, (double)top - 47.5 / scale)));
+  __syncthreads();
+  for (int i = tid; i < kCodes; i += kThreads) count[i] = 0;
+  if (tid == 0) S.total = 0, S.n = 0;
+  __syncthreads();
+  uint64_t middle = 0;
+  uint32_t number = 0;
+  for (int j = 0; j < row.vecs; ++j) {
+    const uint4 raw = row.vector(j);
+    const int at = (row.first + 64 * j) * W;
+    uint32_t bits = 0;
+    row.vec(j, raw, [&](float x, int i) {
+      const int code = codes.of(x);
+      if (x >= codes.low) {
+        if (code != kSide) atomicAdd(&count[code], 1u);
+        else bits |= 1u << (i - at);
+      }
+    });
+    number += __builtin_popcount(bits);
+    row.each_bit(j, raw, bits, [&](float x, int, bool is) {
+      const uint64_t m = weight.mass(x);
+      middle += is ? m : 0;
+    });
+  }
+  middle = wave_sum64(middle);
+  for (int o = 32; o > 0; o >>= 1) number += __shfl_xor(number, o, kWave);
+  if (lane == 0 && number) {
+    atomicAdd((unsigned long long *)&S.total, (unsigned long long)middle);
+    atomicAdd(&S.n, number);
+  }
+  __syncthreads();
+  // The code that the cut falls into, and how many tokens of it are kept: found by the thread whose codes it is among.
+  int cut = kCodes;
+  uint32_t n = 0;
+  const int first = EACH * tid, end = min(first + EACH, kCodes);
+  auto tokens = [&](int code) { return code == kSide ? S.n : count[code]; };
+  if (top_k > 0) {
+    if (tid == 0) S.bin = kCodes;
+    uint32_t sum = 0, all;
+    for (int code = first; code < end; ++code) sum += tokens(code);
+    const uint32_t upto = running(sum, S.wave_count, all);
+    if (upto - sum < top_k && top_k <= upto) {
+      uint32_t before = upto - sum;
+      int code = first;
+      while (before + tokens(code) < top_k) before += tokens(code++);
+      S.bin = code, S.count_above = top_k - before;
+    }
+    __syncthreads();
+    cut = S.bin, n = cut < kCodes ? S.count_above : 0;
+    if (cut == kSide) return false;
+    __syncthreads();
+  }
+  if (share < 1.0) {
+    if (tid == 0) S.bin = kCodes;
+    const int top_cut = cut;
+    auto kept = [&](int code) { return code < top_cut ? tokens(code) : code == top_cut ? n : 0u; };
+    auto mass = [&](int code) {
+      const uint32_t c = kept(code);
+      return c == 0 ? 0 : code == kSide ? S.total : c * weight.mass(codes.value(code));
+    };
+    uint64_t sum = 0, all;
+    for (int code = first; code < end; ++code) sum += mass(code);
+    const uint64_t upto = running(sum, S.wave_mass, all);
+    const double target = fmax(share * (double)all, 1.0);
+    if ((double)(upto - sum) < target && target <= (double)upto) {
+      uint64_t before = upto - sum;
+      int code = first;
+      for (uint64_t m; code + 1 < end && (double)(before + (m = mass(code))) < target; ++code) before += m;
+      const uint64_t one = code == kSide ? 0 : weight.mass(codes.value(code)), c = kept(code);
+      const double more = ceil(target) - (double)before;        // the least whole mass beyond what lies above
+      S.bin = code, S.count_above = (uint32_t)(one ? min(((uint64_t)fmax(more, 1.0) - 1) / one + 1, c) : c);
+    }
+    __syncthreads();
+    if (S.bin < kCodes) cut = S.bin, n = S.count_above;
+    if (cut == kSide) return false;
+  }
+  if (cut == kCodes) {                 // every token that has a mass
+    got = Cut{codes.low, 0x7FFFFFFF, 0, false};
+    return true;
+  }
+  const float value = codes.value(cut);
+  if (tid == 0) S.fill = count[cut];
+  __syncthreads();
+  const uint32_t all = S.fill;
+  got = Cut{value, 0x7FFFFFFF, 0, false};
+  if (n >= all) return true;
+  if (all > kList) return false;
+  // the n-th of those in the vocabulary's order
+  list(row, S, [&](float x, int) { return x == value; });
+  if (tid < (int)all) S.list_w[tid] = 0;
+  __syncthreads();
+  rank(S, (int)all, ByIndex());
+  if (tid < (int)all && S.list_rank[tid] == n - 1) S.index = S.list_i[tid];
+  __syncthreads();
+  got.index = S.index;
+  return true;
+}
+
 template <bool BF16, bool LDS>
 __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
   extern __shared__ __align__(16) uint4 smem[];
@@ -557,10 +696,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
   const Weight weight{S.power, kPowers * scale, top, fmin((double)min_p, 1.0)};
 
   // 1. What may be kept as a list, where that is cheap and short.
+  // (a list of more than 256 tokens takes longer to rank than a cut by the distinct values of a bf16 row does)
+  constexpr int short_list = BF16 ? 256 : kList;
   float least = -__builtin_inff();                   // no token below it is kept
+  bool shorter = true;
   if (top_k == 0 && min_p > 0.f) {                   // w >= min_p, with a margin for the logarithm's and this sum's rounding
     least = (float)fmax((double)kLowest, (double)top + log2(weight.min_p) / scale * 1.000001) - 1e-6f * fabsf(top);
-  } else if (top_k > 0 && top_k <= kList) {
+    const uint32_t some = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= fmaxf(least, kLowest)));
+    if (lane == 0) S.wave_count[wave] = some;
+    __syncthreads();
+    uint32_t threads = 0;                            // each of which has a token for the list
+    for (int i = 0; i < kWaves; ++i) threads += S.wave_count[i];
+    shorter = threads <= short_list;
+  } else if (top_k > 0 && top_k <= short_list) {
     const Bins bins(code_of(bottom), code_of(top), true);
     if (mine >= kLowest) atomicAdd(&S.count[bins.of(mine)], 1u);
     if (tid == 0) S.bin = kBins;
@@ -576,9 +724,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
     __syncthreads();
     if (S.bin < kBins) least = fmaxf(least, value_of(S.lo));
   }
-  const bool lists = (least > -__builtin_inff() || A.V <= kList) && top_k <= kList;
+  const bool lists = (least > -__builtin_inff() || A.V <= short_list) && top_k <= short_list && shorter;
   const uint32_t n = lists ? list(row, S, [&](float x, int) { return x >= least && x >= kLowest; }) : kList + 1;
-  if (n <= kList) {
+  if (n <= (uint32_t)short_list) {
     uint64_t kept = 0;                               // the mass that top_p is a share of
     if (top_k == 0 && top_p < 1.f) {
       uint64_t sum = 0;
@@ -615,14 +763,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
     return;
   }
 
-  // 2. Cuts by histograms.
+  // 2. Cuts: by the distinct values, or by histograms.
   Cut cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V, true};
-  if (top_k > 0) cut = select<false>(row, weight, S, cut, top, bottom, (uint32_t)top_k, 0.0);
+  bool found_cut = top_k == 0 && !(top_p < 1.f);
+  if constexpr (BF16)
+    if (!found_cut)
+      found_cut = cut_by_codes(row, weight, S, top, bottom, (uint32_t)top_k, top_p < 1.f ? (double)top_p : 1.0, scale, cut);
+  if (!found_cut) cut = Cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V, true};
+  if (!found_cut && top_k > 0) cut = select<false>(row, weight, S, cut, top, bottom, (uint32_t)top_k, 0.0);
   uint64_t sum = 0;                                  // kept, of this thread
   bool summed = false;
-  if (top_p < 1.f) {
+  if (!found_cut && top_p < 1.f) {
     Cut got;
-    summed = reach(row, weight, S, cut, top, bottom, (double)top_p, scale, got, sum);
+    if constexpr (!BF16) summed = reach(row, weight, S, cut, top, bottom, (double)top_p, scale, got, sum);
     cut = summed ? got : select<true>(row, weight, S, cut, top, bottom, 0u, (double)top_p);
   }
   sum = summed ? sum : 0;

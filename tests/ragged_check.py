@@ -58,7 +58,8 @@ def causal(T, S):
 
 
 def sample(x, u, temperature, top_k, top_p, min_p):
-    """The token of one row x (V,) at u."""
+    """The token of one row x (V,) at u.  Masses are weights in whole multiples of 2^-45 of the largest, as sample_tokens defines
+    them: a token of weight below 2^-46 is not drawn at u = 0 either, where its weight in 64 bits, e^-700 still above 0, is."""
     x = x.double().clone()
     x[~(x > -3.389e38)] = -3.3895313892515355e38
     V = len(x)
@@ -67,13 +68,13 @@ def sample(x, u, temperature, top_k, top_p, min_p):
         return order[0]
     order = torch.tensor(order[:top_k] if 0 < top_k < V else order)
     w = ((x[order] - x[order[0]]) / temperature).exp()
-    n = len(w)
+    n, mass = len(w), (w * 2.0 ** 45).round()
     if top_p < 1:
-        before = torch.cat([torch.zeros(1, dtype=torch.float64), w.cumsum(0)[:-1]])
-        n = max(1, int((before < top_p * w.sum()).sum()))
+        before = torch.cat([torch.zeros(1, dtype=torch.float64), mass.cumsum(0)[:-1]])
+        n = max(1, int((before < top_p * mass.sum()).sum()))
     n = max(1, min(n, int((w >= min_p).sum())))
     kept, place = order[:n].sort()
-    mass = w[:n][place].cumsum(0)
+    mass = mass[:n][place].cumsum(0)
     return int(kept[min(int((mass <= u * float(mass[-1])).sum()), n - 1)])
 
 

@@ -517,6 +517,25 @@ def test_equal_masked_and_odd_logits():
                 assert got == want, (dtype, T, k, p, m, at)
 
 
+def test_cuts_near_zero_among_equal_tokens_and_on_either_side():
+    """Cuts among tokens that are zero or some 30 binades below the largest, among few and very many equal ones, in rows of one
+    sign, and of tokens whose weights vanish."""
+    V = 9000
+    g = gen(31)
+    x = torch.randn(V, generator=g)
+    relu = x.clamp(min=0) * 0.4                                            # half of them zeros, at the cut
+    tiny = torch.where(torch.rand(V, generator=g) < 0.999, x * 2.0 ** -30, x)   # cuts among magnitudes of 2^-30
+    steps = (x * 4).round() / 4                                            # hundreds of each value
+    signed = torch.where(torch.rand(V, generator=g) < 0.5, x * 1e-38, x * 3)    # subnormal magnitudes of both signs
+    rows = torch.stack([relu, tiny, steps, signed, -x.abs() - 50, x.abs() + 1e4, x * 300, x * 1e-20]).to(bf16)
+    for T, k, p, m in [(1.0, 0, 0.9, 0.0), (0.7, 0, 0.6, 1e-4), (2.0, 6000, 1.0, 0.0), (1.0, 3000, 0.8, 1e-3), (5.0, 0, 0.999, 0.0),
+                       (1.0, 400, 0.9, 0.0), (1e30, 0, 0.3, 0.0), (1e-30, 0, 0.3, 0.0)]:
+        for at in (0.0, 0.41, 0.93, 1 - 2.0 ** -24):
+            u = torch.full((len(rows),), at)
+            got = K.sample_tokens(rows.to(DEV), u.to(DEV), T, k, p, m).tolist()
+            assert got == [R.sample(row, R.f32(at), R.f32(T), k, R.f32(p), R.f32(m)) for row in rows], (T, k, p, m, at)
+
+
 def test_random_numbers_outside_their_range_give_a_token_all_the_same():
     x = torch.randn(4, 1000, generator=gen(0)).to(DEV)
     got = K.sample_tokens(x, torch.tensor([1.0, 5.0, -1.0, NAN], device=DEV), 1.0, 10)

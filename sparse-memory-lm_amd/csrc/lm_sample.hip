@@ -19,7 +19,8 @@
 // Else a cut, the top_k-th token or the one at which the mass reaches top_p, is found in a bf16 row by counting its distinct
 // values, in an fp32 row by a histogram of 1,024 bins, then within its bin.  One row, whole calls: the largest 10 us, no cut 23,
 // top_k 50 with top_p 16, min_p 0.1 13, top_p 0.9 alone 37 by distinct values (55 by the histogram, as in fp32), top_k 2,000 with
-// top_p 36 (57); 256 rows 5 to 15% more, rows in memory that is not 16-byte aligned 15 us more.  (Forming the weights' rough sum
+// top_p 36 (57); 256 rows 5 to 15% more, whatever a row's alignment (read by
+// elements where it is not 16-byte aligned, 25 us for the largest of an fp32 row).  (Forming the weights' rough sum
 // while the row is read took top_p alone from 59 to 54 us and top_p with min_p from 25 to 27; masses looked up per distinct value
 // instead of formed per token, 23 to 33 us without a cut.)
 #include <cstddef>
@@ -80,6 +81,10 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
   return v;
 }
 
+// 16 bytes of a row, which begins at a multiple of a logit's size alone: one load all the same
+typedef uint32_t Four __attribute__((ext_vector_type(4)));
+typedef Four Loose __attribute__((aligned(2)));
+
 // A row as its workgroup reads it, pass after pass: from LDS where it fits, else from memory.  Every lane reads only what it
 // wrote, so the passes need no barrier between them.
 template <bool BF16, bool LDS>
@@ -88,8 +93,6 @@ struct Row {
   const char *base;
   uint4 *kept;
   int V, first, vecs;                 // first vector of this lane, vectors of its run
-  bool aligned;
-
   // (med3 of a NaN is the lowest of the others)
   __device__ __forceinline__ static float fix(float x) { return __builtin_amdgcn_fmed3f(x, kLowest, -kLowest); }
 
@@ -97,9 +100,8 @@ struct Row {
   __device__ __forceinline__ uint4 fetch(int j) const { return fetch_at((first + 64 * j) * W); }
   __device__ __forceinline__ uint4 fetch_at(int at) const {
     float x[W];
-    if (aligned && at + W <= V) {
-      const uint4 raw = *(const uint4 *)(base + (int64_t)at * (BF16 ? 2 : 4));
-      const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+    if (at + W <= V) {
+      const Loose r = *(const Loose *)(base + (int64_t)at * (BF16 ? 2 : 4));
 #pragma unroll
       for (int e = 0; e < W; ++e)
         x[e] = fix(BF16 ? __uint_as_float(e % 2 ? r[e / 2] & 0xFFFF0000u : r[e / 2] << 16) : __uint_as_float(r[e % 4]));
@@ -120,9 +122,7 @@ struct Row {
   }
 
   __device__ __forceinline__ Row(const void *p, int64_t row, int64_t stride, int n, int wave, int lane, int vecs_, uint4 *lds)
-      : base((const char *)p + row * stride * (BF16 ? 2 : 4)), kept(lds), V(n), first(wave * vecs_ * 64 + lane), vecs(vecs_),
-        aligned((uintptr_t)base % 16 == 0) {
-  }
+      : base((const char *)p + row * stride * (BF16 ? 2 : 4)), kept(lds), V(n), first(wave * vecs_ * 64 + lane), vecs(vecs_) {}
   // the first pass: f(x, index) for every element, and the row into LDS
   template <class F>
   __device__ __forceinline__ void load(F &&f) const {

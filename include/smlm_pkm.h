@@ -682,7 +682,7 @@ int smlm_packed_attention(const void *q, const int64_t *q_strides, const void *k
  * q + b * q_row_stride; sequence b has lengths[b] (int32) tokens, token t in row t % page_size of page
  * block_table[b * table_row_stride + t / page_size] (int32, max_pages a sequence); lengths beyond the table count as its size.
  * A page id outside the pages holds no tokens.  y (B, H, head_dim) dense; zeros for a sequence without tokens.  fp32 scores,
- * statistics and sums, probabilities (4 bits: times the row's step) rounded to bf16.  What lies behind a sequence's last token
+ * statistics and sums, probabilities (4 bits: times the row's step) rounded to 16 bits.  What lies behind a sequence's last token
  * counts for nothing.  0 < scale <= 1e38; over 4-bit pages the queries are below 2^100.  workspace:
  * smlm_paged_attention_workspace bytes (may be 0), 16-byte aligned.
  */

@@ -18,10 +18,13 @@
 //
 // 4 bits: a row is lo + step * code, code 0 .. 15.  Codes become fp16 or bf16 by their bits alone (0x4300 | code is 128 + code of
 // bf16, exactly), and step and lo act on sums:  q k = step (q (n + c) - n sum q) + lo sum q,  the accumulator starting from -n
-// sum q,  and  sum_t p_t v_t = sum_t p'_t (128 + c_t) - 135.5 sum_t p'_t + sum_t p_t (lo_t + 7.5 step_t)  with p' = p step
-// rounded to bf16 (as a probability is), whose sum is taken of the same rounded values on the matrix cores: the rounding acts on
-// step (c - 7.5), a value's distance from its row's middle (on step c, from the row's lowest, it took the result's error from
-// 0.0021 to 0.0046).  fp32 sums; the n cost 2^-20 of a sum.
+// sum q,  and  sum_t p_t v_t = sum_t p'_t (128 + c_t) - 135.5 sum_t p'_t + sum_t p_t (lo_t + 7.5 step_t)  with p' = p step,
+// whose sum is taken of the same rounded values on the matrix cores: a rounding acts on step (c - 7.5), a value's distance from
+// its row's middle.  fp32 sums; the n cost 2^-20 of a sum.
+//
+// Probabilities (p') go into the products as two bf16 terms, a value and what its rounding left, 16 bits together: with one the
+// result's error is 1.3 to 1.5 times that of its own rounding to bf16, so 1.0.  The products beside it cost bf16 rows nothing and
+// 4-bit rows 2 to 4%.
 #include <algorithm>
 
 #include "lm_paged.h"
@@ -298,8 +301,13 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
     for (int i = 0; i < 4; ++i) pk[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
     const bf16x8 bp = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pk[i] = pack_bf16x2(p[2 * i] - __uint_as_float(pk[i] << 16), p[2 * i + 1] - __uint_as_float(pk[i] & 0xFFFF0000u));
+    const bf16x8 rest = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
     if constexpr (Q4) {
       pacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp, pacc, 0, 0, 0);
+      pacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, rest, pacc, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < MT / 2; ++j) {     // byte j: dims 2 j and 2 j + 1 of the lane's
         uint32_t a[4], c[4];
@@ -309,10 +317,12 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW
           a[e] = (w & low4) | 0x43004300u;
           c[e] = (w >> 4 & low4) | 0x43004300u;
         }
-        oacc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, uint4{a[0], a[1], a[2], a[3]}), bp,
-                                                              oacc[2 * j], 0, 0, 0);
-        oacc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, uint4{c[0], c[1], c[2], c[3]}), bp,
-                                                                  oacc[2 * j + 1], 0, 0, 0);
+        const bf16x8 even = __builtin_bit_cast(bf16x8, uint4{a[0], a[1], a[2], a[3]});
+        const bf16x8 odd = __builtin_bit_cast(bf16x8, uint4{c[0], c[1], c[2], c[3]});
+        oacc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, bp, oacc[2 * j], 0, 0, 0);
+        oacc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, bp, oacc[2 * j + 1], 0, 0, 0);
+        oacc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, rest, oacc[2 * j], 0, 0, 0);
+        oacc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, rest, oacc[2 * j + 1], 0, 0, 0);
       }
     } else {
 #pragma unroll
@@ -326,8 +336,9 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW
             a[e] = (4 * g + i < valid[kt] ? a[e] & 0xFFFFu : 0u) | (4 * g + i + 1 < valid[kt] ? a[e] & 0xFFFF0000u : 0u);
           }
         }
-        oacc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, uint4{a[0], a[1], a[2], a[3]}), bp,
-                                                           oacc[mt], 0, 0, 0);
+        const bf16x8 v = __builtin_bit_cast(bf16x8, uint4{a[0], a[1], a[2], a[3]});
+        oacc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, bp, oacc[mt], 0, 0, 0);
+        oacc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest, oacc[mt], 0, 0, 0);
       }
     }
     if (t + 1 < t1) load_values();

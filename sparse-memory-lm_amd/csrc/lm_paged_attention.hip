@@ -24,7 +24,7 @@
 //
 // Probabilities (p') go into the products as two bf16 terms, a value and what its rounding left, 16 bits together: with one the
 // result's error is 1.3 to 1.5 times that of its own rounding to bf16, so 1.0.  The products beside it cost bf16 rows nothing and
-// 4-bit rows 2 to 4%.
+// 4-bit rows 5% (48 sequences 68 -> 71 us).
 #include <algorithm>
 
 #include "lm_paged.h"

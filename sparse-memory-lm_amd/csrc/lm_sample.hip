@@ -517,11 +517,12 @@ __device__ __forceinline__ bool reach(const R &row, const Weight &weight, Shared
   return true;
 }
 
-// The mass that the token's running mass has to exceed.
+// The mass that the token's running mass has to exceed: of a total of up to 2^63, and for any u.
 __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
   const double aim = u * (double)total;
-  const uint64_t target = aim > 0.0 ? (uint64_t)fmin(aim, 9.2e18) : 0;
-  return target < total ? target : total - 1;
+  if (aim >= (double)total) return total - 1;
+  const uint64_t target = aim > 0.0 ? (uint64_t)aim : 0;
+  return target < total ? target : total - 1;        // ((double)total may be above it)
 }
 
 // The distinct values of a bf16 row, from the largest down: kSide magnitudes below the largest one of either sign, and all that is

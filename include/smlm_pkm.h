@@ -696,9 +696,9 @@ int smlm_paged_attention(const void *q, int64_t q_row_stride, const smlm_kv_page
  * u (B,) fp32 in [0, 1): weights exp((x - max) / temperature); kept are the top_k largest (all for top_k <= 0), of these the
  * smallest run of largest whose mass reaches top_p of theirs (all for top_p >= 1, at least one), and of these those that are
  * at least min_p of the largest; equal logits rank by index.  token[b]: the first token in the order of the vocabulary whose
- * running kept mass exceeds u times the kept mass.  temperature <= 0 (or NaN): the largest logit's lowest index.  NaN logits
- * count as the lowest; a row of lowest values alone gives each token the same weight.  Each setting is an array (B,) or, where
- * that is NULL, one value for all rows.  Masses in whole multiples of 2^-45 of the largest weight: the same token on every
+ * running kept mass exceeds u times the kept mass.  temperature <= 0 (or NaN): the largest logit's lowest index.  Masked logits
+ * (NaN, -infinity and all values up to the lowest bf16) weigh nothing, at an infinite temperature either; a row of masked ones
+ * alone gives each token the same weight.  Each setting is an array (B,) or, where that is NULL, one value for all rows.  Masses in whole multiples of 2^-45 of the largest weight: the same token on every
  * call.  V <= 2^18.
  */
 int smlm_sample(const void *logits, int dtype, int64_t row_stride, const float *u, const float *temperature,

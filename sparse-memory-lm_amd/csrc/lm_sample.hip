@@ -31,7 +31,7 @@ namespace smlm {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave, kBins = 1024, kList = 512, kPowerBits = 6, kPowers = 1 << kPowerBits;
-constexpr float kLowest = -3.3895313892515355e38f;   // the lowest bf16: masked logits and NaN
+constexpr float kLowest = -3.3895313892515355e38f;   // the lowest bf16: masked logits (-infinity, NaN, all that is lower)
 constexpr double kUnit = 0x1p45;
 
 struct SampleArgs {
@@ -201,11 +201,13 @@ struct Weight {
   double scale;                       // 64 log2(e) / temperature
   float top;
   double min_p;
+  float masked;                       // logits up to here weigh nothing, whatever the temperature (-infinity where all are masked)
 
-  // 2^((x - top) scale / 64), from 2^-47 on, below which a mass is 0 either way.  No branches, so that the chains of a vector's
+  // 2^((x - top) scale / 64), from 2^-47 on, below which a mass is 0 either way (fmax also takes the -infinity times 0 of an
+  // infinite temperature there).  No branches, so that the chains of a vector's
   // elements overlap, and rounding and scaling by additions (conversions and ldexp take four times as long).
   __device__ __forceinline__ double weight(float x) const {
-    const double t = __builtin_fmax(((double)x - (double)top) * scale, -47.0 * kPowers);
+    const double t = __builtin_fmax(((double)(x > masked ? x : -__builtin_inff()) - (double)top) * scale, -47.0 * kPowers);
     const double m = t + 0x1.8p52, r = t - (m - 0x1.8p52);             // t rounded, in m's low bits
     const int k = (int)(uint32_t)__double_as_longlong(m);
     constexpr double c = 0.693147180559945309417 / kPowers;
@@ -694,7 +696,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
   }
 
   const double scale = 1.4426950408889634074 / (double)temperature;
-  const Weight weight{S.power, kPowers * scale, top, fmin((double)min_p, 1.0)};
+  const Weight weight{S.power, kPowers * scale, top, fmin((double)min_p, 1.0), top > kLowest ? kLowest : -__builtin_inff()};
 
   // 1. What may be kept as a list, where that is cheap and short.
   // (a list of more than 256 tokens takes longer to rank than a cut by the distinct values of a bf16 row does)

@@ -1277,6 +1277,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     largest with top_p of their mass (1: all; at least one), of these those of at least min_p (at most 1) times the largest
     weight; equal logits rank by index.  The token is the first in the vocabulary's order whose running kept mass exceeds u times the kept
     mass.  temperature 0: the largest logit's lowest index.  Each setting is a number or a tensor (B,) (fp32, top_k int32).
-    NaN logits count as the lowest.  Masses are exact sums of fp64 weights rounded to 2^-45 of the largest: the same token on
+    Masked logits (NaN, -infinity and all values up to the lowest bf16) weigh nothing at any temperature, and all the same in a
+    row that has no others.  Masses are exact sums of fp64 weights rounded to 2^-45 of the largest: the same token on
     every call."""
     return _lib.serve_ops().sample_tokens(logits, u, temperature, top_k, top_p, min_p)

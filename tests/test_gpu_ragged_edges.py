@@ -34,3 +34,31 @@ def test_the_last_tokens_of_very_large_flat_rows_are_drawn(V, dtype):
         assert K.sample_tokens(x.to(DEV, dtype), u.to(DEV), T).tolist() == want
     for outside in (1.0, 7.0, math.inf):              # the last token all the same
         assert K.sample_tokens(x.to(DEV, dtype), torch.full((4,), outside, device=DEV), T).tolist() == [V - 1] * 4
+
+
+@pytest.mark.parametrize("V", [6000, 50304])
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_masked_logits_weigh_nothing_at_any_temperature(dtype, V):
+    """Few and half of the tokens left by each kind of mask, logits as far apart as the type has them, and a row of masks alone
+    (each token the same weight), up to an infinite temperature, against the definition over the tokens that are left."""
+    g = gen(V)
+    x = torch.randn(V, generator=g)
+    rows, left = [], []
+    for mask in (-math.inf, torch.finfo(dtype).min, NAN):
+        for share in (0.0005, 0.5):
+            keep = torch.rand(V, generator=g) < share
+            keep[77] = True
+            rows.append(torch.where(keep, x, torch.full((V,), mask)))
+            left.append(keep)
+    every = torch.ones(V, dtype=torch.bool)
+    rows += [torch.where(torch.rand(V, generator=g) < 0.5, -2e38, 1e38), torch.full((V,), -math.inf)]
+    left += [every, every]
+    rows = torch.stack(rows).to(dtype)
+    for T in (1e36, 1e38, math.inf):
+        for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.5), (4000, 0.7, 0.0), (40, 1.0, 0.0), (0, 0.8, 0.3)):
+            for at in (0.0, 0.4, 1 - 2.0 ** -24):
+                u = torch.full((len(rows),), at)
+                got = K.sample_tokens(rows.to(DEV), u.to(DEV), T, k, p, m).tolist()
+                ids = [keep.nonzero().flatten() for keep in left]
+                want = [int(i[R.sample(r[i].float(), R.f32(at), R.f32(T), k, R.f32(p), R.f32(m))]) for r, i in zip(rows, ids)]
+                assert got == want, (T, k, p, m, at)

@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t w = x.ks[kt][i];
-          sc[kt][i] = __uint_as_float(w << 16) * sc[kt][i] + __uint_as_float(w & 0xFFFF0000u) * sum_q;
+          const float step = __uint_as_float(w << 16);
+          // (a key that is not finite has an infinite step: its lowest value as NaN, or the infinities might add up to -infinity)
+          sc[kt][i] = step * sc[kt][i] + __builtin_fmaf(step, 0.f, __uint_as_float(w & 0xFFFF0000u)) * sum_q;
         }
       } else {
         sc[kt] = zero4;

@@ -62,3 +62,28 @@ def test_masked_logits_weigh_nothing_at_any_temperature(dtype, V):
                 ids = [keep.nonzero().flatten() for keep in left]
                 want = [int(i[R.sample(r[i].float(), R.f32(at), R.f32(T), k, R.f32(p), R.f32(m))]) for r, i in zip(rows, ids)]
                 assert got == want, (T, k, p, m, at)
+
+
+# ------------------------------------------------------------------------------------------- attention over the pages
+@pytest.mark.parametrize("codes", ["as appended", "of anything"])
+def test_a_key_that_is_not_finite_gives_nan_over_4_bit_pages(codes):
+    """Infinities and NaN among the keys: such a row reads back as NaN, so every query that sees it gets NaN, whatever the signs
+    and the rounding of its sums."""
+    g = gen(50)
+    B, H, D, page, n = 512, 16, 64, 16, 5
+    pages = K.kv_pages(B, 1, page, D, "q4", DEV)
+    qkv = randn(g, B * n, 3 * D)
+    qkv[2::2 * n, D + 5], qkv[2 + n::2 * n, D + 9] = math.inf, NAN
+    cos, sin = torch.ones(n, D // 2, device=DEV), torch.zeros(n, D // 2, device=DEV)
+    pos = torch.arange(n).repeat(B)
+    slots = (torch.arange(B).repeat_interleave(n) * page + pos).to(DEV)
+    K.paged_append(qkv.to(DEV), cos, sin, pos.to(DEV), slots, pages, 1)
+    if codes == "of anything":
+        pages[0][:, 0, 2] = torch.randint(0, 256, (B, D // 2), generator=g, dtype=torch.uint8).to(DEV)
+    k, _ = K.paged_gather(pages, slots)
+    assert torch.isnan(k[2::n]).all() and torch.isfinite(k[3::n]).all()
+    q = randn(g, B, H, D)
+    q[..., ::13] *= 30
+    table, ones = torch.arange(B, dtype=torch.int32, device=DEV).unsqueeze(1), torch.ones(B, dtype=torch.int32, device=DEV)
+    assert torch.isnan(K.paged_attention(q.to(DEV), pages, table, n * ones)).all()
+    assert torch.isfinite(K.paged_attention(q.to(DEV), pages, table, 2 * ones)).all()

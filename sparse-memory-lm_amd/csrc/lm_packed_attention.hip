@@ -23,7 +23,8 @@
 //
 // A masked key weighs exactly nothing, also where its value is an infinity or a NaN (0 times which is NaN): masked tiles sum
 // their values' columns, and where a sum is not finite the values that are not are left out of the products and added key by key,
-// for the queries that see the key.  So a query's result depends, to the bit, on nothing but what it sees.
+// for the queries that see the key.  So neither masked keys and values nor the queries beside it change a bit of a query's result.
+// (Where its sequence lies may: tiles begin at the first key that any query of the workgroup sees, and the order of the sums with them.)
 #include "lm_mm.h"
 
 namespace smlm {
@@ -221,13 +222,14 @@ __global__ void __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(H
               if ((uint32_t)(key - lo[j]) >= (uint32_t)(hi[j] - lo[j])) sacc[kt][j][i] = -__builtin_inff();
             }
       }
-      // P^T as B fragments: 32-key step ks = key tiles 2 ks and 2 ks + 1, slots 4 g .. and 16 + 4 g .. of them.  Returns the or
+      // P^T as B fragments: 32-key step ks = key tiles 2 ks and 2 ks + 1, slots 4 g .. and 16 + 4 g .. of them.  Leaves the or
       // of their bits, in which 0x40004000 is set where one is 2 or more (an infinity or a NaN too).
       bf16x8 bp[kQJ][2];
+      uint32_t bits[kQJ];
       auto probabilities = [&]() __attribute__((always_inline)) {
-        uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < kQJ; ++j)
+        for (int j = 0; j < kQJ; ++j) {
+          bits[j] = 0;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             uint32_t u[4];
@@ -238,24 +240,29 @@ __global__ void __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(H
               for (int i = 0; i < 2; ++i)
                 p[i] = __builtin_amdgcn_exp2f(sacc[2 * ks + e / 2][j][2 * (e % 2) + i] * A.scale_log2 - m[j]);
               u[e] = pack_bf16x2(p[0], p[1]);
-              bits |= u[e];
+              bits[j] |= u[e];
             }
             bp[j][ks] = __builtin_bit_cast(bf16x8, uint4{u[0], u[1], u[2], u[3]});
           }
-        return bits;
+        }
       };
       // Online softmax per query (lane), in the log2 domain, with a reference point m that starts 2^8 above the first tile's
       // maximum and moves, to 2^8 above a tile's, only when an exponential reaches 2: a test of the operands' bits stands in
       // for the maximum of every tile (head dim 64: 753 -> 800 TFLOP/s).  Each query by itself, whatever its neighbours do.
-      if (__builtin_amdgcn_ballot_w64((probabilities() & 0x40004000u) != 0)) {
+      probabilities();
+      if (__builtin_amdgcn_ballot_w64(((bits[0] | bits[1]) & 0x40004000u) != 0)) {
+        static_assert(kQJ == 2);
 #pragma unroll
         for (int j = 0; j < kQJ; ++j) {
+          uint32_t own = bits[j] & 0x40004000u;      // whether one of this query's is
+          own |= xor_lane<16>(own);
+          own |= xor_lane<32>(own);
           float a = -__builtin_inff();
 #pragma unroll
           for (int i = 0; i < 16; ++i) a = fmaxf(a, sacc[i / 4][j][i % 4]);
           a = fmaxf(a, xor_lane_f<16>(a));
           a = fmaxf(a, xor_lane_f<32>(a)) * A.scale_log2;
-          const float mnew = a - m[j] > 0.99f ? a + 8.f : m[j];
+          const float mnew = own && a - m[j] > 0.99f ? a + 8.f : m[j];
           const float alpha = __builtin_amdgcn_exp2f(m[j] - mnew);
           lacc[j] *= alpha;
           m[j] = mnew;

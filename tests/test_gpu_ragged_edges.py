@@ -87,3 +87,28 @@ def test_a_key_that_is_not_finite_gives_nan_over_4_bit_pages(codes):
     table, ones = torch.arange(B, dtype=torch.int32, device=DEV).unsqueeze(1), torch.ones(B, dtype=torch.int32, device=DEV)
     assert torch.isnan(K.paged_attention(q.to(DEV), pages, table, n * ones)).all()
     assert torch.isfinite(K.paged_attention(q.to(DEV), pages, table, 2 * ones)).all()
+
+
+# --------------------------------------------------------------------------------------------- packed prompt attention
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_what_the_neighbours_queries_are_does_not_matter(D):
+    """A query whose later scores exceed its first ones by 8.995 in the log2 domain, just short of what moves its softmax's reference
+    point (a factor that rounds to 2 of bf16, 2^0.995 does not, beyond 2^8): beside queries that stay, that move theirs and that
+    are NaN, in its own group of 16 and in the other, the same bits; and the formula's value."""
+    g = gen(60 + D)
+    T, S, scale = 32, 160, 8.995 / math.log2(math.e)
+    k, v = torch.zeros(S, 1, D), randn(g, S, 1, D)
+    k[64:128, 0, 0] = torch.rand(64, generator=g)
+    k[100, 0, 0], k[128:, 0, 0] = 1.0, 0.25
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device=DEV) for n in (T, S))
+    for at in (0, 21):
+        got = []
+        for other in (0.5, 2.0, NAN):
+            q = torch.zeros(T, 1, D)
+            q[:, 0, 0] = other
+            q[at, 0, 0] = 1.0
+            got.append(K.packed_attention(q.to(DEV, bf16), k.to(DEV, bf16), v.to(DEV), cu_q, cu_k, scale=scale)[at].cpu())
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+        seen = torch.arange(S).unsqueeze(0) <= S - T + at
+        want, bound = R.attention(q[at:at + 1].double(), k.to(bf16).double(), v.double(), seen, scale)
+        assert ((got[0].double() - want[0]).abs() <= R.bound_of(want, bound)[0]).all()

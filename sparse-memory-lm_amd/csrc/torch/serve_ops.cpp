@@ -23,6 +23,14 @@ void row_strides(const Tensor &t, int64_t *s) {
 
 bool is_bf16(const Tensor &t) { return t.scalar_type() == at::kBFloat16; }
 
+// There is no backward: inputs that autograd records would lose their gradients without a word.
+void forward_only(const char *name, std::initializer_list<const Tensor *> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor *t : inputs)
+    TORCH_CHECK_VALUE(!t->defined() || !t->requires_grad(), name, " has no backward pass and an input requires grad: call it under "
+                      "torch.no_grad() or detach the input");
+}
+
 // (k, v) of bf16 pages or (k, v, k_scale, v_scale) of 4-bit ones
 smlm_kv_pages check_pages(const char *name, const Tensor &first, const std::vector<Tensor> &p) {
   TORCH_CHECK_VALUE(p.size() == 2 || p.size() == 4, name, ": pages are (k, v), or (k, v, k_scale, v_scale) in 4 bits; got ",
@@ -30,6 +38,7 @@ smlm_kv_pages check_pages(const char *name, const Tensor &first, const std::vect
   const bool q4 = p.size() == 4;
   for (const Tensor &t : p) {
     check_device(name, first, {&t});
+    forward_only(name, {&t});
     TORCH_CHECK_VALUE(t.dim() == 4 && t.is_contiguous() && !t.is_neg(), name, ": pages must be contiguous and 4-dimensional, got ",
                       t.sizes());
   }
@@ -63,6 +72,7 @@ std::tuple<Tensor, std::optional<Tensor>> paged_append(const Tensor &qkv, const 
                                                        bool keys) {
   const char *name = "paged_append";
   check_device(name, qkv, {&cos, &sin, &positions, &slots});
+  forward_only(name, {&qkv, &cos, &sin});
   const c10::DeviceGuard guard(qkv.device());
   const smlm_kv_pages P = check_pages(name, qkv, pages);
   const int64_t heads = n_heads + 2 * P.kv_heads, hd = P.head_dim;
@@ -134,6 +144,7 @@ Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
   const char *name = "packed_attention";
   const Tensor none;
   check_device(name, q, {&k, &v, &cu_q, cu_k ? &*cu_k : &none, out ? &*out : &none});
+  forward_only(name, {&q, &k, &v, out ? &*out : &none});
   const c10::DeviceGuard guard(q.device());
   TORCH_CHECK_VALUE(is_bf16(q) && is_bf16(k) && is_bf16(v), name, ": q, k and v must be bf16, got ", q.scalar_type(), ", ",
                     k.scalar_type(), " and ", v.scalar_type());
@@ -171,6 +182,7 @@ Tensor paged_attention(const Tensor &q, const std::vector<Tensor> &pages, const 
                        std::optional<double> scale) {
   const char *name = "paged_attention";
   check_device(name, q, {&block_table, &lengths});
+  forward_only(name, {&q});
   const c10::DeviceGuard guard(q.device());
   const smlm_kv_pages P = check_pages(name, q, pages);
   TORCH_CHECK_VALUE(is_bf16(q) && q.dim() == 3 && q.size(2) == P.head_dim && q.size(1) >= 1 && q.size(1) % P.kv_heads == 0, name,

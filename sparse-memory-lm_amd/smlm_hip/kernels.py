@@ -1203,7 +1203,8 @@ def add_rmsnorm_train(x, delta, norm, out_dtype=None):
 
 # ---------------------------------------------------------------------------------------------------------------
 # Serving sequences of different lengths (model.Transformer.generate_ragged): a key-value cache in pages, packed prompts,
-# tokens drawn from the distribution.  Forward only.
+# tokens drawn from the distribution.  Forward only: the functions that return values of their inputs raise a ValueError where
+# autograd would record one of these.
 # ---------------------------------------------------------------------------------------------------------------
 def kv_pages(num_pages, n_kv_heads, page_size, head_dim, kind="bf16", device="cuda"):
     """Empty pages of one attention layer's cache, as the functions below take them: a token lies in slot page id *

@@ -7,6 +7,7 @@ import torch
 
 import ragged_check as R
 from smlm_hip import kernels as K
+from test_gpu_ragged_model import model, prompts
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -112,3 +113,39 @@ def test_what_the_neighbours_queries_are_does_not_matter(D):
         seen = torch.arange(S).unsqueeze(0) <= S - T + at
         want, bound = R.attention(q[at:at + 1].double(), k.to(bf16).double(), v.double(), seen, scale)
         assert ((got[0].double() - want[0]).abs() <= R.bound_of(want, bound)[0]).all()
+
+
+# --------------------------------------------------------------------------------------------------------- refusals
+def test_inputs_that_autograd_records_are_refused():
+    """There is no backward pass: a ValueError instead of outputs that are not in the graph.  Tokens have no gradient anyway."""
+    kv = K.kv_pages(2, 2, 16, 64, device=DEV)
+    z = lambda *s, dtype=bf16: torch.zeros(*s, dtype=dtype, device=DEV)  # noqa: E731
+    q, n, i32 = z(3, 2, 64), z(3, dtype=torch.long), torch.int32
+    cu, cos, table, ones = torch.tensor([0, 3], dtype=i32, device=DEV), z(9, 32, dtype=f32), z(3, 2, dtype=i32), z(3, dtype=i32) + 1
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda r: K.paged_append(r(z(3, 384)), cos, cos, n, n, kv, 2), lambda r: K.paged_append(z(3, 384), cos, r(cos), n, n, kv, 2),
+             lambda r: K.paged_append(z(3, 384), cos, cos, n, n, (kv[0], r(kv[1])), 2), lambda r: K.paged_gather((r(kv[0]), kv[1]), n),
+             lambda r: K.packed_attention(r(q), q, q, cu), lambda r: K.packed_attention(q, r(q), q, cu), lambda r: K.packed_attention(q, q, r(q), cu),
+             lambda r: K.packed_attention(q, q, q, cu, out=r(q)), lambda r: K.paged_attention(r(q), kv, table, ones),
+             lambda r: K.paged_attention(q, (r(kv[0]), kv[1]), table, ones)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no backward"):
+            call(leaf)
+        call(lambda t: t)                                   # no input that records
+        with torch.no_grad():
+            call(leaf)
+    assert K.sample_tokens(leaf(z(3, 5)), z(3, dtype=f32)).tolist() == [0, 0, 0]
+
+
+def test_a_recorded_pass_over_a_paged_cache_is_refused():
+    m = model()
+    cache = m.paged_cache(2, 100)
+    cache.reserve([1, 1])
+    cache.plan = cache.plan_step()
+    tok = torch.zeros(2, 1, dtype=torch.long, device=DEV)
+    with pytest.raises(ValueError, match="no backward"):
+        m(tok, kv_caches=cache.layers)
+    with torch.no_grad():
+        m(tok, kv_caches=cache.layers)
+    m.requires_grad_(False)
+    m(tok, kv_caches=cache.layers)

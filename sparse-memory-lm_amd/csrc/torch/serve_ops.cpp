@@ -85,7 +85,8 @@ std::tuple<Tensor, std::optional<Tensor>> paged_append(const Tensor &qkv, const 
                     name, ": rope tables must be (positions, rotated dims / 2) fp32 or bf16, the rotated dims a multiple of 16 up "
                     "to ", hd, ", got ", cos.sizes(), " ", cos.scalar_type(), " and ", sin.sizes(), " ", sin.scalar_type());
   const Tensor pos = check_slots(name, "positions", positions, N), at = check_slots(name, "slots", slots, N);
-  const Tensor x = aligned(plain(qkv).reshape({N, heads * hd})), c = aligned(plain(cos).contiguous()),
+  const Tensor rows = plain(qkv).reshape({N, heads * hd});
+  const Tensor x = N > 1 && rows.stride(0) < heads * hd ? rows.clone(at::MemoryFormat::Contiguous) : aligned(rows), c = aligned(plain(cos).contiguous()),
                s = aligned(plain(sin).contiguous());
   Tensor q = at::empty({N, n_heads, hd}, qkv.options());
   std::optional<Tensor> k;

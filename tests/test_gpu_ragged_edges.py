@@ -149,3 +149,16 @@ def test_a_recorded_pass_over_a_paged_cache_is_refused():
         m(tok, kv_caches=cache.layers)
     m.requires_grad_(False)
     m(tok, kv_caches=cache.layers)
+
+
+# ------------------------------------------------------------------------------------------------------ odd strides
+def test_append_of_rows_on_top_of_each_other():
+    """One row expanded over several tokens, and rows that overlap in memory, are what they are as copies."""
+    cos, sin = torch.rand(8, 16, generator=gen(1)).to(DEV), torch.rand(8, 16, generator=gen(2)).to(DEV)
+    row = randn(gen(3), 1, 96).to(DEV)
+    for qkv in (row.expand(5, 96), row.view(96).repeat(2).unfold(0, 96, 16)[:5], row.view(1, 1, 96).expand(5, 1, 96)):
+        n, got = torch.arange(5, device=DEV), []
+        for x in (qkv, qkv.contiguous()):
+            pages = K.kv_pages(1, 1, 16, 32, device=DEV)
+            got.append((*K.paged_append(x, cos, sin, n, n, pages, 1, keys=True), *pages))
+        assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][0].any()

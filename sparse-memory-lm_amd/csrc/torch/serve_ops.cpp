@@ -249,7 +249,7 @@ Tensor sample_tokens(const Tensor &logits, const Tensor &u, const py::object &te
                     u.sizes(), " ", u.scalar_type());
   const Setting T = setting("temperature", temperature, logits, at::kFloat), k = setting("top_k", top_k, logits, at::kInt),
                 p = setting("top_p", top_p, logits, at::kFloat), m = setting("min_p", min_p, logits, at::kFloat);
-  const Tensor x0 = plain(logits), x = V == 1 || (x0.stride(1) == 1 && (B <= 1 || x0.stride(0) >= V)) ? x0 : x0.contiguous();
+  const Tensor x0 = plain(logits), x = (V == 1 || x0.stride(1) == 1) && (B <= 1 || x0.stride(0) >= V) ? x0 : x0.contiguous();
   const Tensor r = plain(u).contiguous();
   Tensor token = at::empty({B}, logits.options().dtype(at::kLong));
   if (B == 0) return token;

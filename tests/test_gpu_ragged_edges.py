@@ -162,3 +162,11 @@ def test_append_of_rows_on_top_of_each_other():
             pages = K.kv_pages(1, 1, 16, 32, device=DEV)
             got.append((*K.paged_append(x, cos, sin, n, n, pages, 1, keys=True), *pages))
         assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][0].any()
+
+
+def test_sampled_tokens_of_expanded_rows():
+    g = gen(5)
+    for V in (1, 9):
+        row, u = torch.randn(1, V, generator=g).to(DEV), torch.rand(6, generator=g).to(DEV)
+        for x in (row.expand(6, V), row.t().expand(V, 6).t()):
+            assert torch.equal(K.sample_tokens(x, u), K.sample_tokens(x.clone(memory_format=torch.contiguous_format), u))

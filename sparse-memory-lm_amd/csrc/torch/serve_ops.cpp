@@ -3,6 +3,8 @@
 // include/smlm_pkm.h on torch's current stream of the inputs' device.  Forward only.
 //
 // In C++ because the smallest calls, 6 to 8 us whole, take as long as their argument checks and launches.
+#include <array>
+
 #include "common.h"
 
 namespace {
@@ -14,6 +16,18 @@ Tensor aligned(const Tensor &t) {      // its last dimension dense and every row
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
     fine = fine && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) <= kMaxStride));
   return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Whether rows or heads of t (N, H, hd) lie on top of each other in memory: the smaller stride has to hold hd elements, the larger one
+// all that the smaller one spans.
+bool overlaps(const Tensor &t) {
+  int64_t span = t.size(2);
+  for (const int i : t.size(1) <= 1 || (t.size(0) > 1 && t.stride(0) < t.stride(1)) ? std::array{0, 1} : std::array{1, 0}) {
+    if (t.size(i) <= 1) continue;
+    if (t.stride(i) < span) return true;
+    span += t.stride(i) * (t.size(i) - 1);
+  }
+  return false;
 }
 
 // strides over rows and heads; a dimension of one takes none
@@ -162,10 +176,10 @@ Tensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, const
                     cu_k ? cu_k->scalar_type() : at::kInt);
   TORCH_CHECK_VALUE(cu_k || S == N, name, ": ", S, " keys for ", N, " queries need cu_k");
   TORCH_CHECK_VALUE(!out || (out->sizes() == q.sizes() && is_bf16(*out) && !out->is_neg() && out->stride(2) == 1 &&
-                             (N <= 1 || (out->stride(0) % 4 == 0 && out->stride(0) > 0 && out->stride(0) <= kMaxStride)) &&
-                             (H <= 1 || (out->stride(1) % 4 == 0 && out->stride(1) > 0 && out->stride(1) <= kMaxStride)) &&
+                             (N <= 1 || (out->stride(0) % 4 == 0 && out->stride(0) <= kMaxStride)) &&
+                             (H <= 1 || (out->stride(1) % 4 == 0 && out->stride(1) <= kMaxStride)) && !overlaps(*out) &&
                              (uintptr_t)out->data_ptr() % 8 == 0),
-                    name, ": out must be ", q.sizes(), " bf16 with a dense, 8-byte aligned last dimension");
+                    name, ": out must be ", q.sizes(), " bf16 with a dense, 8-byte aligned last dimension, no element twice");
   const Tensor qa = aligned(plain(q)), ka = aligned(plain(k)), va = aligned(plain(v)), cq = cu_q.contiguous(),
                ck = cu_k ? cu_k->contiguous() : cq;
   Tensor y = out ? *out : at::empty({N, H, hd}, q.options());

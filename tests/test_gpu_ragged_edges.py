@@ -170,3 +170,20 @@ def test_sampled_tokens_of_expanded_rows():
         row, u = torch.randn(1, V, generator=g).to(DEV), torch.rand(6, generator=g).to(DEV)
         for x in (row.expand(6, V), row.t().expand(V, 6).t()):
             assert torch.equal(K.sample_tokens(x, u), K.sample_tokens(x.clone(memory_format=torch.contiguous_format), u))
+
+
+def test_packed_attention_into_views():
+    """`out` with padded rows, heads first, one row or one head is written as it lies; rows or heads on top of each other are refused."""
+    q = randn(gen(2), 5, 2, 64).to(DEV)
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    want = K.packed_attention(q, q, q, cu)
+    room = lambda: torch.zeros(4000, dtype=bf16, device=DEV)  # noqa: E731
+    for strides in ((128, 64, 1), (64, 320, 1), (68, 400, 1), (256, 68, 1)):
+        out = room().as_strided(q.shape, strides)
+        assert torch.equal(K.packed_attention(q, q, q, cu, out=out), want) and torch.equal(out, want)
+    one = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    assert torch.equal(K.packed_attention(q[:1], q[:1], q[:1], one, out=room().as_strided((1, 2, 64), (0, 64, 1))), q[:1])
+    assert torch.equal(K.packed_attention(q[:, :1], q[:, :1], q[:, :1], cu, out=room().as_strided((5, 1, 64), (64, 0, 1))), want[:, :1])
+    for strides in ((64, 64, 1), (0, 64, 1), (128, 0, 1), (60, 320, 1), (64, 316, 1), (124, 64, 1), (128, 60, 1)):
+        with pytest.raises(ValueError, match="twice"):
+            K.packed_attention(q, q, q, cu, out=room().as_strided(q.shape, strides))

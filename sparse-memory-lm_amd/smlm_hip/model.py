@@ -697,6 +697,10 @@ class Transformer(nn.Module):
             raise ValueError(f"the paged cache is for bf16 models (or bf16 autocast) on its own GPU, got {dtype} on {w.device}")
         if self.ngram is not None or len(cache.layers) != len(self.layers):
             raise ValueError(f"a cache of {len(cache.layers)} layers for a model of {len(self.layers)}")
+        shape, cfg = (cache.n_kv_heads, cache.head_dim), self.cfg
+        if shape != (cfg.n_heads, cfg.d_model // cfg.n_heads) or cache.max_len > cfg.max_seq_len:
+            raise ValueError(f"a cache of {shape} heads and dims and {cache.max_len} tokens for a model of {cfg.n_heads} heads, "
+                             f"{cfg.d_model // cfg.n_heads} dims and up to {cfg.max_seq_len} tokens")
 
     @torch.no_grad()
     def generate_ragged(self, prompts, new_tokens, cache=None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None,

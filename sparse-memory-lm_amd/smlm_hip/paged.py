@@ -44,6 +44,7 @@ class PagedKVCache:
         per_seq = -(-max_len // page_size)
         num_pages = n_seqs * per_seq if num_pages is None else num_pages
         self.n_seqs, self.max_len, self.page_size, self.kind, self.num_pages = n_seqs, max_len, page_size, kind, num_pages
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
         self.layers = [PagedLayer(self, kernels.kv_pages(num_pages, n_kv_heads, page_size, head_dim, kind, device))
                        for _ in range(n_layers)]
         self.block_table = torch.full((n_seqs, per_seq), -1, dtype=torch.int32, device=device)

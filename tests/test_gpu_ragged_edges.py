@@ -187,3 +187,15 @@ def test_packed_attention_into_views():
     for strides in ((64, 64, 1), (0, 64, 1), (128, 0, 1), (60, 320, 1), (64, 316, 1), (124, 64, 1), (128, 60, 1)):
         with pytest.raises(ValueError, match="twice"):
             K.packed_attention(q, q, q, cu, out=room().as_strided(q.shape, strides))
+
+
+# ------------------------------------------------------------------------------------------------ the model and its cache
+def test_a_cache_of_another_models_shape_is_refused():
+    """Fewer positions than the cache is long (its later tokens would have no rotation), other heads or dims; nothing changes."""
+    cache, seqs = model().paged_cache(1, 300), prompts([150])
+    for other in (model(max_seq_len=299), model(n_heads=4), model(d_model=64), model(n_layers=3)):
+        for call in (lambda: other.prefill(cache, seqs), lambda: other.generate_ragged(seqs, 3, cache)):
+            with pytest.raises(ValueError, match="cache of"):
+                call()
+    assert cache.seq_lens == [0] and len(cache._free) == cache.num_pages
+    model(max_seq_len=300).prefill(cache, seqs)

@@ -738,13 +738,17 @@ class Transformer(nn.Module):
                 state["fused"] = None
             elif state["fused"] is None or state["fused"]._model() is not self:
                 state["fused"] = _FusedDecodeStep(self)
-            if use_graph and new_tokens:
-                graph = self._ragged_graph(cache, state)
-                for _ in range(new_tokens):
-                    graph.replay()
-            else:
-                for _ in range(new_tokens):
-                    self._ragged_step(cache, state)
+            try:
+                if use_graph and new_tokens:
+                    graph = self._ragged_graph(cache, state)
+                    for _ in range(new_tokens):
+                        graph.replay()
+                else:
+                    for _ in range(new_tokens):
+                        self._ragged_step(cache, state)
+            except BaseException:
+                cache.refresh()                # the prompts are in the cache, and what the steps left counts for nothing
+                raise
         cache.seq_lens = [n + new_tokens for n in cache.seq_lens]
         return torch.cat([first.unsqueeze(1), state["out"][:, 1:new_tokens + 1]], 1)
 
@@ -782,7 +786,7 @@ class Transformer(nn.Module):
         if state.get("graph_of", lambda: None)() is not self or state["graph_key"] != key:
             ctx = (torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False) if ac
                    else torch.autocast("cuda", enabled=False))
-            state["graph"] = None
+            state["graph"] = state["graph_key"] = None
             table = cache.block_table.clone()
             saved = [t.clone() for t in (cache.lengths, state["tok"], state["out"], state["at"])]
             cache.block_table.fill_(-1)          # the steps before the capture (library loads, derived weights) write no page

@@ -65,7 +65,7 @@ class PagedKVCache:
             self._free += self._pages[b]
             self._pages[b] = []
             self.seq_lens[b] = 0
-        self._publish()
+        self.refresh()
 
     def reserve(self, new):
         """Pages for new[b] more tokens of every sequence; ValueError, with nothing changed, where they do not fit."""
@@ -81,9 +81,10 @@ class PagedKVCache:
         for b, n in enumerate(need):
             for _ in range(n):
                 self._pages[b].append(self._free.pop())
-        self._publish()
+        self.refresh()
 
-    def _publish(self):
+    def refresh(self):
+        """The device's block table and lengths as the host has them."""
         rows = [p + [-1] * (self.block_table.shape[1] - len(p)) for p in self._pages]
         self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
         self.lengths.copy_(torch.tensor(self.seq_lens, dtype=torch.int32))

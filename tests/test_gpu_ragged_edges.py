@@ -199,3 +199,35 @@ def test_a_cache_of_another_models_shape_is_refused():
                 call()
     assert cache.seq_lens == [0] and len(cache._free) == cache.num_pages
     model(max_seq_len=300).prefill(cache, seqs)
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+@pytest.mark.parametrize("at", [0, 2])
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_a_step_that_fails_leaves_the_prompts_in_the_cache(at, use_graph):
+    """An error in a step (before the capture, in it, or among eager ones): lengths and block table are those of the prompts, and the
+    next call, of this model or of the one whose graph the cache held, gives what it gives on a fresh cache."""
+    m, n = model(), model(seed=9)
+    seqs = prompts([5, 20])
+    cache = m.paged_cache(2, 100)
+    want = [who.generate_ragged(seqs, 4) for who in (m, n)]
+    assert torch.equal(m.generate_ragged(seqs, 4, cache), want[0])
+    cache.clear()
+    calls, step = [], n._ragged_step
+
+    def failing(*args):
+        calls.append(0)
+        if len(calls) > at:
+            raise RuntimeError("a step that fails")
+        step(*args)
+
+    n._ragged_step = failing
+    with pytest.raises(RuntimeError, match="that fails"):
+        n.generate_ragged(seqs, 4, cache, use_graph=use_graph)
+    assert cache.seq_lens == [5, 20] == cache.lengths.tolist() and cache.plan is None
+    pages = [p + [-1] * (cache.block_table.shape[1] - len(p)) for p in cache._pages]
+    assert cache.block_table.tolist() == pages and pages[1][0] >= 0
+    del n._ragged_step
+    for who, tokens in ((m, want[0]), (n, want[1])):
+        cache.clear()
+        assert torch.equal(who.generate_ragged(seqs, 4, cache), tokens)

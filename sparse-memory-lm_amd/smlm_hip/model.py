@@ -752,6 +752,7 @@ class Transformer(nn.Module):
         cache.seq_lens = [n + new_tokens for n in cache.seq_lens]
         return torch.cat([first.unsqueeze(1), state["out"][:, 1:new_tokens + 1]], 1)
 
+    @torch.inference_mode(False)            # as the cache's tensors
     def _ragged_state(self, cache):
         """The buffers of generate_ragged's steps, kept by the cache."""
         if "tok" not in cache.decoding:

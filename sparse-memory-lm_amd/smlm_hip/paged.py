@@ -38,6 +38,7 @@ class PagedKVCache:
     it grows and gives them back with clear().  The host keeps the lengths; block_table and lengths are on the device,
     where a captured decode step reads them."""
 
+    @torch.inference_mode(False)                       # later calls, outside of it, write what is made here
     def __init__(self, n_layers, n_seqs, max_len, n_kv_heads, head_dim, page_size=64, kind="bf16", num_pages=None, device="cuda"):
         if n_seqs < 1 or max_len < 1:
             raise ValueError(f"PagedKVCache: {n_seqs} sequences of {max_len} tokens")

@@ -231,3 +231,17 @@ def test_a_step_that_fails_leaves_the_prompts_in_the_cache(at, use_graph):
     for who, tokens in ((m, want[0]), (n, want[1])):
         cache.clear()
         assert torch.equal(who.generate_ragged(seqs, 4, cache), tokens)
+
+
+@pytest.mark.parametrize("inside", [True, False])
+def test_inference_mode_and_out_of_it(inside):
+    """A cache made, or first used, in inference mode serves calls outside of it, and the other way round."""
+    m = model()
+    seqs = prompts([5, 20])
+    want = m.generate_ragged(seqs, 4)
+    with torch.inference_mode(inside):
+        cache = m.paged_cache(2, 100)
+    for mode in (True, False, True):
+        with torch.inference_mode(mode):
+            cache.clear()
+            assert torch.equal(m.generate_ragged(seqs, 4, cache), want)

@@ -40,8 +40,8 @@ class PagedKVCache:
 
     @torch.inference_mode(False)                       # later calls, outside of it, write what is made here
     def __init__(self, n_layers, n_seqs, max_len, n_kv_heads, head_dim, page_size=64, kind="bf16", num_pages=None, device="cuda"):
-        if n_seqs < 1 or max_len < 1:
-            raise ValueError(f"PagedKVCache: {n_seqs} sequences of {max_len} tokens")
+        if n_seqs < 1 or max_len < 1 or page_size < 1:
+            raise ValueError(f"PagedKVCache: {n_seqs} sequences of {max_len} tokens in pages of {page_size}")
         per_seq = -(-max_len // page_size)
         num_pages = n_seqs * per_seq if num_pages is None else num_pages
         self.n_seqs, self.max_len, self.page_size, self.kind, self.num_pages = n_seqs, max_len, page_size, kind, num_pages

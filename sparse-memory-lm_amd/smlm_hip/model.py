@@ -679,7 +679,7 @@ class Transformer(nn.Module):
         dev = cache.device
         last = torch.tensor([n > 0 for n in new])
         if sum(new) == 0:
-            return torch.full((cache.n_seqs, self.cfg.vocab_size), float("nan"), device=dev, dtype=self.lm_head.weight.dtype)
+            return torch.full((cache.n_seqs, self.cfg.vocab_size), float("nan"), device=dev, dtype=torch.bfloat16)
         cache.plan = cache.plan_prompts(new)
         try:
             hidden = self._hidden(torch.cat([p.to(dev, torch.long) for p in prompts]).unsqueeze(0), cache.layers, 0)

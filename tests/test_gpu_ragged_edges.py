@@ -245,3 +245,13 @@ def test_inference_mode_and_out_of_it(inside):
         with torch.inference_mode(mode):
             cache.clear()
             assert torch.equal(m.generate_ragged(seqs, 4, cache), want)
+
+
+def test_prefill_of_nothing_is_of_the_type_of_any_other():
+    m = model(f32)
+    cache = m.paged_cache(2, 100)
+    with torch.autocast("cuda", dtype=bf16):
+        none = m.prefill(cache, [[], []])
+        some = m.prefill(cache, [[3], []])
+    assert none.dtype == some.dtype == bf16 and none.shape == some.shape and torch.isnan(none).all()
+    assert torch.isnan(some[1]).all() and torch.isfinite(some[0]).all()

@@ -255,3 +255,116 @@ def test_prefill_of_nothing_is_of_the_type_of_any_other():
         some = m.prefill(cache, [[3], []])
     assert none.dtype == some.dtype == bf16 and none.shape == some.shape and torch.isnan(none).all()
     assert torch.isnan(some[1]).all() and torch.isfinite(some[0]).all()
+
+
+# ------------------------------------------------------------------------------------------- how exact the attention is
+def close_to_64_bits(q, k, v, scale, key_scale=None, value_scale=None):
+    """One query row q (H, D) over keys and values (n, Hk, D), all double: the result, what two bf16 terms a probability and fp32
+    scores and sums may be off by, and the result with one bf16 term a probability.  The scales (n, Hk, 2) of 4-bit rows are their steps
+    and lowest values: there a probability times its row's step is rounded, which acts on a value's distance from its row's middle."""
+    (H, D), n = q.shape, k.shape[0]
+    of = torch.arange(H) // (H // k.shape[1])
+    k, v = k[:, of], v[:, of]
+    s = (k * q).sum(-1) * scale                                           # (n, H)
+    p = ((s - s.max(0).values) / math.log(2) - 8).exp2()                  # as the kernel's first reference point has it
+    w = (p / p.sum(0)).unsqueeze(-1)
+    y = (w * v).sum(0)
+    size = q.abs().sum(-1)
+    if key_scale is None:
+        middle, spread, terms = torch.zeros_like(v), torch.ones_like(v), (k * q).abs().sum(-1)
+        added = v.abs()
+    else:
+        step, low = key_scale[:, of, :1], key_scale[:, of, 1:]
+        spread = value_scale[:, of, :1]
+        middle = value_scale[:, of, 1:] + 7.5 * spread
+        # scores are formed as step (sum (n + code) q - n sum q) + low sum q, n at most 256, q in fp16 to 2^-25 of the largest;
+        # values as sums of (128 + code) steps beside the rows' middles
+        terms = step[..., 0] * (271 * size + 8 * D * q.abs().amax(-1)) + low[..., 0].abs() * size
+        added = 2 * (143 * spread + middle.abs())
+    one = ((p.unsqueeze(-1) * spread).to(bf16).double() * ((v - middle) / spread) + p.unsqueeze(-1) * middle).sum(0) / p.sum(0).unsqueeze(-1)
+    # a score's D products and sums in fp32 move its weight by as much, and the others' sum; an exponential's argument, up to 16,
+    # and the exponential by 2^-18
+    weights = 2 * D * 2.0 ** -24 * scale * terms.amax(0) + 2.0 ** -18
+    bound = (R.HALF * y.abs() + 2.0 ** -16 * (w * (v - middle).abs()).sum(0) + weights.unsqueeze(-1) * (w * v.abs()).sum(0)
+             + (n + 8) * 2.0 ** -24 * (w * added).sum(0))
+    return y, bound, one
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+@pytest.mark.parametrize("H,Hk,D", [(4, 4, 32), (9, 3, 64), (16, 2, 128)])
+def test_probabilities_are_two_bf16_terms_over_pages(kind, H, Hk, D):
+    """Few tokens, weights of nearly the same size, so that results near zero have small roundings of their own: within what two
+    terms allow.  One term a probability is beyond it, by the same formula, on these inputs."""
+    g = gen(D + H)
+    page, scale = 16, 0.1 / D
+    lengths = list(range(2, 34)) + [70, 400]
+    total = sum(-(-n // page) for n in lengths)
+    table = torch.zeros(len(lengths), 25, dtype=torch.int32)
+    ids, at = torch.randperm(total, generator=g), 0
+    for b, n in enumerate(lengths):
+        need = -(-n // page)
+        table[b, :need] = ids[at:at + need]
+        at += need
+    k, v = randn(g, total, Hk, page, D), randn(g, total, Hk, page, D)
+    rows = lambda t: t.transpose(1, 2).flatten(0, 1).double()  # noqa: E731
+    if kind == "bf16":
+        pages, k, v, scales = (k, v), rows(k), rows(v), ()
+    else:
+        (ck, sk), (cv, sv) = R.quantized(k), R.quantized(v)
+        pages, k, v = (ck, cv, sk, sv), rows(R.values(ck, sk)), rows(R.values(cv, sv))
+        scales = rows(sk), rows(sv)
+    q = randn(g, len(lengths), H, D)
+    got = K.paged_attention(q.to(DEV), [p.to(DEV) for p in pages], table.to(DEV),
+                            torch.tensor(lengths, dtype=torch.int32, device=DEV), scale).double().cpu()
+    beyond = 0
+    for b, n in enumerate(lengths):
+        slots = table[b, torch.arange(n) // page].long() * page + torch.arange(n) % page
+        y, bound, one = close_to_64_bits(q[b].double(), k[slots], v[slots], scale, *(t[slots] for t in scales))
+        assert ((got[b] - y).abs() <= bound).all(), (n, ((got[b] - y).abs() / bound).max())
+        beyond += ((one - y).abs() > bound).sum().item()
+    assert beyond > 50
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q4"])
+@torch.no_grad()
+def test_a_models_attention_over_what_its_cache_holds(kind):
+    """A layer's attention, of a second piece of the prompts and of a step, against the formula over the rows that its pages hold
+    afterwards (4-bit ones as the values they stand for): no allowance for what the cache itself rounds."""
+    m = model(mem=False)
+    H, D = m.cfg.n_heads, m.cfg.d_model // m.cfg.n_heads
+    attn, lengths, more = m.layers[1].attn, [1, 7, 64, 130, 33], [5, 0, 70, 1, 20]
+    cache = m.paged_cache(len(lengths), 300, kind, 32)
+    m.prefill(cache, prompts(lengths))
+    layer, g = cache.layers[1], gen(8)
+    rows = lambda t, at: t.transpose(1, 2).flatten(0, 1)[at.to(DEV)].double().cpu()  # noqa: E731
+
+    def projected(n):
+        qkv = randn(g, n, 3 * H * D).to(DEV)
+        copies = [t.clone() for t in layer.pages]
+        q, _ = K.paged_append(qkv, attn.rope.cos, attn.rope.sin, cache.plan.positions, cache.plan.slots, copies, H)
+        return qkv, q.double().cpu()
+
+    cache.reserve(more)
+    cache.plan = cache.plan_prompts(more)
+    qkv, q = projected(sum(more))
+    y = attn._paged(qkv, layer).double().cpu()
+    first = 0
+    for b, (n, new) in enumerate(zip(lengths, more)):
+        k, v = (t.double().cpu() for t in K.paged_gather(layer.pages, cache._slots(b, 0, n + new).to(DEV)))
+        want, bound = R.attention(q[first:first + new], k, v, R.causal(new, n + new), D ** -0.5)
+        assert ((y[first:first + new] - want).abs() <= R.bound_of(want, bound)).all(), b
+        first += new
+    cache.advance(more)
+    cache.reserve([1] * len(lengths))
+    cache.plan = cache.plan_step()
+    qkv, q = projected(len(lengths))
+    y = attn._paged(qkv, layer).double().cpu()
+    for b, n in enumerate(cache.seq_lens):
+        at = cache._slots(b, 0, n + 1)
+        if kind == "bf16":
+            k, v, scales = rows(layer.pages[0], at), rows(layer.pages[1], at), ()
+        else:
+            k, v = (rows(R.values(c, s), at) for c, s in zip(layer.pages[:2], layer.pages[2:]))
+            scales = rows(layer.pages[2], at), rows(layer.pages[3], at)
+        want, bound, _ = close_to_64_bits(q[b], k, v, D ** -0.5, *scales)
+        assert ((y[b] - want).abs() <= bound).all(), b

@@ -229,11 +229,10 @@ struct Weight {
   }
 };
 
-// The kept tokens: those above `value`, and of those equal to it the ones up to `index`; how many.
+// The kept tokens: those above `value`, and of those equal to it the ones up to `index`.
 struct Cut {
   float value;
   int index;
-  uint32_t n;
   bool all;                            // it keeps every token (and what stands behind the row's end weighs nothing)
   __device__ __forceinline__ bool keeps(float x, int i) const { return all | (x > value) | ((x == value) & (i <= index)); }
 };
@@ -394,7 +393,7 @@ __device__ __forceinline__ Cut select(const R &row, const Weight &weight, Shared
       const uint32_t last = S.n;
       if (keep && S.list_rank[tid] == last) S.index = tid;
       __syncthreads();
-      const Cut got{S.list_x[S.index], S.list_i[S.index], above + last + 1, false};
+      const Cut got{S.list_x[S.index], S.list_i[S.index], false};
       __syncthreads();
       return got;
     }
@@ -431,7 +430,7 @@ __device__ __forceinline__ Cut select(const R &row, const Weight &weight, Shared
       else a = mid + 1;
     }
     __syncthreads();
-    return Cut{value, a, above + (uint32_t)c, false};
+    return Cut{value, a, false};
   }
 }
 
@@ -515,7 +514,7 @@ __device__ __forceinline__ bool reach(const R &row, const Weight &weight, Shared
   const uint32_t last = S.n;
   if (keep && S.list_rank[tid] == last) S.index = tid;
   __syncthreads();
-  got = Cut{S.list_x[S.index], S.list_i[S.index], 0, false};      // (how many it keeps is not asked any more)
+  got = Cut{S.list_x[S.index], S.list_i[S.index], false};
   return true;
 }
 
@@ -634,14 +633,14 @@ __device__ __forceinline__ bool cut_by_codes(const R &row, const Weight &weight,
     if (cut == kSide) return false;
   }
   if (cut == kCodes) {                 // every token that has a mass
-    got = Cut{codes.low, 0x7FFFFFFF, 0, false};
+    got = Cut{codes.low, 0x7FFFFFFF, false};
     return true;
   }
   const float value = codes.value(cut);
   if (tid == 0) S.fill = count[cut];
   __syncthreads();
   const uint32_t all = S.fill;
-  got = Cut{value, 0x7FFFFFFF, 0, false};
+  got = Cut{value, 0x7FFFFFFF, false};
   if (n >= all) return true;
   if (all > kList) return false;
   // the n-th of those in the vocabulary's order
@@ -767,12 +766,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs A) {
   }
 
   // 2. Cuts: by the distinct values, or by histograms.
-  Cut cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V, true};
+  Cut cut{kLowest, 0x7FFFFFFF, true};
   bool found_cut = top_k == 0 && !(top_p < 1.f);
   if constexpr (BF16)
     if (!found_cut)
       found_cut = cut_by_codes(row, weight, S, top, bottom, (uint32_t)top_k, top_p < 1.f ? (double)top_p : 1.0, scale, cut);
-  if (!found_cut) cut = Cut{kLowest, 0x7FFFFFFF, (uint32_t)A.V, true};
+  if (!found_cut) cut = Cut{kLowest, 0x7FFFFFFF, true};
   if (!found_cut && top_k > 0) cut = select<false>(row, weight, S, cut, top, bottom, (uint32_t)top_k, 0.0);
   uint64_t sum = 0;                                  // kept, of this thread
   bool summed = false;

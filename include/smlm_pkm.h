@@ -643,8 +643,9 @@ typedef struct smlm_kv_pages {
  *     is not written.  A position outside the tables gives NaN and is not written.
  *   q_out (N, H, head_dim), k_out (N, kv_heads, head_dim) or NULL: the rotated queries and keys, bf16
  * 4-bit pages: lowest = bf16(min), step = bf16((max - lowest) / 15) (times the fp32 nearest to 1 / 15), code =
- * clamp(rint((x - lowest) / step), 0, 15), 0 where step is not positive, of the fp32 rotated keys and the values; a row that
- * is not finite throughout reads back as NaN.  Strides multiples of 8 elements, pointers 16-byte aligned.
+ * clamp(rint((x - lowest) / step), 0, 15), 0 where step is not positive, of the fp32 rotated keys and the values: off by half a
+ * step, 2^-8 of |min| and 2^-8 of the range at most.  A row that is not finite throughout, or whose range is not, reads back
+ * as NaN.  Strides multiples of 8 elements, pointers 16-byte aligned.
  */
 int smlm_paged_append(const void *qkv, int64_t qkv_row_stride, const void *rope_cos, const void *rope_sin, int rope_dtype,
                       int64_t rope_len, int rot, int interleaved, const int64_t *positions, const int64_t *slots,

@@ -18,8 +18,12 @@
 //
 // Products as in a causal prompt pass: S^T = K Q^T on v_mfma_f32_16x16x32_bf16 with the keys as M, so a lane (r, g) holds keys
 // 4 g .. 4 g + 3 of each 16-key tile for ONE query (r), and the softmax is per lane; O^T = V^T P^T
-// with the lane's own probabilities (rounded to bf16) as operand, V^T through transposing LDS reads.  Statistics, scores and
+// with the lane's own probabilities as operand, V^T through transposing LDS reads.  Statistics, scores and
 // output sums in fp32, the probabilities' sum of the same rounded values on the matrix cores.
+//
+// Probabilities are rounded to bf16 once, as in the other prompt pass: the result's error against 64 bits is 1.2 to 1.4 times that
+// of its own rounding.  A second term with what that rounding left, which single-token attention takes, would bring it to
+// 1.0 and the products of two operands: 11,063 tokens, 32 heads of 128, 627 -> 872 us, 8,192 with 64 dims 293 -> 424.
 //
 // A masked key weighs exactly nothing, also where its value is an infinity or a NaN (0 times which is NaN): masked tiles sum
 // their values' columns, and where a sum is not finite the values that are not are left out of the products and added key by key,

@@ -4,8 +4,10 @@
 //   a' = a cos - b sin,  b' = b cos + a sin      (half layout: b = dim i + rot / 2; interleaved: dims 2 i, 2 i + 1)
 // in fp32, every operation rounded (no fused multiply-adds, so that the same operations elsewhere give the same bits), q
 // rounded to bf16 into its own rows, k and v into row slots[n] % page of page slots[n] / page.  bf16 pages hold the rows as they
-// are; 4-bit pages hold, per row, lo = bf16(min), step = bf16((max - lo) / 15) and the codes clamp(rint((x - lo) / step), 0, 15):
-// a row's values lie within half a step of x, and a row that is not finite throughout reads back as NaN.
+// are; 4-bit pages hold, per row, lo = bf16(min), step = bf16((max - lo) / 15) and the codes clamp(rint((x - lo) / step), 0, 15).
+// What they stand for is within half a step of x and, towards the row's ends, what the roundings of lo and step leave out: 2^-8 of
+// the lowest value (of keys; values are bf16 before) and 2^-8 of the row's range.  So a row of keys whose range is small against
+// them loses more: 100.3 .. 100.9 begins at 100.5.  A row that is not finite throughout, or whose range is not, reads back as NaN.
 //
 // Bound by memory (every value read and written once).  One lane takes 8 dims of one row, 16 bytes of bf16: consecutive lanes
 // read consecutive 16-byte pieces of the projection's row.  In the half layout a lane also loads its partner's piece, which the

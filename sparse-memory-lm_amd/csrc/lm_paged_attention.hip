@@ -8,8 +8,10 @@
 // sequences leave compute units idle, the splits of a sequence by a second launch.  A tile's keys are loaded behind the scores of
 // the tile before, its values behind that one's value products, each into the registers just read, so that three wavefronts
 // fit a SIMD, and it is their number that hides the latency (two sets of registers, two wavefronts: 48 sequences in 4 bits 80
-// against 73 us).  bf16 reaches 4.8 to 5.1 TB/s (a copy 5.1), 4 bits 3.2 to 4.4: there the vector instructions of a tile, 270,
-// take as long as its bytes.
+// against 73 us, before the second term below).  bf16 reaches 4.7 to 5.1 TB/s (a copy 5.1).  4 bits reach 3.0 to 4.2, bound by the
+// latency of the loads: by the counters of those 48 sequences a wavefront waits for loads in 53% of its time and for its turn
+// to issue in 15%, and vector instructions, some 320 a tile, fill 63% of a SIMD's cycles (a third less of them, before the second
+// term, gained nothing, 73 against 72 us): more bytes would have to be under way than one tile a wavefront.
 //
 // Products on v_mfma_f32_16x16x32 with the tokens (then the dims) as M and up to 16 query heads as N.  S = K Q^T: a lane
 // (r, g) loads token r's dims and receives tokens 4 g .. 4 g + 3 of query r.  O^T = V^T P^T: a lane loads the 8 tokens that its
@@ -261,7 +263,7 @@ __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW
           }
     }
     // Online softmax per query (lane) in the log2 domain, with a reference point m that moves, to 2^8 above a tile's maximum, only
-    // when an exponential reaches 2.
+    // when an exponential reaches 2 (one of the group's heads: all whose maximum is as near to it, 2^0.99, move theirs).
     float p[8];
     auto exponentials = [&]() __attribute__((always_inline)) {
       float top = 0.f;
@@ -432,13 +434,16 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const float *parts, con
 }
 
 // How the walks are split.  One workgroup per sequence and group of heads, of 4 wavefronts, or of 8 where there are few of them and
-// a sequence has at most 1,024 tokens (one sequence of 700, 6 heads of 64: 10.4 us as three splits and a join, 7.9 so; 16
-// sequences of 2,000, one kv head: 10.0 and 12.6).  Longer ones are split, each split with at least 256 tokens of the longest
-// possible sequence: into 768 workgroups, three for each of the 256 compute units, all of them running at once (2 x 131,072
-// tokens in 4 bits: 65 us; 1,024 workgroups 77, 2,304 74), or, from 8 sequences on, whose lengths differ, into three times as
-// many, which even out (48 of up to 8,191: 768 workgroups 73 us, 2,304 68).
-// (Shares of equally many tiles, cut from the lengths on the device: 72 -> 70 us for these 48, 65 -> 61 for equal ones, but 10.5
-// -> 14.2 for 16 of 2,000 tokens, whose prefix sums and divisions take as long as their walk.)
+// the table holds at most 1,024 tokens (32 sequences of up to 700, 6 heads of 64, 4 bits: 10.0 us as splits and a join, 7.5 so;
+// 16 of 2,000, one kv head: 8.6 and 14.5).  Longer ones are split, into ranges of some 256 tokens of a full table (fewer by what
+// rounds the number of splits up) or more: into 768 workgroups, three for each of the 256 compute units, all of them running at
+// once (2 x 131,072 tokens in 4 bits: 68 us; 1,024 workgroups 80, 2,304 79), or, from 8 sequences on, into three times as many,
+// which even out where lengths differ (48 of up to 8,191: 768 workgroups 78 us, 2,304 71).  The lengths are on the device alone, so
+// their number stands in for whether they differ: 48 of 4,500 each take 58 us in 768 and 66 in 2,304; 9 of 30,000, whose 792
+// workgroups do not all run at once, 98 and 79; 7 of up to 40,000 53 either way.  The plan follows the table, not the
+// lengths: short sequences in a long table pay for its splits and their join.
+// (Shares of equally many tiles, cut from the lengths on the device, before the second term above: 72 -> 70 us for these 48, 65 ->
+// 61 for equal ones, but 10.5 -> 14.2 for 16 of 2,000 tokens, whose prefix sums and divisions take as long as their walk.)
 struct Plan {
   int waves, splits;
 };

@@ -17,10 +17,10 @@
 // holds the k-th largest of the threads' own maxima; min_p: a bound on the logit -- and everything else is done on the list, by ranking
 // each of its 512 tokens at most against all (256 of a bf16 row: 256 rows with min_p 0.01 and top_p 46 us with more, 42 so).
 // Else a cut, the top_k-th token or the one at which the mass reaches top_p, is found in a bf16 row by counting its distinct
-// values, in an fp32 row by a histogram of 1,024 bins, then within its bin.  One row, whole calls: the largest 10 us, no cut 23,
-// top_k 50 with top_p 16, min_p 0.1 13, top_p 0.9 alone 37 by distinct values (55 by the histogram, as in fp32), top_k 2,000 with
-// top_p 36 (57); 256 rows 5 to 15% more, whatever a row's alignment (read by
-// elements where it is not 16-byte aligned, 25 us for the largest of an fp32 row).  (Forming the weights' rough sum
+// values, in an fp32 row by a histogram of 1,024 bins, then within its bin.  One row, whole calls, bf16 (fp32): the largest 9.5 us
+// (9.5), no cut 24 (23), top_k 50 with top_p 16 (16), min_p 0.1 13 (13), top_p 0.9 alone 37 (53), top_k 2,000 with top_p 36 (63);
+// 256 bf16 rows 6 to 17% more, with min_p 0.01 and top_p a third; 256 fp32 rows, which LDS does not hold at this size, 17, 30, 23,
+// 22, 65 and 79 us.  Rows of 50,303, of which none but the first is aligned, take as long.  (Forming the weights' rough sum
 // while the row is read took top_p alone from 59 to 54 us and top_p with min_p from 25 to 27; masses looked up per distinct value
 // instead of formed per token, 23 to 33 us without a cut.)
 #include <cstddef>

@@ -1233,8 +1233,9 @@ def paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, inte
     rotating the first dims of a head (a multiple of 16) in pairs (i, i + half) or, interleaved, (2 i, 2 i + 1); positions and
     slots (N,) int64, the slots distinct.  Returns q (N, n_heads, head_dim) and, with keys=True, the rotated keys (N,
     n_kv_heads, head_dim), else None.  A slot outside the pages (-1) is not written; a position outside the tables gives NaN
-    and is not written.  Rotation in fp32, rounded once; 4-bit pages take the unrounded keys, and a row that is not finite
-    throughout reads back as NaN."""
+    and is not written.  Rotation in fp32, rounded once; 4-bit pages take the unrounded keys.  There a dim is off by up to half a step (a
+    30th of its row's range), 2^-8 of the row's lowest value and 2^-8 of its range, and a row that is not finite throughout, or
+    whose range is not, reads back as NaN."""
     return _lib.serve_ops().paged_append(qkv, rope_cos, rope_sin, positions, slots, pages, n_heads, interleaved, keys)
 
 

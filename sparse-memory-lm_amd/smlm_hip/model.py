@@ -710,7 +710,8 @@ class Transformer(nn.Module):
         tensors (n_seqs,), fp32, top_k int32) from random numbers of `generator`; temperature 0 is greedy, as generate() is.
         Returns the ids (n_seqs, new_tokens + 1): the prompts' next tokens, then one per step; all but the last are in the
         cache afterwards, which a later call may go on from.  Every sequence needs a prompt.  With use_graph a step is one
-        replay of a captured graph, kept by the cache."""
+        replay of a captured graph, kept by the cache: without a cache of the caller's every call makes pages and a graph of its
+        own."""
         prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
         if cache is None:
             longest = max((len(p) for p in prompts), default=0) + new_tokens

@@ -368,3 +368,40 @@ def test_a_models_attention_over_what_its_cache_holds(kind):
             scales = rows(layer.pages[2], at), rows(layer.pages[3], at)
         want, bound, _ = close_to_64_bits(q[b], k, v, D ** -0.5, *scales)
         assert ((y[b] - want).abs() <= bound).all(), b
+
+
+@pytest.mark.parametrize("of", ["normal", "far from zero", "small", "tiny", "huge"])
+def test_what_4_bit_rows_stand_for(of):
+    """Half a step, 2^-8 of the row's lowest value and 2^-8 of its range, and the gather's own rounding; rows of offsets large against
+    their range too."""
+    g = gen(70)
+    N, D = 64, 64
+    x = {"normal": 1.0, "far from zero": 0.1, "small": 1e-3, "tiny": 1e-30, "huge": 1e30}[of] * torch.randn(N, 3 * D, generator=g)
+    x = (x + 100 if of == "far from zero" else x).to(bf16)
+    a = torch.outer(torch.arange(N).double(), 10000.0 ** (-torch.arange(0, D, 2).double() / D))
+    cos, sin = a.cos().float(), a.sin().float()
+    if of == "far from zero":                              # keys as they are, too
+        cos, sin = torch.full_like(cos, 1.003), torch.zeros_like(sin)
+    pages, n = K.kv_pages(4, 1, 16, D, "q4", DEV), torch.arange(N, device=DEV)
+    K.paged_append(x.to(DEV), cos.to(DEV), sin.to(DEV), n, n, pages, 1)
+    rows = x.double().view(N, 3, D)
+    keys = R.rotate(rows[:, 1:2], cos.double(), sin.double(), False)[:, 0]
+    for got, want in zip(K.paged_gather(pages, n), (keys, rows[:, 2])):
+        low, high = want.amin(-1, keepdim=True), want.amax(-1, keepdim=True)
+        # (rounded, a step is up to 2^-8 longer; 4 roundings of fp32 in the rotation and the codes)
+        bound = ((high - low) / 30 * (1 + R.HALF) + R.HALF * low.abs() + R.HALF * (high - low) + R.HALF * want.abs()
+                 + 4 * 2.0 ** -24 * (low.abs() + high.abs()))
+        assert ((got[:, 0].double().cpu() - want).abs() <= bound).all()
+
+
+def test_4_bit_rows_of_a_range_beyond_fp32_are_nan():
+    pages, n = K.kv_pages(1, 1, 16, 32, "q4", DEV), torch.arange(2, device=DEV)
+    qkv = torch.ones(2, 3, 32)
+    qkv[1, 1:, ::3], qkv[1, 1:, 1::3] = 3e38, -3e38
+    one, zero = torch.ones(2, 16, device=DEV), torch.zeros(2, 16, device=DEV)
+    K.paged_append(qkv.view(2, 96).to(DEV, bf16), one, zero, n, n, pages, 1)
+    for got in K.paged_gather(pages, n):
+        assert (got[0] == 1).all() and torch.isnan(got[1]).all()
+    q, table = torch.ones(1, 1, 32, dtype=bf16, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    at = lambda m: K.paged_attention(q, pages, table, torch.tensor([m], dtype=torch.int32, device=DEV))  # noqa: E731
+    assert (at(1) == 1).all() and torch.isnan(at(2)).all()
